@@ -293,6 +293,101 @@ int piper_b200_sage2pp_fwd(const void* query, const int64_t query_strides[3], co
                            int64_t head_dim, double scale, int is_causal, void* workspace,
                            size_t workspace_bytes, void* stream);
 
+/* ---- Decoding over a quantised paged cache -------------------------------
+ * One step of (speculative) decoding.  No counterpart in the reference, which
+ * runs whole prompts.  The cache holds INT8 codes of keys and values and one
+ * fp32 scale for each row (a token of a KV head); a request's tokens lie in
+ * pages that its row of the block table names in order.  `lengths` counts the
+ * committed tokens of each request; a call's new or drafted token i has
+ * position lengths[b] + i.  All pointers are device memory.
+ *
+ *   key_codes, value_codes    int8 [pages, kv_heads, page_size, head_dim]
+ *   key_scales, value_scales  f32  [pages, kv_heads, page_size]
+ *   key_mean                  f32  [kv_heads, head_dim] or NULL: subtracted
+ *                             from keys before quantisation and added when
+ *                             they are read back; a softmax does not see it
+ *   block_table               int32 [batch, table_width], rows table_stride
+ *                             elements apart
+ *   lengths                   int32 [batch]
+ *
+ * page_size is a power of two from 16 to 256, head_dim 64 or 128; the codes
+ * are 16-byte aligned.  Positions outside a request's table row, and table
+ * entries outside [0, pages), name no row: writes and moves skip them, reads
+ * give zeros, attention does not see them. */
+typedef struct piper_b200_kv_cache_s {
+  void* key_codes;
+  float* key_scales;
+  void* value_codes;
+  float* value_scales;
+  const float* key_mean;
+  const int32_t* block_table;
+  const int32_t* lengths;
+  int64_t pages, table_stride;
+  int32_t kv_heads, page_size, head_dim, batch, table_width;
+} piper_b200_kv_cache_t;
+
+/* Quantises `tokens` new rows per request and KV head into the cache at
+ * positions lengths[b] + i, i < counts[b] (counts NULL: all).  key and value
+ * are [batch, kv_heads, tokens, head_dim] with element strides (B, H, N).  A
+ * row's scale is fp32(max|x| * fp32(1/127)), or 1 for a row of zeros; a code
+ * is x / scale rounded half to even.  Rows are expected to be distinct: two
+ * requests that share the page they write to race. */
+int piper_b200_kv_cache_write(const piper_b200_kv_cache_t* cache, const void* key,
+                              const int64_t key_strides[3], const void* value,
+                              const int64_t value_strides[3], int dtype, int64_t tokens,
+                              const int32_t* counts, void* stream);
+
+/* Values of the rows at positions lengths[b] + i into contiguous key_out and
+ * value_out [batch, kv_heads, tokens, head_dim]; zeros where i >= counts[b]. */
+int piper_b200_kv_cache_read(const piper_b200_kv_cache_t* cache, void* key_out, void* value_out,
+                             int dtype, int64_t tokens, const int32_t* counts, void* stream);
+
+/* Moves the row at position lengths[b] + path[b][j] to lengths[b] + j for
+ * 1 <= j < min(counts[b], nodes), as if all rows were read before any is
+ * written.  path is int32 [batch, nodes] (rows path_stride elements apart),
+ * nodes at most 64; entries outside [0, nodes) move nothing. */
+int piper_b200_kv_cache_keep(const piper_b200_kv_cache_t* cache, const int32_t* path,
+                             int64_t path_stride, int64_t nodes, const int32_t* counts,
+                             void* stream);
+
+/* Workspace bytes of piper_b200_tree_attention (0 when it needs none). */
+int piper_b200_tree_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads,
+                                              int64_t nodes, int64_t head_dim, size_t* bytes);
+
+/* Attention of `nodes` (1 to 64) query rows per request and head over the
+ * cache: node t of request b sees positions [0, lengths[b]) and drafted
+ * position lengths[b] + j where bit j of tree_mask[b][t] is set (tree_mask
+ * NULL: j <= t, a chain).  A row that sees nothing is zero.  query is [batch,
+ * heads, nodes, head_dim] with element strides (B, H, N), heads a multiple of
+ * kv_heads (query head h reads KV head h / (heads / kv_heads)); out is
+ * contiguous and of the same type.  tree_mask is int64 [batch, nodes], rows
+ * mask_stride elements apart (0: one tree for all). */
+int piper_b200_tree_attention(const piper_b200_kv_cache_t* cache, const void* query,
+                              const int64_t query_strides[3], void* out, int dtype, int64_t heads,
+                              int64_t nodes, const int64_t* tree_mask, int64_t mask_stride,
+                              double scale, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Rejection sampling over a drafted tree.  Node 0 is the root; node i > 0
+ * carries tokens[b][i] (negative or >= vocab: absent), drawn from
+ * draft[b][parents[b][i]], with parents[b][i] < i.  In node order, a child x
+ * of the current node is accepted when uniform[b][i] * draft[x] < rest[x],
+ * and becomes the current node with rest = its row of `target`; otherwise
+ * rest becomes max(rest - draft, 0) normalised (unchanged where that is zero
+ * everywhere).  path[b] lists the accepted nodes, the root first, then -1;
+ * count[b] is their number; next_token[b] is the lowest index of the largest
+ * rest / noise[b] (a draw from rest when noise is exponential).  target and
+ * draft are f32 [batch, nodes, vocab] with element strides (B, N); tokens
+ * int64, parents int32, uniform f32 [batch, nodes] and noise f32 [batch,
+ * vocab] have one row stride each; path int32 [batch, nodes], count int32 and
+ * next_token int64 [batch] are contiguous.  nodes is at most 64. */
+int piper_b200_verify_draft_tree(const float* target, const int64_t target_strides[2],
+                                 const float* draft, const int64_t draft_strides[2],
+                                 const int64_t* tokens, int64_t tokens_stride,
+                                 const int32_t* parents, int64_t parents_stride,
+                                 const float* uniform, int64_t uniform_stride, const float* noise,
+                                 int64_t noise_stride, int64_t batch, int64_t nodes, int64_t vocab,
+                                 int32_t* path, int32_t* count, int64_t* next_token, void* stream);
+
 /* Scratch capacity of piper_b200_attention_fwd_no_alloc: 16 MiB per GPU. */
 #define PIPER_B200_NO_ALLOC_WORKSPACE_BYTES (16u * 1024u * 1024u)
 

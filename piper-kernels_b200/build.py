@@ -2,8 +2,9 @@
 
 Usage: ``python piper-kernels_b200/build.py [--force] [--verbose]``.
 
-One translation unit (``csrc/piper_b200.cu``) compiled by nvcc for
-``sm_100a`` only, with the C ABI of ``include/piper_b200.h``.  The CUDA
+Each ``csrc/*.cu`` is one translation unit, compiled by nvcc for ``sm_100a``
+only (side by side) and linked into one library with the C ABI of
+``include/piper_b200.h``.  The CUDA
 runtime is linked statically and the driver's tensor-map encoder is looked up
 at run time, so the library has no dependency beyond the NVIDIA driver.
 """
@@ -13,6 +14,7 @@ from __future__ import annotations
 import argparse
 import subprocess
 import sys
+import tempfile
 from pathlib import Path
 
 PKG_ROOT = Path(__file__).resolve().parent
@@ -26,7 +28,6 @@ NVCC_FLAGS = [
     "-O3",
     "-std=c++17",
     "-Xcompiler", "-fPIC",
-    "-shared",
 ]
 
 
@@ -40,13 +41,15 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         if OUTPUT.stat().st_mtime >= newest:
             return OUTPUT
     OUTPUT.parent.mkdir(parents=True, exist_ok=True)
-    cmd = [
-        "nvcc", *NVCC_FLAGS,
-        f"-I{INCLUDE}", f"-I{CSRC}",
-        *(["-Xptxas", "-v"] if verbose else []),
-        "-o", str(OUTPUT), str(CSRC / "piper_b200.cu"),
-    ]
-    subprocess.run(cmd, check=True)
+    common = ["nvcc", *NVCC_FLAGS, f"-I{INCLUDE}", f"-I{CSRC}", *(["-Xptxas", "-v"] if verbose else [])]
+    with tempfile.TemporaryDirectory() as tmp:
+        units = [(src, Path(tmp) / f"{src.stem}.o") for src in sorted(CSRC.glob("*.cu"))]
+        running = [subprocess.Popen([*common, "-c", "-o", str(obj), str(src)]) for src, obj in units]
+        codes = [process.wait() for process in running]
+        for process, code in zip(running, codes):
+            if code != 0:
+                raise subprocess.CalledProcessError(code, process.args)
+        subprocess.run(["nvcc", *NVCC_FLAGS, "-shared", "-o", str(OUTPUT), *(str(obj) for _, obj in units)], check=True)
     return OUTPUT
 
 

@@ -16,6 +16,7 @@
 
 #include "attention.cuh"
 #include "piper_attention.cuh"
+#include "host_api.h"
 #include "layout.h"
 #include "piper_b200.h"
 #include "prepass.cuh"
@@ -176,6 +177,28 @@ int encode_map(CUtensorMap* map, const void* base, uint64_t inner, uint64_t mid,
   if (r != CUDA_SUCCESS) return fail(PIPER_B200_ERR_CUDA, "cuTensorMapEncodeTiled failed: " + std::to_string(r));
   return PIPER_B200_OK;
 }
+
+}  // namespace
+
+namespace piper {
+namespace host {
+
+int fail(int code, const std::string& msg) { return ::fail(code, msg); }
+int cuda_fail(cudaError_t err, const char* what) { return ::cuda_fail(err, what); }
+
+int ensure_device(int* device, unsigned long long* context, int* sms) {
+  const int rc = ::ensure_device(device);
+  if (rc != PIPER_B200_OK) return rc;
+  std::lock_guard<std::mutex> lock(g_init_mutex);
+  *context = g_device_context[*device];
+  *sms = g_device_sms[*device];
+  return PIPER_B200_OK;
+}
+
+}  // namespace host
+}  // namespace piper
+
+namespace {
 
 int check_shape(int dtype, int64_t b, int64_t h, int64_t nq, int64_t nk, int64_t d, int causal) {
   if (dtype != PIPER_B200_FLOAT16 && dtype != PIPER_B200_BFLOAT16)

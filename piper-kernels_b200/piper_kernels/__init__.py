@@ -6,9 +6,34 @@ Drop-in for the reference package's public entry points
 functions and the same ``torch.ops.piper_kernels.*`` custom operators,
 computed by hand-written sm_100a CUDA kernels behind the C ABI in
 ``include/piper_b200.h``.
+
+Next to them, the operators of a (speculative) decoding step over a quantised
+paged KV cache (:mod:`piper_kernels.decoding`), which the reference does not
+have.
 """
 
 from .attention.piper_attention import piper_attention
 from .attention.sage_attention_2pp import sage_attention_2pp
+from .decoding import (
+    DraftVerification,
+    QuantizedKVCache,
+    keep_draft_path,
+    read_kv_cache,
+    tree_attention,
+    tree_mask_from_parents,
+    verify_draft_tree,
+    write_kv_cache,
+)
 
-__all__ = ["piper_attention", "sage_attention_2pp"]
+__all__ = [
+    "DraftVerification",
+    "QuantizedKVCache",
+    "keep_draft_path",
+    "piper_attention",
+    "read_kv_cache",
+    "sage_attention_2pp",
+    "tree_attention",
+    "tree_mask_from_parents",
+    "verify_draft_tree",
+    "write_kv_cache",
+]

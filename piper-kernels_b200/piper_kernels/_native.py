@@ -52,6 +52,12 @@ EXPORTED_SYMBOLS = (
     "piper_b200_sage2pp_prepass",
     "piper_b200_sage2pp_attention_prepared",
     "piper_b200_sage2pp_fwd",
+    "piper_b200_kv_cache_write",
+    "piper_b200_kv_cache_read",
+    "piper_b200_kv_cache_keep",
+    "piper_b200_tree_attention_workspace_bytes",
+    "piper_b200_tree_attention",
+    "piper_b200_verify_draft_tree",
     "piper_b200_device_status",
     "piper_b200_selftest_wait_timeout",
     "piper_b200_selftest_exp2",
@@ -98,10 +104,22 @@ class Sage2ppLayout(ctypes.Structure):
     ] + [(name, ctypes.c_int64) for name in ("nk_pad", "chunks")]
 
 
+class KVCache(ctypes.Structure):
+    """Mirror of ``piper_b200_kv_cache_t``."""
+
+    _fields_ = [
+        (name, ctypes.c_void_p)
+        for name in ("key_codes", "key_scales", "value_codes", "value_scales", "key_mean", "block_table", "lengths")
+    ] + [(name, ctypes.c_int64) for name in ("pages", "table_stride")] + [
+        (name, ctypes.c_int32) for name in ("kv_heads", "page_size", "head_dim", "batch", "table_width")
+    ]
+
+
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 _I64 = ctypes.c_int64
 _STRIDES = ctypes.c_int64 * 3
+_STRIDES2 = ctypes.c_int64 * 2
 _VP = ctypes.c_void_p
 
 
@@ -175,6 +193,21 @@ def _declare(lib: ctypes.CDLL) -> None:
         ctypes.c_double, ctypes.c_int, _VP, ctypes.c_size_t, _VP,
     ]
     lib.piper_b200_sage2pp_fwd.restype = ctypes.c_int
+    cache = ctypes.POINTER(KVCache)
+    lib.piper_b200_kv_cache_write.argtypes = [cache, _VP, _STRIDES, _VP, _STRIDES, ctypes.c_int, _I64, _VP, _VP]
+    lib.piper_b200_kv_cache_write.restype = ctypes.c_int
+    lib.piper_b200_kv_cache_read.argtypes = [cache, _VP, _VP, ctypes.c_int, _I64, _VP, _VP]
+    lib.piper_b200_kv_cache_read.restype = ctypes.c_int
+    lib.piper_b200_kv_cache_keep.argtypes = [cache, _VP, _I64, _I64, _VP, _VP]
+    lib.piper_b200_kv_cache_keep.restype = ctypes.c_int
+    lib.piper_b200_tree_attention_workspace_bytes.argtypes = [_I64] * 5 + [ctypes.POINTER(ctypes.c_size_t)]
+    lib.piper_b200_tree_attention_workspace_bytes.restype = ctypes.c_int
+    lib.piper_b200_tree_attention.argtypes = [cache, _VP, _STRIDES, _VP, ctypes.c_int, _I64, _I64, _VP, _I64] + [
+        ctypes.c_double, _VP, ctypes.c_size_t, _VP,
+    ]
+    lib.piper_b200_tree_attention.restype = ctypes.c_int
+    lib.piper_b200_verify_draft_tree.argtypes = [_VP, _STRIDES2] * 2 + [_VP, _I64] * 4 + [_I64] * 3 + [_VP] * 4
+    lib.piper_b200_verify_draft_tree.restype = ctypes.c_int
     lib.piper_b200_device_status.argtypes = [ctypes.c_int, ctypes.c_int, ctypes.POINTER(ctypes.c_uint32)]
     lib.piper_b200_device_status.restype = ctypes.c_int
     lib.piper_b200_selftest_wait_timeout.argtypes = [ctypes.c_uint64, ctypes.POINTER(ctypes.c_int), _VP]
@@ -222,6 +255,11 @@ def check(status: int, what: str) -> None:
 def strides3(tensor) -> _STRIDES:
     s = tensor.stride()
     return _STRIDES(s[0], s[1], s[2])
+
+
+def strides2(tensor) -> _STRIDES2:
+    s = tensor.stride()
+    return _STRIDES2(s[0], s[1])
 
 
 def workspace_layout(batch: int, heads: int, nq: int, nk: int, d: int) -> WorkspaceLayout:

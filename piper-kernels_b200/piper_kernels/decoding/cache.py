@@ -1,0 +1,354 @@
+"""The quantised paged KV cache: its buffers, and writing, reading and moving rows.
+
+A row is one token of one KV head.  Its ``head_dim`` values ``x`` (for keys
+less ``key_mean``) are held as INT8 codes and one fp32 scale::
+
+    scale = max|x| * fp32(1/127)      (1 for a row of zeros)
+    code  = round half to even (x / scale)
+
+and stand for ``code * scale`` (plus ``key_mean`` for keys).  A constant taken
+off every key does not change a softmax over keys, so attention over the cache
+does not need the mean; it only makes the codes finer, like the K smoothing of
+``piper_attention``.
+
+A request's tokens lie in the pages that its row of ``block_table`` names, in
+order; ``lengths`` counts its committed tokens, and token ``i`` of a call has
+position ``lengths[b] + i``.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+
+import torch
+
+from .. import _native
+from ._common import (
+    DTYPE_CODES,
+    MAX_NODES,
+    SUPPORTED_HEAD_DIMS,
+    check_half,
+    check_no_grad,
+    check_tensor,
+    launch,
+    require_device,
+)
+
+PAGE_SIZES = (16, 32, 64, 128, 256)
+
+
+@dataclass(frozen=True, eq=False)
+class QuantizedKVCache:
+    """Buffers of one layer's cache; a handle that a program keeps.
+
+    ``key_codes`` and ``value_codes`` are int8 ``[pages, kv_heads, page_size,
+    head_dim]``, ``key_scales`` and ``value_scales`` float32 ``[pages,
+    kv_heads, page_size]``, all contiguous on one device.  ``key_mean`` is
+    float32 ``[kv_heads, head_dim]`` or None; it belongs to the rows written
+    with it.  ``page_size`` is 16, 32, 64, 128 or 256, ``head_dim`` 64 or 128.
+    """
+
+    key_codes: torch.Tensor
+    key_scales: torch.Tensor
+    value_codes: torch.Tensor
+    value_scales: torch.Tensor
+    key_mean: torch.Tensor | None = None
+
+    def __post_init__(self) -> None:
+        codes = self.key_codes
+        if codes.ndim != 4:
+            raise ValueError(
+                "QuantizedKVCache key_codes must have shape [pages, kv_heads, page_size, head_dim], "
+                f"got {tuple(codes.shape)}"
+            )
+        pages, kv_heads, page_size, head_dim = codes.shape
+        if head_dim not in SUPPORTED_HEAD_DIMS:
+            raise ValueError(f"QuantizedKVCache supports head dimensions 64 and 128, got {head_dim}")
+        if page_size not in PAGE_SIZES:
+            raise ValueError(f"QuantizedKVCache page_size must be one of {PAGE_SIZES}, got {page_size}")
+        if pages == 0 or kv_heads == 0:
+            raise ValueError("QuantizedKVCache needs at least one page and one KV head")
+        device = codes.device
+        for name, tensor, shape, dtype in (
+            ("key_codes", codes, codes.shape, torch.int8),
+            ("value_codes", self.value_codes, codes.shape, torch.int8),
+            ("key_scales", self.key_scales, codes.shape[:3], torch.float32),
+            ("value_scales", self.value_scales, codes.shape[:3], torch.float32),
+        ):
+            check_tensor("QuantizedKVCache", name, tensor, shape, dtype, device)
+            if not tensor.is_contiguous():
+                raise ValueError(f"QuantizedKVCache {name} must be contiguous")
+        if self.key_mean is not None:
+            check_tensor("QuantizedKVCache", "key_mean", self.key_mean, (kv_heads, head_dim), torch.float32, device)
+            if not self.key_mean.is_contiguous():
+                raise ValueError("QuantizedKVCache key_mean must be contiguous")
+
+    @classmethod
+    def allocate(
+        cls,
+        pages: int,
+        kv_heads: int,
+        page_size: int,
+        head_dim: int,
+        *,
+        device: torch.device | str | int | None = None,
+        key_mean: torch.Tensor | None = None,
+    ) -> "QuantizedKVCache":
+        """A new cache whose rows all stand for zero."""
+        shape = (pages, kv_heads, page_size, head_dim)
+        if device is None:
+            device = "cuda"
+        return cls(
+            torch.zeros(shape, dtype=torch.int8, device=device),
+            torch.ones(shape[:3], dtype=torch.float32, device=device),
+            torch.zeros(shape, dtype=torch.int8, device=device),
+            torch.ones(shape[:3], dtype=torch.float32, device=device),
+            key_mean=key_mean,
+        )
+
+    @property
+    def device(self) -> torch.device:
+        return self.key_codes.device
+
+    @property
+    def kv_heads(self) -> int:
+        return self.key_codes.shape[1]
+
+    @property
+    def page_size(self) -> int:
+        return self.key_codes.shape[2]
+
+    @property
+    def head_dim(self) -> int:
+        return self.key_codes.shape[3]
+
+    def native(self, block_table: torch.Tensor, lengths: torch.Tensor) -> _native.KVCache:
+        """The C ABI's description of this cache for one batch."""
+        pages, kv_heads, page_size, head_dim = self.key_codes.shape
+        return _native.KVCache(
+            self.key_codes.data_ptr(), self.key_scales.data_ptr(), self.value_codes.data_ptr(),
+            self.value_scales.data_ptr(), None if self.key_mean is None else self.key_mean.data_ptr(),
+            block_table.data_ptr(), lengths.data_ptr(), pages, block_table.stride(0), kv_heads, page_size, head_dim,
+            block_table.shape[0], block_table.shape[1],
+        )
+
+
+def check_batch(
+    operator: str, cache: QuantizedKVCache, batch: int, block_table: torch.Tensor, lengths: torch.Tensor
+) -> None:
+    """Check the arguments that say where a batch's tokens lie."""
+    if batch == 0:
+        raise ValueError(f"{operator} does not accept an empty batch")
+    check_tensor(operator, "block_table", block_table, (batch, None), torch.int32, cache.device)
+    check_tensor(operator, "lengths", lengths, (batch,), torch.int32, cache.device)
+    if block_table.shape[1] == 0:
+        raise ValueError(f"{operator} block_table must have at least one column")
+
+
+def write_kv_cache(
+    cache: QuantizedKVCache,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    block_table: torch.Tensor,
+    lengths: torch.Tensor,
+    *,
+    counts: torch.Tensor | None = None,
+) -> None:
+    """Quantise new keys and values into the cache, in place.
+
+    ``key`` and ``value`` are float16 or bfloat16 ``[batch, kv_heads, tokens,
+    head_dim]`` with a contiguous head dimension and any other strides; token
+    ``i`` of request ``b`` goes to position ``lengths[b] + i`` if ``i <
+    counts[b]`` (int32; default: every token).  ``block_table`` is int32
+    ``[batch, columns]``, ``lengths`` int32 ``[batch]``; ``lengths`` is not
+    changed.  Tokens whose position has no page (a column past the table, or an
+    entry that is no page of the cache, such as -1) are not written.  Pages
+    that are written must not be shared between requests.
+    """
+    operator = "write_kv_cache"
+    if key.ndim != 4:
+        raise ValueError(f"{operator} key must have shape [batch, heads, sequence, head_dim], got {tuple(key.shape)}")
+    batch, kv_heads, tokens, head_dim = key.shape
+    check_half(operator, "key", key.dtype)
+    check_tensor(operator, "key", key, (batch, cache.kv_heads, tokens, cache.head_dim), key.dtype, cache.device)
+    check_tensor(operator, "value", value, key.shape, key.dtype, cache.device)
+    if tokens == 0:
+        raise ValueError(f"{operator} does not accept an empty sequence")
+    check_batch(operator, cache, batch, block_table, lengths)
+    if counts is not None:
+        check_tensor(operator, "counts", counts, (batch,), torch.int32, cache.device)
+    check_no_grad(operator, key, value)
+    require_device(operator, cache.device)
+    if torch.compiler.is_compiling():
+        torch.ops.piper_kernels.write_kv_cache(
+            cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales, cache.key_mean, key, value,
+            block_table, lengths, counts,
+        )
+    else:
+        _write(cache, key, value, block_table, lengths, counts)
+
+
+def _write(cache, key, value, block_table, lengths, counts) -> None:
+    launch(
+        "piper_b200_kv_cache_write", cache.device, _native.library().piper_b200_kv_cache_write,
+        ctypes.byref(cache.native(block_table, lengths)), key.data_ptr(), _native.strides3(key), value.data_ptr(),
+        _native.strides3(value), DTYPE_CODES[key.dtype], key.shape[2], None if counts is None else counts.data_ptr(),
+    )
+
+
+def read_kv_cache(
+    cache: QuantizedKVCache,
+    block_table: torch.Tensor,
+    lengths: torch.Tensor,
+    tokens: int,
+    *,
+    counts: torch.Tensor | None = None,
+    dtype: torch.dtype = torch.bfloat16,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values of cached rows, as ``dtype`` ``[batch, kv_heads, tokens, head_dim]``.
+
+    Token ``i`` of request ``b`` is the row at position ``lengths[b] + i``
+    (``lengths`` of zeros reads from the start); tokens from ``counts[b]`` on
+    (default: none), and positions without a page, read as zeros.
+    """
+    operator = "read_kv_cache"
+    check_half(operator, "dtype", dtype)
+    tokens = int(tokens)
+    if tokens <= 0:
+        raise ValueError(f"{operator} tokens must be positive, got {tokens}")
+    if lengths.ndim != 1:
+        raise ValueError(f"{operator} lengths must have shape [batch], got {tuple(lengths.shape)}")
+    check_batch(operator, cache, lengths.shape[0], block_table, lengths)
+    if counts is not None:
+        check_tensor(operator, "counts", counts, (lengths.shape[0],), torch.int32, cache.device)
+    require_device(operator, cache.device)
+    if torch.compiler.is_compiling():
+        return torch.ops.piper_kernels.read_kv_cache(
+            cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales, cache.key_mean, block_table,
+            lengths, counts, tokens, dtype,
+        )
+    return _read(cache, block_table, lengths, counts, tokens, dtype)
+
+
+def _read(cache, block_table, lengths, counts, tokens, dtype) -> tuple[torch.Tensor, torch.Tensor]:
+    shape = (lengths.shape[0], cache.kv_heads, tokens, cache.head_dim)
+    key = torch.empty(shape, dtype=dtype, device=cache.device)
+    value = torch.empty(shape, dtype=dtype, device=cache.device)
+    launch(
+        "piper_b200_kv_cache_read", cache.device, _native.library().piper_b200_kv_cache_read,
+        ctypes.byref(cache.native(block_table, lengths)), key.data_ptr(), value.data_ptr(), DTYPE_CODES[dtype],
+        tokens, None if counts is None else counts.data_ptr(),
+    )
+    return key, value
+
+
+def keep_draft_path(
+    cache: QuantizedKVCache,
+    block_table: torch.Tensor,
+    lengths: torch.Tensor,
+    path: torch.Tensor,
+    counts: torch.Tensor,
+) -> None:
+    """Move the accepted drafted rows together, in place.
+
+    ``path`` (int32 ``[batch, nodes]``) and ``counts`` (int32 ``[batch]``) are
+    :func:`~piper_kernels.verify_draft_tree`'s: the row at position
+    ``lengths[b] + path[b, j]`` moves to ``lengths[b] + j`` for ``1 <= j <
+    counts[b]``.  ``lengths`` is not changed; the committed length is then
+    ``lengths + counts``.
+    """
+    operator = "keep_draft_path"
+    if path.ndim != 2:
+        raise ValueError(f"{operator} path must have shape [batch, nodes], got {tuple(path.shape)}")
+    batch, nodes = path.shape
+    if not 1 <= nodes <= MAX_NODES:
+        raise ValueError(f"{operator} supports 1 to {MAX_NODES} nodes, got {nodes}")
+    check_batch(operator, cache, batch, block_table, lengths)
+    check_tensor(operator, "path", path, (batch, nodes), torch.int32, cache.device)
+    check_tensor(operator, "counts", counts, (batch,), torch.int32, cache.device)
+    require_device(operator, cache.device)
+    if torch.compiler.is_compiling():
+        torch.ops.piper_kernels.keep_draft_path(
+            cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales, block_table, lengths, path,
+            counts,
+        )
+    else:
+        _keep(cache, block_table, lengths, path, counts)
+
+
+def _keep(cache, block_table, lengths, path, counts) -> None:
+    launch(
+        "piper_b200_kv_cache_keep", cache.device, _native.library().piper_b200_kv_cache_keep,
+        ctypes.byref(cache.native(block_table, lengths)), path.data_ptr(), path.stride(0), path.shape[1],
+        counts.data_ptr(),
+    )
+
+
+_BUFFERS = ("key_codes", "key_scales", "value_codes", "value_scales")
+
+
+@torch.library.custom_op("piper_kernels::write_kv_cache", mutates_args=_BUFFERS)
+def _write_op(
+    key_codes: torch.Tensor,
+    key_scales: torch.Tensor,
+    value_codes: torch.Tensor,
+    value_scales: torch.Tensor,
+    key_mean: torch.Tensor | None,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    block_table: torch.Tensor,
+    lengths: torch.Tensor,
+    counts: torch.Tensor | None,
+) -> None:
+    cache = QuantizedKVCache(key_codes, key_scales, value_codes, value_scales, key_mean)
+    _write(cache, key, value, block_table, lengths, counts)
+
+
+@_write_op.register_fake
+def _write_fake(*_args) -> None:
+    return None
+
+
+@torch.library.custom_op("piper_kernels::read_kv_cache", mutates_args=())
+def _read_op(
+    key_codes: torch.Tensor,
+    key_scales: torch.Tensor,
+    value_codes: torch.Tensor,
+    value_scales: torch.Tensor,
+    key_mean: torch.Tensor | None,
+    block_table: torch.Tensor,
+    lengths: torch.Tensor,
+    counts: torch.Tensor | None,
+    tokens: int,
+    dtype: torch.dtype,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    cache = QuantizedKVCache(key_codes, key_scales, value_codes, value_scales, key_mean)
+    return _read(cache, block_table, lengths, counts, tokens, dtype)
+
+
+@_read_op.register_fake
+def _read_fake(
+    key_codes, _key_scales, _value_codes, _value_scales, _key_mean, _block_table, lengths, _counts, tokens, dtype
+):
+    shape = (lengths.shape[0], key_codes.shape[1], tokens, key_codes.shape[3])
+    return key_codes.new_empty(shape, dtype=dtype), key_codes.new_empty(shape, dtype=dtype)
+
+
+@torch.library.custom_op("piper_kernels::keep_draft_path", mutates_args=_BUFFERS)
+def _keep_op(
+    key_codes: torch.Tensor,
+    key_scales: torch.Tensor,
+    value_codes: torch.Tensor,
+    value_scales: torch.Tensor,
+    block_table: torch.Tensor,
+    lengths: torch.Tensor,
+    path: torch.Tensor,
+    counts: torch.Tensor,
+) -> None:
+    _keep(QuantizedKVCache(key_codes, key_scales, value_codes, value_scales), block_table, lengths, path, counts)
+
+
+@_keep_op.register_fake
+def _keep_fake(*_args) -> None:
+    return None

@@ -1,0 +1,206 @@
+"""Decoding operators on the host: refusals, masks, the handle -- CPU only."""
+
+from __future__ import annotations
+
+import ctypes
+
+import pytest
+import torch
+
+import piper_kernels as pk
+from oracle import decoding as oracle
+from piper_kernels import _native
+
+
+def _cache(pages=3, heads=2, page=16, d=64, **kw) -> pk.QuantizedKVCache:
+    return pk.QuantizedKVCache.allocate(pages, heads, page, d, device="cpu", **kw)
+
+
+def _batch(b=2, width=2):
+    return torch.zeros((b, width), dtype=torch.int32), torch.zeros(b, dtype=torch.int32)
+
+
+def test_a_new_cache_stands_for_zeros() -> None:
+    c = _cache()
+    assert (c.kv_heads, c.page_size, c.head_dim) == (2, 16, 64)
+    assert not c.key_codes.any() and bool((c.value_scales == 1).all())
+
+
+@pytest.mark.parametrize(("change", "match"), [
+    (dict(page=24), "page_size"), (dict(page=512), "page_size"), (dict(d=96), "head dimensions"),
+    (dict(pages=0), "at least one page"), (dict(key_mean=torch.zeros(2, 63)), "key_mean"),
+    (dict(key_mean=torch.zeros(2, 64, dtype=torch.float16)), "float32"),
+])
+def test_cache_refuses(change, match) -> None:
+    with pytest.raises(ValueError, match=match):
+        _cache(**change)
+
+
+def test_cache_refuses_buffers_that_do_not_belong_together() -> None:
+    c = _cache()
+    with pytest.raises(ValueError, match="value_codes must have shape"):
+        pk.QuantizedKVCache(c.key_codes, c.key_scales, c.value_codes[:2], c.value_scales)
+    with pytest.raises(ValueError, match="key_scales must use float32"):
+        pk.QuantizedKVCache(c.key_codes, c.key_scales.half(), c.value_codes, c.value_scales)
+    with pytest.raises(ValueError, match="contiguous"):
+        pk.QuantizedKVCache(c.key_codes, c.key_scales, torch.zeros(3, 16, 2, 64, dtype=torch.int8).transpose(1, 2),
+                            c.value_scales)
+
+
+@pytest.mark.parametrize(("change", "match"), [
+    (dict(key=torch.zeros(2, 2, 3, 64)), "float16 or bfloat16"),
+    (dict(key=torch.zeros(2, 2, 64).half()), "shape"),
+    (dict(key=torch.zeros(2, 3, 3, 64).half()), "key must have shape"),
+    (dict(value=torch.zeros(2, 2, 4, 64).half()), "value must have shape"),
+    (dict(value=torch.zeros(2, 2, 3, 64).bfloat16()), "value must use float16"),
+    (dict(value=torch.zeros(2, 2, 64, 3).half().transpose(2, 3)), "last dimension must be contiguous"),
+    (dict(key=torch.zeros(2, 2, 0, 64).half(), value=torch.zeros(2, 2, 0, 64).half()), "empty"),
+    (dict(block_table=torch.zeros((2, 2), dtype=torch.int64)), "block_table must use int32"),
+    (dict(block_table=torch.zeros((3, 2), dtype=torch.int32)), "block_table must have shape"),
+    (dict(block_table=torch.zeros((2, 0), dtype=torch.int32)), "at least one column"),
+    (dict(lengths=torch.zeros(3, dtype=torch.int32)), "lengths"),
+    (dict(counts=torch.zeros(2, dtype=torch.int64)), "counts must use int32"),
+    (dict(lengths=torch.zeros(2, dtype=torch.int32, device="meta")), "must be on cpu"),
+])
+def test_write_refuses(change, match) -> None:
+    table, lengths = _batch()
+    args = dict(key=torch.zeros(2, 2, 3, 64).half(), value=torch.zeros(2, 2, 3, 64).half(), block_table=table,
+                lengths=lengths, counts=None) | change
+    with pytest.raises(ValueError, match=match):
+        pk.write_kv_cache(_cache(), **args)
+
+
+@pytest.mark.parametrize(("change", "match"), [
+    (dict(query=torch.zeros(2, 4, 3, 64)), "float16 or bfloat16"),
+    (dict(query=torch.zeros(2, 4, 64).half()), "shape"),
+    (dict(query=torch.zeros(2, 4, 3, 128).half()), "query must have shape"),
+    (dict(query=torch.zeros(2, 3, 3, 64).half()), "multiple of the cache's 2 KV heads"),
+    (dict(query=torch.zeros(2, 4, 65, 64).half()), "1 to 64 nodes"),
+    (dict(query=torch.zeros(2, 4, 0, 64).half()), "1 to 64 nodes"),
+    (dict(query=torch.zeros(0, 4, 3, 64).half()), "empty batch"),
+    (dict(tree_mask=torch.zeros((2, 3), dtype=torch.int32)), "tree_mask must use int64"),
+    (dict(tree_mask=torch.zeros((2, 4), dtype=torch.int64)), "tree_mask must have shape"),
+    (dict(scale=0.0), "scale must be finite and positive"),
+    (dict(scale=float("nan")), "scale must be finite and positive"),
+])
+def test_attention_refuses(change, match) -> None:
+    table, lengths = _batch()
+    args = dict(query=torch.zeros(2, 4, 3, 64).half(), block_table=table, lengths=lengths) | change
+    with pytest.raises(ValueError, match=match):
+        pk.tree_attention(args.pop("query"), _cache(), **args)
+
+
+@pytest.mark.parametrize(("change", "match"), [
+    (dict(target_probs=torch.zeros(2, 5)), "target_probs must have shape"),
+    (dict(target_probs=torch.zeros(2, 3, 5).half()), "target_probs must use float32"),
+    (dict(draft_probs=torch.zeros(2, 3, 6)), "draft_probs must have shape"),
+    (dict(draft_probs=torch.zeros(2, 5, 3).transpose(1, 2)), "contiguous"),
+    (dict(tokens=torch.zeros((2, 3), dtype=torch.int32)), "tokens must use int64"),
+    (dict(parents=torch.zeros((2, 3), dtype=torch.int64)), "parents must use int32"),
+    (dict(uniform=torch.zeros(2, 4)), "uniform must have shape"),
+    (dict(noise=torch.zeros(2, 4)), "noise must have shape"),
+])
+def test_verify_refuses(change, match) -> None:
+    args = dict(target_probs=torch.zeros(2, 3, 5), draft_probs=torch.zeros(2, 3, 5),
+                tokens=torch.zeros((2, 3), dtype=torch.int64), parents=torch.zeros((2, 3), dtype=torch.int32),
+                uniform=torch.zeros(2, 3), noise=torch.zeros(2, 5)) | change
+    with pytest.raises(ValueError, match=match):
+        pk.verify_draft_tree(**args)
+
+
+def test_keep_and_read_refuse() -> None:
+    table, lengths = _batch()
+    path, counts = torch.zeros((2, 3), dtype=torch.int32), torch.ones(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="path must use int32"):
+        pk.keep_draft_path(_cache(), table, lengths, path.long(), counts)
+    with pytest.raises(ValueError, match="1 to 64 nodes"):
+        pk.keep_draft_path(_cache(), table, lengths, torch.zeros((2, 65), dtype=torch.int32), counts)
+    with pytest.raises(ValueError, match="counts must have shape"):
+        pk.keep_draft_path(_cache(), table, lengths, path, counts[:1])
+    with pytest.raises(ValueError, match="tokens must be positive"):
+        pk.read_kv_cache(_cache(), table, lengths, 0)
+    with pytest.raises(ValueError, match="float16 or bfloat16"):
+        pk.read_kv_cache(_cache(), table, lengths, 1, dtype=torch.float32)
+
+
+def test_there_is_no_cpu_fallback_and_no_autograd() -> None:
+    table, lengths = _batch()
+    x = torch.zeros(2, 2, 3, 64).half()
+    for call in (
+        lambda: pk.write_kv_cache(_cache(), x, x, table, lengths),
+        lambda: pk.read_kv_cache(_cache(), table, lengths, 2),
+        lambda: pk.keep_draft_path(_cache(), table, lengths, torch.zeros((2, 3), dtype=torch.int32), lengths),
+        lambda: pk.tree_attention(x, _cache(), table, lengths),
+        lambda: pk.verify_draft_tree(torch.zeros(1, 1, 5), torch.zeros(1, 1, 5), torch.zeros((1, 1), dtype=torch.int64),
+                                     torch.zeros((1, 1), dtype=torch.int32), torch.zeros(1, 1), torch.zeros(1, 5)),
+    ):
+        with pytest.raises(RuntimeError, match="no CPU or generic-GPU fallback"):
+            call()
+    with pytest.raises(RuntimeError, match="autograd"):
+        pk.tree_attention(x.clone().requires_grad_(), _cache(), table, lengths)
+
+
+def test_entry_points_check_arguments_on_the_host() -> None:
+    lib = _native.library()
+    good = dict(key_codes=256, key_scales=256, value_codes=256, value_scales=256, key_mean=None, block_table=256,
+                lengths=256, pages=2, table_stride=1, kv_heads=1, page_size=16, head_dim=64, batch=1, table_width=1)
+    strides = _native._STRIDES(1, 1, 1)
+
+    def refused(call, *args, match, **change):
+        cache = _native.KVCache(**(good | change))
+        assert call(ctypes.byref(cache), *args) == _native.ERR_INVALID_ARGUMENT
+        assert match in _native.last_error()
+
+    read = (256, 256, 0, 1, None, None)
+    refused(lib.piper_b200_kv_cache_read, *read, match="head_dim", head_dim=32)
+    refused(lib.piper_b200_kv_cache_read, *read, match="page_size", page_size=48)
+    refused(lib.piper_b200_kv_cache_read, *read, match="NULL", lengths=None)
+    refused(lib.piper_b200_kv_cache_read, *read, match="positive", table_width=0)
+    refused(lib.piper_b200_kv_cache_read, *read, match="2^31", pages=1 << 40)
+    refused(lib.piper_b200_kv_cache_read, *read, match="16-byte", key_codes=8)
+    refused(lib.piper_b200_kv_cache_read, 256, 256, 0, 0, None, None, match="tokens")
+    refused(lib.piper_b200_kv_cache_write, None, strides, 256, strides, 0, 1, None, None, match="NULL")
+    refused(lib.piper_b200_kv_cache_write, 256, strides, 256, strides, 5, 1, None, None, match="dtype")
+    refused(lib.piper_b200_kv_cache_keep, 256, 1, 65, 256, None, match="nodes")
+    tree = (256, strides, 256, 0)
+    refused(lib.piper_b200_tree_attention, *tree, 1, 0, None, 0, 0.1, None, 0, None, match="nodes")
+    refused(lib.piper_b200_tree_attention, *tree, 3, 1, None, 0, 0.1, None, 0, None, match="multiple", kv_heads=2)
+    refused(lib.piper_b200_tree_attention, *tree, 1, 1, None, 0, -1.0, None, 0, None, match="scale")
+    two = _native._STRIDES2(1, 1)
+    for vocab, nodes, match in ((0, 1, "vocab"), (5, 65, "nodes")):
+        assert lib.piper_b200_verify_draft_tree(256, two, 256, two, 256, 1, 256, 1, 256, 1, 256, 1, 1, nodes, vocab,
+                                                256, 256, 256, None) == _native.ERR_INVALID_ARGUMENT
+        assert match in _native.last_error()
+
+
+def test_tree_mask_from_parents() -> None:
+    parents = torch.tensor([[-1, 0, 0, 1, 3, 2], [-1, 0, 1, 2, 3, 4]], dtype=torch.int32)
+    mask = pk.tree_mask_from_parents(parents)
+    assert mask.tolist() == [[1, 0b11, 0b101, 0b1011, 0b11011, 0b100101], [1, 3, 7, 15, 31, 63]]
+    assert pk.tree_mask_from_parents(parents[0]).tolist() == mask[0].tolist()
+    chain = pk.tree_mask_from_parents(torch.arange(-1, 63))
+    assert chain[63].item() == -1 and chain[62].item() == (1 << 63) - 1
+    with pytest.raises(ValueError, match="1 to 64"):
+        pk.tree_mask_from_parents(torch.zeros(65, dtype=torch.int32))
+    with pytest.raises(ValueError, match="int32 or int64"):
+        pk.tree_mask_from_parents(torch.zeros(3))
+
+
+def test_oracle_verification_follows_the_target_distribution() -> None:
+    # One root with two drafted children: the first emitted token's frequencies
+    # over many seeds are the target's, whatever the draft.  Each count is
+    # binomial; five standard deviations (plus one) bound it.
+    g = torch.Generator().manual_seed(7)
+    vocab, tries = 4, 4000
+    target = torch.softmax(torch.randn((1, 1, vocab), generator=g), -1)
+    draft = torch.softmax(torch.randn((1, 1, vocab), generator=g), -1)
+    tokens = torch.zeros((tries, 3), dtype=torch.int64)
+    tokens[:, 1:] = torch.multinomial(draft[0, 0], 2 * tries, replacement=True, generator=g).view(tries, 2)
+    parents = torch.tensor([[-1, 0, 0]], dtype=torch.int32).expand(tries, 3)
+    path, count, following = oracle.verify(
+        target.expand(tries, 3, vocab), draft.expand(tries, 3, vocab), tokens, parents,
+        torch.rand((tries, 3), generator=g), torch.empty((tries, vocab)).exponential_(generator=g))
+    first = torch.where(count > 1, tokens.gather(1, path[:, 1:2].long().clamp(min=0))[:, 0], following)
+    for x in range(vocab):
+        p = float(target[0, 0, x])
+        assert abs(int((first == x).sum()) - tries * p) <= 5 * (tries * p * (1 - p)) ** 0.5 + 1
