@@ -5,7 +5,9 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
+#include <mutex>
 #include <string>
 
 #include "host_api.h"
@@ -50,14 +52,9 @@ int check_dtype(int dtype) {
   return PIPER_B200_OK;
 }
 
-int use_device(int* sms = nullptr, unsigned long long* context = nullptr, int* device = nullptr) {
-  int d = 0, s = 0;
-  unsigned long long x = 0;
-  const int rc = piper::host::ensure_device(&d, &x, &s);
-  if (sms) *sms = s;
-  if (context) *context = x;
-  if (device) *device = d;
-  return rc;
+int use_device() {
+  piper::host::Device device;
+  return piper::host::ensure_device(&device);
 }
 
 bool rows_aligned16(const void* p, const int64_t s[3]) {
@@ -96,13 +93,97 @@ void launch_read(const piper::CacheRowsArgs& a, const dim3& grid, cudaStream_t s
     piper::cache_read_kernel<T, 128><<<grid, piper::kCacheThreads, 0, s>>>(a);
 }
 
-template <typename T>
-void launch_tree(const piper::TreeArgs& a, cudaStream_t s) {
-  const dim3 grid(a.nodes, a.heads, a.c.batch);
-  if (a.c.head_dim == 64)
-    piper::tree_attention_simple_kernel<T, 64><<<grid, 128, 0, s>>>(a);
-  else
-    piper::tree_attention_simple_kernel<T, 128><<<grid, 128, 0, s>>>(a);
+constexpr int kMaxDevices = 64;
+std::mutex g_tree_mutex;
+unsigned long long g_tree_context[kMaxDevices] = {};  // context whose kernels have their shared memory
+
+// Rows of a KV head, and the CTAs of one row tile, for which the kernel
+// instances are made: 16 rows on four warps, or 32 rows on eight.
+bool few_rows(int64_t rows) { return rows <= 16; }
+
+template <int D>
+size_t part_bytes(int64_t rows) {
+  return few_rows(rows) ? size_t(4) * 2 * piper::TreeTile<D, 1, 4>::kPart : size_t(4) * 2 * piper::TreeTile<D, 2, 8>::kPart;
+}
+
+int tree_slots(int64_t rows, int sms) {
+  return sms * (few_rows(rows) ? piper::TreeTile<128, 1, 4>::kCtas : piper::TreeTile<128, 2, 8>::kCtas);
+}
+
+template <typename T, int D, int MT, int WARPS>
+int allow_smem() {
+  PIPER_HOST_CUDA(cudaFuncSetAttribute(piper::tree_attention_kernel<T, D, MT, WARPS>,
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       piper::TreeTile<D, MT, WARPS>::kAlloc));
+  return PIPER_B200_OK;
+}
+
+template <typename T, int D>
+int allow_smem_both() {
+  const int rc = allow_smem<T, D, 1, 4>();
+  return rc != PIPER_B200_OK ? rc : allow_smem<T, D, 2, 8>();
+}
+
+int set_up_tree(const piper::host::Device& device) {
+  std::lock_guard<std::mutex> lock(g_tree_mutex);
+  if (device.context != 0 && g_tree_context[device.index] == device.context) return PIPER_B200_OK;
+  int rc = PIPER_B200_OK;
+  if ((rc = allow_smem_both<__half, 64>()) != PIPER_B200_OK) return rc;
+  if ((rc = allow_smem_both<__half, 128>()) != PIPER_B200_OK) return rc;
+  if ((rc = allow_smem_both<__nv_bfloat16, 64>()) != PIPER_B200_OK) return rc;
+  if ((rc = allow_smem_both<__nv_bfloat16, 128>()) != PIPER_B200_OK) return rc;
+  g_tree_context[device.index] = device.context;
+  return PIPER_B200_OK;
+}
+
+template <typename T, int D, int MT, int WARPS>
+int launch_tree(piper::TreeArgs a, int slots, size_t workspace_bytes, cudaStream_t stream) {
+  using S = piper::TreeTile<D, MT, WARPS>;
+  a.row_tiles = (a.rows + S::kRows - 1) / S::kRows;
+  const int64_t segments = static_cast<int64_t>(a.c.batch) * a.c.kv_heads * a.row_tiles;
+  const int64_t most = ((static_cast<int64_t>(a.c.table_width) << a.page_shift) + S::kKeys - 1) / S::kKeys;
+  // Tables of a few tiles: a CTA for each (request, head, row tile), one
+  // launch and nothing to merge.
+  a.whole = most <= 8 && segments < (int64_t(1) << 31);
+  int64_t grid = segments;
+  if (!a.whole) {
+    grid = most > 2 * int64_t(slots) / segments ? slots : std::max<int64_t>(1, segments * most / 2);
+    if (workspace_bytes < static_cast<size_t>(grid) * 2 * S::kPart * 4)
+      return fail(PIPER_B200_ERR_WORKSPACE_TOO_SMALL,
+                  "workspace needs " + std::to_string(static_cast<size_t>(grid) * 2 * S::kPart * 4) + " bytes, got " +
+                      std::to_string(workspace_bytes));
+    if (a.parts == nullptr || reinterpret_cast<uintptr_t>(a.parts) % 256 != 0)
+      return invalid("workspace must be 256-byte aligned and not NULL");
+  }
+  const uint32_t box = static_cast<uint32_t>(std::min(a.c.page_size, 64));
+  CUtensorMap key_map, value_map;
+  const uint64_t outer = static_cast<uint64_t>(a.c.pages) * a.c.kv_heads;
+  int rc = piper::host::encode_rows_map(&key_map, a.c.key_codes, D, a.c.page_size, outer, box);
+  if (rc != PIPER_B200_OK) return rc;
+  if ((rc = piper::host::encode_rows_map(&value_map, a.c.value_codes, D, a.c.page_size, outer, box)) != PIPER_B200_OK)
+    return rc;
+  piper::tree_attention_kernel<T, D, MT, WARPS>
+      <<<static_cast<unsigned>(grid), S::kThreads, S::kAlloc, stream>>>(key_map, value_map, a);
+  PIPER_HOST_CUDA(cudaGetLastError());
+  if (a.whole || grid == 1) return PIPER_B200_OK;
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(grid - 1), S::kRows / 4);
+  config.blockDim = dim3(128);
+  config.stream = stream;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  PIPER_HOST_CUDA(cudaLaunchKernelEx(&config, piper::tree_merge_kernel<T, D, MT, WARPS>, a, static_cast<int>(grid)));
+  return PIPER_B200_OK;
+}
+
+template <typename T, int D>
+int launch_tree_rows(const piper::TreeArgs& a, int sms, size_t workspace_bytes, cudaStream_t stream) {
+  const int slots = tree_slots(a.rows, sms);
+  return few_rows(a.rows) ? launch_tree<T, D, 1, 4>(a, slots, workspace_bytes, stream)
+                          : launch_tree<T, D, 2, 8>(a, slots, workspace_bytes, stream);
 }
 
 }  // namespace
@@ -195,7 +276,14 @@ extern "C" int piper_b200_tree_attention_workspace_bytes(int64_t batch, int64_t 
   if (bytes == nullptr) return invalid("bytes is NULL");
   if (batch <= 0 || heads <= 0 || kv_heads <= 0 || nodes <= 0 || head_dim <= 0)
     return invalid("sizes must be positive");
-  *bytes = 0;
+  int device = 0, sms = 148;
+  if (cudaGetDevice(&device) != cudaSuccess ||
+      cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
+    cudaGetLastError();
+    sms = 148;
+  }
+  const int64_t rows = heads / kv_heads * nodes;
+  *bytes = tree_slots(rows, sms) * (head_dim == 64 ? part_bytes<64>(rows) : part_bytes<128>(rows));
   return PIPER_B200_OK;
 }
 
@@ -212,9 +300,12 @@ extern "C" int piper_b200_tree_attention(const piper_b200_kv_cache_t* cache, con
     return invalid("heads must be a multiple of kv_heads, at most 65535");
   if (!(std::isfinite(scale) && scale > 0.0)) return invalid("scale must be finite and positive");
   if (reinterpret_cast<uintptr_t>(out) % 16 != 0) return invalid("output must be 16-byte aligned");
-  (void)workspace;
-  (void)workspace_bytes;
-  if ((rc = use_device()) != PIPER_B200_OK) return rc;
+  if (reinterpret_cast<uintptr_t>(cache->key_scales) % 16 != 0 ||
+      reinterpret_cast<uintptr_t>(cache->value_scales) % 16 != 0)
+    return invalid("the cache's scales must be 16-byte aligned");
+  piper::host::Device device;
+  if ((rc = piper::host::ensure_device(&device)) != PIPER_B200_OK) return rc;
+  if ((rc = set_up_tree(device)) != PIPER_B200_OK) return rc;
   piper::TreeArgs a{};
   a.c = *cache;
   a.query = query;
@@ -222,18 +313,23 @@ extern "C" int piper_b200_tree_attention(const piper_b200_kv_cache_t* cache, con
   a.out = out;
   a.mask = tree_mask;
   a.mask_stride = mask_stride;
+  a.parts = static_cast<float*>(workspace);
+  a.status = device.status;
+  a.wait_budget_ns = 2000000000ull;
   a.heads = static_cast<int>(heads);
   a.nodes = static_cast<int>(nodes);
   a.group = static_cast<int>(heads / cache->kv_heads);
+  a.rows = a.group * a.nodes;
   a.page_shift = page_shift_of(cache->page_size);
+  a.vec = reinterpret_cast<uintptr_t>(query) % 8 == 0 && query_strides[0] % 4 == 0 && query_strides[1] % 4 == 0 &&
+          query_strides[2] % 4 == 0;
   a.scale_log2e = static_cast<float>(scale * 1.4426950408889634);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (dtype == PIPER_B200_FLOAT16)
-    launch_tree<__half>(a, s);
-  else
-    launch_tree<__nv_bfloat16>(a, s);
-  PIPER_HOST_CUDA(cudaGetLastError());
-  return PIPER_B200_OK;
+    return cache->head_dim == 64 ? launch_tree_rows<__half, 64>(a, device.sms, workspace_bytes, s)
+                                 : launch_tree_rows<__half, 128>(a, device.sms, workspace_bytes, s);
+  return cache->head_dim == 64 ? launch_tree_rows<__nv_bfloat16, 64>(a, device.sms, workspace_bytes, s)
+                               : launch_tree_rows<__nv_bfloat16, 128>(a, device.sms, workspace_bytes, s);
 }
 
 extern "C" int piper_b200_verify_draft_tree(const float* target, const int64_t target_strides[2], const float* draft,

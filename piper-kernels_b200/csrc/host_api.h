@@ -19,7 +19,18 @@ int cuda_fail(cudaError_t err, const char* what);
 // The calling thread's device, checked to be sm_100 and set up.  `context`
 // identifies the CUDA context the set-up belongs to: what another translation
 // unit sets up itself (kernel attributes) it redoes when that changes.
-int ensure_device(int* device, unsigned long long* context, int* sms);
+struct Device {
+  int index = 0;
+  int sms = 0;
+  unsigned long long context = 0;
+  uint32_t* status = nullptr;  // the status word, in device memory
+};
+int ensure_device(Device* device);
+
+// A 3-D tensor map of bytes: a box of `box_mid` rows of `inner` (64 or 128)
+// bytes, swizzled for that width.
+int encode_rows_map(CUtensorMap* map, const void* base, uint64_t inner, uint64_t mid, uint64_t outer,
+                    uint32_t box_mid);
 
 }  // namespace host
 }  // namespace piper

@@ -53,6 +53,7 @@ std::mutex g_init_mutex;
 bool g_device_ready[kMaxDevices] = {};
 unsigned long long g_device_context[kMaxDevices] = {};  // context the set-up was done in
 int g_device_sms[kMaxDevices] = {};
+uint32_t* g_device_status[kMaxDevices] = {};  // the status word's address in that context
 EncodeTiledFn g_encode = nullptr;
 CtxGetCurrentFn g_ctx_get_current = nullptr;
 CtxGetIdFn g_ctx_get_id = nullptr;
@@ -152,6 +153,9 @@ int ensure_device(int* device_out) {
     if (resident < 1)
       return fail(PIPER_B200_ERR_UNSUPPORTED_DEVICE, "an attention CTA does not fit on one SM of this device");
   }
+  void* status = nullptr;
+  PIPER_CUDA(cudaGetSymbolAddress(&status, piper::g_piper_status));
+  g_device_status[device] = static_cast<uint32_t*>(status);
   g_device_ready[device] = true;
   g_device_context[device] = current_context_id();
   return PIPER_B200_OK;
@@ -186,13 +190,19 @@ namespace host {
 int fail(int code, const std::string& msg) { return ::fail(code, msg); }
 int cuda_fail(cudaError_t err, const char* what) { return ::cuda_fail(err, what); }
 
-int ensure_device(int* device, unsigned long long* context, int* sms) {
-  const int rc = ::ensure_device(device);
+int ensure_device(Device* device) {
+  const int rc = ::ensure_device(&device->index);
   if (rc != PIPER_B200_OK) return rc;
   std::lock_guard<std::mutex> lock(g_init_mutex);
-  *context = g_device_context[*device];
-  *sms = g_device_sms[*device];
+  device->sms = g_device_sms[device->index];
+  device->context = g_device_context[device->index];
+  device->status = g_device_status[device->index];
   return PIPER_B200_OK;
+}
+
+int encode_rows_map(CUtensorMap* map, const void* base, uint64_t inner, uint64_t mid, uint64_t outer,
+                    uint32_t box_mid) {
+  return encode_map(map, base, inner, mid, outer, inner, inner * mid, static_cast<uint32_t>(inner), box_mid);
 }
 
 }  // namespace host

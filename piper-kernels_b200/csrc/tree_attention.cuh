@@ -1,12 +1,45 @@
-// Attention of a drafted tree's nodes over the quantised cache (simple form:
-// one CTA per query row).
+// Attention of a drafted tree's nodes over the quantised paged cache.
+//
+// For a request and a KV head the `group * nodes` query rows that read that
+// head are one small matrix Q.  With K codes k, V codes v and the row scales
+// a (keys) and b (values), a row's output is
+//   o = sum_j p_j b_j v_j / sum_j p_j,   p_j = exp(scale * a_j (q . k_j) - m)
+// over the keys j that the row sees.  Reading the cache once (2 D + 8 bytes a
+// key) bounds it while the rows are few: 16 rows need 64 products a byte.
+//
+// Products: fp16 tensor-core MMAs (m16n8k16, fp32 accumulators).  Codes are
+// exact in fp16.  fp16 queries are used as they are; a bf16 row is scaled by
+// a power of two to [1, 2) at its largest element, which loses only what lies
+// 2^-25 and more below it.  Weights w_j = p_j b_j / u are rounded to fp16 (11
+// bits, against 8 or 11 of the output): u, a unit for each row, follows the
+// largest p_j b_j, so w neither overflows nor goes subnormal where it counts.
+// Scores, weights, totals and numerators are fp32.
+//
+// Layout: a code of a page is the byte that a lane's fragment wants.  As 16-bit
+// elements, ldmatrix gives lane (g, t) the bytes 4t .. 4t+3 of key g: the
+// fragment's two pairs, if query elements are permuted alike.  ldmatrix.trans
+// gives keys 2t, 2t+1 of bytes 2g, 2g+1: fragments of the even and of the odd
+// head dimensions.  A byte becomes fp16 by a byte permute under 0x64 (1024 +
+// code + 128) and one subtraction.
+//
+// Work: a unit is one key tile of one (request, KV head, row tile); the units
+// of the whole batch are cut into equal runs, one for each CTA, so that ragged
+// lengths balance.  A run that covers a (request, head, row tile) writes its
+// output; one that covers a part leaves its maximum, total and numerator in
+// the workspace, and tree_merge_kernel joins the parts.
 #pragma once
 
 #include <math.h>
 
+#include <type_traits>
+
 #include "kv_cache.cuh"
+#include "sm100.cuh"
 
 namespace piper {
+
+constexpr float kSlack = 8.0f;         // log2 by which a weight may exceed 1 before the maximum moves
+constexpr float kUnitMin = 0x1p-120f;  // smallest unit of a numerator
 
 struct TreeArgs {
   piper_b200_kv_cache_t c;
@@ -15,69 +48,722 @@ struct TreeArgs {
   void* out;
   const int64_t* mask;
   int64_t mask_stride;
-  int heads, nodes, group, page_shift;
+  float* parts;      // [CTAs, 2] parts: rows x D numerators, then rows x (maximum, total)
+  uint32_t* status;
+  uint64_t wait_budget_ns;
+  int heads, nodes, group, rows, row_tiles, page_shift;
+  int whole;         // each CTA takes one whole (request, head, row tile)
+  int vec;           // query rows allow 8-byte loads
   float scale_log2e;
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(128) tree_attention_simple_kernel(TreeArgs a) {
-  constexpr int kPer = D / 32;
-  const int node = blockIdx.x, head = blockIdx.y, b = blockIdx.z;
-  const int kv = head / a.group;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const T* q = static_cast<const T*>(a.query) + b * a.qs[0] + head * a.qs[1] + node * a.qs[2] + lane * kPer;
-  float qf[kPer], acc[kPer];
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    qf[i] = to_f32<T>(q[i]);
-    acc[i] = 0.0f;
-  }
+// Tile shape of one kernel instance: MT m16 row tiles for each of WARPS
+// warps, 16 keys of the tile for each warp.
+template <int D, int MT, int WARPS>
+struct TreeTile {
+  static constexpr int kRows = 16 * MT;
+  static constexpr int kKeys = 16 * WARPS;
+  static constexpr int kThreads = 32 * (WARPS + 1);  // and one warp that fetches
+  static constexpr int kCodes = kKeys * D;
+  static constexpr int kScales = kKeys * 4;
+  static constexpr int kStage = 2 * kCodes + 2 * kScales;
+  static constexpr int kStageAlloc = (kStage + 1023) / 1024 * 1024;
+  static constexpr int kJoinStride = 80;  // floats; 16 banks between rows
+  static constexpr int kJoin = WARPS * 16 * kJoinStride * 4;
+  static constexpr int kQuery = MT > 1 ? MT * (D / 16) * 32 * 16 : 0;
+  static constexpr int kState = 3 * WARPS * kRows * 4;
+  static constexpr int kFixed = kJoin + kQuery + kState + kRows * 8 + 1024;
+  static constexpr int kCtas = MT == 1 ? 2 : 1;  // per SM
+  static constexpr int kStages = (227 * 1024 / kCtas - 1024 * 2 - kFixed) / kStageAlloc > 8
+                                     ? 8
+                                     : (227 * 1024 / kCtas - 1024 * 2 - kFixed) / kStageAlloc;
+  static constexpr int kAlloc = kStages * kStageAlloc + kFixed + 1024;
+  static constexpr int kPart = kRows * (D + 2);  // floats of one part
+};
+
+// Key tiles of request b (at least one: it has a node).
+template <int kKeys>
+__device__ __forceinline__ int tree_tiles(const TreeArgs& a, int b) {
   const int64_t length = max(0, __ldg(a.c.lengths + b));
-  const uint64_t mask = a.mask != nullptr ? static_cast<uint64_t>(a.mask[b * a.mask_stride + node])
-                                          : (~0ull >> (63 - node));
-  float m = -INFINITY, l = 0.0f;
-  for (int64_t pos = warp; pos < length + a.nodes; pos += 4) {
-    if (pos >= length && !((mask >> (pos - length)) & 1)) continue;
-    const int64_t row = cache_row(a.c, a.page_shift, b, kv, pos);
-    if (row < 0) continue;
-    const int8_t* kc = static_cast<const int8_t*>(a.c.key_codes) + row * D + lane * kPer;
-    const int8_t* vc = static_cast<const int8_t*>(a.c.value_codes) + row * D + lane * kPer;
-    float s = 0.0f;
+  const int64_t keys = min(length + a.nodes, static_cast<int64_t>(a.c.table_width) << a.page_shift);
+  return static_cast<int>((keys + kKeys - 1) / kKeys);
+}
+
+// A run of units: [begin, end) over the batch, and where `begin` lies.
+struct TreeRun {
+  int64_t begin, end;
+  int b, hr, tile, tiles;  // request, head * row_tiles + row tile, key tile and its count
+};
+
+// Units of the batch; every lane gets the result.
+template <int kKeys>
+__device__ __forceinline__ int64_t tree_units(const TreeArgs& a) {
+  const int lane = threadIdx.x % 32;
+  int64_t sum = 0;
+  for (int b = lane; b < a.c.batch; b += 32) sum += tree_tiles<kKeys>(a, b);
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) s += qf[i] * static_cast<float>(kc[i]);
+  for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+  return sum * (static_cast<int64_t>(a.c.kv_heads) * a.row_tiles);
+}
+
+// The request that unit u belongs to, and its first unit.
+template <int kKeys>
+__device__ __forceinline__ void tree_find(const TreeArgs& a, int64_t u, int* request, int* tiles, int64_t* first) {
+  const int lane = threadIdx.x % 32;
+  const int64_t per = static_cast<int64_t>(a.c.kv_heads) * a.row_tiles;
+  int64_t base = 0;
+  for (int b0 = 0; b0 < a.c.batch; b0 += 32) {
+    const int b = b0 + lane;
+    const int n = b < a.c.batch ? tree_tiles<kKeys>(a, b) : 0;
+    int64_t upto = n;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    s *= a.c.key_scales[row] * a.scale_log2e;
-    const float m_new = fmaxf(m, s);
-    const float rescale = exp2f(m - m_new), p = exp2f(s - m_new);
-    const float pv = p * a.c.value_scales[row];
-    m = m_new;
-    l = l * rescale + p;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) acc[i] = acc[i] * rescale + pv * static_cast<float>(vc[i]);
-  }
-  __shared__ float sm[4], sl[4], so[4][D];
-  if (lane == 0) {
-    sm[warp] = m;
-    sl[warp] = l;
-  }
-#pragma unroll
-  for (int i = 0; i < kPer; ++i) so[warp][lane * kPer + i] = acc[i];
-  __syncthreads();
-  if (threadIdx.x < D) {
-    float top = -INFINITY;
-    for (int w = 0; w < 4; ++w) top = fmaxf(top, sm[w]);
-    float o = 0.0f, total = 0.0f;
-    for (int w = 0; w < 4; ++w) {
-      if (sl[w] == 0.0f) continue;
-      const float r = exp2f(sm[w] - top);
-      total += sl[w] * r;
-      o += so[w][threadIdx.x] * r;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t below = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += below;
     }
-    const float y = total == 0.0f ? 0.0f : o / total;
-    const int64_t at = ((static_cast<int64_t>(b) * a.heads + head) * a.nodes + node) * D + threadIdx.x;
-    static_cast<T*>(a.out)[at] = static_cast<T>(y);
+    const unsigned past = __ballot_sync(0xffffffffu, u < base + upto * per);
+    if (past != 0) {
+      const int at = __ffs(past) - 1;
+      *request = b0 + at;
+      *tiles = __shfl_sync(0xffffffffu, n, at);
+      *first = base + (__shfl_sync(0xffffffffu, upto, at) - *tiles) * per;
+      return;
+    }
+    base += __shfl_sync(0xffffffffu, upto, 31) * per;
   }
+  *request = a.c.batch;
+  *tiles = 1;
+  *first = base;
+}
+
+// CTAs that share the units: at least two units each.
+__device__ __forceinline__ int64_t tree_ctas(int64_t units, int grid) {
+  return max(static_cast<int64_t>(1), min(static_cast<int64_t>(grid), units / 2));
+}
+__device__ __forceinline__ int64_t tree_bound(int64_t units, int64_t ctas, int64_t i) { return units * i / ctas; }
+
+template <int kKeys>
+__device__ __forceinline__ TreeRun tree_run(const TreeArgs& a) {
+  TreeRun r;
+  const int per = a.c.kv_heads * a.row_tiles;
+  if (a.whole) {
+    r.b = blockIdx.x / per;
+    r.hr = blockIdx.x % per;
+    r.tile = 0;
+    r.tiles = tree_tiles<kKeys>(a, r.b);
+    r.begin = 0;
+    r.end = r.tiles;
+    return r;
+  }
+  const int64_t units = tree_units<kKeys>(a);
+  const int64_t ctas = tree_ctas(units, gridDim.x);
+  r.begin = blockIdx.x < ctas ? tree_bound(units, ctas, blockIdx.x) : 0;
+  r.end = blockIdx.x < ctas ? tree_bound(units, ctas, blockIdx.x + 1) : 0;
+  int64_t first = 0;
+  tree_find<kKeys>(a, r.begin, &r.b, &r.tiles, &first);
+  r.hr = static_cast<int>((r.begin - first) / r.tiles);
+  r.tile = static_cast<int>((r.begin - first) % r.tiles);
+  return r;
+}
+
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Two of the four codes in x (each plus 128), chosen by `select`, as fp16.
+template <uint32_t select>
+__device__ __forceinline__ uint32_t codes_f16(uint32_t x) {
+  const uint32_t h = __byte_perm(x, 0x64646464u, select);
+  const __half2 y = __hsub2(*reinterpret_cast<const __half2*>(&h), __half2half2(__ushort_as_half(0x6480)));
+  return *reinterpret_cast<const uint32_t*>(&y);
+}
+
+// Shared-memory address of 16-byte chunk `c` of row `r` of a tile that TMA
+// wrote with the swizzle of D-byte rows.
+template <int D>
+__device__ __forceinline__ uint32_t tile_chunk(uint32_t base, int r, int c) {
+  const int x = D == 128 ? (r & 7) : ((r >> 1) & 3);
+  return base + r * D + ((c ^ x) << 4);
+}
+
+__device__ __forceinline__ void bar_sync(int id, int threads) {
+  asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
+}
+
+// Four consecutive query elements as floats.
+template <typename T>
+__device__ __forceinline__ void query4(const T* p, bool vec, float (&x)[4]) {
+  uint16_t e[4];
+  if (vec) {
+    *reinterpret_cast<uint2*>(e) = __ldg(reinterpret_cast<const uint2*>(p));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) e[i] = reinterpret_cast<const uint16_t*>(p)[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) x[i] = to_f32<T>(reinterpret_cast<const T*>(e)[i]);
+}
+
+// The fragments of query rows r0 + lane / 4 and that plus 8 (zeros past the
+// last row), scaled to fp16, and what undoes the scaling times the softmax
+// scale.
+template <typename T, int D>
+__device__ __forceinline__ void query_fragments(const TreeArgs& a, int b, int kv, int r0, uint32_t (&q)[D / 16][4],
+                                                float (&factor)[2]) {
+  const int lane = threadIdx.x % 32;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int row = r0 + lane / 4 + 8 * half;
+    float x[D / 16][4] = {};
+    if (row < a.rows) {
+      const int head = kv * a.group + row / a.nodes;
+      const int node = row % a.nodes;
+      const T* p = static_cast<const T*>(a.query) + b * a.qs[0] + head * a.qs[1] + node * a.qs[2] + (lane % 4) * 4;
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c) query4<T>(p + c * 16, a.vec, x[c]);
+    }
+    float up = 1.0f;
+    factor[half] = a.scale_log2e;
+    if constexpr (!std::is_same<T, __half>::value) {
+      uint32_t top = 0u;
+#pragma unroll
+      for (int c = 0; c < D / 16; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) top = max(top, __float_as_uint(x[c][i]) & 0x7fffffffu);
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const uint32_t e = max(1u, min(253u, top >> 23));
+      up = __uint_as_float((254u - e) << 23);
+      factor[half] = __uint_as_float(e << 23) * a.scale_log2e;
+    }
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c) {
+      q[c][half] = pack2(x[c][0] * up, x[c][1] * up, __half());
+      q[c][half + 2] = pack2(x[c][2] * up, x[c][3] * up, __half());
+    }
+  }
+}
+
+template <typename T, int D, int MT, int WARPS>
+__global__ void __launch_bounds__(TreeTile<D, MT, WARPS>::kThreads, TreeTile<D, MT, WARPS>::kCtas)
+    tree_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map,
+                          TreeArgs a) {
+  using S = TreeTile<D, MT, WARPS>;
+  constexpr int kStages = S::kStages;
+  constexpr int kChunks = D / 16;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* join = reinterpret_cast<float*>(smem + kStages * S::kStageAlloc);
+  uint4* query_smem = reinterpret_cast<uint4*>(smem + kStages * S::kStageAlloc + S::kJoin);
+  float* state = reinterpret_cast<float*>(smem + kStages * S::kStageAlloc + S::kJoin + S::kQuery);
+  uint64_t* words = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(state) + S::kState);
+  __shared__ __align__(8) uint64_t full_bar[kStages], empty_bar[kStages];
+  __shared__ uint32_t valid[kStages];
+  __shared__ uint32_t abort_word;
+  const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
+  const uint32_t abort_flag = smem_u32(&abort_word);
+  if (tid == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(smem_u32(&full_bar[s]), 1);
+      mbar_init(smem_u32(&empty_bar[s]), WARPS);
+    }
+    abort_word = 0u;
+    fence_mbarrier_init();
+  }
+  __syncthreads();
+  // Lets tree_merge_kernel's CTAs be placed; they wait for this grid's end.
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  TreeRun run = tree_run<S::kKeys>(a);
+  const int per = a.c.kv_heads * a.row_tiles;
+  const int box = min(a.c.page_size, 64);
+  const int box_shift = min(a.page_shift, 6);
+  const int boxes = S::kKeys >> box_shift;
+
+  if (warp == WARPS) {
+    // ---- fetching warp: lane i brings box i of each tile.
+    int64_t u = run.begin;
+    int stage = 0, issued = 0;
+    uint32_t phase = 1;  // a fresh barrier's previous phase counts as done
+    bool ok = true;
+    int b = run.b, hr = run.hr, tile = run.tile, tiles = run.tiles;
+    const int32_t* row = a.c.block_table + b * a.c.table_stride;
+    int have = -1, entry = -1;  // table columns [have, have + 32), one a lane
+    while (u < run.end && ok) {
+      const int64_t position = static_cast<int64_t>(tile) * S::kKeys + static_cast<int64_t>(lane) * box;
+      const int column = static_cast<int>(position >> a.page_shift);
+      const int column0 = static_cast<int>((static_cast<int64_t>(tile) * S::kKeys) >> a.page_shift);
+      const int column1 =
+          static_cast<int>((static_cast<int64_t>(tile) * S::kKeys + S::kKeys - 1) >> a.page_shift);
+      if (have < 0 || column0 < have || column1 >= have + 32) {
+        have = column0;
+        entry = have + lane < a.c.table_width ? __ldg(row + have + lane) : -1;
+      }
+      const int page = __shfl_sync(0xffffffffu, entry, (column - have) & 31);
+      ok = mbar_wait_warp(smem_u32(&empty_bar[stage]), phase, a.wait_budget_ns, a.status, kStatusTimeoutEmpty,
+                          abort_flag);
+      if (!ok) break;
+      const bool good = lane < boxes && column < a.c.table_width && page >= 0 && page < a.c.pages;
+      const uint32_t goods = __ballot_sync(0xffffffffu, good);
+      const uint32_t bar = smem_u32(&full_bar[stage]);
+      if (lane == 0) {
+        valid[stage] = goods;
+        mbar_arrive_expect_tx(bar, __popc(goods) * box * (2 * D + 8));
+      }
+      __syncwarp();
+      if (good) {
+        const int head = hr / a.row_tiles;
+        const int z = page * a.c.kv_heads + head;
+        const int y = static_cast<int>(position & (a.c.page_size - 1));
+        const uint32_t base = smem_u32(smem + stage * S::kStageAlloc);
+        const int64_t at = (static_cast<int64_t>(z) << a.page_shift) + y;
+        tma_load_3d(base + lane * box * D, &key_map, bar, 0, y, z);
+        bulk_load(base + 2 * S::kCodes + lane * box * 4, a.c.key_scales + at, box * 4, bar);
+        tma_load_3d(base + S::kCodes + lane * box * D, &value_map, bar, 0, y, z);
+        bulk_load(base + 2 * S::kCodes + S::kScales + lane * box * 4, a.c.value_scales + at, box * 4, bar);
+      }
+      ++issued;
+      if (++stage == kStages) {
+        stage = 0;
+        phase ^= 1;
+      }
+      ++u;
+      if (++tile == tiles) {
+        tile = 0;
+        if (++hr == per && u < run.end) {
+          hr = 0;
+          ++b;
+          have = -1;
+          tiles = tree_tiles<S::kKeys>(a, b);
+          row = a.c.block_table + b * a.c.table_stride;
+        }
+      }
+    }
+    // Every copy has landed before the CTA's shared memory goes (the
+    // consumers have waited for all of them unless something gave up).
+    if (!ok)
+      for (int i = max(0, issued - kStages); i < issued; ++i)
+        mbar_wait_warp(smem_u32(&full_bar[i % kStages]), (i / kStages) & 1, a.wait_budget_ns, a.status,
+                       kStatusTimeoutDrain, 0u);
+    return;
+  }
+
+  // ---- computing warps: 16 keys of each tile, all rows.
+  const int g = lane / 4, t = lane % 4;
+  int64_t u = run.begin;
+  int stage = 0;
+  uint32_t phase = 0;
+  bool ok = true;
+  int b = run.b, hr = run.hr, tile = run.tile, tiles = run.tiles;
+  int part = 0;
+  while (u < run.end) {
+    const int kv = hr / a.row_tiles;
+    const int row0 = (hr % a.row_tiles) * S::kRows;
+    const int tile_end = static_cast<int>(min(static_cast<int64_t>(tiles), tile + (run.end - u)));
+    const bool all = tile == 0 && tile_end == tiles;
+    const int64_t length = max(0, __ldg(a.c.lengths + b));
+    uint32_t q[MT == 1 ? kChunks : 1][4];
+    float factor[MT][2];
+    if constexpr (MT == 1) {
+      query_fragments<T, D>(a, b, kv, row0, q, factor[0]);
+    } else {
+      // Row tile i's fragments come from warp i; the factors go with them.
+      if (warp < MT) {
+        uint32_t f[kChunks][4];
+        float r[2];
+        query_fragments<T, D>(a, b, kv, row0 + warp * 16, f, r);
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c)
+          query_smem[(warp * kChunks + c) * 32 + lane] = make_uint4(f[c][0], f[c][1], f[c][2], f[c][3]);
+        if (t == 0) {
+          state[warp * 16 + g] = r[0];
+          state[warp * 16 + g + 8] = r[1];
+        }
+      }
+    }
+    if (tid < S::kRows) {
+      const int row = row0 + tid;
+      uint64_t word = 0;
+      if (row < a.rows) {
+        const int node = row % a.nodes;
+        word = a.mask != nullptr ? static_cast<uint64_t>(__ldg(reinterpret_cast<const unsigned long long*>(
+                                       a.mask + b * a.mask_stride + node)))
+                                 : ~0ull >> (63 - node);
+        word &= ~0ull >> (64 - a.nodes);
+      }
+      words[tid] = word;
+    }
+    bar_sync(1, WARPS * 32);
+    if constexpr (MT > 1) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        factor[i][0] = state[i * 16 + g];
+        factor[i][1] = state[i * 16 + g + 8];
+      }
+    }
+    float o[MT][2 * kChunks][4] = {};
+    float m[MT][2], l[MT][2], unit[MT][2], inv[MT][2];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        m[i][h] = -INFINITY;
+        l[i][h] = unit[i][h] = inv[i][h] = 0.0f;
+      }
+    for (; tile < tile_end; ++tile, ++u) {
+      if (ok) ok = mbar_wait_warp(smem_u32(&full_bar[stage]), phase, a.wait_budget_ns, a.status, kStatusTimeoutFull,
+                                  abort_flag);
+      if (ok) {
+        const uint32_t base = smem_u32(smem + stage * S::kStageAlloc);
+        const float* scales = reinterpret_cast<const float*>(smem + stage * S::kStageAlloc + 2 * S::kCodes);
+        const int key0 = warp * 16;
+        // ---- scores of 16 keys
+        float s[MT][2][4] = {};
+#pragma unroll
+        for (int c = 0; c < kChunks; c += 2) {
+          uint32_t k[4];
+          ldmatrix4(tile_chunk<D>(base, key0 + (lane & 15), c + (lane >> 4)), k);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) k[x] ^= 0x80808080u;
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+              const uint32_t b0 = codes_f16<0x4140>(k[2 * x + n]);
+              const uint32_t b1 = codes_f16<0x4342>(k[2 * x + n]);
+#pragma unroll
+              for (int i = 0; i < MT; ++i) {
+                if constexpr (MT == 1) {
+                  mma16816(s[i][n], q[c + x], b0, b1);
+                } else {
+                  const uint4 f = query_smem[(i * kChunks + c + x) * 32 + lane];
+                  const uint32_t fr[4] = {f.x, f.y, f.z, f.w};
+                  mma16816(s[i][n], fr, b0, b1);
+                }
+              }
+            }
+          }
+        }
+        const float2 ks0 = *reinterpret_cast<const float2*>(scales + key0 + 2 * t);
+        const float2 ks1 = *reinterpret_cast<const float2*>(scales + key0 + 8 + 2 * t);
+        const float2 vs0 = *reinterpret_cast<const float2*>(scales + S::kKeys + key0 + 2 * t);
+        const float2 vs1 = *reinterpret_cast<const float2*>(scales + S::kKeys + key0 + 8 + 2 * t);
+        const float ks[2][2] = {{ks0.x, ks0.y}, {ks1.x, ks1.y}};
+        const float vs[2][2] = {{vs0.x, vs0.y}, {vs1.x, vs1.y}};
+        const uint32_t goods = valid[stage];
+        const int64_t first = static_cast<int64_t>(tile) * S::kKeys;
+        const bool masked = first + S::kKeys > length || goods != (boxes == 32 ? ~0u : (1u << boxes) - 1u);
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[i][n][e] *= ks[n][e & 1];
+        // A key that a row does not see may hold anything: its score is
+        // replaced, and its weight again after the product with its scale.
+        uint32_t unseen = 0u;
+        if (masked) {
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int key = key0 + n * 8 + 2 * t + e;
+              const int64_t j = first + key - length;
+              const bool there = (goods >> (key >> box_shift)) & 1u;
+              const bool open = there && j < 0;
+              const bool drafted = there && j >= 0 && j < a.nodes;
+#pragma unroll
+              for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  const bool seen = open || (drafted && ((words[i * 16 + g + 8 * h] >> (j & 63)) & 1u));
+                  if (!seen) {
+                    s[i][n][2 * h + e] = -INFINITY;
+                    unseen |= 1u << (i * 8 + n * 4 + 2 * h + e);
+                  }
+                }
+            }
+        }
+        // ---- weights
+        bool grow = false;
+        float top[MT][2];
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            top[i][h] = fmaxf(fmaxf(s[i][0][2 * h], s[i][0][2 * h + 1]), fmaxf(s[i][1][2 * h], s[i][1][2 * h + 1]));
+            grow |= (top[i][h] - m[i][h]) * factor[i][h] > kSlack;
+          }
+        if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float x = top[i][h];
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+              if (x > m[i][h]) {
+                const float shrink = ex2_approx((m[i][h] - x) * factor[i][h]);
+                m[i][h] = x;
+                l[i][h] *= shrink;
+                unit[i][h] *= shrink;
+                inv[i][h] = unit[i][h] >= kUnitMin ? 1.0f / unit[i][h] : 0.0f;
+              }
+            }
+        }
+        bool over = false;
+        float most[MT][2];
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float shift = m[i][h] == -INFINITY ? 0.0f : -m[i][h] * factor[i][h];
+#pragma unroll
+            for (int n = 0; n < 2; ++n)
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                const float p = ex2_approx(fmaf(s[i][n][2 * h + e], factor[i][h], shift));
+                l[i][h] += p;
+                s[i][n][2 * h + e] = p * vs[n][e];
+              }
+          }
+        if (masked) {
+#pragma unroll
+          for (int x = 0; x < 8 * MT; ++x)
+            if ((unseen >> x) & 1u) s[x / 8][(x / 4) & 1][x & 3] = 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            most[i][h] = fmaxf(fmaxf(s[i][0][2 * h], s[i][0][2 * h + 1]), fmaxf(s[i][1][2 * h], s[i][1][2 * h + 1]));
+            over |= most[i][h] > unit[i][h] * 256.0f;
+          }
+        if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+          for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float x = most[i][h];
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+              if (x > unit[i][h]) {
+                const float shrink = unit[i][h] / x;
+                unit[i][h] = x;
+                inv[i][h] = x >= kUnitMin ? 1.0f / x : 0.0f;
+#pragma unroll
+                for (int c = 0; c < 2 * kChunks; ++c) {
+                  o[i][c][2 * h] *= shrink;
+                  o[i][c][2 * h + 1] *= shrink;
+                }
+              }
+            }
+        }
+        uint32_t w[MT][4];
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              w[i][2 * n + h] =
+                  pack2(s[i][n][2 * h] * inv[i][h], s[i][n][2 * h + 1] * inv[i][h], __half());
+        // ---- numerators: even, then odd head dimensions of each chunk
+#pragma unroll
+        for (int c = 0; c < kChunks; c += 2) {
+          uint32_t v[4];
+          ldmatrix4_trans(tile_chunk<D>(base + S::kCodes, key0 + (lane & 15), c + (lane >> 4)), v);
+#pragma unroll
+          for (int x = 0; x < 4; ++x) v[x] ^= 0x80808080u;
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const uint32_t e0 = codes_f16<0x4240>(v[2 * x]), e1 = codes_f16<0x4240>(v[2 * x + 1]);
+            const uint32_t d0 = codes_f16<0x4341>(v[2 * x]), d1 = codes_f16<0x4341>(v[2 * x + 1]);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+              mma16816(o[i][2 * (c + x)], w[i], e0, e1);
+              mma16816(o[i][2 * (c + x) + 1], w[i], d0, d1);
+            }
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&empty_bar[stage]));
+      if (++stage == kStages) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+    // ---- join the warps' parts: each row's maximum and total, then the
+    // numerators, 16 rows and 64 head dimensions at a time.
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        l[i][h] += __shfl_xor_sync(0xffffffffu, l[i][h], 1);
+        l[i][h] += __shfl_xor_sync(0xffffffffu, l[i][h], 2);
+        m[i][h] *= factor[i][h];
+      }
+    bar_sync(1, WARPS * 32);  // the factors in `state` have been read
+    if (t == 0) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          state[(0 * WARPS + warp) * S::kRows + i * 16 + g + 8 * h] = m[i][h];
+          state[(1 * WARPS + warp) * S::kRows + i * 16 + g + 8 * h] = l[i][h];
+        }
+    }
+    bar_sync(1, WARPS * 32);
+    float whole_m[MT][2], whole_l[MT][2], share[MT][2];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int r = i * 16 + g + 8 * h;
+        float top = -INFINITY, total = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, state[w * S::kRows + r]);
+        const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w)
+          total += state[(WARPS + w) * S::kRows + r] * ex2_approx(state[w * S::kRows + r] - ref);
+        whole_m[i][h] = top;
+        whole_l[i][h] = total;
+        share[i][h] = unit[i][h] * ex2_approx(m[i][h] - ref);
+      }
+    float* to = a.parts + (static_cast<int64_t>(blockIdx.x) * 2 + part) * S::kPart;
+    if (!all && warp == 0 && t == 0) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = i * 16 + g + 8 * h;
+          to[S::kRows * D + 2 * r] = whole_m[i][h];
+          to[S::kRows * D + 2 * r + 1] = whole_l[i][h];
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+#pragma unroll
+      for (int d0 = 0; d0 < D; d0 += 64) {
+        float* mine = join + warp * 16 * S::kJoinStride;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float(&even)[4] = o[i][2 * (d0 / 16 + c)];
+            const float(&odd)[4] = o[i][2 * (d0 / 16 + c) + 1];
+            const float f = share[i][h];
+            *reinterpret_cast<float4*>(mine + (g + 8 * h) * S::kJoinStride + c * 16 + 4 * t) =
+                make_float4(even[2 * h] * f, odd[2 * h] * f, even[2 * h + 1] * f, odd[2 * h + 1] * f);
+          }
+        bar_sync(1, WARPS * 32);
+        // 16 rows x 64 columns, four columns a thread.
+        for (int x = tid; x < 256; x += WARPS * 32) {
+          const int r = x / 16, d = (x % 16) * 4;
+          float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+          for (int w = 0; w < WARPS; ++w) {
+            const float4 y = *reinterpret_cast<const float4*>(join + (w * 16 + r) * S::kJoinStride + d);
+            sum.x += y.x;
+            sum.y += y.y;
+            sum.z += y.z;
+            sum.w += y.w;
+          }
+          const int row = row0 + i * 16 + r;
+          if (!all) {
+            *reinterpret_cast<float4*>(to + (i * 16 + r) * D + d0 + d) = sum;
+          } else if (row < a.rows) {
+            float total = 0.0f, top = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w) top = fmaxf(top, state[w * S::kRows + i * 16 + r]);
+            const float ref = top == -INFINITY ? 0.0f : top;
+#pragma unroll
+            for (int w = 0; w < WARPS; ++w)
+              total += state[(WARPS + w) * S::kRows + i * 16 + r] * ex2_approx(state[w * S::kRows + i * 16 + r] - ref);
+            const float f = total == 0.0f ? 0.0f : 1.0f / total;
+            const int64_t at =
+                ((static_cast<int64_t>(b) * a.heads + kv * a.group + row / a.nodes) * a.nodes + row % a.nodes) * D;
+            uint2 y;
+            y.x = pack2(sum.x * f, sum.y * f, T());
+            y.y = pack2(sum.z * f, sum.w * f, T());
+            *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at + d0 + d) = y;
+          }
+        }
+        bar_sync(1, WARPS * 32);
+      }
+    }
+    part = 1;
+    if (tile == tiles) {
+      tile = 0;
+      if (++hr == per && u < run.end) {
+        hr = 0;
+        ++b;
+        tiles = tree_tiles<S::kKeys>(a, b);
+      }
+    }
+  }
+}
+
+// Joins the parts of every (request, head, row tile) that a boundary between
+// two runs cuts.  CTA x looks at the boundary before run x + 1 and works if it
+// is the first inside its row tile; a warp takes a row, and CTAs y share the
+// rows.
+template <typename T, int D, int MT, int WARPS>
+__global__ void __launch_bounds__(128) tree_merge_kernel(TreeArgs a, int grid) {
+  using S = TreeTile<D, MT, WARPS>;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int64_t units = tree_units<S::kKeys>(a);
+  const int64_t ctas = tree_ctas(units, grid);
+  const int64_t i = blockIdx.x + 1;
+  if (i >= ctas) return;
+  const int64_t at = tree_bound(units, ctas, i);
+  int b = 0, tiles = 1;
+  int64_t first = 0;
+  tree_find<S::kKeys>(a, at, &b, &tiles, &first);
+  const int hr = static_cast<int>((at - first) / tiles);
+  const int64_t begin = first + static_cast<int64_t>(hr) * tiles;
+  if (at == begin || tree_bound(units, ctas, i - 1) > begin) return;
+  const int r = blockIdx.y * 4 + threadIdx.x / 32;
+  const int row = (hr % a.row_tiles) * S::kRows + r;
+  if (row >= a.rows) return;
+  const int lane = threadIdx.x % 32;
+  constexpr int kPer = D / 32;
+  float m = -INFINITY, l = 0.0f, o[kPer] = {};
+  for (int64_t c = i - 1; c < ctas && tree_bound(units, ctas, c) < begin + tiles; ++c) {
+    // The row tile is run c's second part unless the run starts in it.
+    const float* part = a.parts + (c * 2 + (tree_bound(units, ctas, c) < begin ? 1 : 0)) * S::kPart;
+    const float pm = part[S::kRows * D + 2 * r], pl = part[S::kRows * D + 2 * r + 1];
+    const float top = fmaxf(m, pm);
+    const float ref = top == -INFINITY ? 0.0f : top;
+    const float f = ex2_approx(m - ref), pf = ex2_approx(pm - ref);
+    m = top;
+    l = l * f + pl * pf;
+#pragma unroll
+    for (int x = 0; x < kPer; ++x) o[x] = o[x] * f + part[r * D + lane * kPer + x] * pf;
+  }
+  const int kv = hr / a.row_tiles;
+  const float f = l == 0.0f ? 0.0f : 1.0f / l;
+  T* out = static_cast<T*>(a.out) +
+           ((static_cast<int64_t>(b) * a.heads + kv * a.group + row / a.nodes) * a.nodes + row % a.nodes) * D;
+#pragma unroll
+  for (int x = 0; x < kPer; x += 2)
+    *reinterpret_cast<uint32_t*>(out + lane * kPer + x) = pack2(o[x] * f, o[x + 1] * f, T());
 }
 
 }  // namespace piper
