@@ -350,9 +350,12 @@ int piper_b200_kv_cache_keep(const piper_b200_kv_cache_t* cache, const int32_t* 
                              int64_t path_stride, int64_t nodes, const int32_t* counts,
                              void* stream);
 
-/* Workspace bytes of piper_b200_tree_attention (0 when it needs none). */
+/* Workspace bytes of piper_b200_tree_attention on the current device for a
+ * block table with room for `positions` tokens a request (table_width *
+ * page_size); 0 when it needs none. */
 int piper_b200_tree_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads,
-                                              int64_t nodes, int64_t head_dim, size_t* bytes);
+                                              int64_t nodes, int64_t head_dim, int64_t positions,
+                                              size_t* bytes);
 
 /* Attention of `nodes` (1 to 64) query rows per request and head over the
  * cache: node t of request b sees positions [0, lengths[b]) and drafted

@@ -97,18 +97,40 @@ constexpr int kMaxDevices = 64;
 std::mutex g_tree_mutex;
 unsigned long long g_tree_context[kMaxDevices] = {};  // context whose kernels have their shared memory
 
-// Rows of a KV head, and the CTAs of one row tile, for which the kernel
-// instances are made: 16 rows on four warps, or 32 rows on eight.
-bool few_rows(int64_t rows) { return rows <= 16; }
+// How one call is spread over the GPU.
+struct TreePlan {
+  int64_t grid = 0;
+  size_t bytes = 0;  // of the workspace
+  int row_tiles = 0;
+  bool whole = false;
+};
 
+template <typename S>
+TreePlan tree_plan(int64_t batch, int64_t kv_heads, int64_t rows, int64_t positions, int sms) {
+  TreePlan p;
+  p.row_tiles = static_cast<int>((rows + S::kRows - 1) / S::kRows);
+  const int64_t segments = batch * kv_heads * p.row_tiles;
+  const int64_t most = (positions + S::kKeys - 1) / S::kKeys;
+  // Tables of a few tiles: a CTA for each (request, head, row tile), one
+  // launch and nothing to merge.
+  p.whole = most <= 8 && segments < (int64_t(1) << 31);
+  if (p.whole) {
+    p.grid = segments;
+    return p;
+  }
+  const int64_t slots = static_cast<int64_t>(sms) * S::kCtas;
+  p.grid = most > 2 * slots / segments ? slots : std::max<int64_t>(1, segments * most / 2);
+  p.bytes = static_cast<size_t>(p.grid) * 2 * S::kPart * 4;
+  return p;
+}
+
+// Up to 16 rows of a KV head go to one m16 tile on four warps, more to two on
+// eight.
 template <int D>
-size_t part_bytes(int64_t rows) {
-  return few_rows(rows) ? size_t(4) * 2 * piper::TreeTile<D, 1, 4>::kPart : size_t(4) * 2 * piper::TreeTile<D, 2, 8>::kPart;
-}
-
-int tree_slots(int64_t rows, int sms) {
-  return sms * (few_rows(rows) ? piper::TreeTile<128, 1, 4>::kCtas : piper::TreeTile<128, 2, 8>::kCtas);
-}
+using FewRows = piper::TreeTile<D, 1, 4>;
+template <int D>
+using ManyRows = piper::TreeTile<D, 2, 8>;
+bool few_rows(int64_t rows) { return rows <= 16; }
 
 template <typename T, int D, int MT, int WARPS>
 int allow_smem() {
@@ -137,24 +159,17 @@ int set_up_tree(const piper::host::Device& device) {
 }
 
 template <typename T, int D, int MT, int WARPS>
-int launch_tree(piper::TreeArgs a, int slots, size_t workspace_bytes, cudaStream_t stream) {
+int launch_tree(piper::TreeArgs a, int sms, size_t workspace_bytes, cudaStream_t stream) {
   using S = piper::TreeTile<D, MT, WARPS>;
-  a.row_tiles = (a.rows + S::kRows - 1) / S::kRows;
-  const int64_t segments = static_cast<int64_t>(a.c.batch) * a.c.kv_heads * a.row_tiles;
-  const int64_t most = ((static_cast<int64_t>(a.c.table_width) << a.page_shift) + S::kKeys - 1) / S::kKeys;
-  // Tables of a few tiles: a CTA for each (request, head, row tile), one
-  // launch and nothing to merge.
-  a.whole = most <= 8 && segments < (int64_t(1) << 31);
-  int64_t grid = segments;
-  if (!a.whole) {
-    grid = most > 2 * int64_t(slots) / segments ? slots : std::max<int64_t>(1, segments * most / 2);
-    if (workspace_bytes < static_cast<size_t>(grid) * 2 * S::kPart * 4)
-      return fail(PIPER_B200_ERR_WORKSPACE_TOO_SMALL,
-                  "workspace needs " + std::to_string(static_cast<size_t>(grid) * 2 * S::kPart * 4) + " bytes, got " +
-                      std::to_string(workspace_bytes));
-    if (a.parts == nullptr || reinterpret_cast<uintptr_t>(a.parts) % 256 != 0)
-      return invalid("workspace must be 256-byte aligned and not NULL");
-  }
+  const TreePlan plan =
+      tree_plan<S>(a.c.batch, a.c.kv_heads, a.rows, static_cast<int64_t>(a.c.table_width) << a.page_shift, sms);
+  a.row_tiles = plan.row_tiles;
+  a.whole = plan.whole;
+  if (workspace_bytes < plan.bytes)
+    return fail(PIPER_B200_ERR_WORKSPACE_TOO_SMALL, "workspace needs " + std::to_string(plan.bytes) + " bytes, got " +
+                                                        std::to_string(workspace_bytes));
+  if (plan.bytes > 0 && (a.parts == nullptr || reinterpret_cast<uintptr_t>(a.parts) % 256 != 0))
+    return invalid("workspace must be 256-byte aligned and not NULL");
   const uint32_t box = static_cast<uint32_t>(std::min(a.c.page_size, 64));
   CUtensorMap key_map, value_map;
   const uint64_t outer = static_cast<uint64_t>(a.c.pages) * a.c.kv_heads;
@@ -163,27 +178,26 @@ int launch_tree(piper::TreeArgs a, int slots, size_t workspace_bytes, cudaStream
   if ((rc = piper::host::encode_rows_map(&value_map, a.c.value_codes, D, a.c.page_size, outer, box)) != PIPER_B200_OK)
     return rc;
   piper::tree_attention_kernel<T, D, MT, WARPS>
-      <<<static_cast<unsigned>(grid), S::kThreads, S::kAlloc, stream>>>(key_map, value_map, a);
+      <<<static_cast<unsigned>(plan.grid), S::kThreads, S::kAlloc, stream>>>(key_map, value_map, a);
   PIPER_HOST_CUDA(cudaGetLastError());
-  if (a.whole || grid == 1) return PIPER_B200_OK;
+  if (plan.whole || plan.grid == 1) return PIPER_B200_OK;
   cudaLaunchAttribute attribute{};
   attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attribute.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(static_cast<unsigned>(grid - 1), S::kRows / 4);
+  config.gridDim = dim3(static_cast<unsigned>(plan.grid - 1), S::kRows / 4);
   config.blockDim = dim3(128);
   config.stream = stream;
   config.attrs = &attribute;
   config.numAttrs = 1;
-  PIPER_HOST_CUDA(cudaLaunchKernelEx(&config, piper::tree_merge_kernel<T, D, MT, WARPS>, a, static_cast<int>(grid)));
+  PIPER_HOST_CUDA(cudaLaunchKernelEx(&config, piper::tree_merge_kernel<T, D, MT, WARPS>, a, static_cast<int>(plan.grid)));
   return PIPER_B200_OK;
 }
 
 template <typename T, int D>
 int launch_tree_rows(const piper::TreeArgs& a, int sms, size_t workspace_bytes, cudaStream_t stream) {
-  const int slots = tree_slots(a.rows, sms);
-  return few_rows(a.rows) ? launch_tree<T, D, 1, 4>(a, slots, workspace_bytes, stream)
-                          : launch_tree<T, D, 2, 8>(a, slots, workspace_bytes, stream);
+  return few_rows(a.rows) ? launch_tree<T, D, 1, 4>(a, sms, workspace_bytes, stream)
+                          : launch_tree<T, D, 2, 8>(a, sms, workspace_bytes, stream);
 }
 
 }  // namespace
@@ -272,10 +286,12 @@ extern "C" int piper_b200_kv_cache_keep(const piper_b200_kv_cache_t* cache, cons
 }
 
 extern "C" int piper_b200_tree_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t nodes,
-                                                         int64_t head_dim, size_t* bytes) {
+                                                         int64_t head_dim, int64_t positions, size_t* bytes) {
   if (bytes == nullptr) return invalid("bytes is NULL");
-  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || nodes <= 0 || head_dim <= 0)
+  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || nodes <= 0 || positions <= 0)
     return invalid("sizes must be positive");
+  if (head_dim != 64 && head_dim != 128)
+    return invalid("head_dim must be 64 or 128, got " + std::to_string(head_dim));
   int device = 0, sms = 148;
   if (cudaGetDevice(&device) != cudaSuccess ||
       cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
@@ -283,7 +299,12 @@ extern "C" int piper_b200_tree_attention_workspace_bytes(int64_t batch, int64_t 
     sms = 148;
   }
   const int64_t rows = heads / kv_heads * nodes;
-  *bytes = tree_slots(rows, sms) * (head_dim == 64 ? part_bytes<64>(rows) : part_bytes<128>(rows));
+  if (head_dim == 64)
+    *bytes = few_rows(rows) ? tree_plan<FewRows<64>>(batch, kv_heads, rows, positions, sms).bytes
+                            : tree_plan<ManyRows<64>>(batch, kv_heads, rows, positions, sms).bytes;
+  else
+    *bytes = few_rows(rows) ? tree_plan<FewRows<128>>(batch, kv_heads, rows, positions, sms).bytes
+                            : tree_plan<ManyRows<128>>(batch, kv_heads, rows, positions, sms).bytes;
   return PIPER_B200_OK;
 }
 

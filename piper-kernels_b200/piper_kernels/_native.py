@@ -200,7 +200,7 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.piper_b200_kv_cache_read.restype = ctypes.c_int
     lib.piper_b200_kv_cache_keep.argtypes = [cache, _VP, _I64, _I64, _VP, _VP]
     lib.piper_b200_kv_cache_keep.restype = ctypes.c_int
-    lib.piper_b200_tree_attention_workspace_bytes.argtypes = [_I64] * 5 + [ctypes.POINTER(ctypes.c_size_t)]
+    lib.piper_b200_tree_attention_workspace_bytes.argtypes = [_I64] * 6 + [ctypes.POINTER(ctypes.c_size_t)]
     lib.piper_b200_tree_attention_workspace_bytes.restype = ctypes.c_int
     lib.piper_b200_tree_attention.argtypes = [cache, _VP, _STRIDES, _VP, ctypes.c_int, _I64, _I64, _VP, _I64] + [
         ctypes.c_double, _VP, ctypes.c_size_t, _VP,

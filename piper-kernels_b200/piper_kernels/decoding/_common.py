@@ -1,12 +1,12 @@
 """Checks and launch helpers that the decoding operators share.
 
 Everything here runs on the host before any device work.  These operators are
-called once per layer and token, so the checks read tensor attributes only.
+called once per layer and token, often with a few microseconds of GPU work, so
+a call first asks :func:`fits` of each argument, one expression without
+messages; only a misfit goes to :func:`check_tensor`, which says what is wrong.
 """
 
 from __future__ import annotations
-
-from functools import lru_cache
 
 import torch
 
@@ -17,21 +17,33 @@ DTYPE_CODES = {torch.float16: _native.FLOAT16, torch.bfloat16: _native.BFLOAT16}
 SUPPORTED_HEAD_DIMS = (64, 128)
 MAX_NODES = 64
 
-
-@lru_cache(maxsize=None)
-def _is_sm100(index: int) -> bool:
-    return AcceleratorTarget.from_device(torch.device("cuda", index)).supports_tcgen05_int8
+_sm100_devices: dict[int, bool] = {}
 
 
 def require_device(operator: str, device: torch.device) -> None:
     """Raise unless ``device`` is an sm_100 GPU."""
-    if device.type == "cuda" and _is_sm100(device.index if device.index is not None else torch.cuda.current_device()):
-        return
+    if device.type == "cuda":
+        if device.index in _sm100_devices:
+            return
+        if AcceleratorTarget.from_device(device).supports_tcgen05_int8:
+            _sm100_devices[device.index] = True
+            return
     target = AcceleratorTarget.from_device(device)
     raise RuntimeError(
         f"{operator}'s B200 backend requires CUDA tensors on an sm_100 GPU, "
         f"got device {device} ({target.architecture or target.backend}); "
         "this package has no CPU or generic-GPU fallback"
+    )
+
+
+def fits(tensor: torch.Tensor, shape: tuple[int, ...], dtype: torch.dtype, device: torch.device) -> bool:
+    """Whether :func:`check_tensor` would accept the argument (``shape`` in whole numbers, not empty)."""
+    return (
+        tensor.shape == shape
+        and tensor.dtype is dtype
+        and tensor.device == device
+        and tensor.layout is torch.strided
+        and (tensor.stride(-1) == 1 or shape[-1] <= 1)
     )
 
 
@@ -62,9 +74,8 @@ def check_half(operator: str, name: str, dtype: torch.dtype) -> None:
         raise ValueError(f"{operator} {name} must use float16 or bfloat16, got {dtype}")
 
 
-def check_no_grad(operator: str, *tensors: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise RuntimeError(f"{operator} is an inference-only operator and does not support autograd")
+def refuse_grad(operator: str) -> None:
+    raise RuntimeError(f"{operator} is an inference-only operator and does not support autograd")
 
 
 def launch(what: str, device: torch.device, call, *args) -> None:

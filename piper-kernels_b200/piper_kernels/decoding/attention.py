@@ -4,11 +4,12 @@ from __future__ import annotations
 
 import ctypes
 import math
+from functools import lru_cache
 
 import torch
 
 from .. import _native
-from ._common import DTYPE_CODES, MAX_NODES, check_half, check_no_grad, check_tensor, launch, require_device
+from ._common import DTYPE_CODES, MAX_NODES, check_half, check_tensor, fits, launch, refuse_grad, require_device
 from .cache import QuantizedKVCache, check_batch
 
 OPERATOR = "tree_attention"
@@ -47,9 +48,11 @@ def tree_attention(
             f"{OPERATOR} query must have shape [batch, heads, sequence, head_dim], got {tuple(query.shape)}"
         )
     batch, heads, nodes, _ = query.shape
-    device = cache.device
-    check_half(OPERATOR, "query", query.dtype)
-    check_tensor(OPERATOR, "query", query, (batch, heads, nodes, cache.head_dim), query.dtype, device)
+    device, dtype, head_dim = cache.device, query.dtype, cache.head_dim
+    if dtype not in DTYPE_CODES:
+        check_half(OPERATOR, "query", dtype)
+    if not fits(query, (batch, heads, nodes, head_dim), dtype, device):
+        check_tensor(OPERATOR, "query", query, (batch, heads, nodes, head_dim), dtype, device)
     if not 1 <= nodes <= MAX_NODES:
         raise ValueError(f"{OPERATOR} supports 1 to {MAX_NODES} nodes, got {nodes}")
     if heads == 0 or heads % cache.kv_heads != 0:
@@ -57,9 +60,11 @@ def tree_attention(
     check_batch(OPERATOR, cache, batch, block_table, lengths)
     if tree_mask is not None:
         shape = (nodes,) if tree_mask.ndim == 1 else (batch, nodes)
-        check_tensor(OPERATOR, "tree_mask", tree_mask, shape, torch.int64, device)
-    check_no_grad(OPERATOR, query)
-    effective = cache.head_dim**-0.5 if scale is None else float(scale)
+        if not fits(tree_mask, shape, torch.int64, device):
+            check_tensor(OPERATOR, "tree_mask", tree_mask, shape, torch.int64, device)
+    if query.requires_grad and torch.is_grad_enabled():
+        refuse_grad(OPERATOR)
+    effective = head_dim**-0.5 if scale is None else float(scale)
     if not math.isfinite(effective) or effective <= 0:
         raise ValueError(f"{OPERATOR} scale must be finite and positive, got {scale}")
     require_device(OPERATOR, device)
@@ -71,27 +76,34 @@ def tree_attention(
     return _run(query, cache, block_table, lengths, tree_mask, effective)
 
 
-def workspace_bytes(batch: int, heads: int, kv_heads: int, nodes: int, head_dim: int) -> int:
+def workspace_bytes(batch: int, heads: int, kv_heads: int, nodes: int, head_dim: int, positions: int) -> int:
+    """Workspace of one call whose block table has room for ``positions`` tokens (0: it needs none)."""
     size = ctypes.c_size_t(0)
     _native.check(
         _native.library().piper_b200_tree_attention_workspace_bytes(
-            batch, heads, kv_heads, nodes, head_dim, ctypes.byref(size)
+            batch, heads, kv_heads, nodes, head_dim, positions, ctypes.byref(size)
         ),
         "piper_b200_tree_attention_workspace_bytes",
     )
     return int(size.value)
 
 
+_workspace_bytes = lru_cache(maxsize=4096)(workspace_bytes)  # the same few shapes come back every step
+
+
 def _run(query, cache, block_table, lengths, tree_mask, scale) -> torch.Tensor:
     batch, heads, nodes, head_dim = query.shape
-    out = torch.empty((batch, heads, nodes, head_dim), dtype=query.dtype, device=query.device)
-    nbytes = workspace_bytes(batch, heads, cache.kv_heads, nodes, head_dim)
-    workspace = torch.empty(nbytes, dtype=torch.uint8, device=query.device) if nbytes else None
+    device = query.device
+    out = torch.empty((batch, heads, nodes, head_dim), dtype=query.dtype, device=device)
+    nbytes = _workspace_bytes(
+        batch, heads, cache.kv_heads, nodes, head_dim, block_table.shape[1] * cache.page_size
+    )
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     mask_ptr, mask_stride = None, 0
     if tree_mask is not None:
         mask_ptr, mask_stride = tree_mask.data_ptr(), tree_mask.stride(0) if tree_mask.ndim == 2 else 0
     launch(
-        "piper_b200_tree_attention", query.device, _native.library().piper_b200_tree_attention,
+        "piper_b200_tree_attention", device, _native.library().piper_b200_tree_attention,
         ctypes.byref(cache.native(block_table, lengths)), query.data_ptr(), _native.strides3(query), out.data_ptr(),
         DTYPE_CODES[query.dtype], heads, nodes, mask_ptr, mask_stride, scale,
         None if workspace is None else workspace.data_ptr(), nbytes,

@@ -19,7 +19,6 @@ position ``lengths[b] + i``.
 from __future__ import annotations
 
 import ctypes
-from dataclasses import dataclass
 
 import torch
 
@@ -29,16 +28,16 @@ from ._common import (
     MAX_NODES,
     SUPPORTED_HEAD_DIMS,
     check_half,
-    check_no_grad,
     check_tensor,
+    fits,
     launch,
+    refuse_grad,
     require_device,
 )
 
 PAGE_SIZES = (16, 32, 64, 128, 256)
 
 
-@dataclass(frozen=True, eq=False)
 class QuantizedKVCache:
     """Buffers of one layer's cache; a handle that a program keeps.
 
@@ -47,42 +46,41 @@ class QuantizedKVCache:
     kv_heads, page_size]``, all contiguous on one device.  ``key_mean`` is
     float32 ``[kv_heads, head_dim]`` or None; it belongs to the rows written
     with it.  ``page_size`` is 16, 32, 64, 128 or 256, ``head_dim`` 64 or 128.
+    The buffers are read-only attributes, like the sizes ``pages``,
+    ``kv_heads``, ``page_size`` and ``head_dim`` and the ``device``.
     """
 
-    key_codes: torch.Tensor
-    key_scales: torch.Tensor
-    value_codes: torch.Tensor
-    value_scales: torch.Tensor
-    key_mean: torch.Tensor | None = None
+    __slots__ = ("_buffers", "device", "pages", "kv_heads", "page_size", "head_dim")
 
-    def __post_init__(self) -> None:
-        codes = self.key_codes
-        if codes.ndim != 4:
-            raise ValueError(
-                "QuantizedKVCache key_codes must have shape [pages, kv_heads, page_size, head_dim], "
-                f"got {tuple(codes.shape)}"
-            )
-        pages, kv_heads, page_size, head_dim = codes.shape
-        if head_dim not in SUPPORTED_HEAD_DIMS:
-            raise ValueError(f"QuantizedKVCache supports head dimensions 64 and 128, got {head_dim}")
-        if page_size not in PAGE_SIZES:
-            raise ValueError(f"QuantizedKVCache page_size must be one of {PAGE_SIZES}, got {page_size}")
-        if pages == 0 or kv_heads == 0:
-            raise ValueError("QuantizedKVCache needs at least one page and one KV head")
-        device = codes.device
-        for name, tensor, shape, dtype in (
-            ("key_codes", codes, codes.shape, torch.int8),
-            ("value_codes", self.value_codes, codes.shape, torch.int8),
-            ("key_scales", self.key_scales, codes.shape[:3], torch.float32),
-            ("value_scales", self.value_scales, codes.shape[:3], torch.float32),
+    def __init__(
+        self,
+        key_codes: torch.Tensor,
+        key_scales: torch.Tensor,
+        value_codes: torch.Tensor,
+        value_scales: torch.Tensor,
+        key_mean: torch.Tensor | None = None,
+    ) -> None:
+        shape, device = key_codes.shape, key_codes.device
+        if not (
+            len(shape) == 4
+            and shape[0] > 0
+            and shape[1] > 0
+            and shape[2] in PAGE_SIZES
+            and shape[3] in SUPPORTED_HEAD_DIMS
+            and key_codes.dtype is torch.int8
+            and key_codes.is_contiguous()
+            and fits(value_codes, shape, torch.int8, device)
+            and value_codes.is_contiguous()
+            and fits(key_scales, shape[:3], torch.float32, device)
+            and key_scales.is_contiguous()
+            and fits(value_scales, shape[:3], torch.float32, device)
+            and value_scales.is_contiguous()
+            and (key_mean is None or fits(key_mean, shape[1::2], torch.float32, device) and key_mean.is_contiguous())
         ):
-            check_tensor("QuantizedKVCache", name, tensor, shape, dtype, device)
-            if not tensor.is_contiguous():
-                raise ValueError(f"QuantizedKVCache {name} must be contiguous")
-        if self.key_mean is not None:
-            check_tensor("QuantizedKVCache", "key_mean", self.key_mean, (kv_heads, head_dim), torch.float32, device)
-            if not self.key_mean.is_contiguous():
-                raise ValueError("QuantizedKVCache key_mean must be contiguous")
+            _refuse_buffers(key_codes, key_scales, value_codes, value_scales, key_mean)
+        self._buffers = (key_codes, key_scales, value_codes, value_scales, key_mean)
+        self.device = device
+        self.pages, self.kv_heads, self.page_size, self.head_dim = shape
 
     @classmethod
     def allocate(
@@ -108,36 +106,77 @@ class QuantizedKVCache:
         )
 
     @property
-    def device(self) -> torch.device:
-        return self.key_codes.device
+    def key_codes(self) -> torch.Tensor:
+        return self._buffers[0]
 
     @property
-    def kv_heads(self) -> int:
-        return self.key_codes.shape[1]
+    def key_scales(self) -> torch.Tensor:
+        return self._buffers[1]
 
     @property
-    def page_size(self) -> int:
-        return self.key_codes.shape[2]
+    def value_codes(self) -> torch.Tensor:
+        return self._buffers[2]
 
     @property
-    def head_dim(self) -> int:
-        return self.key_codes.shape[3]
+    def value_scales(self) -> torch.Tensor:
+        return self._buffers[3]
+
+    @property
+    def key_mean(self) -> torch.Tensor | None:
+        return self._buffers[4]
 
     def native(self, block_table: torch.Tensor, lengths: torch.Tensor) -> _native.KVCache:
         """The C ABI's description of this cache for one batch."""
-        pages, kv_heads, page_size, head_dim = self.key_codes.shape
+        key_codes, key_scales, value_codes, value_scales, key_mean = self._buffers
+        batch, width = block_table.shape
         return _native.KVCache(
-            self.key_codes.data_ptr(), self.key_scales.data_ptr(), self.value_codes.data_ptr(),
-            self.value_scales.data_ptr(), None if self.key_mean is None else self.key_mean.data_ptr(),
-            block_table.data_ptr(), lengths.data_ptr(), pages, block_table.stride(0), kv_heads, page_size, head_dim,
-            block_table.shape[0], block_table.shape[1],
+            key_codes.data_ptr(), key_scales.data_ptr(), value_codes.data_ptr(), value_scales.data_ptr(),
+            None if key_mean is None else key_mean.data_ptr(), block_table.data_ptr(), lengths.data_ptr(),
+            self.pages, block_table.stride(0), self.kv_heads, self.page_size, self.head_dim, batch, width,
         )
+
+
+def _refuse_buffers(key_codes, key_scales, value_codes, value_scales, key_mean) -> None:
+    """Say what is wrong with a cache's buffers."""
+    name = "QuantizedKVCache"
+    if key_codes.ndim != 4:
+        raise ValueError(
+            f"{name} key_codes must have shape [pages, kv_heads, page_size, head_dim], got {tuple(key_codes.shape)}"
+        )
+    pages, kv_heads, page_size, head_dim = key_codes.shape
+    if head_dim not in SUPPORTED_HEAD_DIMS:
+        raise ValueError(f"{name} supports head dimensions 64 and 128, got {head_dim}")
+    if page_size not in PAGE_SIZES:
+        raise ValueError(f"{name} page_size must be one of {PAGE_SIZES}, got {page_size}")
+    if pages == 0 or kv_heads == 0:
+        raise ValueError(f"{name} needs at least one page and one KV head")
+    for label, tensor, shape, dtype in (
+        ("key_codes", key_codes, key_codes.shape, torch.int8),
+        ("value_codes", value_codes, key_codes.shape, torch.int8),
+        ("key_scales", key_scales, key_codes.shape[:3], torch.float32),
+        ("value_scales", value_scales, key_codes.shape[:3], torch.float32),
+        ("key_mean", key_mean, (kv_heads, head_dim), torch.float32),
+    ):
+        if tensor is not None:
+            check_tensor(name, label, tensor, shape, dtype, key_codes.device)
+            if not tensor.is_contiguous():
+                raise ValueError(f"{name} {label} must be contiguous")
+    raise ValueError(f"{name} buffers do not belong together")
 
 
 def check_batch(
     operator: str, cache: QuantizedKVCache, batch: int, block_table: torch.Tensor, lengths: torch.Tensor
 ) -> None:
     """Check the arguments that say where a batch's tokens lie."""
+    table = block_table.shape
+    if (
+        batch > 0
+        and len(table) == 2
+        and table[1] > 0
+        and fits(block_table, (batch, table[1]), torch.int32, cache.device)
+        and fits(lengths, (batch,), torch.int32, cache.device)
+    ):
+        return
     if batch == 0:
         raise ValueError(f"{operator} does not accept an empty batch")
     check_tensor(operator, "block_table", block_table, (batch, None), torch.int32, cache.device)
@@ -169,16 +208,20 @@ def write_kv_cache(
     operator = "write_kv_cache"
     if key.ndim != 4:
         raise ValueError(f"{operator} key must have shape [batch, heads, sequence, head_dim], got {tuple(key.shape)}")
-    batch, kv_heads, tokens, head_dim = key.shape
-    check_half(operator, "key", key.dtype)
-    check_tensor(operator, "key", key, (batch, cache.kv_heads, tokens, cache.head_dim), key.dtype, cache.device)
-    check_tensor(operator, "value", value, key.shape, key.dtype, cache.device)
+    batch, _, tokens, _ = key.shape
+    device, dtype, shape = cache.device, key.dtype, (batch, cache.kv_heads, tokens, cache.head_dim)
+    if dtype not in DTYPE_CODES:
+        check_half(operator, "key", dtype)
+    if not (fits(key, shape, dtype, device) and fits(value, shape, dtype, device)):
+        check_tensor(operator, "key", key, shape, dtype, device)
+        check_tensor(operator, "value", value, shape, dtype, device)
     if tokens == 0:
         raise ValueError(f"{operator} does not accept an empty sequence")
     check_batch(operator, cache, batch, block_table, lengths)
-    if counts is not None:
-        check_tensor(operator, "counts", counts, (batch,), torch.int32, cache.device)
-    check_no_grad(operator, key, value)
+    if counts is not None and not fits(counts, (batch,), torch.int32, device):
+        check_tensor(operator, "counts", counts, (batch,), torch.int32, device)
+    if (key.requires_grad or value.requires_grad) and torch.is_grad_enabled():
+        refuse_grad(operator)
     require_device(operator, cache.device)
     if torch.compiler.is_compiling():
         torch.ops.piper_kernels.write_kv_cache(
@@ -213,14 +256,15 @@ def read_kv_cache(
     (default: none), and positions without a page, read as zeros.
     """
     operator = "read_kv_cache"
-    check_half(operator, "dtype", dtype)
+    if dtype not in DTYPE_CODES:
+        check_half(operator, "dtype", dtype)
     tokens = int(tokens)
     if tokens <= 0:
         raise ValueError(f"{operator} tokens must be positive, got {tokens}")
     if lengths.ndim != 1:
         raise ValueError(f"{operator} lengths must have shape [batch], got {tuple(lengths.shape)}")
     check_batch(operator, cache, lengths.shape[0], block_table, lengths)
-    if counts is not None:
+    if counts is not None and not fits(counts, (lengths.shape[0],), torch.int32, cache.device):
         check_tensor(operator, "counts", counts, (lengths.shape[0],), torch.int32, cache.device)
     require_device(operator, cache.device)
     if torch.compiler.is_compiling():
@@ -265,8 +309,10 @@ def keep_draft_path(
     if not 1 <= nodes <= MAX_NODES:
         raise ValueError(f"{operator} supports 1 to {MAX_NODES} nodes, got {nodes}")
     check_batch(operator, cache, batch, block_table, lengths)
-    check_tensor(operator, "path", path, (batch, nodes), torch.int32, cache.device)
-    check_tensor(operator, "counts", counts, (batch,), torch.int32, cache.device)
+    device = cache.device
+    if not (fits(path, (batch, nodes), torch.int32, device) and fits(counts, (batch,), torch.int32, device)):
+        check_tensor(operator, "path", path, (batch, nodes), torch.int32, device)
+        check_tensor(operator, "counts", counts, (batch,), torch.int32, device)
     require_device(operator, cache.device)
     if torch.compiler.is_compiling():
         torch.ops.piper_kernels.keep_draft_path(

@@ -7,7 +7,7 @@ from typing import NamedTuple
 import torch
 
 from .. import _native
-from ._common import MAX_NODES, check_no_grad, check_tensor, launch, require_device
+from ._common import MAX_NODES, check_tensor, fits, launch, refuse_grad, require_device
 
 OPERATOR = "verify_draft_tree"
 
@@ -62,17 +62,27 @@ def verify_draft_tree(
         )
     batch, nodes, vocab = target_probs.shape
     device = target_probs.device
-    check_tensor(OPERATOR, "target_probs", target_probs, (batch, nodes, vocab), torch.float32, device)
-    check_tensor(OPERATOR, "draft_probs", draft_probs, (batch, nodes, vocab), torch.float32, device)
-    check_tensor(OPERATOR, "tokens", tokens, (batch, nodes), torch.int64, device)
-    check_tensor(OPERATOR, "parents", parents, (batch, nodes), torch.int32, device)
-    check_tensor(OPERATOR, "uniform", uniform, (batch, nodes), torch.float32, device)
-    check_tensor(OPERATOR, "noise", noise, (batch, vocab), torch.float32, device)
+    rows, pair, single = (batch, nodes, vocab), (batch, nodes), torch.float32
+    if not (
+        fits(target_probs, rows, single, device)
+        and fits(draft_probs, rows, single, device)
+        and fits(tokens, pair, torch.int64, device)
+        and fits(parents, pair, torch.int32, device)
+        and fits(uniform, pair, single, device)
+        and fits(noise, (batch, vocab), single, device)
+    ):
+        check_tensor(OPERATOR, "target_probs", target_probs, rows, single, device)
+        check_tensor(OPERATOR, "draft_probs", draft_probs, rows, single, device)
+        check_tensor(OPERATOR, "tokens", tokens, pair, torch.int64, device)
+        check_tensor(OPERATOR, "parents", parents, pair, torch.int32, device)
+        check_tensor(OPERATOR, "uniform", uniform, pair, single, device)
+        check_tensor(OPERATOR, "noise", noise, (batch, vocab), single, device)
     if batch == 0 or vocab == 0:
         raise ValueError(f"{OPERATOR} does not accept an empty batch or vocabulary")
     if not 1 <= nodes <= MAX_NODES:
         raise ValueError(f"{OPERATOR} supports 1 to {MAX_NODES} nodes, got {nodes}")
-    check_no_grad(OPERATOR, target_probs, draft_probs)
+    if (target_probs.requires_grad or draft_probs.requires_grad) and torch.is_grad_enabled():
+        refuse_grad(OPERATOR)
     require_device(OPERATOR, device)
     if torch.compiler.is_compiling():
         return DraftVerification(
