@@ -14,6 +14,7 @@
 #include "kv_cache.cuh"
 #include "piper_b200.h"
 #include "tree_attention.cuh"
+#include "tree_wide.cuh"
 #include "verify_tree.cuh"
 
 namespace {
@@ -124,43 +125,67 @@ TreePlan tree_plan(int64_t batch, int64_t kv_heads, int64_t rows, int64_t positi
   return p;
 }
 
-// Up to 16 rows of a KV head go to one m16 tile on four warps, more to two on
-// eight.
+// The kernel for a number of query rows of a KV head: up to 16 one m16 tile
+// on four warps, up to 128 a tcgen05 tile whose streams take alternate keys,
+// more a pair of them over the same keys.
+enum class TreeKind { kFew, kAlternate, kPair };
+TreeKind tree_kind(int64_t rows) {
+  return rows <= 16 ? TreeKind::kFew : rows <= 128 ? TreeKind::kAlternate : TreeKind::kPair;
+}
 template <int D>
 using FewRows = piper::TreeTile<D, 1, 4>;
-template <int D>
-using ManyRows = piper::TreeTile<D, 2, 8>;
-bool few_rows(int64_t rows) { return rows <= 16; }
 
-template <typename T, int D, int MT, int WARPS>
-int allow_smem() {
-  PIPER_HOST_CUDA(cudaFuncSetAttribute(piper::tree_attention_kernel<T, D, MT, WARPS>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       piper::TreeTile<D, MT, WARPS>::kAlloc));
+template <int D>
+TreePlan tree_plan(int64_t batch, int64_t kv_heads, int64_t rows, int64_t positions, int sms) {
+  switch (tree_kind(rows)) {
+    case TreeKind::kFew: return tree_plan<FewRows<D>>(batch, kv_heads, rows, positions, sms);
+    case TreeKind::kAlternate: return tree_plan<piper::WideTile<D, false>>(batch, kv_heads, rows, positions, sms);
+    default: return tree_plan<piper::WideTile<D, true>>(batch, kv_heads, rows, positions, sms);
+  }
+}
+
+int allow_smem(const void* kernel, int bytes) {
+  PIPER_HOST_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  return PIPER_B200_OK;
+}
+
+template <typename T, int D, bool kShared>
+int set_up_wide() {
+  const void* kernel = reinterpret_cast<const void*>(piper::tree_wide_kernel<T, D, kShared>);
+  const int rc = allow_smem(kernel, piper::WideTile<D, kShared>::kAlloc);
+  if (rc != PIPER_B200_OK) return rc;
+  // Its setmaxnreg split needs exactly this many registers at launch.
+  cudaFuncAttributes attr;
+  PIPER_HOST_CUDA(cudaFuncGetAttributes(&attr, kernel));
+  if (attr.numRegs != piper::kWideLaunchRegs)
+    return fail(PIPER_B200_ERR_CUDA, "tree attention kernel compiled with " + std::to_string(attr.numRegs) +
+                                         " registers per thread; its warpgroup register split needs " +
+                                         std::to_string(piper::kWideLaunchRegs));
   return PIPER_B200_OK;
 }
 
 template <typename T, int D>
-int allow_smem_both() {
-  const int rc = allow_smem<T, D, 1, 4>();
-  return rc != PIPER_B200_OK ? rc : allow_smem<T, D, 2, 8>();
+int set_up_instances() {
+  int rc = allow_smem(reinterpret_cast<const void*>(piper::tree_attention_kernel<T, D, 1, 4>), FewRows<D>::kAlloc);
+  if (rc != PIPER_B200_OK) return rc;
+  if ((rc = set_up_wide<T, D, false>()) != PIPER_B200_OK) return rc;
+  return set_up_wide<T, D, true>();
 }
 
 int set_up_tree(const piper::host::Device& device) {
   std::lock_guard<std::mutex> lock(g_tree_mutex);
   if (device.context != 0 && g_tree_context[device.index] == device.context) return PIPER_B200_OK;
   int rc = PIPER_B200_OK;
-  if ((rc = allow_smem_both<__half, 64>()) != PIPER_B200_OK) return rc;
-  if ((rc = allow_smem_both<__half, 128>()) != PIPER_B200_OK) return rc;
-  if ((rc = allow_smem_both<__nv_bfloat16, 64>()) != PIPER_B200_OK) return rc;
-  if ((rc = allow_smem_both<__nv_bfloat16, 128>()) != PIPER_B200_OK) return rc;
+  if ((rc = set_up_instances<__half, 64>()) != PIPER_B200_OK) return rc;
+  if ((rc = set_up_instances<__half, 128>()) != PIPER_B200_OK) return rc;
+  if ((rc = set_up_instances<__nv_bfloat16, 64>()) != PIPER_B200_OK) return rc;
+  if ((rc = set_up_instances<__nv_bfloat16, 128>()) != PIPER_B200_OK) return rc;
   g_tree_context[device.index] = device.context;
   return PIPER_B200_OK;
 }
 
-template <typename T, int D, int MT, int WARPS>
-int launch_tree(piper::TreeArgs a, int sms, size_t workspace_bytes, cudaStream_t stream) {
-  using S = piper::TreeTile<D, MT, WARPS>;
+template <typename T, int D, typename S, typename Kernel>
+int launch_tree(piper::TreeArgs a, Kernel kernel, int threads, int sms, size_t workspace_bytes, cudaStream_t stream) {
   const TreePlan plan =
       tree_plan<S>(a.c.batch, a.c.kv_heads, a.rows, static_cast<int64_t>(a.c.table_width) << a.page_shift, sms);
   a.row_tiles = plan.row_tiles;
@@ -177,8 +202,7 @@ int launch_tree(piper::TreeArgs a, int sms, size_t workspace_bytes, cudaStream_t
   if (rc != PIPER_B200_OK) return rc;
   if ((rc = piper::host::encode_rows_map(&value_map, a.c.value_codes, D, a.c.page_size, outer, box)) != PIPER_B200_OK)
     return rc;
-  piper::tree_attention_kernel<T, D, MT, WARPS>
-      <<<static_cast<unsigned>(plan.grid), S::kThreads, S::kAlloc, stream>>>(key_map, value_map, a);
+  kernel<<<static_cast<unsigned>(plan.grid), threads, S::kAlloc, stream>>>(key_map, value_map, a);
   PIPER_HOST_CUDA(cudaGetLastError());
   if (plan.whole || plan.grid == 1) return PIPER_B200_OK;
   cudaLaunchAttribute attribute{};
@@ -190,14 +214,23 @@ int launch_tree(piper::TreeArgs a, int sms, size_t workspace_bytes, cudaStream_t
   config.stream = stream;
   config.attrs = &attribute;
   config.numAttrs = 1;
-  PIPER_HOST_CUDA(cudaLaunchKernelEx(&config, piper::tree_merge_kernel<T, D, MT, WARPS>, a, static_cast<int>(plan.grid)));
+  PIPER_HOST_CUDA(cudaLaunchKernelEx(&config, piper::tree_merge_kernel<T, D, S>, a, static_cast<int>(plan.grid)));
   return PIPER_B200_OK;
 }
 
 template <typename T, int D>
 int launch_tree_rows(const piper::TreeArgs& a, int sms, size_t workspace_bytes, cudaStream_t stream) {
-  return few_rows(a.rows) ? launch_tree<T, D, 1, 4>(a, sms, workspace_bytes, stream)
-                          : launch_tree<T, D, 2, 8>(a, sms, workspace_bytes, stream);
+  switch (tree_kind(a.rows)) {
+    case TreeKind::kFew:
+      return launch_tree<T, D, FewRows<D>>(a, piper::tree_attention_kernel<T, D, 1, 4>, FewRows<D>::kThreads, sms,
+                                           workspace_bytes, stream);
+    case TreeKind::kAlternate:
+      return launch_tree<T, D, piper::WideTile<D, false>>(a, piper::tree_wide_kernel<T, D, false>,
+                                                          piper::kWideThreads, sms, workspace_bytes, stream);
+    default:
+      return launch_tree<T, D, piper::WideTile<D, true>>(a, piper::tree_wide_kernel<T, D, true>, piper::kWideThreads,
+                                                         sms, workspace_bytes, stream);
+  }
 }
 
 }  // namespace
@@ -299,12 +332,8 @@ extern "C" int piper_b200_tree_attention_workspace_bytes(int64_t batch, int64_t 
     sms = 148;
   }
   const int64_t rows = heads / kv_heads * nodes;
-  if (head_dim == 64)
-    *bytes = few_rows(rows) ? tree_plan<FewRows<64>>(batch, kv_heads, rows, positions, sms).bytes
-                            : tree_plan<ManyRows<64>>(batch, kv_heads, rows, positions, sms).bytes;
-  else
-    *bytes = few_rows(rows) ? tree_plan<FewRows<128>>(batch, kv_heads, rows, positions, sms).bytes
-                            : tree_plan<ManyRows<128>>(batch, kv_heads, rows, positions, sms).bytes;
+  *bytes = head_dim == 64 ? tree_plan<64>(batch, kv_heads, rows, positions, sms).bytes
+                          : tree_plan<128>(batch, kv_heads, rows, positions, sms).bytes;
   return PIPER_B200_OK;
 }
 

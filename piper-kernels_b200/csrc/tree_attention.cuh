@@ -724,9 +724,8 @@ __global__ void __launch_bounds__(TreeTile<D, MT, WARPS>::kThreads, TreeTile<D, 
 // two runs cuts.  CTA x looks at the boundary before run x + 1 and works if it
 // is the first inside its row tile; a warp takes a row, and CTAs y share the
 // rows.
-template <typename T, int D, int MT, int WARPS>
+template <typename T, int D, typename S>
 __global__ void __launch_bounds__(128) tree_merge_kernel(TreeArgs a, int grid) {
-  using S = TreeTile<D, MT, WARPS>;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int64_t units = tree_units<S::kKeys>(a);
   const int64_t ctas = tree_ctas(units, grid);
