@@ -152,16 +152,7 @@ int allow_smem(const void* kernel, int bytes) {
 template <typename T, int D, bool kShared>
 int set_up_wide() {
   const void* kernel = reinterpret_cast<const void*>(piper::tree_wide_kernel<T, D, kShared>);
-  const int rc = allow_smem(kernel, piper::WideTile<D, kShared>::kAlloc);
-  if (rc != PIPER_B200_OK) return rc;
-  // Its setmaxnreg split needs exactly this many registers at launch.
-  cudaFuncAttributes attr;
-  PIPER_HOST_CUDA(cudaFuncGetAttributes(&attr, kernel));
-  if (attr.numRegs != piper::kWideLaunchRegs)
-    return fail(PIPER_B200_ERR_CUDA, "tree attention kernel compiled with " + std::to_string(attr.numRegs) +
-                                         " registers per thread; its warpgroup register split needs " +
-                                         std::to_string(piper::kWideLaunchRegs));
-  return PIPER_B200_OK;
+  return allow_smem(kernel, piper::WideTile<D, kShared>::kAlloc);
 }
 
 template <typename T, int D>

@@ -149,6 +149,43 @@ __device__ __forceinline__ bool mbar_wait_sleep_warp(uint32_t bar, uint32_t pari
   return __all_sync(0xffffffffu, ok) != 0;
 }
 
+// mbar_wait with try_wait and no time hint: the thread sleeps until the phase
+// completes or the hardware's own (short) limit passes, so that it takes few
+// issue slots and does not oversleep.  Bounded in the same way; the clock is
+// read once in sixteen tries.
+__device__ __forceinline__ bool mbar_wait_block(uint32_t bar, uint32_t parity, uint64_t budget_ns, uint32_t* status,
+                                                uint32_t status_bit, uint32_t abort_addr) {
+  uint64_t start = 0;
+  while (true) {
+#pragma unroll 1
+    for (int tries = 0; tries < 16; ++tries) {
+      uint32_t ok;
+      asm volatile(
+          "{\n\t.reg .pred p;\n\t"
+          "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+          "selp.u32 %0, 1, 0, p;\n\t}"
+          : "=r"(ok)
+          : "r"(bar), "r"(parity)
+          : "memory");
+      if (ok != 0) return true;
+    }
+    if (abort_addr != 0 && flag_get(abort_addr) != 0) return false;
+    const uint64_t now = global_timer_ns();
+    if (start == 0) start = now;
+    if (now - start > budget_ns) {
+      if (status != nullptr) atomicOr(status, status_bit);
+      if (abort_addr != 0) flag_set(abort_addr, 1u);
+      return false;
+    }
+  }
+}
+
+__device__ __forceinline__ bool mbar_wait_block_warp(uint32_t bar, uint32_t parity, uint64_t budget_ns,
+                                                     uint32_t* status, uint32_t status_bit, uint32_t abort_addr) {
+  const bool ok = mbar_wait_block(bar, parity, budget_ns, status, status_bit, abort_addr);
+  return __all_sync(0xffffffffu, ok) != 0;
+}
+
 // Warp-uniform variant for code that synchronises the warp afterwards: every
 // lane waits (each bounded), then the warp agrees on success, so no lane can
 // leave a loop that its siblings stay in.
@@ -346,6 +383,32 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t* v) {
                : "memory");
 }
 
+// 16x256b shape: 16 lanes (from the address's lane, a multiple of 16 within the
+// warp's 32), eight columns for each four registers: lane 4 g + t holds rows g
+// (first two) and g + 8 (last two) of columns 2 t and 2 t + 1.  .x4: 32 columns.
+__device__ __forceinline__ void tmem_ld_16x256b_x4(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st_16x256b_x4(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+// 16x128b shape: four columns for each two registers: lane 4 g + t holds rows g
+// and g + 8 of column t.  .x4: 16 columns.
+__device__ __forceinline__ void tmem_st_16x128b_x4(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
 // Writes the same 32-bit value into 4 consecutive columns of this thread's lane.
 __device__ __forceinline__ void tmem_st4_same(uint32_t taddr, uint32_t v) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1,%1,%1,%1};" ::"r"(taddr), "r"(v) : "memory");
@@ -357,6 +420,12 @@ __device__ __forceinline__ void tmem_st4_same(uint32_t taddr, uint32_t v) {
 __device__ __forceinline__ float4 lds128(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr));
+  return v;
+}
+
+__device__ __forceinline__ float2 lds64(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr));
   return v;
 }
 

@@ -16,24 +16,24 @@
 // 128-255 of the row tile over the same keys (more than 128 rows).  Otherwise
 // they are alternate key tiles of the same 128 rows, joined at the end.
 //
-// Warps: 0-3 and 4-7 softmax of streams 0 and 1 (a thread owns a row), 8-11
-// conversion (a thread owns a key), 12 fetches, 13 issues MMAs, 14 owns TMEM.
+// A softmax warp reads its 16 rows' scores twice, 32 columns at a time, first
+// for the maxima, then for the weights.  A row has one reference, the unit of
+// its numerators and of its total: 2^unit follows the largest weight times its
+// value scale, trails by a factor of at most 2^14, and moves only when a tile
+// could outgrow it.
+//
+// Warps: 0-7 and 8-15 softmax of streams 0 and 1 (two for each 32 TMEM lanes),
+// 16-19 conversion (a thread owns a key), 20 fetches, 21 issues MMAs, 22 owns
+// TMEM.
 #pragma once
 
 #include "tree_attention.cuh"
 
 namespace piper {
 
-constexpr int kWideThreads = 512;
-// Register split (setmaxnreg), launch = 128 x 512: the softmax holds 128
-// scores a thread.  128 * (2 * 192 + 72 + 56) = 65536.
-constexpr int kWideLaunchRegs = 128;
-constexpr int kWideRegsSoftmax = 192;
-constexpr int kWideRegsConvert = 72;
-constexpr int kWideRegsControl = 56;
-static_assert(2 * kWideRegsSoftmax + kWideRegsConvert + kWideRegsControl <= 4 * kWideLaunchRegs,
-              "setmaxnreg split exceeds the launch register allocation");
-
+constexpr int kWideThreads = 768;
+constexpr float kWideSlack = 14.0f;      // log2 by which a weight may exceed 1: fp16 holds 2^15
+constexpr float kScaleLogMin = -90.0f;   // smaller value scales count as 2^-90 in the references
 template <int D, bool kShared>
 struct WideTile {
   static constexpr int kRows = kShared ? 256 : 128;
@@ -44,12 +44,13 @@ struct WideTile {
   static constexpr int kQuery = (kShared ? 2 : 1) * kHalf;
   static constexpr int kBuffers = kShared ? 1 : 2;  // fp16 K and V tiles
   static constexpr int kScaleRing = 4;
+  static constexpr int kEntry = kKeys * 8;          // scales of keys and of values
   static constexpr int kOffQuery = 0;
   static constexpr int kOffK = kOffQuery + kQuery;
   static constexpr int kOffV = kOffK + kBuffers * kHalf;
   static constexpr int kOffScales = kOffV + kBuffers * kHalf;
-  static constexpr int kOffState = kOffScales + kScaleRing * kKeys * 8;
-  static constexpr int kOffRing = (kOffState + 3 * 128 * 4 + 1023) / 1024 * 1024;
+  static constexpr int kOffState = kOffScales + kScaleRing * kEntry;
+  static constexpr int kOffRing = (kOffState + 256 * (3 * 4 + 8) + 1023) / 1024 * 1024;
   static constexpr int kFit = (225 * 1024 - kOffRing) / kCodes;
   static constexpr int kRing = kFit > 8 ? 8 : kFit;
   static constexpr int kAlloc = kOffRing + kRing * kCodes + 1024;
@@ -103,6 +104,14 @@ __device__ __forceinline__ void wide_next(const TreeArgs& a, int per, WideWalk& 
   w.all = w.count == w.tiles;
 }
 
+constexpr float kNoReference = -1e30f;
+
+__device__ __forceinline__ float lg2_approx(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 __device__ __forceinline__ float2 mul2(float2 x, float2 y) { return __fmul2_rn(x, y); }
 
 // Query row `row` into shared memory at lane row r (K-major, SW128, blocks of
@@ -111,32 +120,30 @@ __device__ __forceinline__ float2 mul2(float2 x, float2 y) { return __fmul2_rn(x
 template <typename T, int D>
 __device__ __forceinline__ float wide_query_row(const TreeArgs& a, uint8_t* to, int b, int kv, int row, int r,
                                                 bool store) {
-  uint4 raw[D / 8];
-  if (row < a.rows) {
-    const T* p = static_cast<const T*>(a.query) + b * a.qs[0] + (kv * a.group + row / a.nodes) * a.qs[1] +
-                 (row % a.nodes) * a.qs[2];
-    if (a.vec) {
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
+  const bool there = row < a.rows;
+  const T* p = static_cast<const T*>(a.query) + b * a.qs[0];
+  if (there) p += (kv * a.group + row / a.nodes) * a.qs[1] + (row % a.nodes) * a.qs[2];
+  // Read twice (the second time from L1) to hold few registers.
+  auto eight = [&](int c, float (&x)[8]) {
+    uint4 raw = make_uint4(0u, 0u, 0u, 0u);
+    if (there) {
+      if (a.vec) {
         const uint2 lo = __ldg(reinterpret_cast<const uint2*>(p) + 2 * c);
         const uint2 hi = __ldg(reinterpret_cast<const uint2*>(p) + 2 * c + 1);
-        raw[c] = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        raw = make_uint4(lo.x, lo.y, hi.x, hi.y);
+      } else {
+        raw = load_raw8<T, false>(p + c * 8);
       }
-    } else {
-#pragma unroll
-      for (int c = 0; c < D / 8; ++c) raw[c] = load_raw8<T, false>(p + c * 8);
     }
-  } else {
-#pragma unroll
-    for (int c = 0; c < D / 8; ++c) raw[c] = make_uint4(0u, 0u, 0u, 0u);
-  }
+    unpack8<T>(raw, x);
+  };
   float up = 1.0f, factor = a.scale_log2e;
   if constexpr (!std::is_same<T, __half>::value) {
     uint32_t top = 0u;
-#pragma unroll
+#pragma unroll 2
     for (int c = 0; c < D / 8; ++c) {
       float x[8];
-      unpack8<T>(raw[c], x);
+      eight(c, x);
 #pragma unroll
       for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
     }
@@ -145,10 +152,10 @@ __device__ __forceinline__ float wide_query_row(const TreeArgs& a, uint8_t* to, 
     factor = __uint_as_float(e << 23) * a.scale_log2e;
   }
   if (store) {
-#pragma unroll
+#pragma unroll 2
     for (int c = 0; c < D / 8; ++c) {
       float x[8];
-      unpack8<T>(raw[c], x);
+      eight(c, x);
       uint4 w;
       w.x = pack2(x[0] * up, x[1] * up, __half());
       w.y = pack2(x[2] * up, x[3] * up, __half());
@@ -160,25 +167,30 @@ __device__ __forceinline__ float wide_query_row(const TreeArgs& a, uint8_t* to, 
   return factor;
 }
 
-// The keys of a tile that a row sees, 32 to a word.
-__device__ __forceinline__ void wide_seen(uint32_t (&seen)[4], uint32_t goods, int box_shift, int open, uint64_t word) {
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const int n = open - 32 * c;  // committed keys from this word's first on
-    uint32_t bits = n >= 32 ? ~0u : n > 0 ? (1u << n) - 1u : 0u;
-    if (n >= 0) {
-      if (n < 32) bits |= static_cast<uint32_t>(word << n);
-    } else if (n > -64) {
-      bits |= static_cast<uint32_t>(word >> -n);
-    }
-    uint32_t there = 0u;
-    if (box_shift >= 5) {
-      there = (goods >> ((32 * c) >> box_shift)) & 1u ? ~0u : 0u;
-    } else {
-      there = ((goods >> (2 * c)) & 1u ? 0xffffu : 0u) | ((goods >> (2 * c + 1)) & 1u ? 0xffff0000u : 0u);
-    }
-    seen[c] = bits & there;
+// Which of keys 32 c .. 32 c + 31 of a tile a row sees: the first `open` of the
+// tile are committed, those after it follow `word`.
+__device__ __forceinline__ uint32_t wide_seen(uint32_t goods, int box_shift, int open, uint64_t word, int c) {
+  const int n = open - 32 * c;
+  uint32_t bits = n >= 32 ? ~0u : n > 0 ? (1u << n) - 1u : 0u;
+  if (n >= 0) {
+    if (n < 32) bits |= static_cast<uint32_t>(word << n);
+  } else if (n > -64) {
+    bits |= static_cast<uint32_t>(word >> -n);
   }
+  const uint32_t there = box_shift >= 5 ? ((goods >> ((32 * c) >> box_shift)) & 1u ? ~0u : 0u)
+                                        : ((goods >> (2 * c)) & 1u ? 0xffffu : 0u) |
+                                              ((goods >> (2 * c + 1)) & 1u ? 0xffff0000u : 0u);
+  return bits & there;
+}
+
+// Scores of keys that a row does not see, by the two lowest bits.
+__device__ __forceinline__ void hide(float2& y, uint32_t seen) {
+  if (!(seen & 1u)) y.x = -INFINITY;
+  if (!(seen & 2u)) y.y = -INFINITY;
+}
+
+__device__ __forceinline__ float2 f2_of(uint32_t x, uint32_t y) {
+  return make_float2(__uint_as_float(x), __uint_as_float(y));
 }
 
 template <typename T, int D, bool kShared>
@@ -204,7 +216,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     }
     for (int i = 0; i < S::kScaleRing; ++i) {
       mbar_init(smem_u32(&scale_full[i]), 1);
-      mbar_init(smem_u32(&scale_empty[i]), kShared ? 8 : 4);
+      mbar_init(smem_u32(&scale_empty[i]), kShared ? 16 : 8);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&k_full[i]), 4);
@@ -212,7 +224,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       mbar_init(smem_u32(&v_full[i]), 4);
       mbar_init(smem_u32(&v_empty[i]), 1);
       mbar_init(smem_u32(&s_full[i]), 1);
-      mbar_init(smem_u32(&p_full[i]), 4);
+      mbar_init(smem_u32(&p_full[i]), 8);
       mbar_init(smem_u32(&o_done[i]), 1);
       mbar_init(smem_u32(&q_full[i]), 4);
     }
@@ -220,7 +232,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     abort_word = 0u;
     fence_mbarrier_init();
   }
-  if (warp == 14) {
+  if (warp == 22) {
     tmem_alloc(&tmem_slot, 512);
     tmem_relinquish();
   }
@@ -237,260 +249,319 @@ __global__ void __launch_bounds__(kWideThreads, 1)
   const int box_shift = min(a.page_shift, 6);
   const int boxes = S::kKeys >> box_shift;
 
-  if (warp < 8) {
+  if (warp < 16) {
     // ------------------------------------------------------------ softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWideRegsSoftmax));
-    const int x = warp / 4;
-    const int r = tid % 128;
-    const uint32_t lane_base = static_cast<uint32_t>((warp % 4) * 32) << 16;
-    const uint32_t tm_s = tmem_base + lane_base + x * 128;
-    const uint32_t tm_o = tmem_base + lane_base + 256 + x * 128;
-    float* state = reinterpret_cast<float*>(smem + S::kOffState);
+    const int x = warp / 8;              // stream
+    const int half = (warp / 4) & 1;     // of the 32 TMEM lanes that the warp reaches
+    const int lane0 = (warp % 4) * 32;   // the first of them
+    const int g = lane / 4, t = lane % 4;
+    const int r16 = lane0 + half * 16 + g;  // a lane has rows r16 and r16 + 8 of the stream
+    const uint32_t tm_s = tmem_base + (static_cast<uint32_t>(lane0 + half * 16) << 16) + x * 128;
+    const uint32_t tm_o = tmem_base + (static_cast<uint32_t>(lane0 + half * 16) << 16) + 256 + x * 128;
+    float* totals = reinterpret_cast<float*>(smem + S::kOffState);  // [stream][128]
+    float* units = totals + 256;
+    float* factors = units + 256;
+    uint64_t* words = reinterpret_cast<uint64_t*>(factors + 256);  // visible nodes
+    const int bar_id = kShared ? 1 + x : 1;
+    constexpr int kBarThreads = kShared ? 256 : 512;
     bool ok = true;
     uint32_t jobs = 0;      // of this stream so far
     uint32_t done = 0;      // segments of this stream that had a job
-    int64_t counter = 0;    // key tiles of the run so far
+    uint32_t counter = 0;   // key tiles of the run so far
     int part = 0;
     while (w.left > 0) {
       const int kv = w.hr / a.row_tiles;
-      const int row = (w.hr % a.row_tiles) * S::kRows + (kShared ? x * 128 : 0) + r;
+      const int row0 = (w.hr % a.row_tiles) * S::kRows + (kShared ? x * 128 : 0);
       const int64_t length = max(0, __ldg(a.c.lengths + w.b));
-      uint64_t word = 0;
-      if (row < a.rows) {
-        const int node = row % a.nodes;
-        word = a.mask != nullptr ? static_cast<uint64_t>(__ldg(reinterpret_cast<const unsigned long long*>(
-                                       a.mask + w.b * a.mask_stride + node)))
-                                 : ~0ull >> (63 - node);
-        word &= ~0ull >> (64 - a.nodes);
+      if (half == 0) {
+        const int r = lane0 + lane, row = row0 + r;
+        uint64_t word = 0;
+        if (row < a.rows) {
+          const int node = row % a.nodes;
+          word = a.mask != nullptr ? static_cast<uint64_t>(__ldg(reinterpret_cast<const unsigned long long*>(
+                                         a.mask + w.b * a.mask_stride + node)))
+                                   : ~0ull >> (63 - node);
+          word &= ~0ull >> (64 - a.nodes);
+        }
+        words[x * 128 + r] = word;
+        factors[x * 128 + r] = wide_query_row<T, D>(a, smem + S::kOffQuery + (kShared ? x * S::kHalf : 0), w.b, kv,
+                                                    row, r, kShared || x == 0);
+        if (kShared || x == 0) {
+          fence_proxy_async_shared();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(smem_u32(&q_full[kShared ? x : 0]));
+        }
       }
-      const float factor = wide_query_row<T, D>(a, smem + S::kOffQuery + (kShared ? x * S::kHalf : 0), w.b, kv, row, r,
-                                                kShared || x == 0);
-      if (kShared || x == 0) {
-        fence_proxy_async_shared();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&q_full[kShared ? x : 0]));
+      bar_sync(bar_id, kBarThreads);
+      // A row's reference `unit`: the logarithm of the numerators' unit, and of
+      // the total's.
+      float factor[2], unit[2], l[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        factor[h] = factors[x * 128 + r16 + 8 * h];
+        unit[h] = kNoReference;
+        l[h] = 0.0f;
       }
-      float m = -INFINITY, l = 0.0f, unit = 0.0f, inv = 0.0f;
+      // Warps whose rows are all past the last only take part in the hand-over.
+      const bool idle = row0 + lane0 + half * 16 >= a.rows;
       bool first_job = true;
       for (int j = kShared ? 0 : x; j < w.count; j += kShared ? 1 : 2) {
-        const int64_t c = counter + j;
-        const int entry = static_cast<int>(c % S::kScaleRing);
-        if (ok) ok = mbar_wait_warp(smem_u32(&scale_full[entry]), static_cast<uint32_t>(c / S::kScaleRing) & 1, budget,
-                                    a.status, kStatusTimeoutFull, abort_flag);
-        if (ok) ok = mbar_wait_sleep_warp(smem_u32(&s_full[x]), jobs & 1, budget, a.status, kStatusTimeoutMma,
+        const uint32_t c0 = counter + j;
+        const int entry = static_cast<int>(c0 % S::kScaleRing);
+        if (ok) ok = mbar_wait_block_warp(smem_u32(&scale_full[entry]), (c0 / S::kScaleRing) & 1, budget, a.status,
+                                          kStatusTimeoutFull, abort_flag);
+        if (ok) ok = mbar_wait_block_warp(smem_u32(&s_full[x]), jobs & 1, budget, a.status, kStatusTimeoutMma,
                                           abort_flag);
         ++jobs;
         if (!ok) continue;
         tc_fence_after();
-        const uint32_t scales = sbase + S::kOffScales + entry * S::kKeys * 8;
-        float2 y[64];
-        {
-          uint32_t t0[32], t1[32], t2[32], t3[32];
-          tmem_ld32(tm_s, t0);
-          tmem_ld32(tm_s + 32, t1);
-          tmem_ld32(tm_s + 64, t2);
-          tmem_ld32(tm_s + 96, t3);
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            y[i] = make_float2(__uint_as_float(t0[2 * i]), __uint_as_float(t0[2 * i + 1]));
-            y[16 + i] = make_float2(__uint_as_float(t1[2 * i]), __uint_as_float(t1[2 * i + 1]));
-            y[32 + i] = make_float2(__uint_as_float(t2[2 * i]), __uint_as_float(t2[2 * i + 1]));
-            y[48 + i] = make_float2(__uint_as_float(t3[2 * i]), __uint_as_float(t3[2 * i + 1]));
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float4 ks = lds128(scales + 16 * i);
-          y[2 * i] = mul2(y[2 * i], make_float2(ks.x, ks.y));
-          y[2 * i + 1] = mul2(y[2 * i + 1], make_float2(ks.z, ks.w));
-        }
-        const int64_t first = static_cast<int64_t>(w.tile + j) * S::kKeys;
-        const uint32_t goods = valid[entry];
-        const bool masked = first + S::kKeys > length || goods != (1u << boxes) - 1u;
-        uint32_t seen[4];
-        if (masked) {
-          wide_seen(seen, goods, box_shift, static_cast<int>(max(min(length - first, int64_t(256)), int64_t(-256))),
-                    word);
-#pragma unroll
-          for (int i = 0; i < 64; ++i) {
-            if (!((seen[i / 16] >> (2 * (i % 16))) & 1u)) y[i].x = -INFINITY;
-            if (!((seen[i / 16] >> (2 * (i % 16) + 1)) & 1u)) y[i].y = -INFINITY;
-          }
-        }
-        float top0 = -INFINITY, top1 = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 64; i += 2) {
-          top0 = fmax3(top0, y[i].x, y[i].y);
-          top1 = fmax3(top1, y[i + 1].x, y[i + 1].y);
-        }
-        const float top = fmaxf(top0, top1);
-        if ((top - m) * factor > kSlack) {
-          const float shrink = ex2_approx((m - top) * factor);
-          m = top;
-          l *= shrink;
-          unit *= shrink;
-          inv = unit >= kUnitMin ? 1.0f / unit : 0.0f;
-        }
-        const float shift = m == -INFINITY ? 0.0f : -m * factor;
-        const float2 f2 = make_float2(factor, factor), s2 = make_float2(shift, shift);
-        float2 sum0 = make_float2(0.0f, 0.0f), sum1 = sum0;
-        float most0 = 0.0f, most1 = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float4 vs = lds128(scales + S::kKeys * 4 + 16 * i);
-          float2 p = __ffma2_rn(y[2 * i], f2, s2);
-          p.x = ex2_approx(p.x);
-          p.y = ex2_approx(p.y);
-          sum0 = __fadd2_rn(sum0, p);
-          y[2 * i] = mul2(p, make_float2(vs.x, vs.y));
-          float2 q = __ffma2_rn(y[2 * i + 1], f2, s2);
-          q.x = ex2_approx(q.x);
-          q.y = ex2_approx(q.y);
-          sum1 = __fadd2_rn(sum1, q);
-          y[2 * i + 1] = mul2(q, make_float2(vs.z, vs.w));
-        }
-        if (masked) {
-#pragma unroll
-          for (int i = 0; i < 64; ++i) {
-            if (!((seen[i / 16] >> (2 * (i % 16))) & 1u)) y[i].x = 0.0f;
-            if (!((seen[i / 16] >> (2 * (i % 16) + 1)) & 1u)) y[i].y = 0.0f;
-          }
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&scale_empty[entry]));
-        l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
-#pragma unroll
-        for (int i = 0; i < 64; i += 2) {
-          most0 = fmax3(most0, y[i].x, y[i].y);
-          most1 = fmax3(most1, y[i + 1].x, y[i + 1].y);
-        }
-        const float most = fmaxf(most0, most1);
-        const bool over = most > unit * 256.0f;
-        if (__any_sync(0xffffffffu, over)) {
-          const float shrink = over ? unit / most : 1.0f;
-          if (over) {
-            unit = most;
-            inv = most >= kUnitMin ? 1.0f / most : 0.0f;
-          }
-          // The stream's last numerator MMAs are complete: the scores of this
-          // tile were committed after them.
-          if (!first_job) {
-            const float2 k2 = make_float2(shrink, shrink);
+        if (!idle) {
+          const uint32_t scales = sbase + S::kOffScales + entry * S::kEntry;
+          const int64_t first = static_cast<int64_t>(w.tile + j) * S::kKeys;
+          const uint32_t goods = valid[entry];
+          const bool masked = first + S::kKeys > length || goods != (1u << boxes) - 1u;
+          const int open = static_cast<int>(max(min(length - first, int64_t(256)), int64_t(-256)));
+          // Bit 8 n + e: column 32 c + 8 n + 2 t + e of row h is seen.
+          auto seen_of = [&](int c, int h) {
+            return wide_seen(goods, box_shift, open, words[x * 128 + r16 + 8 * h], c) >> (2 * t);
+          };
+          // ---- first reading: the largest scores and value scale
+          float top[2] = {-INFINITY, -INFINITY};
+          const float4 four = lds128(scales + S::kKeys * 4 + 16 * lane);
+          float reach = fmaxf(fmaxf(four.x, four.y), fmaxf(four.z, four.w));
+          // (A masked tile has a body of its own: branches inside would cut
+          // the other's instructions into short chains.)
+          auto largest = [&](auto hidden) {
 #pragma unroll 1
-            for (int d = 0; d < D; d += 16) {
+            for (int c = 0; c < 4; ++c) {
               uint32_t v[16];
-              tmem_ld8(tm_o + d, v);
-              tmem_ld8(tm_o + d + 8, v + 8);
+              tmem_ld_16x256b_x4(tm_s + 32 * c, v);
+              float2 ks[4];
+#pragma unroll
+              for (int n = 0; n < 4; ++n) ks[n] = lds64(scales + 128 * c + 32 * n + 8 * t);
+              tmem_ld_wait();
+              uint32_t seen[2];
+              if constexpr (hidden.value) {
+                seen[0] = seen_of(c, 0);
+                seen[1] = seen_of(c, 1);
+              }
+#pragma unroll
+              for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  float2 y = mul2(f2_of(v[4 * n + 2 * h], v[4 * n + 2 * h + 1]), ks[n]);
+                  if constexpr (hidden.value) hide(y, seen[h] >> (8 * n));
+                  top[h] = fmax3(top[h], y.x, y.y);
+                }
+            }
+          };
+          if (masked)
+            largest(std::true_type());
+          else
+            largest(std::false_type());
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) reach = fmaxf(reach, __shfl_xor_sync(0xffffffffu, reach, o));
+          const float reach_log = fmaxf(lg2_approx(reach), kScaleLogMin);
+          // A weight times its value scale is at most 2^(top + reach_log - unit).
+          bool renew = false;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) renew |= fmaf(top[h], factor[h], reach_log - unit[h]) > kWideSlack;
+          if (__any_sync(0xffffffffu, renew)) {
+            // The largest logarithm of a weight times its value scale.
+            float most[2] = {-INFINITY, -INFINITY};
+            uint32_t v[16];
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              tmem_ld_16x256b_x4(tm_s + 32 * c, v);
               tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const float2 z = mul2(make_float2(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), k2);
-                v[2 * i] = __float_as_uint(z.x);
-                v[2 * i + 1] = __float_as_uint(z.y);
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t seen = masked ? seen_of(c, h) : ~0u;
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                  const float2 ks = lds64(scales + 128 * c + 32 * n + 8 * t);
+                  const float2 vs = lds64(scales + S::kKeys * 4 + 128 * c + 32 * n + 8 * t);
+                  const float zx = fmaf(__uint_as_float(v[4 * n + 2 * h]) * ks.x, factor[h],
+                                        fmaxf(lg2_approx(vs.x), kScaleLogMin));
+                  const float zy = fmaf(__uint_as_float(v[4 * n + 2 * h + 1]) * ks.y, factor[h],
+                                        fmaxf(lg2_approx(vs.y), kScaleLogMin));
+                  if ((seen >> (8 * n)) & 1u) most[h] = fmaxf(most[h], zx);
+                  if ((seen >> (8 * n + 1)) & 1u) most[h] = fmaxf(most[h], zy);
+                }
               }
-              tmem_st8(tm_o + d, v);
-              tmem_st8(tm_o + d + 8, v + 8);
+            }
+            float shrink[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 1));
+              most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 2));
+              shrink[h] = 1.0f;
+              if (most[h] > unit[h]) {
+                shrink[h] = ex2_approx(unit[h] - most[h]);
+                unit[h] = most[h];
+                l[h] *= shrink[h];
+              }
+            }
+            // The stream's last numerator MMAs are complete: the scores of
+            // this tile were committed after them.
+            if (!first_job) {
+#pragma unroll 1
+              for (int d = 0; d < D; d += 32) {
+                tmem_ld_16x256b_x4(tm_o + d, v);
+                tmem_ld_wait();
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e)
+                    v[4 * n + e] = __float_as_uint(__uint_as_float(v[4 * n + e]) * shrink[e / 2]);
+                tmem_st_16x256b_x4(tm_o + d, v);
+              }
             }
           }
+          // ---- second reading: the weights, over the spent scores (column
+          // c / 2: what it covers has been read)
+          float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+          auto weigh = [&](auto hidden) {
+#pragma unroll 1
+            for (int c = 0; c < 4; ++c) {
+              uint32_t v[16];
+              tmem_ld_16x256b_x4(tm_s + 32 * c, v);
+              float2 ks[4], vs[4];
+#pragma unroll
+              for (int n = 0; n < 4; ++n) {
+                ks[n] = lds64(scales + 128 * c + 32 * n + 8 * t);
+                vs[n] = lds64(scales + S::kKeys * 4 + 128 * c + 32 * n + 8 * t);
+              }
+              tmem_ld_wait();
+              uint32_t seen[2];
+              if constexpr (hidden.value) {
+                seen[0] = seen_of(c, 0);
+                seen[1] = seen_of(c, 1);
+              }
+              uint32_t p16[8];
+#pragma unroll
+              for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  float2 p = __ffma2_rn(mul2(f2_of(v[4 * n + 2 * h], v[4 * n + 2 * h + 1]), ks[n]),
+                                        make_float2(factor[h], factor[h]), make_float2(-unit[h], -unit[h]));
+                  if constexpr (hidden.value) hide(p, seen[h] >> (8 * n));
+                  p.x = ex2_approx(p.x);
+                  p.y = ex2_approx(p.y);
+                  sum[h] = __fadd2_rn(sum[h], p);
+                  p = mul2(p, vs[n]);
+                  uint32_t x16 = pack2(p.x, p.y, __half());
+                  if constexpr (hidden.value)  // an unseen key's value scale may be anything
+                    x16 &= ((seen[h] >> (8 * n)) & 1u ? 0xffffu : 0u) |
+                           ((seen[h] >> (8 * n + 1)) & 1u ? 0xffff0000u : 0u);
+                  p16[2 * n + h] = x16;
+                }
+              tmem_st_16x128b_x4(tm_s + 16 * c, p16);
+            }
+          };
+          if (masked)
+            weigh(std::true_type());
+          else
+            weigh(std::false_type());
+#pragma unroll
+          for (int h = 0; h < 2; ++h) l[h] += sum[h].x + sum[h].y;
+          tmem_st_wait();
         }
         first_job = false;
-        const float2 i2 = make_float2(inv, inv);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          uint32_t h[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float2 z = mul2(y[8 * i + e], i2);
-            h[e] = pack2(z.x, z.y, __half());
-          }
-          tmem_st8(tm_s + 8 * i, h);
-        }
-        tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&p_full[x]));
+        if (lane == 0) {
+          mbar_arrive(smem_u32(&scale_empty[entry]));
+          mbar_arrive(smem_u32(&p_full[x]));
+        }
       }
       counter += w.count;
       // ---- the segment's end
       const bool mine = kShared || x < w.count;  // this stream had a job
       if (mine) {
-        if (ok) ok = mbar_wait_sleep_warp(smem_u32(&o_done[x]), done & 1, budget, a.status, kStatusTimeoutMma,
+        if (ok) ok = mbar_wait_block_warp(smem_u32(&o_done[x]), done & 1, budget, a.status, kStatusTimeoutMma,
                                           abort_flag);
         ++done;
-        tc_fence_after();
       }
-      m *= factor;
-      float m1 = -INFINITY, l1 = 0.0f, unit1 = 0.0f;
-      if constexpr (!kShared) {
-        if (x == 1) {
-          state[r] = mine ? m : -INFINITY;
-          state[128 + r] = mine ? l : 0.0f;
-          state[256 + r] = mine ? unit : 0.0f;
-          tc_fence_before();
-        }
-        bar_sync(1, 256);
-        if (x == 0) {
-          tc_fence_after();
-          m1 = state[r];
-          l1 = state[128 + r];
-          unit1 = state[256 + r];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+        if (t == 0) {
+          totals[x * 128 + r16 + 8 * h] = l[h];
+          units[x * 128 + r16 + 8 * h] = unit[h] == kNoReference ? -INFINITY : unit[h];
         }
       }
-      if (kShared || x == 0) {
+      tc_fence_before();
+      bar_sync(bar_id, kBarThreads);
+      tc_fence_after();
+      {
+        // A thread writes its share of the head dimensions of one row.  The
+        // warps that reach the row's lane: two, or four with both streams'.
+        constexpr int kShare = D / (kShared ? 2 : 4);
+        const int share = kShared ? half : 2 * x + half;
+        const int s0 = kShared ? x : 0;  // the stream, or the first of two
         const bool two = !kShared && w.count > 1;
-        const float whole_m = fmaxf(m, m1);
+        const int r = lane0 + lane, row = row0 + r;
+        const float unit0 = units[s0 * 128 + r], unit1 = two ? units[128 + r] : -INFINITY;
+        const float whole_m = fmaxf(unit0, unit1);
         const float ref = whole_m == -INFINITY ? 0.0f : whole_m;
-        const float g0 = ex2_approx(m - ref), g1 = two ? ex2_approx(m1 - ref) : 0.0f;
-        const float whole_l = l * g0 + l1 * g1;
-        const float inv_l = whole_l == 0.0f ? 0.0f : 1.0f / whole_l;
-        const float f0 = unit * g0 * (w.all ? inv_l : 1.0f), f1 = unit1 * g1 * (w.all ? inv_l : 1.0f);
-        const int lr = (kShared ? x * 128 : 0) + r;  // row of the row tile
+        const float g0 = ex2_approx(unit0 - ref), g1 = two ? ex2_approx(unit1 - ref) : 0.0f;
+        const float whole_l = totals[s0 * 128 + r] * g0 + (two ? totals[128 + r] * g1 : 0.0f);
+        const float over_l = !w.all ? 1.0f : whole_l == 0.0f ? 0.0f : 1.0f / whole_l;
+        const float f0 = g0 * over_l, f1 = g1 * over_l;
+        const int lr = s0 * 128 + r;  // row of the row tile
+        const uint32_t from = tmem_base + (static_cast<uint32_t>(lane0) << 16) + 256 + s0 * 128;
         float* to = a.parts + (static_cast<int64_t>(blockIdx.x) * 2 + part) * S::kPart;
-        T* out = static_cast<T*>(a.out) +
-                 ((static_cast<int64_t>(w.b) * a.heads + kv * a.group + row / a.nodes) * a.nodes + row % a.nodes) * D;
-        if (!w.all && row < a.rows) {
+        if (!w.all && ok && share == 0 && row < a.rows) {
           to[S::kRows * D + 2 * lr] = whole_m;
           to[S::kRows * D + 2 * lr + 1] = whole_l;
         }
 #pragma unroll 1
-        for (int d = 0; d < D; d += 32) {
-          uint32_t v[32], u[32];
-          tmem_ld32(tm_o + d, v);
-          if (two) tmem_ld32(tm_o + 128 + d, u);
+        for (int d = share * kShare; d < (share + 1) * kShare; d += 16) {
+          uint32_t u0[16], u1[16];
+          tmem_ld8(from + d, u0);
+          tmem_ld8(from + d + 8, u0 + 8);
+          if (two) {
+            tmem_ld8(from + 128 + d, u1);
+            tmem_ld8(from + 128 + d + 8, u1 + 8);
+          }
           tmem_ld_wait();
-          float z[32];
+          float z[16];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            z[i] = __uint_as_float(v[i]) * f0;
-            if (two) z[i] += __uint_as_float(u[i]) * f1;
+          for (int i = 0; i < 16; ++i) {
+            z[i] = __uint_as_float(u0[i]) * f0;
+            if (two) z[i] += __uint_as_float(u1[i]) * f1;
           }
           if (!ok || row >= a.rows) continue;
           if (w.all) {
+            T* out = static_cast<T*>(a.out) + ((static_cast<int64_t>(w.b) * a.heads + kv * a.group + row / a.nodes) *
+                                                   a.nodes + row % a.nodes) * D + d;
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
+            for (int i = 0; i < 16; i += 8) {
               uint4 h;
               h.x = pack2(z[i], z[i + 1], T());
               h.y = pack2(z[i + 2], z[i + 3], T());
               h.z = pack2(z[i + 4], z[i + 5], T());
               h.w = pack2(z[i + 6], z[i + 7], T());
-              *reinterpret_cast<uint4*>(out + d + i) = h;
+              *reinterpret_cast<uint4*>(out + i) = h;
             }
           } else {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4)
+            for (int i = 0; i < 16; i += 4)
               *reinterpret_cast<float4*>(to + lr * D + d + i) = make_float4(z[i], z[i + 1], z[i + 2], z[i + 3]);
           }
         }
         tc_fence_before();
       }
-      if constexpr (!kShared) bar_sync(1, 256);
+      // The numerators have been read, before any warp hands over the next
+      // segment's first weights.
+      if constexpr (!kShared) bar_sync(bar_id, kBarThreads);
       part = 1;
       wide_next<S::kKeys>(a, per, w);
     }
-  } else if (warp < 12) {
+  } else if (warp < 20) {
     // --------------------------------------------------------- conversion
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWideRegsConvert));
     const int r = tid % 128;
     bool ok = true;
     uint32_t uses[2] = {0, 0};
@@ -502,18 +573,20 @@ __global__ void __launch_bounds__(kWideThreads, 1)
 #pragma unroll 1
         for (int side = 0; ok && side < 2; ++side, ++op) {
           const int slot = static_cast<int>(op % kRing);
-          ok = mbar_wait_warp(smem_u32(&ring_full[slot]), static_cast<uint32_t>(op / kRing) & 1, budget, a.status,
+          ok = mbar_wait_block_warp(smem_u32(&ring_full[slot]), static_cast<uint32_t>(op / kRing) & 1, budget, a.status,
                               kStatusTimeoutFull, abort_flag) &&
-               mbar_wait_sleep_warp(smem_u32(side == 0 ? &k_empty[buffer] : &v_empty[buffer]), (use & 1) ^ 1, budget,
+               mbar_wait_block_warp(smem_u32(side == 0 ? &k_empty[buffer] : &v_empty[buffer]), (use & 1) ^ 1, budget,
                                     a.status, kStatusTimeoutMma, abort_flag);
           if (!ok) break;
           const uint32_t from = sbase + S::kOffRing + slot * S::kCodes;
           uint8_t* to = smem + (side == 0 ? S::kOffK : S::kOffV) + buffer * S::kHalf + r * 128;
+          float4 raw[D / 16];
+#pragma unroll
+          for (int c = 0; c < D / 16; ++c) raw[c] = lds128(tile_chunk<D>(from, r, c));
 #pragma unroll
           for (int c = 0; c < D / 16; ++c) {
-            const float4 raw = lds128(tile_chunk<D>(from, r, c));
-            const uint32_t code[4] = {__float_as_uint(raw.x) ^ 0x80808080u, __float_as_uint(raw.y) ^ 0x80808080u,
-                                      __float_as_uint(raw.z) ^ 0x80808080u, __float_as_uint(raw.w) ^ 0x80808080u};
+            const uint32_t code[4] = {__float_as_uint(raw[c].x) ^ 0x80808080u, __float_as_uint(raw[c].y) ^ 0x80808080u,
+                                      __float_as_uint(raw[c].z) ^ 0x80808080u, __float_as_uint(raw[c].w) ^ 0x80808080u};
             uint32_t h[8];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -536,8 +609,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       wide_next<S::kKeys>(a, per, w);
     }
   } else {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWideRegsControl));
-    if (warp == 12) {
+    if (warp == 20) {
       // ----------------------------------------------- fetching, a box a lane
       bool ok = true;
       int64_t op = 0, counter = 0;
@@ -562,7 +634,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
           const int y = static_cast<int>(position & (a.c.page_size - 1));
           const int64_t at = (static_cast<int64_t>(z) << a.page_shift) + y;
           const int ring = static_cast<int>(counter % S::kScaleRing);
-          ok = mbar_wait_sleep_warp(smem_u32(&scale_empty[ring]),
+          ok = mbar_wait_block_warp(smem_u32(&scale_empty[ring]),
                                     (static_cast<uint32_t>(counter / S::kScaleRing) & 1) ^ 1, budget, a.status,
                                     kStatusTimeoutEmpty, abort_flag);
           if (!ok) break;
@@ -572,7 +644,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
           }
           __syncwarp();
           if (good) {
-            const uint32_t to = sbase + S::kOffScales + ring * S::kKeys * 8 + lane * box * 4;
+            const uint32_t to = sbase + S::kOffScales + ring * S::kEntry + lane * box * 4;
             bulk_load(to, a.c.key_scales + at, box * 4, smem_u32(&scale_full[ring]));
             bulk_load(to + S::kKeys * 4, a.c.value_scales + at, box * 4, smem_u32(&scale_full[ring]));
           }
@@ -580,7 +652,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
           for (int side = 0; ok && side < 2; ++side, ++op) {
             const int slot = static_cast<int>(op % kRing);
             const uint32_t bar = smem_u32(&ring_full[slot]);
-            ok = mbar_wait_sleep_warp(smem_u32(&ring_empty[slot]), (static_cast<uint32_t>(op / kRing) & 1) ^ 1, budget,
+            ok = mbar_wait_block_warp(smem_u32(&ring_empty[slot]), (static_cast<uint32_t>(op / kRing) & 1) ^ 1, budget,
                                       a.status, kStatusTimeoutEmpty, abort_flag);
             if (!ok) break;
             if (lane == 0) mbar_arrive_expect_tx(bar, __popc(goods) * box * D);
@@ -594,13 +666,13 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       }
       // Every copy has landed before the CTA's shared memory goes.
       for (int64_t i = max(int64_t(0), op - kRing); i < op; ++i)
-        mbar_wait_warp(smem_u32(&ring_full[i % kRing]), static_cast<uint32_t>(i / kRing) & 1, budget, a.status,
+        mbar_wait_block_warp(smem_u32(&ring_full[i % kRing]), static_cast<uint32_t>(i / kRing) & 1, budget, a.status,
                        kStatusTimeoutDrain, 0u);
       if (!ok)
         for (int64_t i = max(int64_t(0), counter - S::kScaleRing); i < counter; ++i)
-          mbar_wait_warp(smem_u32(&scale_full[i % S::kScaleRing]), static_cast<uint32_t>(i / S::kScaleRing) & 1, budget,
+          mbar_wait_block_warp(smem_u32(&scale_full[i % S::kScaleRing]), static_cast<uint32_t>(i / S::kScaleRing) & 1, budget,
                          a.status, kStatusTimeoutDrain, 0u);
-    } else if (warp == 13 && lane == 0) {
+    } else if (warp == 21 && lane == 0) {
       // -------------------------------------------------------- MMA issue
       constexpr uint32_t kIdescQK = umma_idesc_f16(128, S::kKeys);
       constexpr uint32_t kIdescPV = umma_idesc_f16(128, D) | (1u << 16);  // B with N contiguous
@@ -616,7 +688,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         const int x = job & 1;
         const int buffer = kShared ? 0 : x;
         if (!kShared || x == 0) {
-          ok = mbar_wait(smem_u32(&k_full[buffer]), k_use[buffer] & 1, budget, a.status, kStatusTimeoutFull,
+          ok = mbar_wait_block(smem_u32(&k_full[buffer]), k_use[buffer] & 1, budget, a.status, kStatusTimeoutFull,
                          abort_flag);
           ++k_use[buffer];
           if (!ok) return;
@@ -635,7 +707,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       while (w.left > 0 && ok) {
         const int jobs = kShared ? 2 * w.count : w.count;
         for (int x = 0; ok && x < (kShared ? 2 : 1); ++x)
-          ok = mbar_wait(smem_u32(&q_full[x]), segment & 1, budget, a.status, kStatusTimeoutFull, abort_flag);
+          ok = mbar_wait_block(smem_u32(&q_full[x]), segment & 1, budget, a.status, kStatusTimeoutFull, abort_flag);
         ++segment;
         if (!ok) break;
         tc_fence_after();
@@ -644,12 +716,12 @@ __global__ void __launch_bounds__(kWideThreads, 1)
           const int x = job & 1;
           const int buffer = kShared ? 0 : x;
           if (!kShared || x == 0) {
-            ok = mbar_wait(smem_u32(&v_full[buffer]), v_use[buffer] & 1, budget, a.status, kStatusTimeoutFull,
+            ok = mbar_wait_block(smem_u32(&v_full[buffer]), v_use[buffer] & 1, budget, a.status, kStatusTimeoutFull,
                            abort_flag);
             ++v_use[buffer];
             if (!ok) break;
           }
-          ok = mbar_wait(smem_u32(&p_full[x]), p_use[x] & 1, budget, a.status, kStatusTimeoutFull, abort_flag);
+          ok = mbar_wait_block(smem_u32(&p_full[x]), p_use[x] & 1, budget, a.status, kStatusTimeoutFull, abort_flag);
           ++p_use[x];
           if (!ok) break;
           tc_fence_after();
@@ -674,7 +746,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (warp == 14) {
+  if (warp == 22) {
     tc_fence_after();
     tmem_dealloc(tmem_base, 512);
   }
