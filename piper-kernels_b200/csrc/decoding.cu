@@ -200,7 +200,7 @@ int launch_tree(piper::TreeArgs a, Kernel kernel, int threads, int sms, size_t w
   attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attribute.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(static_cast<unsigned>(plan.grid - 1), S::kRows / 4);
+  config.gridDim = dim3(static_cast<unsigned>(plan.grid - 1), (std::min(a.rows, S::kRows) + 3) / 4);
   config.blockDim = dim3(128);
   config.stream = stream;
   config.attrs = &attribute;

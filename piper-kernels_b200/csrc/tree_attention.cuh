@@ -723,10 +723,11 @@ __global__ void __launch_bounds__(TreeTile<D, MT, WARPS>::kThreads, TreeTile<D, 
 // Joins the parts of every (request, head, row tile) that a boundary between
 // two runs cuts.  CTA x looks at the boundary before run x + 1 and works if it
 // is the first inside its row tile; a warp takes a row, and CTAs y share the
-// rows.
+// rows.  A lane holds the maximum and total of one of 32 parts, so that the
+// numerators' loads do not wait for one another.
 template <typename T, int D, typename S>
 __global__ void __launch_bounds__(128) tree_merge_kernel(TreeArgs a, int grid) {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // (The lengths were there before the attention kernel began.)
   const int64_t units = tree_units<S::kKeys>(a);
   const int64_t ctas = tree_ctas(units, grid);
   const int64_t i = blockIdx.x + 1;
@@ -737,32 +738,66 @@ __global__ void __launch_bounds__(128) tree_merge_kernel(TreeArgs a, int grid) {
   tree_find<S::kKeys>(a, at, &b, &tiles, &first);
   const int hr = static_cast<int>((at - first) / tiles);
   const int64_t begin = first + static_cast<int64_t>(hr) * tiles;
-  if (at == begin || tree_bound(units, ctas, i - 1) > begin) return;
-  const int r = blockIdx.y * 4 + threadIdx.x / 32;
-  const int row = (hr % a.row_tiles) * S::kRows + r;
-  if (row >= a.rows) return;
+  const int64_t before = tree_bound(units, ctas, i - 1);
+  if (at == begin || before > begin) return;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // Runs i - 1 to `last` have parts of the row tile: `last` holds its last unit.
+  int64_t last = ((begin + tiles - 1) * ctas) / units;
+  while (last + 1 < ctas && tree_bound(units, ctas, last + 1) < begin + tiles) ++last;
+  while (tree_bound(units, ctas, last) >= begin + tiles) --last;
+  const int count = static_cast<int>(last - (i - 1) + 1);
   const int lane = threadIdx.x % 32;
+  const int kv = hr / a.row_tiles, row0 = (hr % a.row_tiles) * S::kRows;
   constexpr int kPer = D / 32;
-  float m = -INFINITY, l = 0.0f, o[kPer] = {};
-  for (int64_t c = i - 1; c < ctas && tree_bound(units, ctas, c) < begin + tiles; ++c) {
-    // The row tile is run c's second part unless the run starts in it.
-    const float* part = a.parts + (c * 2 + (tree_bound(units, ctas, c) < begin ? 1 : 0)) * S::kPart;
-    const float pm = part[S::kRows * D + 2 * r], pl = part[S::kRows * D + 2 * r + 1];
-    const float top = fmaxf(m, pm);
-    const float ref = top == -INFINITY ? 0.0f : top;
-    const float f = ex2_approx(m - ref), pf = ex2_approx(pm - ref);
-    m = top;
-    l = l * f + pl * pf;
+  // Part k is run i - 1 + k's first one if the run starts inside the row tile
+  // or at its start.
+  auto part_of = [&](int k) {
+    return a.parts + ((i - 1 + k) * 2 + (k == 0 && before < begin ? 1 : 0)) * S::kPart;
+  };
+  for (int r = blockIdx.y * 4 + threadIdx.x / 32; r < S::kRows && row0 + r < a.rows; r += 4 * gridDim.y) {
+    float m = -INFINITY, l = 0.0f, o[kPer] = {};
+    for (int k0 = 0; k0 < count; k0 += 32) {
+      float pm = -INFINITY, pl = 0.0f;
+      if (k0 + lane < count) {
+        const float2 ml = *reinterpret_cast<const float2*>(part_of(k0 + lane) + S::kRows * D + 2 * r);
+        pm = ml.x;
+        pl = ml.y;
+      }
+      float top = pm;
 #pragma unroll
-    for (int x = 0; x < kPer; ++x) o[x] = o[x] * f + part[r * D + lane * kPer + x] * pf;
+      for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+      top = fmaxf(top, m);
+      const float ref = top == -INFINITY ? 0.0f : top;
+      const float pf = ex2_approx(pm - ref), f = ex2_approx(m - ref);
+      float sum = pl * pf;
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+      m = top;
+      l = l * f + sum;
+#pragma unroll
+      for (int x = 0; x < kPer; ++x) o[x] *= f;
+      const int n = min(32, count - k0);
+#pragma unroll 8
+      for (int k = 0; k < n; ++k) {
+        const float g = __shfl_sync(0xffffffffu, pf, k);
+        const float* from = part_of(k0 + k) + r * D + lane * kPer;
+        float v[kPer];
+        if constexpr (kPer == 4)
+          *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(from);
+        else
+          *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(from);
+#pragma unroll
+        for (int x = 0; x < kPer; ++x) o[x] = fmaf(v[x], g, o[x]);
+      }
+    }
+    const int row = row0 + r;
+    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+    T* out = static_cast<T*>(a.out) +
+             ((static_cast<int64_t>(b) * a.heads + kv * a.group + row / a.nodes) * a.nodes + row % a.nodes) * D;
+#pragma unroll
+    for (int x = 0; x < kPer; x += 2)
+      *reinterpret_cast<uint32_t*>(out + lane * kPer + x) = pack2(o[x] * f, o[x + 1] * f, T());
   }
-  const int kv = hr / a.row_tiles;
-  const float f = l == 0.0f ? 0.0f : 1.0f / l;
-  T* out = static_cast<T*>(a.out) +
-           ((static_cast<int64_t>(b) * a.heads + kv * a.group + row / a.nodes) * a.nodes + row % a.nodes) * D;
-#pragma unroll
-  for (int x = 0; x < kPer; x += 2)
-    *reinterpret_cast<uint32_t*>(out + lane * kPer + x) = pack2(o[x] * f, o[x + 1] * f, T());
 }
 
 }  // namespace piper

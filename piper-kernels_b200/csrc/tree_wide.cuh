@@ -23,7 +23,7 @@
 // could outgrow it.
 //
 // Warps: 0-7 and 8-15 softmax of streams 0 and 1 (two for each 32 TMEM lanes),
-// 16-19 conversion (a thread owns a key), 20 fetches, 21 issues MMAs, 22 owns
+// 16-17 conversion of K, 18-19 of V, 20 fetches, 21 issues MMAs, 22 owns
 // TMEM.
 #pragma once
 
@@ -114,57 +114,72 @@ __device__ __forceinline__ float lg2_approx(float x) {
 
 __device__ __forceinline__ float2 mul2(float2 x, float2 y) { return __fmul2_rn(x, y); }
 
-// Query row `row` into shared memory at lane row r (K-major, SW128, blocks of
-// 64 head dimensions), scaled to fp16; returns what undoes that, times the
-// softmax scale.
+// Sixteen query rows, from row r0 of the stream (row `row0` of the KV head),
+// into shared memory (K-major, SW128, blocks of 64 head dimensions), scaled to
+// fp16, and what undoes that, times the softmax scale, into `factors`.  A warp
+// reads a row at a time, eight in flight.
 template <typename T, int D>
-__device__ __forceinline__ float wide_query_row(const TreeArgs& a, uint8_t* to, int b, int kv, int row, int r,
-                                                bool store) {
-  const bool there = row < a.rows;
-  const T* p = static_cast<const T*>(a.query) + b * a.qs[0];
-  if (there) p += (kv * a.group + row / a.nodes) * a.qs[1] + (row % a.nodes) * a.qs[2];
-  // Read twice (the second time from L1) to hold few registers.
-  auto eight = [&](int c, float (&x)[8]) {
-    uint4 raw = make_uint4(0u, 0u, 0u, 0u);
-    if (there) {
-      if (a.vec) {
-        const uint2 lo = __ldg(reinterpret_cast<const uint2*>(p) + 2 * c);
-        const uint2 hi = __ldg(reinterpret_cast<const uint2*>(p) + 2 * c + 1);
-        raw = make_uint4(lo.x, lo.y, hi.x, hi.y);
-      } else {
-        raw = load_raw8<T, false>(p + c * 8);
+__device__ __forceinline__ void wide_query_rows(const TreeArgs& a, uint8_t* to, float* factors, int b, int kv, int row0,
+                                                int r0) {
+  constexpr int kPer = D / 32;  // elements a lane
+  const int lane = threadIdx.x % 32;
+  const int mine = row0 + r0 + (lane & 15);
+  int64_t at = -1;
+  if (mine < a.rows)
+    at = b * a.qs[0] + (kv * a.group + mine / a.nodes) * a.qs[1] + (mine % a.nodes) * a.qs[2];
+  const uint16_t* base = static_cast<const uint16_t*>(a.query) + lane * kPer;
+#pragma unroll 1
+  for (int k0 = 0; k0 < 16; k0 += 8) {
+    uint32_t raw[8][kPer / 2];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int64_t row_at = __shfl_sync(0xffffffffu, at, k0 + k);
+#pragma unroll
+      for (int i = 0; i < kPer / 2; ++i) raw[k][i] = 0u;
+      if (row_at >= 0) {
+        const uint16_t* p = base + row_at;
+        if (a.vec) {
+          if constexpr (kPer == 4) {
+            const uint2 w = __ldg(reinterpret_cast<const uint2*>(p));
+            raw[k][0] = w.x;
+            raw[k][1] = w.y;
+          } else {
+            raw[k][0] = __ldg(reinterpret_cast<const uint32_t*>(p));
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < kPer / 2; ++i)
+            raw[k][i] = static_cast<uint32_t>(p[2 * i]) | (static_cast<uint32_t>(p[2 * i + 1]) << 16);
+        }
       }
     }
-    unpack8<T>(raw, x);
-  };
-  float up = 1.0f, factor = a.scale_log2e;
-  if constexpr (!std::is_same<T, __half>::value) {
-    uint32_t top = 0u;
-#pragma unroll 2
-    for (int c = 0; c < D / 8; ++c) {
-      float x[8];
-      eight(c, x);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+    for (int k = 0; k < 8; ++k) {
+      const int r = r0 + k0 + k;
+      float x[kPer];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const uint16_t e = static_cast<uint16_t>(raw[k][i / 2] >> (16 * (i % 2)));
+        x[i] = to_f32<T>(*reinterpret_cast<const T*>(&e));
+      }
+      float up = 1.0f, factor = a.scale_log2e;
+      if constexpr (!std::is_same<T, __half>::value) {
+        uint32_t top = 0u;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+        top = __reduce_max_sync(0xffffffffu, top);
+        const uint32_t e = max(1u, min(253u, top >> 23));
+        up = __uint_as_float((254u - e) << 23);
+        factor = __uint_as_float(e << 23) * a.scale_log2e;
+      }
+      if (lane == 0) factors[r] = factor;
+      const int chunk = lane * kPer / 8;
+      uint8_t* p = to + (chunk / 8) * 16384 + r * 128 + (((chunk & 7) ^ (r & 7)) << 4) + (lane * kPer % 8) * 2;
+#pragma unroll
+      for (int i = 0; i < kPer / 2; ++i)
+        reinterpret_cast<uint32_t*>(p)[i] = pack2(x[2 * i] * up, x[2 * i + 1] * up, __half());
     }
-    const uint32_t e = max(1u, min(253u, top >> 23));
-    up = __uint_as_float((254u - e) << 23);
-    factor = __uint_as_float(e << 23) * a.scale_log2e;
   }
-  if (store) {
-#pragma unroll 2
-    for (int c = 0; c < D / 8; ++c) {
-      float x[8];
-      eight(c, x);
-      uint4 w;
-      w.x = pack2(x[0] * up, x[1] * up, __half());
-      w.y = pack2(x[2] * up, x[3] * up, __half());
-      w.z = pack2(x[4] * up, x[5] * up, __half());
-      w.w = pack2(x[6] * up, x[7] * up, __half());
-      *reinterpret_cast<uint4*>(to + (c / 8) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = w;
-    }
-  }
-  return factor;
 }
 
 // Which of keys 32 c .. 32 c + 31 of a tile a row sees: the first `open` of the
@@ -212,21 +227,21 @@ __global__ void __launch_bounds__(kWideThreads, 1)
   if (tid == 0) {
     for (int i = 0; i < kRing; ++i) {
       mbar_init(smem_u32(&ring_full[i]), 1);
-      mbar_init(smem_u32(&ring_empty[i]), 4);
+      mbar_init(smem_u32(&ring_empty[i]), 2);
     }
     for (int i = 0; i < S::kScaleRing; ++i) {
       mbar_init(smem_u32(&scale_full[i]), 1);
       mbar_init(smem_u32(&scale_empty[i]), kShared ? 16 : 8);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_u32(&k_full[i]), 4);
+      mbar_init(smem_u32(&k_full[i]), 2);
       mbar_init(smem_u32(&k_empty[i]), 1);
-      mbar_init(smem_u32(&v_full[i]), 4);
+      mbar_init(smem_u32(&v_full[i]), 2);
       mbar_init(smem_u32(&v_empty[i]), 1);
       mbar_init(smem_u32(&s_full[i]), 1);
       mbar_init(smem_u32(&p_full[i]), 8);
       mbar_init(smem_u32(&o_done[i]), 1);
-      mbar_init(smem_u32(&q_full[i]), 4);
+      mbar_init(smem_u32(&q_full[i]), 8);
     }
     mbar_init(smem_u32(&mma_done), 1);
     abort_word = 0u;
@@ -262,6 +277,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     float* units = totals + 256;
     float* factors = units + 256;
     uint64_t* words = reinterpret_cast<uint64_t*>(factors + 256);  // visible nodes
+    const int own = kShared ? x * 128 : 0;  // of factors and words: alternate streams share their rows
     const int bar_id = kShared ? 1 + x : 1;
     constexpr int kBarThreads = kShared ? 256 : 512;
     bool ok = true;
@@ -273,24 +289,24 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       const int kv = w.hr / a.row_tiles;
       const int row0 = (w.hr % a.row_tiles) * S::kRows + (kShared ? x * 128 : 0);
       const int64_t length = max(0, __ldg(a.c.lengths + w.b));
-      if (half == 0) {
-        const int r = lane0 + lane, row = row0 + r;
-        uint64_t word = 0;
-        if (row < a.rows) {
-          const int node = row % a.nodes;
-          word = a.mask != nullptr ? static_cast<uint64_t>(__ldg(reinterpret_cast<const unsigned long long*>(
-                                         a.mask + w.b * a.mask_stride + node)))
-                                   : ~0ull >> (63 - node);
-          word &= ~0ull >> (64 - a.nodes);
+      if (kShared || x == 0) {
+        if (half == 0) {
+          const int row = row0 + lane0 + lane;
+          uint64_t word = 0;
+          if (row < a.rows) {
+            const int node = row % a.nodes;
+            word = a.mask != nullptr ? static_cast<uint64_t>(__ldg(reinterpret_cast<const unsigned long long*>(
+                                           a.mask + w.b * a.mask_stride + node)))
+                                     : ~0ull >> (63 - node);
+            word &= ~0ull >> (64 - a.nodes);
+          }
+          words[own + lane0 + lane] = word;
         }
-        words[x * 128 + r] = word;
-        factors[x * 128 + r] = wide_query_row<T, D>(a, smem + S::kOffQuery + (kShared ? x * S::kHalf : 0), w.b, kv,
-                                                    row, r, kShared || x == 0);
-        if (kShared || x == 0) {
-          fence_proxy_async_shared();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(smem_u32(&q_full[kShared ? x : 0]));
-        }
+        wide_query_rows<T, D>(a, smem + S::kOffQuery + (kShared ? x * S::kHalf : 0), factors + own, w.b, kv, row0,
+                              (warp % 8) * 16);
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&q_full[kShared ? x : 0]));
       }
       bar_sync(bar_id, kBarThreads);
       // A row's reference `unit`: the logarithm of the numerators' unit, and of
@@ -298,7 +314,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       float factor[2], unit[2], l[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        factor[h] = factors[x * 128 + r16 + 8 * h];
+        factor[h] = factors[own + r16 + 8 * h];
         unit[h] = kNoReference;
         l[h] = 0.0f;
       }
@@ -323,7 +339,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
           const int open = static_cast<int>(max(min(length - first, int64_t(256)), int64_t(-256)));
           // Bit 8 n + e: column 32 c + 8 n + 2 t + e of row h is seen.
           auto seen_of = [&](int c, int h) {
-            return wide_seen(goods, box_shift, open, words[x * 128 + r16 + 8 * h], c) >> (2 * t);
+            return wide_seen(goods, box_shift, open, words[own + r16 + 8 * h], c) >> (2 * t);
           };
           // ---- first reading: the largest scores and value scale
           float top[2] = {-INFINITY, -INFINITY};
@@ -562,27 +578,30 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     }
   } else if (warp < 20) {
     // --------------------------------------------------------- conversion
-    const int r = tid % 128;
+    // Two warps turn K tiles, two V tiles: a V tile waits for the numerators
+    // before it, which must not hold up the next K tile.
+    const int side = (warp - 16) / 2;
+    const int r = tid % 64;
     bool ok = true;
     uint32_t uses[2] = {0, 0};
-    int64_t op = 0;
+    uint32_t op = side;
     while (w.left > 0) {
-      for (int j = 0; ok && j < w.count; ++j) {
+      for (int j = 0; ok && j < w.count; ++j, op += 2) {
         const int buffer = kShared ? 0 : (j & 1);
         const uint32_t use = uses[buffer]++;
+        const uint32_t slot = op % kRing;
+        ok = mbar_wait_block_warp(smem_u32(&ring_full[slot]), (op / kRing) & 1, budget, a.status, kStatusTimeoutFull,
+                                  abort_flag) &&
+             mbar_wait_block_warp(smem_u32(side == 0 ? &k_empty[buffer] : &v_empty[buffer]), (use & 1) ^ 1, budget,
+                                  a.status, kStatusTimeoutMma, abort_flag);
+        if (!ok) break;
+        const uint32_t from = sbase + S::kOffRing + slot * S::kCodes;
+        uint8_t* to = smem + (side == 0 ? S::kOffK : S::kOffV) + buffer * S::kHalf;
 #pragma unroll 1
-        for (int side = 0; ok && side < 2; ++side, ++op) {
-          const int slot = static_cast<int>(op % kRing);
-          ok = mbar_wait_block_warp(smem_u32(&ring_full[slot]), static_cast<uint32_t>(op / kRing) & 1, budget, a.status,
-                              kStatusTimeoutFull, abort_flag) &&
-               mbar_wait_block_warp(smem_u32(side == 0 ? &k_empty[buffer] : &v_empty[buffer]), (use & 1) ^ 1, budget,
-                                    a.status, kStatusTimeoutMma, abort_flag);
-          if (!ok) break;
-          const uint32_t from = sbase + S::kOffRing + slot * S::kCodes;
-          uint8_t* to = smem + (side == 0 ? S::kOffK : S::kOffV) + buffer * S::kHalf + r * 128;
+        for (int row = r; row < S::kKeys; row += 64) {
           float4 raw[D / 16];
 #pragma unroll
-          for (int c = 0; c < D / 16; ++c) raw[c] = lds128(tile_chunk<D>(from, r, c));
+          for (int c = 0; c < D / 16; ++c) raw[c] = lds128(tile_chunk<D>(from, row, c));
 #pragma unroll
           for (int c = 0; c < D / 16; ++c) {
             const uint32_t code[4] = {__float_as_uint(raw[c].x) ^ 0x80808080u, __float_as_uint(raw[c].y) ^ 0x80808080u,
@@ -593,17 +612,17 @@ __global__ void __launch_bounds__(kWideThreads, 1)
               h[2 * i] = codes_f16<0x4140>(code[i]);
               h[2 * i + 1] = codes_f16<0x4342>(code[i]);
             }
-            uint8_t* block = to + (c / 4) * 16384;
-            *reinterpret_cast<uint4*>(block + ((((c & 3) * 2) ^ (r & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
-            *reinterpret_cast<uint4*>(block + ((((c & 3) * 2 + 1) ^ (r & 7)) << 4)) =
+            uint8_t* block = to + row * 128 + (c / 4) * 16384;
+            *reinterpret_cast<uint4*>(block + ((((c & 3) * 2) ^ (row & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<uint4*>(block + ((((c & 3) * 2 + 1) ^ (row & 7)) << 4)) =
                 make_uint4(h[4], h[5], h[6], h[7]);
           }
-          fence_proxy_async_shared();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(smem_u32(&ring_empty[slot]));
-            mbar_arrive(smem_u32(side == 0 ? &k_full[buffer] : &v_full[buffer]));
-          }
+        }
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(smem_u32(&ring_empty[slot]));
+          mbar_arrive(smem_u32(side == 0 ? &k_full[buffer] : &v_full[buffer]));
         }
       }
       wide_next<S::kKeys>(a, per, w);
