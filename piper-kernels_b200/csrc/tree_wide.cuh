@@ -31,7 +31,7 @@
 
 namespace piper {
 
-constexpr int kWideThreads = 768;
+constexpr int kWideThreads = 736;
 constexpr float kWideSlack = 14.0f;      // log2 by which a weight may exceed 1: fp16 holds 2^15
 constexpr float kScaleLogMin = -90.0f;   // smaller value scales count as 2^-90 in the references
 template <int D, bool kShared>
@@ -42,13 +42,13 @@ struct WideTile {
   static constexpr int kCodes = kKeys * D;          // one ring slot: K or V codes
   static constexpr int kHalf = kKeys * D * 2;       // one fp16 operand tile
   static constexpr int kQuery = (kShared ? 2 : 1) * kHalf;
-  static constexpr int kBuffers = kShared ? 1 : 2;  // fp16 K and V tiles
+  static constexpr int kBuffers = kShared ? 1 : 2;  // fp16 K tiles (one V tile: a V tile is needed later)
   static constexpr int kScaleRing = 4;
   static constexpr int kEntry = kKeys * 8;          // scales of keys and of values
   static constexpr int kOffQuery = 0;
   static constexpr int kOffK = kOffQuery + kQuery;
   static constexpr int kOffV = kOffK + kBuffers * kHalf;
-  static constexpr int kOffScales = kOffV + kBuffers * kHalf;
+  static constexpr int kOffScales = kOffV + kHalf;
   static constexpr int kOffState = kOffScales + kScaleRing * kEntry;
   static constexpr int kOffRing = (kOffState + 256 * (3 * 4 + 8) + 1023) / 1024 * 1024;
   static constexpr int kFit = (225 * 1024 - kOffRing) / kCodes;
@@ -218,7 +218,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t sbase = smem_u32(smem);
   __shared__ __align__(8) uint64_t ring_full[kRing], ring_empty[kRing], scale_full[S::kScaleRing],
-      scale_empty[S::kScaleRing], k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_full[2], o_done[2],
+      scale_empty[S::kScaleRing], k_full[2], k_empty[2], v_full, v_empty, s_full[2], p_full[2], o_done[2],
       q_full[2], mma_done;
   __shared__ uint32_t valid[S::kScaleRing];
   __shared__ uint32_t abort_word, tmem_slot;
@@ -236,13 +236,13 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&k_full[i]), 2);
       mbar_init(smem_u32(&k_empty[i]), 1);
-      mbar_init(smem_u32(&v_full[i]), 2);
-      mbar_init(smem_u32(&v_empty[i]), 1);
       mbar_init(smem_u32(&s_full[i]), 1);
       mbar_init(smem_u32(&p_full[i]), 8);
       mbar_init(smem_u32(&o_done[i]), 1);
       mbar_init(smem_u32(&q_full[i]), 8);
     }
+    mbar_init(smem_u32(&v_full), 2);
+    mbar_init(smem_u32(&v_empty), 1);
     mbar_init(smem_u32(&mma_done), 1);
     abort_word = 0u;
     fence_mbarrier_init();
@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
           // ---- first reading: the largest scores and value scale
           float top[2] = {-INFINITY, -INFINITY};
           const float4 four = lds128(scales + S::kKeys * 4 + 16 * lane);
-          float reach = fmaxf(fmaxf(four.x, four.y), fmaxf(four.z, four.w));
+          float reach = fmaxf(fmaxf(fmaxf(four.x, four.y), fmaxf(four.z, four.w)), 0.0f);  // (NaN: 0)
           // (A masked tile has a body of its own: branches inside would cut
           // the other's instructions into short chains.)
           auto largest = [&](auto hidden) {
@@ -356,27 +356,30 @@ __global__ void __launch_bounds__(kWideThreads, 1)
 #pragma unroll
               for (int n = 0; n < 4; ++n) ks[n] = lds64(scales + 128 * c + 32 * n + 8 * t);
               tmem_ld_wait();
-              uint32_t seen[2];
-              if constexpr (hidden.value) {
-                seen[0] = seen_of(c, 0);
-                seen[1] = seen_of(c, 1);
-              }
 #pragma unroll
-              for (int n = 0; n < 4; ++n)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                  float2 y = mul2(f2_of(v[4 * n + 2 * h], v[4 * n + 2 * h + 1]), ks[n]);
-                  if constexpr (hidden.value) hide(y, seen[h] >> (8 * n));
-                  top[h] = fmax3(top[h], y.x, y.y);
+              for (int k = 0; k < 1; ++k) {
+                uint32_t seen[2];
+                if constexpr (hidden.value) {
+                  seen[0] = seen_of(c + k, 0);
+                  seen[1] = seen_of(c + k, 1);
                 }
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+#pragma unroll
+                  for (int h = 0; h < 2; ++h) {
+                    float2 y = mul2(f2_of(v[16 * k + 4 * n + 2 * h], v[16 * k + 4 * n + 2 * h + 1]), ks[4 * k + n]);
+                    if constexpr (hidden.value) hide(y, seen[h] >> (8 * n));
+                    top[h] = fmax3(top[h], y.x, y.y);
+                  }
+              }
             }
           };
           if (masked)
             largest(std::true_type());
           else
             largest(std::false_type());
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) reach = fmaxf(reach, __shfl_xor_sync(0xffffffffu, reach, o));
+          // (Floats that are not negative order as their bits.)
+          reach = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(reach)));
           const float reach_log = fmaxf(lg2_approx(reach), kScaleLogMin);
           // A weight times its value scale is at most 2^(top + reach_log - unit).
           bool renew = false;
@@ -440,39 +443,41 @@ __global__ void __launch_bounds__(kWideThreads, 1)
           auto weigh = [&](auto hidden) {
 #pragma unroll 1
             for (int c = 0; c < 4; ++c) {
-              uint32_t v[16];
-              tmem_ld_16x256b_x4(tm_s + 32 * c, v);
-              float2 ks[4], vs[4];
+              {
+                uint32_t v[16];
+                tmem_ld_16x256b_x4(tm_s + 32 * c, v);
+                float2 ks[4], vs[4];
 #pragma unroll
-              for (int n = 0; n < 4; ++n) {
-                ks[n] = lds64(scales + 128 * c + 32 * n + 8 * t);
-                vs[n] = lds64(scales + S::kKeys * 4 + 128 * c + 32 * n + 8 * t);
-              }
-              tmem_ld_wait();
-              uint32_t seen[2];
-              if constexpr (hidden.value) {
-                seen[0] = seen_of(c, 0);
-                seen[1] = seen_of(c, 1);
-              }
-              uint32_t p16[8];
-#pragma unroll
-              for (int n = 0; n < 4; ++n)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                  float2 p = __ffma2_rn(mul2(f2_of(v[4 * n + 2 * h], v[4 * n + 2 * h + 1]), ks[n]),
-                                        make_float2(factor[h], factor[h]), make_float2(-unit[h], -unit[h]));
-                  if constexpr (hidden.value) hide(p, seen[h] >> (8 * n));
-                  p.x = ex2_approx(p.x);
-                  p.y = ex2_approx(p.y);
-                  sum[h] = __fadd2_rn(sum[h], p);
-                  p = mul2(p, vs[n]);
-                  uint32_t x16 = pack2(p.x, p.y, __half());
-                  if constexpr (hidden.value)  // an unseen key's value scale may be anything
-                    x16 &= ((seen[h] >> (8 * n)) & 1u ? 0xffffu : 0u) |
-                           ((seen[h] >> (8 * n + 1)) & 1u ? 0xffff0000u : 0u);
-                  p16[2 * n + h] = x16;
+                for (int n = 0; n < 4; ++n) {
+                  ks[n] = lds64(scales + 128 * c + 32 * n + 8 * t);
+                  vs[n] = lds64(scales + S::kKeys * 4 + 128 * c + 32 * n + 8 * t);
                 }
-              tmem_st_16x128b_x4(tm_s + 16 * c, p16);
+                tmem_ld_wait();
+                uint32_t seen[2];
+                if constexpr (hidden.value) {
+                  seen[0] = seen_of(c, 0);
+                  seen[1] = seen_of(c, 1);
+                }
+                uint32_t p16[8];
+#pragma unroll
+                for (int n = 0; n < 4; ++n)
+#pragma unroll
+                  for (int h = 0; h < 2; ++h) {
+                    float2 p = __ffma2_rn(mul2(f2_of(v[4 * n + 2 * h], v[4 * n + 2 * h + 1]), ks[n]),
+                                          make_float2(factor[h], factor[h]), make_float2(-unit[h], -unit[h]));
+                    if constexpr (hidden.value) hide(p, seen[h] >> (8 * n));
+                    p.x = ex2_approx(p.x);
+                    p.y = ex2_approx(p.y);
+                    sum[h] = __fadd2_rn(sum[h], p);
+                    p = mul2(p, vs[n]);
+                    uint32_t x16 = pack2(p.x, p.y, __half());
+                    if constexpr (hidden.value)  // an unseen key's value scale may be anything
+                      x16 &= ((seen[h] >> (8 * n)) & 1u ? 0xffffu : 0u) |
+                             ((seen[h] >> (8 * n + 1)) & 1u ? 0xffff0000u : 0u);
+                    p16[2 * n + h] = x16;
+                  }
+                tmem_st_16x128b_x4(tm_s + 16 * c, p16);
+              }
             }
           };
           if (masked)
@@ -587,12 +592,12 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     uint32_t op = side;
     while (w.left > 0) {
       for (int j = 0; ok && j < w.count; ++j, op += 2) {
-        const int buffer = kShared ? 0 : (j & 1);
+        const int buffer = kShared || side == 1 ? 0 : (j & 1);
         const uint32_t use = uses[buffer]++;
         const uint32_t slot = op % kRing;
         ok = mbar_wait_block_warp(smem_u32(&ring_full[slot]), (op / kRing) & 1, budget, a.status, kStatusTimeoutFull,
                                   abort_flag) &&
-             mbar_wait_block_warp(smem_u32(side == 0 ? &k_empty[buffer] : &v_empty[buffer]), (use & 1) ^ 1, budget,
+             mbar_wait_block_warp(smem_u32(side == 0 ? &k_empty[buffer] : &v_empty), (use & 1) ^ 1, budget,
                                   a.status, kStatusTimeoutMma, abort_flag);
         if (!ok) break;
         const uint32_t from = sbase + S::kOffRing + slot * S::kCodes;
@@ -622,7 +627,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         __syncwarp();
         if (lane == 0) {
           mbar_arrive(smem_u32(&ring_empty[slot]));
-          mbar_arrive(smem_u32(side == 0 ? &k_full[buffer] : &v_full[buffer]));
+          mbar_arrive(smem_u32(side == 0 ? &k_full[buffer] : &v_full));
         }
       }
       wide_next<S::kKeys>(a, per, w);
@@ -699,7 +704,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       const uint64_t desc_k = umma_desc_kmajor(sbase + S::kOffK, 128);
       const uint64_t desc_v = umma_desc_nmajor(sbase + S::kOffV, 16384u);
       bool ok = true;
-      uint32_t k_use[2] = {0, 0}, v_use[2] = {0, 0}, p_use[2] = {0, 0};
+      uint32_t k_use[2] = {0, 0}, v_use = 0, p_use[2] = {0, 0};
       uint32_t segment = 0;
       // A job is one stream's tile; a segment's jobs alternate between the
       // streams.  Shared keys: jobs 2i and 2i + 1 use tile i.
@@ -733,23 +738,20 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         for (int job = 0; ok && job < 2 && job < jobs; ++job) scores(job);
         for (int job = 0; ok && job < jobs; ++job) {
           const int x = job & 1;
-          const int buffer = kShared ? 0 : x;
           if (!kShared || x == 0) {
-            ok = mbar_wait_block(smem_u32(&v_full[buffer]), v_use[buffer] & 1, budget, a.status, kStatusTimeoutFull,
-                           abort_flag);
-            ++v_use[buffer];
+            ok = mbar_wait_block(smem_u32(&v_full), v_use & 1, budget, a.status, kStatusTimeoutFull, abort_flag);
+            ++v_use;
             if (!ok) break;
           }
           ok = mbar_wait_block(smem_u32(&p_full[x]), p_use[x] & 1, budget, a.status, kStatusTimeoutFull, abort_flag);
           ++p_use[x];
           if (!ok) break;
           tc_fence_after();
-          const uint64_t v = desc_v + static_cast<uint64_t>((buffer * S::kHalf) >> 4);
 #pragma unroll
           for (int i = 0; i < S::kKeys / 16; ++i)
-            umma_f16_ts(tmem_base + 256 + x * 128, tmem_base + x * 128 + 8 * i, v + i * (2048u >> 4), kIdescPV,
+            umma_f16_ts(tmem_base + 256 + x * 128, tmem_base + x * 128 + 8 * i, desc_v + i * (2048u >> 4), kIdescPV,
                         job >= 2 || i > 0 ? 1u : 0u);
-          if (!kShared || x == 1) umma_commit(smem_u32(&v_empty[buffer]));
+          if (!kShared || x == 1) umma_commit(smem_u32(&v_empty));
           if (job + 2 < jobs)
             scores(job + 2);
           else
