@@ -10,10 +10,12 @@
 // Products: fp16 tensor-core MMAs (m16n8k16, fp32 accumulators).  Codes are
 // exact in fp16.  fp16 queries are used as they are; a bf16 row is scaled by
 // a power of two to [1, 2) at its largest element, which loses only what lies
-// 2^-25 and more below it.  Weights w_j = p_j b_j / u are rounded to fp16 (11
-// bits, against 8 or 11 of the output): u, a unit for each row, follows the
-// largest p_j b_j, so w neither overflows nor goes subnormal where it counts.
-// Scores, weights, totals and numerators are fp32.
+// 2^-25 and more below it.  A row has one reference, a logarithm `unit` that
+// follows its largest p_j b_j: the total sums p_j / 2^unit, and the weights
+// w_j = p_j b_j / 2^unit are rounded to fp16 (11 bits, against 8 or 11 of the
+// output).  The reference moves, and the numerators with it, only when a
+// weight would exceed 2^14, so that w neither overflows nor goes subnormal
+// where it counts.  Scores, weights, totals and numerators are fp32.
 //
 // Layout: a code of a page is the byte that a lane's fragment wants.  As 16-bit
 // elements, ldmatrix gives lane (g, t) the bytes 4t .. 4t+3 of key g: the
@@ -38,8 +40,9 @@
 
 namespace piper {
 
-constexpr float kSlack = 8.0f;         // log2 by which a weight may exceed 1 before the maximum moves
-constexpr float kUnitMin = 0x1p-120f;  // smallest unit of a numerator
+constexpr float kSlack = 14.0f;         // log2 by which a weight may exceed 1: fp16 holds 2^15
+constexpr float kScaleLogMin = -90.0f;  // smaller value scales count as 2^-90 in the references
+constexpr float kNoReference = -1e30f;
 
 struct TreeArgs {
   piper_b200_kv_cache_t c;
@@ -57,11 +60,10 @@ struct TreeArgs {
   float scale_log2e;
 };
 
-// Tile shape of one kernel instance: MT m16 row tiles for each of WARPS
-// warps, 16 keys of the tile for each warp.
-template <int D, int MT, int WARPS>
+// Tile of up to 16 rows: a warp takes 16 keys of it.
+template <int D, int WARPS>
 struct TreeTile {
-  static constexpr int kRows = 16 * MT;
+  static constexpr int kRows = 16;
   static constexpr int kKeys = 16 * WARPS;
   static constexpr int kThreads = 32 * (WARPS + 1);  // and one warp that fetches
   static constexpr int kCodes = kKeys * D;
@@ -70,13 +72,11 @@ struct TreeTile {
   static constexpr int kStageAlloc = (kStage + 1023) / 1024 * 1024;
   static constexpr int kJoinStride = 80;  // floats; 16 banks between rows
   static constexpr int kJoin = WARPS * 16 * kJoinStride * 4;
-  static constexpr int kQuery = MT > 1 ? MT * (D / 16) * 32 * 16 : 0;
-  static constexpr int kState = 3 * WARPS * kRows * 4;
-  static constexpr int kFixed = kJoin + kQuery + kState + kRows * 8 + 1024;
-  static constexpr int kCtas = MT == 1 ? 2 : 1;  // per SM
-  static constexpr int kStages = (227 * 1024 / kCtas - 1024 * 2 - kFixed) / kStageAlloc > 8
-                                     ? 8
-                                     : (227 * 1024 / kCtas - 1024 * 2 - kFixed) / kStageAlloc;
+  static constexpr int kState = 2 * WARPS * kRows * 4;
+  static constexpr int kFixed = kJoin + kState + kRows * 8 + 1024;
+  static constexpr int kCtas = 2;  // per SM
+  static constexpr int kFit = (227 * 1024 / kCtas - 1024 * 2 - kFixed) / kStageAlloc;
+  static constexpr int kStages = kFit > 8 ? 8 : kFit;
   static constexpr int kAlloc = kStages * kStageAlloc + kFixed + 1024;
   static constexpr int kPart = kRows * (D + 2);  // floats of one part
 };
@@ -201,6 +201,12 @@ __device__ __forceinline__ uint32_t tile_chunk(uint32_t base, int r, int c) {
   return base + r * D + ((c ^ x) << 4);
 }
 
+__device__ __forceinline__ float lg2_approx(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 __device__ __forceinline__ void bar_sync(int id, int threads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory");
 }
@@ -259,18 +265,17 @@ __device__ __forceinline__ void query_fragments(const TreeArgs& a, int b, int kv
   }
 }
 
-template <typename T, int D, int MT, int WARPS>
-__global__ void __launch_bounds__(TreeTile<D, MT, WARPS>::kThreads, TreeTile<D, MT, WARPS>::kCtas)
+template <typename T, int D, int WARPS>
+__global__ void __launch_bounds__(TreeTile<D, WARPS>::kThreads, TreeTile<D, WARPS>::kCtas)
     tree_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map,
                           TreeArgs a) {
-  using S = TreeTile<D, MT, WARPS>;
+  using S = TreeTile<D, WARPS>;
   constexpr int kStages = S::kStages;
   constexpr int kChunks = D / 16;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* join = reinterpret_cast<float*>(smem + kStages * S::kStageAlloc);
-  uint4* query_smem = reinterpret_cast<uint4*>(smem + kStages * S::kStageAlloc + S::kJoin);
-  float* state = reinterpret_cast<float*>(smem + kStages * S::kStageAlloc + S::kJoin + S::kQuery);
+  float* state = reinterpret_cast<float*>(smem + kStages * S::kStageAlloc + S::kJoin);
   uint64_t* words = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(state) + S::kState);
   __shared__ __align__(8) uint64_t full_bar[kStages], empty_bar[kStages];
   __shared__ uint32_t valid[kStages];
@@ -314,7 +319,7 @@ __global__ void __launch_bounds__(TreeTile<D, MT, WARPS>::kThreads, TreeTile<D, 
         entry = have + lane < a.c.table_width ? __ldg(row + have + lane) : -1;
       }
       const int page = __shfl_sync(0xffffffffu, entry, (column - have) & 31);
-      ok = mbar_wait_warp(smem_u32(&empty_bar[stage]), phase, a.wait_budget_ns, a.status, kStatusTimeoutEmpty,
+      ok = mbar_wait_block_warp(smem_u32(&empty_bar[stage]), phase, a.wait_budget_ns, a.status, kStatusTimeoutEmpty,
                           abort_flag);
       if (!ok) break;
       const bool good = lane < boxes && column < a.c.table_width && page >= 0 && page < a.c.pages;
@@ -357,7 +362,7 @@ __global__ void __launch_bounds__(TreeTile<D, MT, WARPS>::kThreads, TreeTile<D, 
     // consumers have waited for all of them unless something gave up).
     if (!ok)
       for (int i = max(0, issued - kStages); i < issued; ++i)
-        mbar_wait_warp(smem_u32(&full_bar[i % kStages]), (i / kStages) & 1, a.wait_budget_ns, a.status,
+        mbar_wait_block_warp(smem_u32(&full_bar[i % kStages]), (i / kStages) & 1, a.wait_budget_ns, a.status,
                        kStatusTimeoutDrain, 0u);
     return;
   }
@@ -376,25 +381,9 @@ __global__ void __launch_bounds__(TreeTile<D, MT, WARPS>::kThreads, TreeTile<D, 
     const int tile_end = static_cast<int>(min(static_cast<int64_t>(tiles), tile + (run.end - u)));
     const bool all = tile == 0 && tile_end == tiles;
     const int64_t length = max(0, __ldg(a.c.lengths + b));
-    uint32_t q[MT == 1 ? kChunks : 1][4];
-    float factor[MT][2];
-    if constexpr (MT == 1) {
-      query_fragments<T, D>(a, b, kv, row0, q, factor[0]);
-    } else {
-      // Row tile i's fragments come from warp i; the factors go with them.
-      if (warp < MT) {
-        uint32_t f[kChunks][4];
-        float r[2];
-        query_fragments<T, D>(a, b, kv, row0 + warp * 16, f, r);
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c)
-          query_smem[(warp * kChunks + c) * 32 + lane] = make_uint4(f[c][0], f[c][1], f[c][2], f[c][3]);
-        if (t == 0) {
-          state[warp * 16 + g] = r[0];
-          state[warp * 16 + g + 8] = r[1];
-        }
-      }
-    }
+    uint32_t q[kChunks][4];
+    float factor[2];
+    query_fragments<T, D>(a, b, kv, row0, q, factor);
     if (tid < S::kRows) {
       const int row = row0 + tid;
       uint64_t word = 0;
@@ -408,31 +397,20 @@ __global__ void __launch_bounds__(TreeTile<D, MT, WARPS>::kThreads, TreeTile<D, 
       words[tid] = word;
     }
     bar_sync(1, WARPS * 32);
-    if constexpr (MT > 1) {
-#pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        factor[i][0] = state[i * 16 + g];
-        factor[i][1] = state[i * 16 + g + 8];
-      }
-    }
-    float o[MT][2 * kChunks][4] = {};
-    float m[MT][2], l[MT][2], unit[MT][2], inv[MT][2];
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        m[i][h] = -INFINITY;
-        l[i][h] = unit[i][h] = inv[i][h] = 0.0f;
-      }
+    float o[2 * kChunks][4] = {};
+    float unit[2] = {kNoReference, kNoReference}, l[2] = {0.0f, 0.0f};
     for (; tile < tile_end; ++tile, ++u) {
-      if (ok) ok = mbar_wait_warp(smem_u32(&full_bar[stage]), phase, a.wait_budget_ns, a.status, kStatusTimeoutFull,
+      if (ok) ok = mbar_wait_block_warp(smem_u32(&full_bar[stage]), phase, a.wait_budget_ns, a.status, kStatusTimeoutFull,
                                   abort_flag);
       if (ok) {
         const uint32_t base = smem_u32(smem + stage * S::kStageAlloc);
         const float* scales = reinterpret_cast<const float*>(smem + stage * S::kStageAlloc + 2 * S::kCodes);
         const int key0 = warp * 16;
-        // ---- scores of 16 keys
-        float s[MT][2][4] = {};
+        const uint32_t goods = valid[stage];
+        const int64_t first = static_cast<int64_t>(tile) * S::kKeys;
+        const bool masked = first + S::kKeys > length || goods != (1u << boxes) - 1u;
+        // ---- scores of 16 keys, in two chains
+        float s[2][2][4] = {};
 #pragma unroll
         for (int c = 0; c < kChunks; c += 2) {
           uint32_t k[4];
@@ -440,148 +418,91 @@ __global__ void __launch_bounds__(TreeTile<D, MT, WARPS>::kThreads, TreeTile<D, 
 #pragma unroll
           for (int x = 0; x < 4; ++x) k[x] ^= 0x80808080u;
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
+          for (int x = 0; x < 2; ++x)
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-              const uint32_t b0 = codes_f16<0x4140>(k[2 * x + n]);
-              const uint32_t b1 = codes_f16<0x4342>(k[2 * x + n]);
-#pragma unroll
-              for (int i = 0; i < MT; ++i) {
-                if constexpr (MT == 1) {
-                  mma16816(s[i][n], q[c + x], b0, b1);
-                } else {
-                  const uint4 f = query_smem[(i * kChunks + c + x) * 32 + lane];
-                  const uint32_t fr[4] = {f.x, f.y, f.z, f.w};
-                  mma16816(s[i][n], fr, b0, b1);
-                }
-              }
-            }
-          }
+            for (int n = 0; n < 2; ++n)
+              mma16816(s[x][n], q[c + x], codes_f16<0x4140>(k[2 * x + n]), codes_f16<0x4342>(k[2 * x + n]));
         }
-        const float2 ks0 = *reinterpret_cast<const float2*>(scales + key0 + 2 * t);
-        const float2 ks1 = *reinterpret_cast<const float2*>(scales + key0 + 8 + 2 * t);
-        const float2 vs0 = *reinterpret_cast<const float2*>(scales + S::kKeys + key0 + 2 * t);
-        const float2 vs1 = *reinterpret_cast<const float2*>(scales + S::kKeys + key0 + 8 + 2 * t);
-        const float ks[2][2] = {{ks0.x, ks0.y}, {ks1.x, ks1.y}};
-        const float vs[2][2] = {{vs0.x, vs0.y}, {vs1.x, vs1.y}};
-        const uint32_t goods = valid[stage];
-        const int64_t first = static_cast<int64_t>(tile) * S::kKeys;
-        const bool masked = first + S::kKeys > length || goods != (boxes == 32 ? ~0u : (1u << boxes) - 1u);
+        float ks[2][2], vs[2][2], lv[2][2];
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[i][n][e] *= ks[n][e & 1];
-        // A key that a row does not see may hold anything: its score is
-        // replaced, and its weight again after the product with its scale.
-        uint32_t unseen = 0u;
-        if (masked) {
-#pragma unroll
-          for (int n = 0; n < 2; ++n)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int key = key0 + n * 8 + 2 * t + e;
-              const int64_t j = first + key - length;
-              const bool there = (goods >> (key >> box_shift)) & 1u;
-              const bool open = there && j < 0;
-              const bool drafted = there && j >= 0 && j < a.nodes;
-#pragma unroll
-              for (int i = 0; i < MT; ++i)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                  const bool seen = open || (drafted && ((words[i * 16 + g + 8 * h] >> (j & 63)) & 1u));
-                  if (!seen) {
-                    s[i][n][2 * h + e] = -INFINITY;
-                    unseen |= 1u << (i * 8 + n * 4 + 2 * h + e);
-                  }
-                }
-            }
+        for (int n = 0; n < 2; ++n) {
+          const float2 k2 = *reinterpret_cast<const float2*>(scales + key0 + 8 * n + 2 * t);
+          const float2 v2 = *reinterpret_cast<const float2*>(scales + S::kKeys + key0 + 8 * n + 2 * t);
+          ks[n][0] = k2.x;
+          ks[n][1] = k2.y;
+          vs[n][0] = v2.x;
+          vs[n][1] = v2.y;
+          lv[n][0] = fmaxf(lg2_approx(v2.x), kScaleLogMin);
+          lv[n][1] = fmaxf(lg2_approx(v2.y), kScaleLogMin);
         }
-        // ---- weights
-        bool grow = false;
-        float top[MT][2];
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            top[i][h] = fmaxf(fmaxf(s[i][0][2 * h], s[i][0][2 * h + 1]), fmaxf(s[i][1][2 * h], s[i][1][2 * h + 1]));
-            grow |= (top[i][h] - m[i][h]) * factor[i][h] > kSlack;
-          }
-        if (__any_sync(0xffffffffu, grow)) {
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float x = top[i][h];
-              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-              if (x > m[i][h]) {
-                const float shrink = ex2_approx((m[i][h] - x) * factor[i][h]);
-                m[i][h] = x;
-                l[i][h] *= shrink;
-                unit[i][h] *= shrink;
-                inv[i][h] = unit[i][h] >= kUnitMin ? 1.0f / unit[i][h] : 0.0f;
-              }
-            }
-        }
-        bool over = false;
-        float most[MT][2];
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float shift = m[i][h] == -INFINITY ? 0.0f : -m[i][h] * factor[i][h];
+        uint32_t w[4];
+        // A masked tile has a body of its own: selections would lengthen the
+        // other's.
+        auto weigh = [&](auto hidden) {
+          uint32_t unseen = 0u;  // bit 4 n + 2 h + e
+          if constexpr (hidden.value) {
 #pragma unroll
             for (int n = 0; n < 2; ++n)
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                const float p = ex2_approx(fmaf(s[i][n][2 * h + e], factor[i][h], shift));
-                l[i][h] += p;
-                s[i][n][2 * h + e] = p * vs[n][e];
+                const int key = key0 + n * 8 + 2 * t + e;
+                const int64_t j = first + key - length;
+                const bool there = (goods >> (key >> box_shift)) & 1u;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                  if (!(there && (j < 0 || (j < a.nodes && ((words[g + 8 * h] >> (j & 63)) & 1u)))))
+                    unseen |= 1u << (4 * n + 2 * h + e);
               }
           }
-        if (masked) {
-#pragma unroll
-          for (int x = 0; x < 8 * MT; ++x)
-            if ((unseen >> x) & 1u) s[x / 8][(x / 4) & 1][x & 3] = 0.0f;
-        }
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            most[i][h] = fmaxf(fmaxf(s[i][0][2 * h], s[i][0][2 * h + 1]), fmaxf(s[i][1][2 * h], s[i][1][2 * h + 1]));
-            over |= most[i][h] > unit[i][h] * 256.0f;
-          }
-        if (__any_sync(0xffffffffu, over)) {
-#pragma unroll
-          for (int i = 0; i < MT; ++i)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float x = most[i][h];
-              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-              x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
-              if (x > unit[i][h]) {
-                const float shrink = unit[i][h] / x;
-                unit[i][h] = x;
-                inv[i][h] = x >= kUnitMin ? 1.0f / x : 0.0f;
-#pragma unroll
-                for (int c = 0; c < 2 * kChunks; ++c) {
-                  o[i][c][2 * h] *= shrink;
-                  o[i][c][2 * h + 1] *= shrink;
-                }
-              }
-            }
-        }
-        uint32_t w[MT][4];
-#pragma unroll
-        for (int i = 0; i < MT; ++i)
+          float y[2][4];
+          float most[2] = {-INFINITY, -INFINITY};
 #pragma unroll
           for (int n = 0; n < 2; ++n)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-              w[i][2 * n + h] =
-                  pack2(s[i][n][2 * h] * inv[i][h], s[i][n][2 * h + 1] * inv[i][h], __half());
+            for (int x = 0; x < 4; ++x) {
+              y[n][x] = (s[0][n][x] + s[1][n][x]) * ks[n][x & 1];
+              // A key that a row does not see may hold anything.
+              if (hidden.value && ((unseen >> (4 * n + x)) & 1u)) y[n][x] = -INFINITY;
+              float z = fmaf(y[n][x], factor[x / 2], lv[n][x & 1]);
+              if (hidden.value && ((unseen >> (4 * n + x)) & 1u)) z = -INFINITY;
+              most[x / 2] = fmaxf(most[x / 2], z);
+            }
+          if (__any_sync(0xffffffffu, most[0] - unit[0] > kSlack || most[1] - unit[1] > kSlack)) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 1));
+              most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 2));
+              if (most[h] > unit[h]) {
+                const float shrink = ex2_approx(unit[h] - most[h]);
+                unit[h] = most[h];
+                l[h] *= shrink;
+#pragma unroll
+                for (int c = 0; c < 2 * kChunks; ++c) {
+                  o[c][2 * h] *= shrink;
+                  o[c][2 * h + 1] *= shrink;
+                }
+              }
+            }
+          }
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float p[2];
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                p[e] = ex2_approx(fmaf(y[n][2 * h + e], factor[h], -unit[h]));
+                l[h] += p[e];
+                p[e] *= vs[n][e];
+                if (hidden.value && ((unseen >> (4 * n + 2 * h + e)) & 1u)) p[e] = 0.0f;
+              }
+              w[2 * n + h] = pack2(p[0], p[1], __half());
+            }
+        };
+        if (masked)
+          weigh(std::true_type());
+        else
+          weigh(std::false_type());
         // ---- numerators: even, then odd head dimensions of each chunk
 #pragma unroll
         for (int c = 0; c < kChunks; c += 2) {
@@ -591,13 +512,8 @@ __global__ void __launch_bounds__(TreeTile<D, MT, WARPS>::kThreads, TreeTile<D, 
           for (int x = 0; x < 4; ++x) v[x] ^= 0x80808080u;
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            const uint32_t e0 = codes_f16<0x4240>(v[2 * x]), e1 = codes_f16<0x4240>(v[2 * x + 1]);
-            const uint32_t d0 = codes_f16<0x4341>(v[2 * x]), d1 = codes_f16<0x4341>(v[2 * x + 1]);
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-              mma16816(o[i][2 * (c + x)], w[i], e0, e1);
-              mma16816(o[i][2 * (c + x) + 1], w[i], d0, d1);
-            }
+            mma16816(o[2 * (c + x)], w, codes_f16<0x4240>(v[2 * x]), codes_f16<0x4240>(v[2 * x + 1]));
+            mma16816(o[2 * (c + x) + 1], w, codes_f16<0x4341>(v[2 * x]), codes_f16<0x4341>(v[2 * x + 1]));
           }
         }
       }
@@ -608,105 +524,84 @@ __global__ void __launch_bounds__(TreeTile<D, MT, WARPS>::kThreads, TreeTile<D, 
         phase ^= 1;
       }
     }
-    // ---- join the warps' parts: each row's maximum and total, then the
-    // numerators, 16 rows and 64 head dimensions at a time.
+    // ---- join the warps' parts: each row's reference and total, then the
+    // numerators, 64 head dimensions at a time.
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        l[i][h] += __shfl_xor_sync(0xffffffffu, l[i][h], 1);
-        l[i][h] += __shfl_xor_sync(0xffffffffu, l[i][h], 2);
-        m[i][h] *= factor[i][h];
+    for (int h = 0; h < 2; ++h) {
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+      if (unit[h] == kNoReference) unit[h] = -INFINITY;
+      if (t == 0) {
+        state[warp * 16 + g + 8 * h] = unit[h];
+        state[(WARPS + warp) * 16 + g + 8 * h] = l[h];
       }
-    bar_sync(1, WARPS * 32);  // the factors in `state` have been read
-    if (t == 0) {
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          state[(0 * WARPS + warp) * S::kRows + i * 16 + g + 8 * h] = m[i][h];
-          state[(1 * WARPS + warp) * S::kRows + i * 16 + g + 8 * h] = l[i][h];
-        }
     }
     bar_sync(1, WARPS * 32);
-    float whole_m[MT][2], whole_l[MT][2], share[MT][2];
+    // A row's reference (0 where it saw nothing) and total over the warps.
+    auto joined = [&](int r, float* total) {
+      float top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+      for (int w = 0; w < WARPS; ++w) top = fmaxf(top, state[w * 16 + r]);
+      const float ref = top == -INFINITY ? 0.0f : top;
+      *total = 0.0f;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = i * 16 + g + 8 * h;
-        float top = -INFINITY, total = 0.0f;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) top = fmaxf(top, state[w * S::kRows + r]);
-        const float ref = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w)
-          total += state[(WARPS + w) * S::kRows + r] * ex2_approx(state[w * S::kRows + r] - ref);
-        whole_m[i][h] = top;
-        whole_l[i][h] = total;
-        share[i][h] = unit[i][h] * ex2_approx(m[i][h] - ref);
-      }
+      for (int w = 0; w < WARPS; ++w) *total += state[(WARPS + w) * 16 + r] * ex2_approx(state[w * 16 + r] - ref);
+      return top;
+    };
+    float share[2];
     float* to = a.parts + (static_cast<int64_t>(blockIdx.x) * 2 + part) * S::kPart;
-    if (!all && warp == 0 && t == 0) {
 #pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int r = i * 16 + g + 8 * h;
-          to[S::kRows * D + 2 * r] = whole_m[i][h];
-          to[S::kRows * D + 2 * r + 1] = whole_l[i][h];
-        }
+    for (int h = 0; h < 2; ++h) {
+      float total;
+      const float top = joined(g + 8 * h, &total);
+      share[h] = ex2_approx(unit[h] - (top == -INFINITY ? 0.0f : top));
+      if (!all && warp == 0 && t == 0) {
+        to[16 * D + 2 * (g + 8 * h)] = top;
+        to[16 * D + 2 * (g + 8 * h) + 1] = total;
+      }
     }
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
+    for (int d0 = 0; d0 < D; d0 += 64) {
+      float* mine = join + warp * 16 * S::kJoinStride;
 #pragma unroll
-      for (int d0 = 0; d0 < D; d0 += 64) {
-        float* mine = join + warp * 16 * S::kJoinStride;
+      for (int c = 0; c < 4; ++c)
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float(&even)[4] = o[i][2 * (d0 / 16 + c)];
-            const float(&odd)[4] = o[i][2 * (d0 / 16 + c) + 1];
-            const float f = share[i][h];
-            *reinterpret_cast<float4*>(mine + (g + 8 * h) * S::kJoinStride + c * 16 + 4 * t) =
-                make_float4(even[2 * h] * f, odd[2 * h] * f, even[2 * h + 1] * f, odd[2 * h + 1] * f);
-          }
-        bar_sync(1, WARPS * 32);
-        // 16 rows x 64 columns, four columns a thread.
-        for (int x = tid; x < 256; x += WARPS * 32) {
-          const int r = x / 16, d = (x % 16) * 4;
-          float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-          for (int w = 0; w < WARPS; ++w) {
-            const float4 y = *reinterpret_cast<const float4*>(join + (w * 16 + r) * S::kJoinStride + d);
-            sum.x += y.x;
-            sum.y += y.y;
-            sum.z += y.z;
-            sum.w += y.w;
-          }
-          const int row = row0 + i * 16 + r;
-          if (!all) {
-            *reinterpret_cast<float4*>(to + (i * 16 + r) * D + d0 + d) = sum;
-          } else if (row < a.rows) {
-            float total = 0.0f, top = -INFINITY;
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w) top = fmaxf(top, state[w * S::kRows + i * 16 + r]);
-            const float ref = top == -INFINITY ? 0.0f : top;
-#pragma unroll
-            for (int w = 0; w < WARPS; ++w)
-              total += state[(WARPS + w) * S::kRows + i * 16 + r] * ex2_approx(state[w * S::kRows + i * 16 + r] - ref);
-            const float f = total == 0.0f ? 0.0f : 1.0f / total;
-            const int64_t at =
-                ((static_cast<int64_t>(b) * a.heads + kv * a.group + row / a.nodes) * a.nodes + row % a.nodes) * D;
-            uint2 y;
-            y.x = pack2(sum.x * f, sum.y * f, T());
-            y.y = pack2(sum.z * f, sum.w * f, T());
-            *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at + d0 + d) = y;
-          }
+        for (int h = 0; h < 2; ++h) {
+          const float(&even)[4] = o[2 * (d0 / 16 + c)];
+          const float(&odd)[4] = o[2 * (d0 / 16 + c) + 1];
+          const float f = share[h];
+          *reinterpret_cast<float4*>(mine + (g + 8 * h) * S::kJoinStride + c * 16 + 4 * t) =
+              make_float4(even[2 * h] * f, odd[2 * h] * f, even[2 * h + 1] * f, odd[2 * h + 1] * f);
         }
-        bar_sync(1, WARPS * 32);
+      bar_sync(1, WARPS * 32);
+      // 16 rows x 64 columns, four columns a thread.
+      for (int x = tid; x < 256; x += WARPS * 32) {
+        const int r = x / 16, d = (x % 16) * 4;
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+          const float4 y = *reinterpret_cast<const float4*>(join + (w * 16 + r) * S::kJoinStride + d);
+          sum.x += y.x;
+          sum.y += y.y;
+          sum.z += y.z;
+          sum.w += y.w;
+        }
+        const int row = row0 + r;
+        if (!all) {
+          *reinterpret_cast<float4*>(to + r * D + d0 + d) = sum;
+        } else if (row < a.rows) {
+          float total;
+          joined(r, &total);
+          const float f = total == 0.0f ? 0.0f : 1.0f / total;
+          const int64_t at =
+              ((static_cast<int64_t>(b) * a.heads + kv * a.group + row / a.nodes) * a.nodes + row % a.nodes) * D;
+          uint2 y;
+          y.x = pack2(sum.x * f, sum.y * f, T());
+          y.y = pack2(sum.z * f, sum.w * f, T());
+          *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + at + d0 + d) = y;
+        }
       }
+      bar_sync(1, WARPS * 32);
     }
     part = 1;
     if (tile == tiles) {

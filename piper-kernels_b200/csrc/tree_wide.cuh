@@ -32,8 +32,7 @@
 namespace piper {
 
 constexpr int kWideThreads = 736;
-constexpr float kWideSlack = 14.0f;      // log2 by which a weight may exceed 1: fp16 holds 2^15
-constexpr float kScaleLogMin = -90.0f;   // smaller value scales count as 2^-90 in the references
+
 template <int D, bool kShared>
 struct WideTile {
   static constexpr int kRows = kShared ? 256 : 128;
@@ -102,14 +101,6 @@ __device__ __forceinline__ void wide_next(const TreeArgs& a, int per, WideWalk& 
   }
   w.count = static_cast<int>(min(static_cast<int64_t>(w.tiles), w.left));
   w.all = w.count == w.tiles;
-}
-
-constexpr float kNoReference = -1e30f;
-
-__device__ __forceinline__ float lg2_approx(float x) {
-  float y;
-  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 __device__ __forceinline__ float2 mul2(float2 x, float2 y) { return __fmul2_rn(x, y); }
@@ -384,7 +375,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
           // A weight times its value scale is at most 2^(top + reach_log - unit).
           bool renew = false;
 #pragma unroll
-          for (int h = 0; h < 2; ++h) renew |= fmaf(top[h], factor[h], reach_log - unit[h]) > kWideSlack;
+          for (int h = 0; h < 2; ++h) renew |= fmaf(top[h], factor[h], reach_log - unit[h]) > kSlack;
           if (__any_sync(0xffffffffu, renew)) {
             // The largest logarithm of a weight times its value scale.
             float most[2] = {-INFINITY, -INFINITY};
