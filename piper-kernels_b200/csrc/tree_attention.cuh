@@ -24,9 +24,11 @@
 // head dimensions.  A byte becomes fp16 by a byte permute under 0x64 (1024 +
 // code + 128) and one subtraction.
 //
-// Work: a unit is one key tile of one (request, KV head, row tile); the units
-// of the whole batch are cut into equal runs, one for each CTA, so that ragged
-// lengths balance.  A run that covers a (request, head, row tile) writes its
+// Work: a segment is one (request, KV head, row tile); it has S::kLead units
+// for its start and end (query rows, join), then a unit for each key tile.  The
+// units of the whole batch are cut into equal runs, one for each CTA, so that
+// ragged lengths balance (without the lead, runs of short requests took twice
+// as long as the others).  A run that covers a (request, head, row tile) writes its
 // output; one that covers a part leaves its maximum, total and numerator in
 // the workspace, and tree_merge_kernel joins the parts.
 #pragma once
@@ -75,6 +77,7 @@ struct TreeTile {
   static constexpr int kState = 2 * WARPS * kRows * 4;
   static constexpr int kFixed = kJoin + kState + kRows * 8 + 1024;
   static constexpr int kCtas = 2;  // per SM
+  static constexpr int kLead = 3;  // a segment's start and end, in key tiles
   static constexpr int kFit = (227 * 1024 / kCtas - 1024 * 2 - kFixed) / kStageAlloc;
   static constexpr int kStages = kFit > 8 ? 8 : kFit;
   static constexpr int kAlloc = kStages * kStageAlloc + kFixed + 1024;
@@ -89,33 +92,37 @@ __device__ __forceinline__ int tree_tiles(const TreeArgs& a, int b) {
   return static_cast<int>((keys + kKeys - 1) / kKeys);
 }
 
-// A run of units: [begin, end) over the batch, and where `begin` lies.
+// A run's place in the batch: `left` units from position `at` of segment
+// (b, hr) on, hr being head * row_tiles + row tile; of the segment it has key
+// tiles [tile, tile + count) of `tiles`.
 struct TreeRun {
-  int64_t begin, end;
-  int b, hr, tile, tiles;  // request, head * row_tiles + row tile, key tile and its count
+  int64_t left;
+  int b, hr, at, tiles, tile, count;
+  bool all;
 };
 
 // Units of the batch; every lane gets the result.
-template <int kKeys>
+template <typename S>
 __device__ __forceinline__ int64_t tree_units(const TreeArgs& a) {
   const int lane = threadIdx.x % 32;
   int64_t sum = 0;
-  for (int b = lane; b < a.c.batch; b += 32) sum += tree_tiles<kKeys>(a, b);
+  for (int b = lane; b < a.c.batch; b += 32) sum += S::kLead + tree_tiles<S::kKeys>(a, b);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   return sum * (static_cast<int64_t>(a.c.kv_heads) * a.row_tiles);
 }
 
-// The request that unit u belongs to, and its first unit.
-template <int kKeys>
+// The request that unit u belongs to, its key tiles, and its first unit.
+template <typename S>
 __device__ __forceinline__ void tree_find(const TreeArgs& a, int64_t u, int* request, int* tiles, int64_t* first) {
   const int lane = threadIdx.x % 32;
   const int64_t per = static_cast<int64_t>(a.c.kv_heads) * a.row_tiles;
   int64_t base = 0;
   for (int b0 = 0; b0 < a.c.batch; b0 += 32) {
     const int b = b0 + lane;
-    const int n = b < a.c.batch ? tree_tiles<kKeys>(a, b) : 0;
-    int64_t upto = n;
+    const int n = b < a.c.batch ? tree_tiles<S::kKeys>(a, b) : 0;
+    const int64_t mine = b < a.c.batch ? S::kLead + n : 0;
+    int64_t upto = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t below = __shfl_up_sync(0xffffffffu, upto, o);
@@ -126,7 +133,7 @@ __device__ __forceinline__ void tree_find(const TreeArgs& a, int64_t u, int* req
       const int at = __ffs(past) - 1;
       *request = b0 + at;
       *tiles = __shfl_sync(0xffffffffu, n, at);
-      *first = base + (__shfl_sync(0xffffffffu, upto, at) - *tiles) * per;
+      *first = base + __shfl_sync(0xffffffffu, upto - mine, at) * per;
       return;
     }
     base += __shfl_sync(0xffffffffu, upto, 31) * per;
@@ -136,34 +143,60 @@ __device__ __forceinline__ void tree_find(const TreeArgs& a, int64_t u, int* req
   *first = base;
 }
 
-// CTAs that share the units: at least two units each.
+// CTAs that share the units: at least two key tiles' worth each.
+template <typename S>
 __device__ __forceinline__ int64_t tree_ctas(int64_t units, int grid) {
-  return max(static_cast<int64_t>(1), min(static_cast<int64_t>(grid), units / 2));
+  return max(static_cast<int64_t>(1), min(static_cast<int64_t>(grid), units / (S::kLead + 2)));
 }
 __device__ __forceinline__ int64_t tree_bound(int64_t units, int64_t ctas, int64_t i) { return units * i / ctas; }
 
-template <int kKeys>
+// The key tiles of the run's segment, from its units.
+template <typename S>
+__device__ __forceinline__ void tree_range(TreeRun& r) {
+  const int end = static_cast<int>(min(static_cast<int64_t>(S::kLead + r.tiles), r.at + r.left));
+  r.tile = max(0, r.at - S::kLead);
+  r.count = max(0, end - S::kLead) - r.tile;
+  r.all = r.count == r.tiles;
+}
+
+template <typename S>
 __device__ __forceinline__ TreeRun tree_run(const TreeArgs& a) {
   TreeRun r;
   const int per = a.c.kv_heads * a.row_tiles;
+  r.at = 0;
   if (a.whole) {
     r.b = blockIdx.x / per;
     r.hr = blockIdx.x % per;
-    r.tile = 0;
-    r.tiles = tree_tiles<kKeys>(a, r.b);
-    r.begin = 0;
-    r.end = r.tiles;
-    return r;
+    r.tiles = tree_tiles<S::kKeys>(a, r.b);
+    r.left = S::kLead + r.tiles;
+  } else {
+    const int64_t units = tree_units<S>(a);
+    const int64_t ctas = tree_ctas<S>(units, gridDim.x);
+    const int64_t begin = blockIdx.x < ctas ? tree_bound(units, ctas, blockIdx.x) : 0;
+    r.left = blockIdx.x < ctas ? tree_bound(units, ctas, blockIdx.x + 1) - begin : 0;
+    int64_t first = 0;
+    tree_find<S>(a, begin, &r.b, &r.tiles, &first);
+    const int length = S::kLead + r.tiles;
+    r.hr = static_cast<int>((begin - first) / length);
+    r.at = static_cast<int>((begin - first) % length);
   }
-  const int64_t units = tree_units<kKeys>(a);
-  const int64_t ctas = tree_ctas(units, gridDim.x);
-  r.begin = blockIdx.x < ctas ? tree_bound(units, ctas, blockIdx.x) : 0;
-  r.end = blockIdx.x < ctas ? tree_bound(units, ctas, blockIdx.x + 1) : 0;
-  int64_t first = 0;
-  tree_find<kKeys>(a, r.begin, &r.b, &r.tiles, &first);
-  r.hr = static_cast<int>((r.begin - first) / r.tiles);
-  r.tile = static_cast<int>((r.begin - first) % r.tiles);
+  tree_range<S>(r);
+  if (r.left == 0) r.count = 0;
   return r;
+}
+
+// The run's next segment.
+template <typename S>
+__device__ __forceinline__ void tree_next(const TreeArgs& a, TreeRun& r) {
+  r.left -= S::kLead + r.tiles - r.at;
+  if (r.left <= 0) return;
+  r.at = 0;
+  if (++r.hr == a.c.kv_heads * a.row_tiles) {
+    r.hr = 0;
+    ++r.b;
+    r.tiles = tree_tiles<S::kKeys>(a, r.b);
+  }
+  tree_range<S>(r);
 }
 
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
@@ -293,28 +326,27 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS>::kThreads, TreeTile<D, WARP
   __syncthreads();
   // Lets tree_merge_kernel's CTAs be placed; they wait for this grid's end.
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  TreeRun run = tree_run<S::kKeys>(a);
-  const int per = a.c.kv_heads * a.row_tiles;
+  TreeRun run = tree_run<S>(a);
   const int box = min(a.c.page_size, 64);
   const int box_shift = min(a.page_shift, 6);
   const int boxes = S::kKeys >> box_shift;
 
   if (warp == WARPS) {
     // ---- fetching warp: lane i brings box i of each tile.
-    int64_t u = run.begin;
     int stage = 0, issued = 0;
     uint32_t phase = 1;  // a fresh barrier's previous phase counts as done
     bool ok = true;
-    int b = run.b, hr = run.hr, tile = run.tile, tiles = run.tiles;
-    const int32_t* row = a.c.block_table + b * a.c.table_stride;
+    for (; run.left > 0 && ok; tree_next<S>(a, run)) {
+    const int32_t* row = a.c.block_table + run.b * a.c.table_stride;
+    const int head = run.hr / a.row_tiles;
     int have = -1, entry = -1;  // table columns [have, have + 32), one a lane
-    while (u < run.end && ok) {
+    for (int tile = run.tile; tile < run.tile + run.count && ok; ++tile) {
       const int64_t position = static_cast<int64_t>(tile) * S::kKeys + static_cast<int64_t>(lane) * box;
       const int column = static_cast<int>(position >> a.page_shift);
       const int column0 = static_cast<int>((static_cast<int64_t>(tile) * S::kKeys) >> a.page_shift);
       const int column1 =
           static_cast<int>((static_cast<int64_t>(tile) * S::kKeys + S::kKeys - 1) >> a.page_shift);
-      if (have < 0 || column0 < have || column1 >= have + 32) {
+      if (have < 0 || column1 >= have + 32) {
         have = column0;
         entry = have + lane < a.c.table_width ? __ldg(row + have + lane) : -1;
       }
@@ -331,7 +363,6 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS>::kThreads, TreeTile<D, WARP
       }
       __syncwarp();
       if (good) {
-        const int head = hr / a.row_tiles;
         const int z = page * a.c.kv_heads + head;
         const int y = static_cast<int>(position & (a.c.page_size - 1));
         const uint32_t base = smem_u32(smem + stage * S::kStageAlloc);
@@ -346,17 +377,7 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS>::kThreads, TreeTile<D, WARP
         stage = 0;
         phase ^= 1;
       }
-      ++u;
-      if (++tile == tiles) {
-        tile = 0;
-        if (++hr == per && u < run.end) {
-          hr = 0;
-          ++b;
-          have = -1;
-          tiles = tree_tiles<S::kKeys>(a, b);
-          row = a.c.block_table + b * a.c.table_stride;
-        }
-      }
+    }
     }
     // Every copy has landed before the CTA's shared memory goes (the
     // consumers have waited for all of them unless something gave up).
@@ -369,17 +390,15 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS>::kThreads, TreeTile<D, WARP
 
   // ---- computing warps: 16 keys of each tile, all rows.
   const int g = lane / 4, t = lane % 4;
-  int64_t u = run.begin;
   int stage = 0;
   uint32_t phase = 0;
   bool ok = true;
-  int b = run.b, hr = run.hr, tile = run.tile, tiles = run.tiles;
   int part = 0;
-  while (u < run.end) {
-    const int kv = hr / a.row_tiles;
-    const int row0 = (hr % a.row_tiles) * S::kRows;
-    const int tile_end = static_cast<int>(min(static_cast<int64_t>(tiles), tile + (run.end - u)));
-    const bool all = tile == 0 && tile_end == tiles;
+  for (; run.left > 0; tree_next<S>(a, run)) {
+    if (run.count == 0) continue;
+    const int b = run.b, kv = run.hr / a.row_tiles;
+    const int row0 = (run.hr % a.row_tiles) * S::kRows;
+    const bool all = run.all;
     const int64_t length = max(0, __ldg(a.c.lengths + b));
     uint32_t q[kChunks][4];
     float factor[2];
@@ -399,7 +418,7 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS>::kThreads, TreeTile<D, WARP
     bar_sync(1, WARPS * 32);
     float o[2 * kChunks][4] = {};
     float unit[2] = {kNoReference, kNoReference}, l[2] = {0.0f, 0.0f};
-    for (; tile < tile_end; ++tile, ++u) {
+    for (int tile = run.tile; tile < run.tile + run.count; ++tile) {
       if (ok) ok = mbar_wait_block_warp(smem_u32(&full_bar[stage]), phase, a.wait_budget_ns, a.status, kStatusTimeoutFull,
                                   abort_flag);
       if (ok) {
@@ -604,50 +623,42 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS>::kThreads, TreeTile<D, WARP
       bar_sync(1, WARPS * 32);
     }
     part = 1;
-    if (tile == tiles) {
-      tile = 0;
-      if (++hr == per && u < run.end) {
-        hr = 0;
-        ++b;
-        tiles = tree_tiles<S::kKeys>(a, b);
-      }
-    }
   }
 }
 
-// Joins the parts of every (request, head, row tile) that a boundary between
-// two runs cuts.  CTA x looks at the boundary before run x + 1 and works if it
-// is the first inside its row tile; a warp takes a row, and CTAs y share the
+// Joins the parts of every segment whose key tiles a boundary between two runs
+// cuts.  CTA x looks at the boundary before run x + 1 and works if it is the
+// first such one of its segment; a warp takes a row, and CTAs y share the
 // rows.  A lane holds the maximum and total of one of 32 parts, so that the
 // numerators' loads do not wait for one another.
 template <typename T, int D, typename S>
 __global__ void __launch_bounds__(128) tree_merge_kernel(TreeArgs a, int grid) {
   // (The lengths were there before the attention kernel began.)
-  const int64_t units = tree_units<S::kKeys>(a);
-  const int64_t ctas = tree_ctas(units, grid);
+  const int64_t units = tree_units<S>(a);
+  const int64_t ctas = tree_ctas<S>(units, grid);
   const int64_t i = blockIdx.x + 1;
   if (i >= ctas) return;
   const int64_t at = tree_bound(units, ctas, i);
   int b = 0, tiles = 1;
   int64_t first = 0;
-  tree_find<S::kKeys>(a, at, &b, &tiles, &first);
-  const int hr = static_cast<int>((at - first) / tiles);
-  const int64_t begin = first + static_cast<int64_t>(hr) * tiles;
+  tree_find<S>(a, at, &b, &tiles, &first);
+  const int hr = static_cast<int>((at - first) / (S::kLead + tiles));
+  const int64_t start = first + static_cast<int64_t>(hr) * (S::kLead + tiles);
+  const int64_t begin = start + S::kLead, end = begin + tiles;  // its key tiles
   const int64_t before = tree_bound(units, ctas, i - 1);
-  if (at == begin || before > begin) return;
+  if (at <= begin || before > begin) return;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  // Runs i - 1 to `last` have parts of the row tile: `last` holds its last unit.
-  int64_t last = ((begin + tiles - 1) * ctas) / units;
-  while (last + 1 < ctas && tree_bound(units, ctas, last + 1) < begin + tiles) ++last;
-  while (tree_bound(units, ctas, last) >= begin + tiles) --last;
+  // Runs i - 1 to `last` have parts of it: `last` holds its last unit.
+  int64_t last = ((end - 1) * ctas) / units;
+  while (last + 1 < ctas && tree_bound(units, ctas, last + 1) < end) ++last;
+  while (tree_bound(units, ctas, last) >= end) --last;
   const int count = static_cast<int>(last - (i - 1) + 1);
   const int lane = threadIdx.x % 32;
   const int kv = hr / a.row_tiles, row0 = (hr % a.row_tiles) * S::kRows;
   constexpr int kPer = D / 32;
-  // Part k is run i - 1 + k's first one if the run starts inside the row tile
-  // or at its start.
+  // Part k is run i - 1 + k's first one if the run starts in the segment.
   auto part_of = [&](int k) {
-    return a.parts + ((i - 1 + k) * 2 + (k == 0 && before < begin ? 1 : 0)) * S::kPart;
+    return a.parts + ((i - 1 + k) * 2 + (k == 0 && before < start ? 1 : 0)) * S::kPart;
   };
   for (int r = blockIdx.y * 4 + threadIdx.x / 32; r < S::kRows && row0 + r < a.rows; r += 4 * gridDim.y) {
     float m = -INFINITY, l = 0.0f, o[kPer] = {};

@@ -38,6 +38,7 @@ struct WideTile {
   static constexpr int kRows = kShared ? 256 : 128;
   static constexpr int kKeys = 128;
   static constexpr int kCtas = 1;
+  static constexpr int kLead = 2;
   static constexpr int kCodes = kKeys * D;          // one ring slot: K or V codes
   static constexpr int kHalf = kKeys * D * 2;       // one fp16 operand tile
   static constexpr int kQuery = (kShared ? 2 : 1) * kHalf;
@@ -68,39 +69,6 @@ __device__ __forceinline__ uint64_t umma_desc_nmajor(uint32_t smem_addr, uint32_
   d |= 1ull << 46;
   d |= 2ull << 61;
   return d;
-}
-
-// Walks a run's segments: (request, head, row tile) and the key tiles of it
-// that the run has.
-struct WideWalk {
-  int b, hr, tile, tiles, count;
-  int64_t left;
-  bool all;
-};
-template <int kKeys>
-__device__ __forceinline__ WideWalk wide_begin(const TreeRun& r) {
-  WideWalk w;
-  w.b = r.b;
-  w.hr = r.hr;
-  w.tile = r.tile;
-  w.tiles = r.tiles;
-  w.left = r.end - r.begin;
-  w.count = static_cast<int>(min(static_cast<int64_t>(w.tiles - w.tile), w.left));
-  w.all = w.tile == 0 && w.count == w.tiles;
-  return w;
-}
-template <int kKeys>
-__device__ __forceinline__ void wide_next(const TreeArgs& a, int per, WideWalk& w) {
-  w.left -= w.count;
-  if (w.left <= 0) return;
-  w.tile = 0;
-  if (++w.hr == per) {
-    w.hr = 0;
-    ++w.b;
-    w.tiles = tree_tiles<kKeys>(a, w.b);
-  }
-  w.count = static_cast<int>(min(static_cast<int64_t>(w.tiles), w.left));
-  w.all = w.count == w.tiles;
 }
 
 __device__ __forceinline__ float2 mul2(float2 x, float2 y) { return __fmul2_rn(x, y); }
@@ -248,9 +216,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint32_t tmem_base = tmem_slot;
   const uint64_t budget = a.wait_budget_ns;
-  const int per = a.c.kv_heads * a.row_tiles;
-  const TreeRun run = tree_run<S::kKeys>(a);
-  WideWalk w = wide_begin<S::kKeys>(run);
+  TreeRun w = tree_run<S>(a);
   const int box = min(a.c.page_size, 64);
   const int box_shift = min(a.page_shift, 6);
   const int boxes = S::kKeys >> box_shift;
@@ -276,7 +242,8 @@ __global__ void __launch_bounds__(kWideThreads, 1)
     uint32_t done = 0;      // segments of this stream that had a job
     uint32_t counter = 0;   // key tiles of the run so far
     int part = 0;
-    while (w.left > 0) {
+    for (; w.left > 0; tree_next<S>(a, w)) {
+      if (w.count == 0) continue;
       const int kv = w.hr / a.row_tiles;
       const int row0 = (w.hr % a.row_tiles) * S::kRows + (kShared ? x * 128 : 0);
       const int64_t length = max(0, __ldg(a.c.lengths + w.b));
@@ -570,7 +537,6 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       // segment's first weights.
       if constexpr (!kShared) bar_sync(bar_id, kBarThreads);
       part = 1;
-      wide_next<S::kKeys>(a, per, w);
     }
   } else if (warp < 20) {
     // --------------------------------------------------------- conversion
@@ -621,7 +587,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
           mbar_arrive(smem_u32(side == 0 ? &k_full[buffer] : &v_full));
         }
       }
-      wide_next<S::kKeys>(a, per, w);
+      tree_next<S>(a, w);
     }
   } else {
     if (warp == 20) {
@@ -677,7 +643,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                           bar, 0, y, z);
           }
         }
-        wide_next<S::kKeys>(a, per, w);
+        tree_next<S>(a, w);
       }
       // Every copy has landed before the CTA's shared memory goes.
       for (int64_t i = max(int64_t(0), op - kRing); i < op; ++i)
@@ -719,7 +685,8 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         umma_commit(smem_u32(&s_full[x]));
         if (!kShared || x == 1) umma_commit(smem_u32(&k_empty[buffer]));
       };
-      while (w.left > 0 && ok) {
+      for (; w.left > 0 && ok; tree_next<S>(a, w)) {
+        if (w.count == 0) continue;
         const int jobs = kShared ? 2 * w.count : w.count;
         for (int x = 0; ok && x < (kShared ? 2 : 1); ++x)
           ok = mbar_wait_block(smem_u32(&q_full[x]), segment & 1, budget, a.status, kStatusTimeoutFull, abort_flag);
@@ -748,7 +715,6 @@ __global__ void __launch_bounds__(kWideThreads, 1)
           else
             umma_commit(smem_u32(&o_done[x]));
         }
-        wide_next<S::kKeys>(a, per, w);
       }
       // Everything issued completes before TMEM is freed.
       umma_commit(smem_u32(&mma_done));
