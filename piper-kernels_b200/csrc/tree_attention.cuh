@@ -72,12 +72,13 @@ struct TreeTile {
   static constexpr int kScales = kKeys * 4;
   static constexpr int kStage = 2 * kCodes + 2 * kScales;
   static constexpr int kStageAlloc = (kStage + 1023) / 1024 * 1024;
-  static constexpr int kJoinStride = 80;  // floats; 16 banks between rows
+  static constexpr int kJoinStride = 48;  // floats, 32 of them used; 16 banks between rows
   static constexpr int kJoin = WARPS * 16 * kJoinStride * 4;
   static constexpr int kState = 2 * WARPS * kRows * 4;
-  static constexpr int kFixed = kJoin + kState + kRows * 8 + 1024;
-  static constexpr int kCtas = 2;  // per SM
-  static constexpr int kLead = 3;  // a segment's start and end, in key tiles
+  static constexpr int kQuery = (D / 16) * 32 * 16;  // fragments
+  static constexpr int kFixed = kJoin + kState + kQuery + kRows * 8 + 512;
+  static constexpr int kCtas = D == 64 ? 4 : 2;  // per SM, what registers and stages allow
+  static constexpr int kLead = 5;  // a segment's start and end, in key tiles
   static constexpr int kFit = (227 * 1024 / kCtas - 1024 * 2 - kFixed) / kStageAlloc;
   static constexpr int kStages = kFit > 8 ? 8 : kFit;
   static constexpr int kAlloc = kStages * kStageAlloc + kFixed + 1024;
@@ -309,7 +310,8 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS>::kThreads, TreeTile<D, WARP
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   float* join = reinterpret_cast<float*>(smem + kStages * S::kStageAlloc);
   float* state = reinterpret_cast<float*>(smem + kStages * S::kStageAlloc + S::kJoin);
-  uint64_t* words = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(state) + S::kState);
+  uint4* query = reinterpret_cast<uint4*>(reinterpret_cast<uint8_t*>(state) + S::kState);
+  uint64_t* words = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(query) + S::kQuery);
   __shared__ __align__(8) uint64_t full_bar[kStages], empty_bar[kStages];
   __shared__ uint32_t valid[kStages];
   __shared__ uint32_t abort_word;
@@ -400,9 +402,17 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS>::kThreads, TreeTile<D, WARP
     const int row0 = (run.hr % a.row_tiles) * S::kRows;
     const bool all = run.all;
     const int64_t length = max(0, __ldg(a.c.lengths + b));
-    uint32_t q[kChunks][4];
+    // Every warp has the rows' factors; warp 0's fragments serve all (holding
+    // them cost each thread 32 registers, and the SM a CTA).
     float factor[2];
-    query_fragments<T, D>(a, b, kv, row0, q, factor);
+    {
+      uint32_t q[kChunks][4];
+      query_fragments<T, D>(a, b, kv, row0, q, factor);
+      if (warp == 0) {
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) query[c * 32 + lane] = make_uint4(q[c][0], q[c][1], q[c][2], q[c][3]);
+      }
+    }
     if (tid < S::kRows) {
       const int row = row0 + tid;
       uint64_t word = 0;
@@ -437,10 +447,13 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS>::kThreads, TreeTile<D, WARP
 #pragma unroll
           for (int x = 0; x < 4; ++x) k[x] ^= 0x80808080u;
 #pragma unroll
-          for (int x = 0; x < 2; ++x)
+          for (int x = 0; x < 2; ++x) {
+            const uint4 f = query[(c + x) * 32 + lane];
+            const uint32_t q[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
             for (int n = 0; n < 2; ++n)
-              mma16816(s[x][n], q[c + x], codes_f16<0x4140>(k[2 * x + n]), codes_f16<0x4342>(k[2 * x + n]));
+              mma16816(s[x][n], q, codes_f16<0x4140>(k[2 * x + n]), codes_f16<0x4342>(k[2 * x + n]));
+          }
         }
         float ks[2][2], vs[2][2], lv[2][2];
 #pragma unroll
@@ -544,7 +557,7 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS>::kThreads, TreeTile<D, WARP
       }
     }
     // ---- join the warps' parts: each row's reference and total, then the
-    // numerators, 64 head dimensions at a time.
+    // numerators, 32 head dimensions at a time.
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
@@ -580,10 +593,10 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS>::kThreads, TreeTile<D, WARP
       }
     }
 #pragma unroll
-    for (int d0 = 0; d0 < D; d0 += 64) {
+    for (int d0 = 0; d0 < D; d0 += 32) {
       float* mine = join + warp * 16 * S::kJoinStride;
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+      for (int c = 0; c < 2; ++c)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const float(&even)[4] = o[2 * (d0 / 16 + c)];
@@ -593,9 +606,9 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS>::kThreads, TreeTile<D, WARP
               make_float4(even[2 * h] * f, odd[2 * h] * f, even[2 * h + 1] * f, odd[2 * h + 1] * f);
         }
       bar_sync(1, WARPS * 32);
-      // 16 rows x 64 columns, four columns a thread.
-      for (int x = tid; x < 256; x += WARPS * 32) {
-        const int r = x / 16, d = (x % 16) * 4;
+      // 16 rows x 32 columns, four columns a thread.
+      for (int x = tid; x < 128; x += WARPS * 32) {
+        const int r = x / 8, d = (x % 8) * 4;
         float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {

@@ -38,7 +38,7 @@ struct WideTile {
   static constexpr int kRows = kShared ? 256 : 128;
   static constexpr int kKeys = 128;
   static constexpr int kCtas = 1;
-  static constexpr int kLead = 2;
+  static constexpr int kLead = 4;
   static constexpr int kCodes = kKeys * D;          // one ring slot: K or V codes
   static constexpr int kHalf = kKeys * D * 2;       // one fp16 operand tile
   static constexpr int kQuery = (kShared ? 2 : 1) * kHalf;
