@@ -385,7 +385,8 @@ extern "C" int piper_b200_verify_draft_tree(const float* target, const int64_t t
   if (batch <= 0 || batch > 65535) return invalid("batch must be in [1, 65535]");
   if (nodes <= 0 || nodes > piper::kMaxNodes) return invalid("nodes must be in [1, 64], got " + std::to_string(nodes));
   if (vocab <= 0 || vocab > (int64_t(1) << 30)) return invalid("vocab must be in [1, 2^30]");
-  int rc = use_device();
+  piper::host::Device device;
+  int rc = piper::host::ensure_device(&device);
   if (rc != PIPER_B200_OK) return rc;
   piper::VerifyArgs a{};
   a.target = target;
@@ -407,8 +408,24 @@ extern "C" int piper_b200_verify_draft_tree(const float* target, const int64_t t
   a.path = path;
   a.count = count;
   a.next = next_token;
-  piper::verify_simple_kernel<<<static_cast<unsigned>(batch), piper::kVerifyThreads, 0,
-                                static_cast<cudaStream_t>(stream)>>>(a);
-  PIPER_HOST_CUDA(cudaGetLastError());
+  a.vec = reinterpret_cast<uintptr_t>(target) % 16 == 0 && reinterpret_cast<uintptr_t>(draft) % 16 == 0 &&
+          reinterpret_cast<uintptr_t>(noise) % 16 == 0 && target_strides[0] % 4 == 0 && target_strides[1] % 4 == 0 &&
+          draft_strides[0] % 4 == 0 && draft_strides[1] % 4 == 0 && noise_stride % 4 == 0;
+  // CTAs a request: enough to fill the GPU, while each has 2048 words or more
+  // (fewer are read in the time that a join takes).
+  int ranks = 1;
+  while (ranks < 8 && vocab > int64_t(ranks) * 2048 && batch * ranks < 2 * device.sms) ranks *= 2;
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = static_cast<unsigned>(ranks);
+  attribute.val.clusterDim.y = 1;
+  attribute.val.clusterDim.z = 1;
+  cudaLaunchConfig_t config{};
+  config.gridDim = dim3(static_cast<unsigned>(ranks), static_cast<unsigned>(batch));
+  config.blockDim = dim3(piper::kVerifyThreads);
+  config.stream = static_cast<cudaStream_t>(stream);
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  PIPER_HOST_CUDA(cudaLaunchKernelEx(&config, piper::verify_tree_kernel, a));
   return PIPER_B200_OK;
 }

@@ -1,12 +1,32 @@
-// Rejection sampling over a drafted tree (simple form: one CTA per request).
+// Rejection sampling over a drafted tree.
+//
+// A request's walk needs few numbers while it accepts: target[x] and draft[x]
+// of each drafted token at its parent, which are fetched for all nodes at
+// once.  A whole row is read only where the walk rejects: with r the rest of
+// the target's distribution and q the draft's,
+//   total = sum_v max(r[v] - q[v], 0),   r <- max(r - q, 0) / total
+// before a further sibling can be tested, and at the end for the next token,
+//   argmax_v r[v] / noise[v].
+// The rest after several rejections is computed again from the rows and the
+// totals, so that nothing is written back.  Divisions are IEEE and the decisions
+// follow the definition's roundings; only the totals' sums are in another order.
+//
+// Bound: memory (12 bytes a word for the last pass), and with few requests the
+// latency of the passes that follow one another.  A cluster of CTAs shares a
+// request's vocabulary and joins its sums and maxima through distributed
+// shared memory, in rank order.
 #pragma once
 
+#include <cooperative_groups.h>
 #include <math.h>
 #include <stdint.h>
 
+#include "kv_cache.cuh"
+
 namespace piper {
 
-constexpr int kVerifyThreads = 1024;
+constexpr int kVerifyThreads = 512;
+constexpr int kVerifyUnroll = 4;  // 16-byte loads in flight of each row
 
 struct VerifyArgs {
   const float* target;
@@ -19,6 +39,7 @@ struct VerifyArgs {
   int64_t tokens_stride, parents_stride, uniform_stride, noise_stride;
   int nodes;
   int64_t vocab;
+  int vec;  // rows of target, draft and noise allow 16-byte loads
   int32_t* path;
   int32_t* count;
   int64_t* next;
@@ -33,77 +54,171 @@ __device__ __forceinline__ float rest_of(float p, float q, const float* totals, 
   return r;
 }
 
-__global__ void __launch_bounds__(kVerifyThreads) verify_simple_kernel(VerifyArgs a) {
-  __shared__ float totals[64];
-  __shared__ float part[32];
-  __shared__ float best_s[32];
-  __shared__ int64_t best_i[32];
-  const int64_t b = blockIdx.x;
+struct VerifyBest {
+  float score;
+  int64_t at;
+};
+__device__ __forceinline__ VerifyBest verify_better(VerifyBest x, VerifyBest y) {
+  return y.score > x.score || (y.score == x.score && y.at < x.at) ? y : x;
+}
+
+// Calls body(v, p, q, e) for this thread's words of [begin, end): the target's,
+// the draft's and the noise's values (0 where a pass does not read them).
+template <bool kDraft, bool kNoise, typename Body>
+__device__ __forceinline__ void verify_words(const VerifyArgs& a, const float* p, const float* q, const float* e,
+                                             int64_t begin, int64_t end, Body body) {
+  int64_t v = begin + threadIdx.x;
+  if (a.vec) {
+    // `begin` is a multiple of 4.
+    const int64_t whole = begin + (end - begin) / 4 * 4;
+    int64_t u = begin + threadIdx.x * 4;
+    for (; u < whole; u += int64_t(kVerifyThreads) * 4 * kVerifyUnroll) {
+      float4 pw[kVerifyUnroll], qw[kVerifyUnroll], ew[kVerifyUnroll];
+#pragma unroll
+      for (int k = 0; k < kVerifyUnroll; ++k) {
+        const int64_t w = u + int64_t(k) * kVerifyThreads * 4;
+        pw[k] = qw[k] = ew[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (w < whole) {
+          pw[k] = __ldg(reinterpret_cast<const float4*>(p + w));
+          if (kDraft) qw[k] = __ldg(reinterpret_cast<const float4*>(q + w));
+          if (kNoise) ew[k] = __ldg(reinterpret_cast<const float4*>(e + w));
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < kVerifyUnroll; ++k) {
+        const int64_t w = u + int64_t(k) * kVerifyThreads * 4;
+        if (w < whole) {
+          body(w, pw[k].x, qw[k].x, ew[k].x);
+          body(w + 1, pw[k].y, qw[k].y, ew[k].y);
+          body(w + 2, pw[k].z, qw[k].z, ew[k].z);
+          body(w + 3, pw[k].w, qw[k].w, ew[k].w);
+        }
+      }
+    }
+    v = whole + threadIdx.x;
+  }
+  for (; v < end; v += int64_t(kVerifyThreads) * kVerifyUnroll) {
+    float pw[kVerifyUnroll], qw[kVerifyUnroll], ew[kVerifyUnroll];
+#pragma unroll
+    for (int k = 0; k < kVerifyUnroll; ++k) {
+      const int64_t w = v + int64_t(k) * kVerifyThreads;
+      pw[k] = qw[k] = ew[k] = 0.0f;
+      if (w < end) {
+        pw[k] = __ldg(p + w);
+        if (kDraft) qw[k] = __ldg(q + w);
+        if (kNoise) ew[k] = __ldg(e + w);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kVerifyUnroll; ++k)
+      if (v + int64_t(k) * kVerifyThreads < end) body(v + int64_t(k) * kVerifyThreads, pw[k], qw[k], ew[k]);
+  }
+}
+
+// grid (CTAs of a cluster, batch), a cluster to a request.
+__global__ void __launch_bounds__(kVerifyThreads) verify_tree_kernel(VerifyArgs a) {
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  constexpr int kWarps = kVerifyThreads / 32;
+  __shared__ float node_p[kMaxNodes], node_q[kMaxNodes], node_u[kMaxNodes];
+  __shared__ int node_parent[kMaxNodes];  // -1: absent
+  __shared__ float totals[kMaxNodes];
+  __shared__ float warp_sum[kWarps], joined_sum[2];  // by turn
+  __shared__ VerifyBest warp_best[kWarps], joined_best;
+  const int64_t b = blockIdx.y;
+  const int ranks = static_cast<int>(cluster.num_blocks());
+  const int rank = static_cast<int>(cluster.block_rank());
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
-  int current = 0, rejected = 0, count = 1;
+  // This CTA's words: a multiple of 4 to each rank.
+  const int64_t per = ((a.vocab + ranks - 1) / ranks + 3) / 4 * 4;
+  const int64_t begin = min(a.vocab, per * rank), end = min(a.vocab, begin + per);
+  if (tid < a.nodes) {
+    const int64_t x = tid == 0 ? -1 : __ldg(reinterpret_cast<const long long*>(a.tokens) + b * a.tokens_stride + tid);
+    const int parent = tid == 0 ? -1 : __ldg(a.parents + b * a.parents_stride + tid);
+    const bool there = x >= 0 && x < a.vocab && parent >= 0 && parent < tid;
+    node_parent[tid] = there ? parent : -1;
+    if (there) {
+      node_p[tid] = __ldg(a.target + b * a.ts[0] + parent * a.ts[1] + x);
+      node_q[tid] = __ldg(a.draft + b * a.ds[0] + parent * a.ds[1] + x);
+      node_u[tid] = __ldg(a.uniform + b * a.uniform_stride + tid);
+    }
+  }
+  __syncthreads();
+  // Every thread of the cluster takes the same walk.
+  int current = 0, rejected = 0, count = 1, turn = 0;
   int32_t* path = a.path + b * a.nodes;
-  if (tid == 0) path[0] = 0;
+  if (rank == 0 && tid == 0) path[0] = 0;
   for (int i = 1; i < a.nodes; ++i) {
-    const int64_t x = a.tokens[b * a.tokens_stride + i];
-    if (a.parents[b * a.parents_stride + i] != current || x < 0 || x >= a.vocab) continue;
-    const float* p = a.target + b * a.ts[0] + current * a.ts[1];
-    const float* q = a.draft + b * a.ds[0] + current * a.ds[1];
-    if (a.uniform[b * a.uniform_stride + i] * q[x] < rest_of(p[x], q[x], totals, rejected)) {
-      if (tid == 0) path[count] = i;
+    if (node_parent[i] != current) continue;
+    const float p = node_p[i], q = node_q[i];
+    if (node_u[i] * q < rest_of(p, q, totals, rejected)) {
+      if (rank == 0 && tid == 0) path[count] = i;
       ++count;
       current = i;
       rejected = 0;
       continue;
     }
+    const float* pr = a.target + b * a.ts[0] + current * a.ts[1];
+    const float* qr = a.draft + b * a.ds[0] + current * a.ds[1];
     float sum = 0.0f;
-    for (int64_t v = tid; v < a.vocab; v += kVerifyThreads)
-      sum += fmaxf(rest_of(p[v], q[v], totals, rejected) - q[v], 0.0f);
+    verify_words<true, false>(a, pr, qr, nullptr, begin, end, [&](int64_t, float x, float y, float) {
+      sum += fmaxf(rest_of(x, y, totals, rejected) - y, 0.0f);
+    });
+#pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) part[warp] = sum;
+    if (lane == 0) warp_sum[warp] = sum;
     __syncthreads();
     if (tid == 0) {
+      float mine = 0.0f;
+      for (int w = 0; w < kWarps; ++w) mine += warp_sum[w];
+      joined_sum[turn] = mine;
+    }
+    cluster.sync();
+    if (tid == 0) {
       float total = 0.0f;
-      for (int w = 0; w < 32; ++w) total += part[w];
+      for (int r = 0; r < ranks; ++r) total += *cluster.map_shared_rank(&joined_sum[turn], r);
       totals[rejected] = total;
     }
+    // The other turn's sums are written only after every rank has read these:
+    // each passes the next cluster.sync after its reading.
+    turn ^= 1;
     __syncthreads();
     ++rejected;
   }
-  const float* p = a.target + b * a.ts[0] + current * a.ts[1];
-  const float* q = a.draft + b * a.ds[0] + current * a.ds[1];
-  float best = -1.0f;
-  int64_t at = 0;
-  for (int64_t v = tid; v < a.vocab; v += kVerifyThreads) {
-    const float r = rejected == 0 ? p[v] : rest_of(p[v], q[v], totals, rejected);
-    const float s = __fdiv_rn(r, a.noise[b * a.noise_stride + v]);
-    if (s > best) {
-      best = s;
-      at = v;
-    }
-  }
-  for (int o = 16; o > 0; o >>= 1) {
-    const float s = __shfl_xor_sync(0xffffffffu, best, o);
-    const int64_t j = __shfl_xor_sync(0xffffffffu, at, o);
-    if (s > best || (s == best && j < at)) {
-      best = s;
-      at = j;
-    }
-  }
-  if (lane == 0) {
-    best_s[warp] = best;
-    best_i[warp] = at;
-  }
+  const float* pr = a.target + b * a.ts[0] + current * a.ts[1];
+  const float* qr = a.draft + b * a.ds[0] + current * a.ds[1];
+  const float* er = a.noise + b * a.noise_stride;
+  VerifyBest best{-1.0f, 0};
+  auto race = [&](int64_t v, float r, float e) {
+    const float s = __fdiv_rn(r, e);
+    if (s > best.score) best = VerifyBest{s, v};  // (a thread's words ascend)
+  };
+  if (rejected == 0)
+    verify_words<false, true>(a, pr, qr, er, begin, end, [&](int64_t v, float x, float, float e) { race(v, x, e); });
+  else
+    verify_words<true, true>(a, pr, qr, er, begin, end, [&](int64_t v, float x, float y, float e) {
+      race(v, rest_of(x, y, totals, rejected), e);
+    });
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    best = verify_better(best, VerifyBest{__shfl_xor_sync(0xffffffffu, best.score, o),
+                                          __shfl_xor_sync(0xffffffffu, best.at, o)});
+  if (lane == 0) warp_best[warp] = best;
   __syncthreads();
   if (tid == 0) {
-    for (int w = 1; w < 32; ++w)
-      if (best_s[w] > best || (best_s[w] == best && best_i[w] < at)) {
-        best = best_s[w];
-        at = best_i[w];
-      }
-    a.next[b] = best < 0.0f ? 0 : at;
-    a.count[b] = count;
+    for (int w = 1; w < kWarps; ++w) best = verify_better(best, warp_best[w]);
+    joined_best = best;
   }
-  for (int i = count + tid; i < a.nodes; i += kVerifyThreads) path[i] = -1;
+  cluster.sync();
+  if (rank == 0) {
+    if (tid == 0) {
+      for (int r = 1; r < ranks; ++r) best = verify_better(best, *cluster.map_shared_rank(&joined_best, r));
+      a.next[b] = best.score < 0.0f ? 0 : best.at;
+      a.count[b] = count;
+    }
+    for (int i = count + tid; i < a.nodes; i += kVerifyThreads) path[i] = -1;
+  }
+  cluster.sync();  // shared memory stays until rank 0 has read it
 }
 
 }  // namespace piper
