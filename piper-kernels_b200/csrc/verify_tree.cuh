@@ -8,8 +8,10 @@
 // before a further sibling can be tested, and at the end for the next token,
 //   argmax_v r[v] / noise[v].
 // The rest after several rejections is computed again from the rows and the
-// totals, so that nothing is written back.  Divisions are IEEE and the decisions
-// follow the definition's roundings; only the totals' sums are in another order.
+// over, so that nothing is written back.  All is fp32; a total divides as its
+// reciprocal multiplies (an IEEE division for each word and rejection made the
+// passes twice as long), the last division, by the noise, is IEEE: equal
+// quotients are equal, and go to the lowest index.
 //
 // Bound: memory (12 bytes a word for the last pass), and with few requests the
 // latency of the passes that follow one another.  A cluster of CTAs shares a
@@ -45,18 +47,17 @@ struct VerifyArgs {
   int64_t* next;
 };
 
-// What is left of probability p after taking out the draft's q once for each
-// of the n totals: max(r - q, 0) / total, or r where the total is zero.
-__device__ __forceinline__ float rest_of(float p, float q, const float* totals, int n) {
+// What is left of probability p after taking out the draft's q n times:
+// max(r - q, 0) over each total, given as reciprocals.
+__device__ __forceinline__ float rest_of(float p, float q, const float* over, int n) {
   float r = p;
-  for (int k = 0; k < n; ++k)
-    if (totals[k] > 0.0f) r = __fdiv_rn(fmaxf(r - q, 0.0f), totals[k]);
+  for (int k = 0; k < n; ++k) r = fmaxf(r - q, 0.0f) * over[k];
   return r;
 }
 
 struct VerifyBest {
   float score;
-  int64_t at;
+  int at;
 };
 __device__ __forceinline__ VerifyBest verify_better(VerifyBest x, VerifyBest y) {
   return y.score > x.score || (y.score == x.score && y.at < x.at) ? y : x;
@@ -64,29 +65,28 @@ __device__ __forceinline__ VerifyBest verify_better(VerifyBest x, VerifyBest y) 
 
 // Calls body(v, p, q, e) for this thread's words of [begin, end): the target's,
 // the draft's and the noise's values (0 where a pass does not read them).
+// `begin` is a multiple of 4.
 template <bool kDraft, bool kNoise, typename Body>
 __device__ __forceinline__ void verify_words(const VerifyArgs& a, const float* p, const float* q, const float* e,
-                                             int64_t begin, int64_t end, Body body) {
-  int64_t v = begin + threadIdx.x;
+                                             int begin, int end, Body body) {
+  int v = begin + threadIdx.x;
   if (a.vec) {
-    // `begin` is a multiple of 4.
-    const int64_t whole = begin + (end - begin) / 4 * 4;
-    int64_t u = begin + threadIdx.x * 4;
-    for (; u < whole; u += int64_t(kVerifyThreads) * 4 * kVerifyUnroll) {
+    const int whole = begin + (end - begin) / 4 * 4;
+    constexpr int kStep = kVerifyThreads * 4;
+    for (int u = begin + threadIdx.x * 4; u < whole; u += kStep * kVerifyUnroll) {
       float4 pw[kVerifyUnroll], qw[kVerifyUnroll], ew[kVerifyUnroll];
 #pragma unroll
       for (int k = 0; k < kVerifyUnroll; ++k) {
-        const int64_t w = u + int64_t(k) * kVerifyThreads * 4;
         pw[k] = qw[k] = ew[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (w < whole) {
-          pw[k] = __ldg(reinterpret_cast<const float4*>(p + w));
-          if (kDraft) qw[k] = __ldg(reinterpret_cast<const float4*>(q + w));
-          if (kNoise) ew[k] = __ldg(reinterpret_cast<const float4*>(e + w));
+        if (u + k * kStep < whole) {
+          pw[k] = __ldg(reinterpret_cast<const float4*>(p + u + k * kStep));
+          if (kDraft) qw[k] = __ldg(reinterpret_cast<const float4*>(q + u + k * kStep));
+          if (kNoise) ew[k] = __ldg(reinterpret_cast<const float4*>(e + u + k * kStep));
         }
       }
 #pragma unroll
       for (int k = 0; k < kVerifyUnroll; ++k) {
-        const int64_t w = u + int64_t(k) * kVerifyThreads * 4;
+        const int w = u + k * kStep;
         if (w < whole) {
           body(w, pw[k].x, qw[k].x, ew[k].x);
           body(w + 1, pw[k].y, qw[k].y, ew[k].y);
@@ -97,11 +97,11 @@ __device__ __forceinline__ void verify_words(const VerifyArgs& a, const float* p
     }
     v = whole + threadIdx.x;
   }
-  for (; v < end; v += int64_t(kVerifyThreads) * kVerifyUnroll) {
+  for (; v < end; v += kVerifyThreads * kVerifyUnroll) {
     float pw[kVerifyUnroll], qw[kVerifyUnroll], ew[kVerifyUnroll];
 #pragma unroll
     for (int k = 0; k < kVerifyUnroll; ++k) {
-      const int64_t w = v + int64_t(k) * kVerifyThreads;
+      const int w = v + k * kVerifyThreads;
       pw[k] = qw[k] = ew[k] = 0.0f;
       if (w < end) {
         pw[k] = __ldg(p + w);
@@ -111,18 +111,18 @@ __device__ __forceinline__ void verify_words(const VerifyArgs& a, const float* p
     }
 #pragma unroll
     for (int k = 0; k < kVerifyUnroll; ++k)
-      if (v + int64_t(k) * kVerifyThreads < end) body(v + int64_t(k) * kVerifyThreads, pw[k], qw[k], ew[k]);
+      if (v + k * kVerifyThreads < end) body(v + k * kVerifyThreads, pw[k], qw[k], ew[k]);
   }
 }
 
 // grid (CTAs of a cluster, batch), a cluster to a request.
-__global__ void __launch_bounds__(kVerifyThreads) verify_tree_kernel(VerifyArgs a) {
+__global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(VerifyArgs a) {
   namespace cg = cooperative_groups;
   cg::cluster_group cluster = cg::this_cluster();
   constexpr int kWarps = kVerifyThreads / 32;
   __shared__ float node_p[kMaxNodes], node_q[kMaxNodes], node_u[kMaxNodes];
   __shared__ int node_parent[kMaxNodes];  // -1: absent
-  __shared__ float totals[kMaxNodes];
+  __shared__ float over[kMaxNodes];
   __shared__ float warp_sum[kWarps], joined_sum[2];  // by turn
   __shared__ VerifyBest warp_best[kWarps], joined_best;
   const int64_t b = blockIdx.y;
@@ -130,8 +130,9 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_tree_kernel(VerifyArgs 
   const int rank = static_cast<int>(cluster.block_rank());
   const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
   // This CTA's words: a multiple of 4 to each rank.
-  const int64_t per = ((a.vocab + ranks - 1) / ranks + 3) / 4 * 4;
-  const int64_t begin = min(a.vocab, per * rank), end = min(a.vocab, begin + per);
+  const int vocab = static_cast<int>(a.vocab);
+  const int per = ((vocab + ranks - 1) / ranks + 3) / 4 * 4;
+  const int begin = min(vocab, per * rank), end = min(vocab, begin + per);
   if (tid < a.nodes) {
     const int64_t x = tid == 0 ? -1 : __ldg(reinterpret_cast<const long long*>(a.tokens) + b * a.tokens_stride + tid);
     const int parent = tid == 0 ? -1 : __ldg(a.parents + b * a.parents_stride + tid);
@@ -151,7 +152,7 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_tree_kernel(VerifyArgs 
   for (int i = 1; i < a.nodes; ++i) {
     if (node_parent[i] != current) continue;
     const float p = node_p[i], q = node_q[i];
-    if (node_u[i] * q < rest_of(p, q, totals, rejected)) {
+    if (node_u[i] * q < rest_of(p, q, over, rejected)) {
       if (rank == 0 && tid == 0) path[count] = i;
       ++count;
       current = i;
@@ -161,8 +162,8 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_tree_kernel(VerifyArgs 
     const float* pr = a.target + b * a.ts[0] + current * a.ts[1];
     const float* qr = a.draft + b * a.ds[0] + current * a.ds[1];
     float sum = 0.0f;
-    verify_words<true, false>(a, pr, qr, nullptr, begin, end, [&](int64_t, float x, float y, float) {
-      sum += fmaxf(rest_of(x, y, totals, rejected) - y, 0.0f);
+    verify_words<true, false>(a, pr, qr, nullptr, begin, end, [&](int, float x, float y, float) {
+      sum += fmaxf(rest_of(x, y, over, rejected) - y, 0.0f);
     });
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
@@ -174,30 +175,30 @@ __global__ void __launch_bounds__(kVerifyThreads) verify_tree_kernel(VerifyArgs 
       joined_sum[turn] = mine;
     }
     cluster.sync();
-    if (tid == 0) {
-      float total = 0.0f;
-      for (int r = 0; r < ranks; ++r) total += *cluster.map_shared_rank(&joined_sum[turn], r);
-      totals[rejected] = total;
-    }
+    float total = 0.0f;
+    for (int r = 0; r < ranks; ++r) total += *cluster.map_shared_rank(&joined_sum[turn], r);
     // The other turn's sums are written only after every rank has read these:
     // each passes the next cluster.sync after its reading.
     turn ^= 1;
+    if (total > 0.0f) {  // else nothing would be left: rest stays as it was
+      if (tid == 0) over[rejected] = 1.0f / total;
+      ++rejected;
+    }
     __syncthreads();
-    ++rejected;
   }
   const float* pr = a.target + b * a.ts[0] + current * a.ts[1];
   const float* qr = a.draft + b * a.ds[0] + current * a.ds[1];
   const float* er = a.noise + b * a.noise_stride;
   VerifyBest best{-1.0f, 0};
-  auto race = [&](int64_t v, float r, float e) {
+  auto race = [&](int v, float r, float e) {
     const float s = __fdiv_rn(r, e);
     if (s > best.score) best = VerifyBest{s, v};  // (a thread's words ascend)
   };
   if (rejected == 0)
-    verify_words<false, true>(a, pr, qr, er, begin, end, [&](int64_t v, float x, float, float e) { race(v, x, e); });
+    verify_words<false, true>(a, pr, qr, er, begin, end, [&](int v, float x, float, float e) { race(v, x, e); });
   else
-    verify_words<true, true>(a, pr, qr, er, begin, end, [&](int64_t v, float x, float y, float e) {
-      race(v, rest_of(x, y, totals, rejected), e);
+    verify_words<true, true>(a, pr, qr, er, begin, end, [&](int v, float x, float y, float e) {
+      race(v, rest_of(x, y, over, rejected), e);
     });
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
