@@ -306,6 +306,7 @@ int piper_b200_sage2pp_fwd(const void* query, const int64_t query_strides[3], co
  *   key_mean                  f32  [kv_heads, head_dim] or NULL: subtracted
  *                             from keys before quantisation and added when
  *                             they are read back; a softmax does not see it
+ *                             (16-byte aligned)
  *   block_table               int32 [batch, table_width], rows table_stride
  *                             elements apart
  *   lengths                   int32 [batch]

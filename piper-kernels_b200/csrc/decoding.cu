@@ -44,6 +44,7 @@ int check_cache(const piper_b200_kv_cache_t* c) {
   if (c->table_stride < 0) return invalid("table_stride must not be negative");
   if (reinterpret_cast<uintptr_t>(c->key_codes) % 16 != 0 || reinterpret_cast<uintptr_t>(c->value_codes) % 16 != 0)
     return invalid("the cache's codes must be 16-byte aligned");
+  if (reinterpret_cast<uintptr_t>(c->key_mean) % 16 != 0) return invalid("key_mean must be 16-byte aligned");
   return PIPER_B200_OK;
 }
 
@@ -64,7 +65,7 @@ bool rows_aligned16(const void* p, const int64_t s[3]) {
 
 // CTAs for `rows` rows of D/8 lanes each.
 int row_blocks(int64_t rows, int d, unsigned* blocks) {
-  const int64_t per = piper::kCacheThreads / (d / 8);
+  const int64_t per = piper::kCacheThreads / (d / 8) * piper::kCachePasses;
   const int64_t n = (rows + per - 1) / per;
   if (n > 0x7fffffff) return invalid("too many rows for one call");
   *blocks = static_cast<unsigned>(n);

@@ -43,8 +43,11 @@ struct CacheRowsArgs {
   int page_shift;
 };
 
-// Codes of eight values, packed.
+// Codes of eight values, packed.  The division-free rounding of the prepass is
+// exact while the scale and its reciprocal are normal numbers; other rows
+// (nearly subnormal, or not finite) divide.
 __device__ __forceinline__ uint2 row_codes(const float (&x)[8], float scale) {
+  if (scale >= 0x1p-100f && scale <= 0x1p+121f) return pack_codes(x, scale, __frcp_rn(scale));
   uint32_t w[2] = {0u, 0u};
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -54,44 +57,88 @@ __device__ __forceinline__ uint2 row_codes(const float (&x)[8], float scale) {
   return make_uint2(w[0], w[1]);
 }
 
+// Eight fp32 of the key mean.
+__device__ __forceinline__ void mean8(const float* p, float (&m)[8]) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+  m[0] = a.x, m[1] = a.y, m[2] = a.z, m[3] = a.w, m[4] = b.x, m[5] = b.y, m[6] = b.z, m[7] = b.w;
+}
+
+// (token, head) of the rows that a thread takes: `row0` and every `step`-th
+// after it.  `inner` varies fastest; one 64-bit division for all of them.
+struct CacheRowWalk {
+  int64_t outer0;
+  unsigned inner0, inner;
+  __device__ CacheRowWalk(int64_t row0, int64_t inner_count) {
+    inner = static_cast<unsigned>(inner_count);
+    outer0 = row0 / inner_count;
+    inner0 = static_cast<unsigned>(row0 - outer0 * inner_count);
+  }
+  __device__ __forceinline__ void at(unsigned ahead, int64_t* outer, unsigned* in) const {
+    const unsigned x = inner0 + ahead, more = x / inner;
+    *outer = outer0 + more;
+    *in = x - more * inner;
+  }
+};
+
 // D/8 consecutive lanes hold a row, eight values each: K and V of one (token,
-// head) per lane group.  grid (ceil(tokens * kv_heads / rows per CTA), batch);
-// heads vary fastest, the order in which a projection leaves them.
+// head) per lane group, kCachePasses rows a thread with all their loads in
+// flight.  grid (ceil(tokens * kv_heads / rows per CTA), batch); heads vary
+// fastest, the order in which a projection leaves them.
+constexpr int kCachePasses = 2;
+
 template <typename T, int D, bool kVec16>
 __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(CacheRowsArgs a) {
   constexpr int kLanes = D / 8;
+  constexpr int kRows = kCacheThreads / kLanes;  // a pass
   const int b = blockIdx.y;
-  const int64_t row = (static_cast<int64_t>(blockIdx.x) * kCacheThreads + threadIdx.x) / kLanes;
   const int lane = threadIdx.x % kLanes;
-  const int64_t token = row / a.c.kv_heads;
-  const int head = static_cast<int>(row - token * a.c.kv_heads);
+  const CacheRowWalk walk(static_cast<int64_t>(blockIdx.x) * (kRows * kCachePasses), a.c.kv_heads);
   int64_t n = a.tokens;
   if (a.counts != nullptr) n = min(n, static_cast<int64_t>(__ldg(a.counts + b)));
-  const int64_t at = token < n ? cache_row(a.c, a.page_shift, b, head, __ldg(a.c.lengths + b) + token) : -1;
+  const int64_t length = __ldg(a.c.lengths + b);
+  uint4 raw[kCachePasses][2];
+  int64_t token[kCachePasses];
+  unsigned head[kCachePasses];
 #pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    float x[8] = {};
-    if (at >= 0) {
-      const T* p = static_cast<const T*>(a.in[side]) + b * a.stride[side][0] + head * a.stride[side][1] +
-                   token * a.stride[side][2] + lane * 8;
-      unpack8<T>(load_raw8<T, kVec16>(p), x);
-      if (side == 0 && a.c.key_mean != nullptr) {
+  for (int p = 0; p < kCachePasses; ++p) {
+    walk.at(threadIdx.x / kLanes + p * kRows, &token[p], &head[p]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = __fsub_rn(x[i], __ldg(a.c.key_mean + head * D + lane * 8 + i));
-      }
+    for (int side = 0; side < 2; ++side) {
+      raw[p][side] = make_uint4(0u, 0u, 0u, 0u);
+      if (token[p] < n)
+        raw[p][side] = load_raw8<T, kVec16>(static_cast<const T*>(a.in[side]) + b * a.stride[side][0] +
+                                            head[p] * a.stride[side][1] + token[p] * a.stride[side][2] + lane * 8);
     }
-    // The largest magnitude; fmaxf would drop a NaN, so the bits are compared
-    // as integers (NaN above infinity above every finite magnitude).
-    uint32_t amax = 0u;
+  }
+  int64_t at[kCachePasses];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(x[i]) & 0x7fffffffu);
+  for (int p = 0; p < kCachePasses; ++p)
+    at[p] = token[p] < n ? cache_row(a.c, a.page_shift, b, head[p], length + token[p]) : -1;
 #pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    if (at < 0) continue;
-    const float scale = amax == 0u ? 1.0f : __fmul_rn(__uint_as_float(amax), 1.0f / 127.0f);
-    int8_t* codes = static_cast<int8_t*>(side == 0 ? a.c.key_codes : a.c.value_codes);
-    *reinterpret_cast<uint2*>(codes + at * D + lane * 8) = row_codes(x, scale);
-    if (lane == 0) (side == 0 ? a.c.key_scales : a.c.value_scales)[at] = scale;
+  for (int p = 0; p < kCachePasses; ++p) {
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      float x[8];
+      unpack8<T>(raw[p][side], x);
+      if (side == 0 && a.c.key_mean != nullptr && at[p] >= 0) {
+        float m[8];
+        mean8(a.c.key_mean + head[p] * D + lane * 8, m);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = __fsub_rn(x[i], m[i]);
+      }
+      // The largest magnitude; fmaxf would drop a NaN, so the bits are compared
+      // as integers (NaN above infinity above every finite magnitude).
+      uint32_t amax = 0u;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(x[i]) & 0x7fffffffu);
+#pragma unroll
+      for (int o = kLanes / 2; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      if (at[p] < 0) continue;
+      const float scale = amax == 0u ? 1.0f : __fmul_rn(__uint_as_float(amax), 1.0f / 127.0f);
+      int8_t* codes = static_cast<int8_t*>(side == 0 ? a.c.key_codes : a.c.value_codes);
+      *reinterpret_cast<uint2*>(codes + at[p] * D + lane * 8) = row_codes(x, scale);
+      if (lane == 0) (side == 0 ? a.c.key_scales : a.c.value_scales)[at[p]] = scale;
+    }
   }
 }
 
@@ -109,38 +156,59 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
 template <typename T, int D>
 __global__ void __launch_bounds__(kCacheThreads) cache_read_kernel(CacheRowsArgs a) {
   constexpr int kLanes = D / 8;
+  constexpr int kRows = kCacheThreads / kLanes;
   const int b = blockIdx.y;
-  const int64_t row = (static_cast<int64_t>(blockIdx.x) * kCacheThreads + threadIdx.x) / kLanes;
   const int lane = threadIdx.x % kLanes;
-  const int64_t head64 = row / a.tokens;
-  if (head64 >= a.c.kv_heads) return;
-  const int head = static_cast<int>(head64);
-  const int64_t token = row - head64 * a.tokens;
+  const CacheRowWalk walk(static_cast<int64_t>(blockIdx.x) * (kRows * kCachePasses), a.tokens);
   int64_t n = a.tokens;
   if (a.counts != nullptr) n = min(n, static_cast<int64_t>(__ldg(a.counts + b)));
-  const int64_t at = token < n ? cache_row(a.c, a.page_shift, b, head, __ldg(a.c.lengths + b) + token) : -1;
+  const int64_t length = __ldg(a.c.lengths + b);
+  int64_t at[kCachePasses], head[kCachePasses];
+  unsigned token[kCachePasses];
 #pragma unroll
-  for (int side = 0; side < 2; ++side) {
-    float x[8] = {};
-    if (at >= 0) {
-      const int8_t* codes = static_cast<const int8_t*>(side == 0 ? a.c.key_codes : a.c.value_codes);
-      const uint2 w = *reinterpret_cast<const uint2*>(codes + at * D + lane * 8);
-      const float scale = (side == 0 ? a.c.key_scales : a.c.value_scales)[at];
-      const int8_t* q = reinterpret_cast<const int8_t*>(&w);
+  for (int p = 0; p < kCachePasses; ++p) {
+    walk.at(threadIdx.x / kLanes + p * kRows, &head[p], &token[p]);
+    at[p] = head[p] < a.c.kv_heads && token[p] < n
+                ? cache_row(a.c, a.page_shift, b, static_cast<int>(head[p]), length + token[p])
+                : -1;
+  }
+  uint2 w[kCachePasses][2];
+  float scale[kCachePasses][2];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(static_cast<float>(q[i]), scale);
-      if (side == 0 && a.c.key_mean != nullptr) {
+  for (int p = 0; p < kCachePasses; ++p)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = __fadd_rn(x[i], __ldg(a.c.key_mean + head * D + lane * 8 + i));
+    for (int side = 0; side < 2; ++side) {
+      w[p][side] = make_uint2(0u, 0u);
+      scale[p][side] = 0.0f;
+      if (at[p] >= 0) {
+        const int8_t* codes = static_cast<const int8_t*>(side == 0 ? a.c.key_codes : a.c.value_codes);
+        w[p][side] = *reinterpret_cast<const uint2*>(codes + at[p] * D + lane * 8);
+        scale[p][side] = (side == 0 ? a.c.key_scales : a.c.value_scales)[at[p]];
       }
     }
-    uint4 w;
-    w.x = pack2(x[0], x[1], T());
-    w.y = pack2(x[2], x[3], T());
-    w.z = pack2(x[4], x[5], T());
-    w.w = pack2(x[6], x[7], T());
-    const int64_t o = ((static_cast<int64_t>(b) * a.c.kv_heads + head) * a.tokens + token) * D + lane * 8;
-    *reinterpret_cast<uint4*>(static_cast<T*>(a.out[side]) + o) = w;
+#pragma unroll
+  for (int p = 0; p < kCachePasses; ++p) {
+    if (head[p] >= a.c.kv_heads) continue;
+#pragma unroll
+    for (int side = 0; side < 2; ++side) {
+      float x[8];
+      const int8_t* q = reinterpret_cast<const int8_t*>(&w[p][side]);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(static_cast<float>(q[i]), scale[p][side]);
+      if (side == 0 && a.c.key_mean != nullptr && at[p] >= 0) {
+        float m[8];
+        mean8(a.c.key_mean + head[p] * D + lane * 8, m);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = __fadd_rn(x[i], m[i]);
+      }
+      uint4 y;
+      y.x = pack2(x[0], x[1], T());
+      y.y = pack2(x[2], x[3], T());
+      y.z = pack2(x[4], x[5], T());
+      y.w = pack2(x[6], x[7], T());
+      const int64_t o = ((static_cast<int64_t>(b) * a.c.kv_heads + head[p]) * a.tokens + token[p]) * D + lane * 8;
+      *reinterpret_cast<uint4*>(static_cast<T*>(a.out[side]) + o) = y;
+    }
   }
 }
 
