@@ -63,9 +63,9 @@ bool rows_aligned16(const void* p, const int64_t s[3]) {
   return reinterpret_cast<uintptr_t>(p) % 16 == 0 && s[0] % 8 == 0 && s[1] % 8 == 0 && s[2] % 8 == 0;
 }
 
-// CTAs for `rows` rows of D/8 lanes each.
+// CTAs for `rows` rows of D/16 lanes each.
 int row_blocks(int64_t rows, int d, unsigned* blocks) {
-  const int64_t per = piper::kCacheThreads / (d / 8) * piper::kCachePasses;
+  const int64_t per = piper::kCacheThreads / (d / 16) * piper::kCachePasses;
   const int64_t n = (rows + per - 1) / per;
   if (n > 0x7fffffff) return invalid("too many rows for one call");
   *blocks = static_cast<unsigned>(n);

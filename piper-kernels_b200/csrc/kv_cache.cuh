@@ -43,11 +43,16 @@ struct CacheRowsArgs {
   int page_shift;
 };
 
-// Codes of eight values, packed.  The division-free rounding of the prepass is
-// exact while the scale and its reciprocal are normal numbers; other rows
+// Codes of eight values, packed.  The prepass's division-free rounding needs
+// the quotient to 2^-14: |x / s| <= 127 and an approximate reciprocal (2^-23)
+// give 2^-15, while the scale and its reciprocal are normal numbers; other rows
 // (nearly subnormal, or not finite) divide.
 __device__ __forceinline__ uint2 row_codes(const float (&x)[8], float scale) {
-  if (scale >= 0x1p-100f && scale <= 0x1p+121f) return pack_codes(x, scale, __frcp_rn(scale));
+  if (scale >= 0x1p-100f && scale <= 0x1p+121f) {
+    float over;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(over) : "f"(scale));
+    return pack_codes(x, scale, over);
+  }
   uint32_t w[2] = {0u, 0u};
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
@@ -57,10 +62,30 @@ __device__ __forceinline__ uint2 row_codes(const float (&x)[8], float scale) {
   return make_uint2(w[0], w[1]);
 }
 
+// Largest magnitude; a NaN wins.
+__device__ __forceinline__ float amax3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(fabsf(b)), "f"(fabsf(c)));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // Eight fp32 of the key mean.
 __device__ __forceinline__ void mean8(const float* p, float (&m)[8]) {
   const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
   m[0] = a.x, m[1] = a.y, m[2] = a.z, m[3] = a.w, m[4] = b.x, m[5] = b.y, m[6] = b.z, m[7] = b.w;
+}
+
+// Four codes as floats: the byte plus 128 under the exponent of 2^23.
+__device__ __forceinline__ void codes_f32(uint32_t w, float (&x)[8], int at) {
+  const uint32_t u = w ^ 0x80808080u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    x[at + i] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7540u + i)) - 8388736.0f;
 }
 
 // (token, head) of the rows that a thread takes: `row0` and every `step`-th
@@ -80,15 +105,15 @@ struct CacheRowWalk {
   }
 };
 
-// D/8 consecutive lanes hold a row, eight values each: K and V of one (token,
-// head) per lane group, kCachePasses rows a thread with all their loads in
-// flight.  grid (ceil(tokens * kv_heads / rows per CTA), batch); heads vary
-// fastest, the order in which a projection leaves them.
-constexpr int kCachePasses = 2;
+// D/16 consecutive lanes hold a row, sixteen values each: K and V of one
+// (token, head) per lane group, kCachePasses rows a thread with all their
+// loads in flight.  grid (ceil(tokens * kv_heads / rows per CTA), batch); heads
+// vary fastest, the order in which a projection leaves them.
+constexpr int kCachePasses = 1;
 
 template <typename T, int D, bool kVec16>
 __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(CacheRowsArgs a) {
-  constexpr int kLanes = D / 8;
+  constexpr int kLanes = D / 16;
   constexpr int kRows = kCacheThreads / kLanes;  // a pass
   const int b = blockIdx.y;
   const int lane = threadIdx.x % kLanes;
@@ -96,7 +121,7 @@ __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(CacheRowsArg
   int64_t n = a.tokens;
   if (a.counts != nullptr) n = min(n, static_cast<int64_t>(__ldg(a.counts + b)));
   const int64_t length = __ldg(a.c.lengths + b);
-  uint4 raw[kCachePasses][2];
+  uint4 raw[kCachePasses][2][2];
   int64_t token[kCachePasses];
   unsigned head[kCachePasses];
 #pragma unroll
@@ -104,10 +129,13 @@ __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(CacheRowsArg
     walk.at(threadIdx.x / kLanes + p * kRows, &token[p], &head[p]);
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
-      raw[p][side] = make_uint4(0u, 0u, 0u, 0u);
-      if (token[p] < n)
-        raw[p][side] = load_raw8<T, kVec16>(static_cast<const T*>(a.in[side]) + b * a.stride[side][0] +
-                                            head[p] * a.stride[side][1] + token[p] * a.stride[side][2] + lane * 8);
+      raw[p][side][0] = raw[p][side][1] = make_uint4(0u, 0u, 0u, 0u);
+      if (token[p] < n) {
+        const T* from = static_cast<const T*>(a.in[side]) + b * a.stride[side][0] + head[p] * a.stride[side][1] +
+                        token[p] * a.stride[side][2] + lane * 16;
+        raw[p][side][0] = load_raw8<T, kVec16>(from);
+        raw[p][side][1] = load_raw8<T, kVec16>(from + 8);
+      }
     }
   }
   int64_t at[kCachePasses];
@@ -118,25 +146,27 @@ __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(CacheRowsArg
   for (int p = 0; p < kCachePasses; ++p) {
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
-      float x[8];
-      unpack8<T>(raw[p][side], x);
-      if (side == 0 && a.c.key_mean != nullptr && at[p] >= 0) {
-        float m[8];
-        mean8(a.c.key_mean + head[p] * D + lane * 8, m);
+      float x[2][8];
+      float amax = 0.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = __fsub_rn(x[i], m[i]);
+      for (int k = 0; k < 2; ++k) {
+        unpack8<T>(raw[p][side][k], x[k]);
+        if (side == 0 && a.c.key_mean != nullptr && at[p] >= 0) {
+          float m[8];
+          mean8(a.c.key_mean + head[p] * D + lane * 16 + k * 8, m);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[k][i] = __fsub_rn(x[k][i], m[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) amax = amax3(amax, x[k][i], x[k][i + 1]);
       }
-      // The largest magnitude; fmaxf would drop a NaN, so the bits are compared
-      // as integers (NaN above infinity above every finite magnitude).
-      uint32_t amax = 0u;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) amax = max(amax, __float_as_uint(x[i]) & 0x7fffffffu);
-#pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+      for (int o = kLanes / 2; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
       if (at[p] < 0) continue;
-      const float scale = amax == 0u ? 1.0f : __fmul_rn(__uint_as_float(amax), 1.0f / 127.0f);
+      const float scale = amax == 0.0f ? 1.0f : __fmul_rn(amax, 1.0f / 127.0f);
       int8_t* codes = static_cast<int8_t*>(side == 0 ? a.c.key_codes : a.c.value_codes);
-      *reinterpret_cast<uint2*>(codes + at[p] * D + lane * 8) = row_codes(x, scale);
+      const uint2 lo = row_codes(x[0], scale), hi = row_codes(x[1], scale);
+      *reinterpret_cast<uint4*>(codes + at[p] * D + lane * 16) = make_uint4(lo.x, lo.y, hi.x, hi.y);
       if (lane == 0) (side == 0 ? a.c.key_scales : a.c.value_scales)[at[p]] = scale;
     }
   }
@@ -155,7 +185,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
 // contiguous [batch, kv_heads, tokens, D].
 template <typename T, int D>
 __global__ void __launch_bounds__(kCacheThreads) cache_read_kernel(CacheRowsArgs a) {
-  constexpr int kLanes = D / 8;
+  constexpr int kLanes = D / 16;
   constexpr int kRows = kCacheThreads / kLanes;
   const int b = blockIdx.y;
   const int lane = threadIdx.x % kLanes;
@@ -172,42 +202,45 @@ __global__ void __launch_bounds__(kCacheThreads) cache_read_kernel(CacheRowsArgs
                 ? cache_row(a.c, a.page_shift, b, static_cast<int>(head[p]), length + token[p])
                 : -1;
   }
-  uint2 w[kCachePasses][2];
+  uint4 w[kCachePasses][2];
   float scale[kCachePasses][2];
 #pragma unroll
   for (int p = 0; p < kCachePasses; ++p)
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
-      w[p][side] = make_uint2(0u, 0u);
-      scale[p][side] = 0.0f;
-      if (at[p] >= 0) {
-        const int8_t* codes = static_cast<const int8_t*>(side == 0 ? a.c.key_codes : a.c.value_codes);
-        w[p][side] = *reinterpret_cast<const uint2*>(codes + at[p] * D + lane * 8);
-        scale[p][side] = (side == 0 ? a.c.key_scales : a.c.value_scales)[at[p]];
-      }
+      if (at[p] < 0) continue;
+      const int8_t* codes = static_cast<const int8_t*>(side == 0 ? a.c.key_codes : a.c.value_codes);
+      w[p][side] = *reinterpret_cast<const uint4*>(codes + at[p] * D + lane * 16);
+      scale[p][side] = (side == 0 ? a.c.key_scales : a.c.value_scales)[at[p]];
     }
 #pragma unroll
   for (int p = 0; p < kCachePasses; ++p) {
     if (head[p] >= a.c.kv_heads) continue;
+    const int64_t o = ((static_cast<int64_t>(b) * a.c.kv_heads + head[p]) * a.tokens + token[p]) * D + lane * 16;
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
-      float x[8];
-      const int8_t* q = reinterpret_cast<const int8_t*>(&w[p][side]);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(static_cast<float>(q[i]), scale[p][side]);
-      if (side == 0 && a.c.key_mean != nullptr && at[p] >= 0) {
-        float m[8];
-        mean8(a.c.key_mean + head[p] * D + lane * 8, m);
+      for (int k = 0; k < 2; ++k) {
+        uint4 y = make_uint4(0u, 0u, 0u, 0u);
+        if (at[p] >= 0) {
+          float x[8];
+          codes_f32(k == 0 ? w[p][side].x : w[p][side].z, x, 0);
+          codes_f32(k == 0 ? w[p][side].y : w[p][side].w, x, 4);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = __fadd_rn(x[i], m[i]);
+          for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(x[i], scale[p][side]);
+          if (side == 0 && a.c.key_mean != nullptr) {
+            float m[8];
+            mean8(a.c.key_mean + head[p] * D + lane * 16 + k * 8, m);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = __fadd_rn(x[i], m[i]);
+          }
+          y.x = pack2(x[0], x[1], T());
+          y.y = pack2(x[2], x[3], T());
+          y.z = pack2(x[4], x[5], T());
+          y.w = pack2(x[6], x[7], T());
+        }
+        *reinterpret_cast<uint4*>(static_cast<T*>(a.out[side]) + o + k * 8) = y;
       }
-      uint4 y;
-      y.x = pack2(x[0], x[1], T());
-      y.y = pack2(x[2], x[3], T());
-      y.z = pack2(x[4], x[5], T());
-      y.w = pack2(x[6], x[7], T());
-      const int64_t o = ((static_cast<int64_t>(b) * a.c.kv_heads + head[p]) * a.tokens + token[p]) * D + lane * 8;
-      *reinterpret_cast<uint4*>(static_cast<T*>(a.out[side]) + o) = y;
     }
   }
 }
