@@ -247,8 +247,12 @@ extern "C" int piper_b200_kv_cache_write(const piper_b200_kv_cache_t* cache, con
   a.counts = counts;
   a.tokens = tokens;
   a.page_shift = page_shift_of(cache->page_size);
+  while (a.block_shift < 3 && (int64_t(2) << a.block_shift) <= tokens) ++a.block_shift;
+  const int64_t block = int64_t(1) << a.block_shift;
   unsigned blocks = 0;
-  if ((rc = row_blocks(tokens * cache->kv_heads, cache->head_dim, &blocks)) != PIPER_B200_OK) return rc;
+  if ((rc = row_blocks((tokens + block - 1) / block * block * cache->kv_heads, cache->head_dim, &blocks)) !=
+      PIPER_B200_OK)
+    return rc;
   if ((rc = use_device()) != PIPER_B200_OK) return rc;
   const dim3 grid(blocks, static_cast<unsigned>(cache->batch));
   const bool v16 = rows_aligned16(key, key_strides) && rows_aligned16(value, value_strides);

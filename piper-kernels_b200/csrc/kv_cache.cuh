@@ -41,6 +41,7 @@ struct CacheRowsArgs {
   const int32_t* counts;
   int64_t tokens;
   int page_shift;
+  int block_shift;     // write: log2 of the tokens of a head that follow one another
 };
 
 // Codes of eight values, packed.  The prepass's division-free rounding needs
@@ -107,8 +108,10 @@ struct CacheRowWalk {
 
 // D/16 consecutive lanes hold a row, sixteen values each: K and V of one
 // (token, head) per lane group, kCachePasses rows a thread with all their
-// loads in flight.  grid (ceil(tokens * kv_heads / rows per CTA), batch); heads
-// vary fastest, the order in which a projection leaves them.
+// loads in flight.  grid (ceil(rows / rows per CTA), batch).  Rows go by blocks
+// of up to 8 tokens, then heads, then tokens: a projection leaves the heads of
+// a token side by side, the cache has the tokens of a head side by side, and
+// such a block is a kilobyte in both.
 constexpr int kCachePasses = 1;
 
 template <typename T, int D, bool kVec16>
@@ -117,7 +120,8 @@ __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(CacheRowsArg
   constexpr int kRows = kCacheThreads / kLanes;  // a pass
   const int b = blockIdx.y;
   const int lane = threadIdx.x % kLanes;
-  const CacheRowWalk walk(static_cast<int64_t>(blockIdx.x) * (kRows * kCachePasses), a.c.kv_heads);
+  const CacheRowWalk walk(static_cast<int64_t>(blockIdx.x) * (kRows * kCachePasses),
+                          static_cast<int64_t>(a.c.kv_heads) << a.block_shift);
   int64_t n = a.tokens;
   if (a.counts != nullptr) n = min(n, static_cast<int64_t>(__ldg(a.counts + b)));
   const int64_t length = __ldg(a.c.lengths + b);
@@ -127,6 +131,8 @@ __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(CacheRowsArg
 #pragma unroll
   for (int p = 0; p < kCachePasses; ++p) {
     walk.at(threadIdx.x / kLanes + p * kRows, &token[p], &head[p]);
+    token[p] = (token[p] << a.block_shift) + (head[p] & ((1u << a.block_shift) - 1u));
+    head[p] >>= a.block_shift;
 #pragma unroll
     for (int side = 0; side < 2; ++side) {
       raw[p][side][0] = raw[p][side][1] = make_uint4(0u, 0u, 0u, 0u);
