@@ -78,12 +78,21 @@ def refuse_grad(operator: str) -> None:
     raise RuntimeError(f"{operator} is an inference-only operator and does not support autograd")
 
 
+def _stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# The same handle without a Stream object around it (0.1 against 2.2 us), where torch has it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _stream)
+
+
 def launch(what: str, device: torch.device, call, *args) -> None:
     """Call a C entry point on ``device``'s current stream (its last argument)."""
-    if device.index == torch.cuda.current_device():
-        status = call(*args, torch.cuda.current_stream(device).cuda_stream)
+    index = device.index
+    if index == torch.cuda.current_device():
+        status = call(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
-            status = call(*args, torch.cuda.current_stream(device).cuda_stream)
+            status = call(*args, _raw_stream(index))
     if status:
         _native.check(status, what)

@@ -94,11 +94,11 @@ _workspace_bytes = lru_cache(maxsize=4096)(workspace_bytes)  # the same few shap
 def _run(query, cache, block_table, lengths, tree_mask, scale) -> torch.Tensor:
     batch, heads, nodes, head_dim = query.shape
     device = query.device
-    out = torch.empty((batch, heads, nodes, head_dim), dtype=query.dtype, device=device)
+    out = torch.empty_like(query, memory_format=torch.contiguous_format)
     nbytes = _workspace_bytes(
         batch, heads, cache.kv_heads, nodes, head_dim, block_table.shape[1] * cache.page_size
     )
-    workspace = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+    workspace = out.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     mask_ptr, mask_stride = None, 0
     if tree_mask is not None:
         mask_ptr, mask_stride = tree_mask.data_ptr(), tree_mask.stride(0) if tree_mask.ndim == 2 else 0

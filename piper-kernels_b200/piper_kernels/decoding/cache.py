@@ -277,8 +277,8 @@ def read_kv_cache(
 
 def _read(cache, block_table, lengths, counts, tokens, dtype) -> tuple[torch.Tensor, torch.Tensor]:
     shape = (lengths.shape[0], cache.kv_heads, tokens, cache.head_dim)
-    key = torch.empty(shape, dtype=dtype, device=cache.device)
-    value = torch.empty(shape, dtype=dtype, device=cache.device)
+    key = cache.key_codes.new_empty(shape, dtype=dtype)
+    value = torch.empty_like(key)
     launch(
         "piper_b200_kv_cache_read", cache.device, _native.library().piper_b200_kv_cache_read,
         ctypes.byref(cache.native(block_table, lengths)), key.data_ptr(), value.data_ptr(), DTYPE_CODES[dtype],

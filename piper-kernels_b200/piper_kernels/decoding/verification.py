@@ -94,9 +94,9 @@ def verify_draft_tree(
 def _run(target, draft, tokens, parents, uniform, noise) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     batch, nodes, vocab = target.shape
     device = target.device
-    path = torch.empty((batch, nodes), dtype=torch.int32, device=device)
-    count = torch.empty(batch, dtype=torch.int32, device=device)
-    next_token = torch.empty(batch, dtype=torch.int64, device=device)
+    path = parents.new_empty((batch, nodes))
+    count = parents.new_empty(batch)
+    next_token = tokens.new_empty(batch)
     launch(
         "piper_b200_verify_draft_tree", device, _native.library().piper_b200_verify_draft_tree,
         target.data_ptr(), _native.strides2(target), draft.data_ptr(), _native.strides2(draft),
