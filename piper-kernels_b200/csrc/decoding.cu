@@ -133,8 +133,9 @@ enum class TreeKind { kFew, kAlternate, kPair };
 TreeKind tree_kind(int64_t rows) {
   return rows <= 16 ? TreeKind::kFew : rows <= 128 ? TreeKind::kAlternate : TreeKind::kPair;
 }
+constexpr int kFewGroups = 2;
 template <int D>
-using FewRows = piper::TreeTile<D, 4>;
+using FewRows = piper::TreeTile<D, 4, kFewGroups>;
 
 template <int D>
 TreePlan tree_plan(int64_t batch, int64_t kv_heads, int64_t rows, int64_t positions, int sms) {
@@ -158,7 +159,7 @@ int set_up_wide() {
 
 template <typename T, int D>
 int set_up_instances() {
-  int rc = allow_smem(reinterpret_cast<const void*>(piper::tree_attention_kernel<T, D, 4>), FewRows<D>::kAlloc);
+  int rc = allow_smem(reinterpret_cast<const void*>(piper::tree_attention_kernel<T, D, 4, kFewGroups>), FewRows<D>::kAlloc);
   if (rc != PIPER_B200_OK) return rc;
   if ((rc = set_up_wide<T, D, false>()) != PIPER_B200_OK) return rc;
   return set_up_wide<T, D, true>();
@@ -214,7 +215,7 @@ template <typename T, int D>
 int launch_tree_rows(const piper::TreeArgs& a, int sms, size_t workspace_bytes, cudaStream_t stream) {
   switch (tree_kind(a.rows)) {
     case TreeKind::kFew:
-      return launch_tree<T, D, FewRows<D>>(a, piper::tree_attention_kernel<T, D, 4>, FewRows<D>::kThreads, sms,
+      return launch_tree<T, D, FewRows<D>>(a, piper::tree_attention_kernel<T, D, 4, kFewGroups>, FewRows<D>::kThreads, sms,
                                            workspace_bytes, stream);
     case TreeKind::kAlternate:
       return launch_tree<T, D, piper::WideTile<D, false>>(a, piper::tree_wide_kernel<T, D, false>,

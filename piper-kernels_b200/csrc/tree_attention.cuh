@@ -62,11 +62,11 @@ struct TreeArgs {
   float scale_log2e;
 };
 
-// Tile of up to 16 rows: a warp takes 16 keys of it.
-template <int D, int WARPS>
+// Tile of up to 16 rows: a warp takes 16 * GROUPS keys of it.
+template <int D, int WARPS, int GROUPS>
 struct TreeTile {
   static constexpr int kRows = 16;
-  static constexpr int kKeys = 16 * WARPS;
+  static constexpr int kKeys = 16 * GROUPS * WARPS;
   static constexpr int kThreads = 32 * (WARPS + 1);  // and one warp that fetches
   static constexpr int kCodes = kKeys * D;
   static constexpr int kScales = kKeys * 4;
@@ -77,8 +77,8 @@ struct TreeTile {
   static constexpr int kState = 2 * WARPS * kRows * 4;
   static constexpr int kQuery = (D / 16) * 32 * 16;  // fragments
   static constexpr int kFixed = kJoin + kState + kQuery + kRows * 8 + 512;
-  static constexpr int kCtas = D == 64 ? 4 : 2;  // per SM, what registers and stages allow
-  static constexpr int kLead = 5;  // a segment's start and end, in key tiles
+  static constexpr int kCtas = D == 64 ? 3 : 2;  // per SM, what registers and stages allow
+  static constexpr int kLead = 4;  // a segment's start and end, in key tiles
   static constexpr int kFit = (227 * 1024 / kCtas - 1024 * 2 - kFixed) / kStageAlloc;
   static constexpr int kStages = kFit > 8 ? 8 : kFit;
   static constexpr int kAlloc = kStages * kStageAlloc + kFixed + 1024;
@@ -299,11 +299,12 @@ __device__ __forceinline__ void query_fragments(const TreeArgs& a, int b, int kv
   }
 }
 
-template <typename T, int D, int WARPS>
-__global__ void __launch_bounds__(TreeTile<D, WARPS>::kThreads, TreeTile<D, WARPS>::kCtas)
+template <typename T, int D, int WARPS, int GROUPS>
+__global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS>::kThreads, TreeTile<D, WARPS, GROUPS>::kCtas)
     tree_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map,
                           TreeArgs a) {
-  using S = TreeTile<D, WARPS>;
+  using S = TreeTile<D, WARPS, GROUPS>;
+  constexpr int kN = 2 * GROUPS;  // groups of eight keys of a warp
   constexpr int kStages = S::kStages;
   constexpr int kChunks = D / 16;
   extern __shared__ uint8_t smem_raw[];
@@ -434,47 +435,40 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS>::kThreads, TreeTile<D, WARP
       if (ok) {
         const uint32_t base = smem_u32(smem + stage * S::kStageAlloc);
         const float* scales = reinterpret_cast<const float*>(smem + stage * S::kStageAlloc + 2 * S::kCodes);
-        const int key0 = warp * 16;
+        const int key0 = warp * 16 * GROUPS;
         const uint32_t goods = valid[stage];
         const int64_t first = static_cast<int64_t>(tile) * S::kKeys;
         const bool masked = first + S::kKeys > length || goods != (1u << boxes) - 1u;
-        // ---- scores of 16 keys, in two chains
-        float s[2][2][4] = {};
+        // ---- scores
+        float y[kN][4] = {};
 #pragma unroll
         for (int c = 0; c < kChunks; c += 2) {
-          uint32_t k[4];
-          ldmatrix4(tile_chunk<D>(base, key0 + (lane & 15), c + (lane >> 4)), k);
+          uint4 f[2];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) k[x] ^= 0x80808080u;
+          for (int x = 0; x < 2; ++x) f[x] = query[(c + x) * 32 + lane];
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const uint4 f = query[(c + x) * 32 + lane];
-            const uint32_t q[4] = {f.x, f.y, f.z, f.w};
+          for (int i = 0; i < GROUPS; ++i) {
+            uint32_t k[4];
+            ldmatrix4(tile_chunk<D>(base, key0 + 16 * i + (lane & 15), c + (lane >> 4)), k);
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
-              mma16816(s[x][n], q, codes_f16<0x4140>(k[2 * x + n]), codes_f16<0x4342>(k[2 * x + n]));
+            for (int x = 0; x < 4; ++x) k[x] ^= 0x80808080u;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const uint32_t q[4] = {f[x].x, f[x].y, f[x].z, f[x].w};
+#pragma unroll
+              for (int n = 0; n < 2; ++n)
+                mma16816(y[2 * i + n], q, codes_f16<0x4140>(k[2 * x + n]), codes_f16<0x4342>(k[2 * x + n]));
+            }
           }
         }
-        float ks[2][2], vs[2][2], lv[2][2];
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const float2 k2 = *reinterpret_cast<const float2*>(scales + key0 + 8 * n + 2 * t);
-          const float2 v2 = *reinterpret_cast<const float2*>(scales + S::kKeys + key0 + 8 * n + 2 * t);
-          ks[n][0] = k2.x;
-          ks[n][1] = k2.y;
-          vs[n][0] = v2.x;
-          vs[n][1] = v2.y;
-          lv[n][0] = fmaxf(lg2_approx(v2.x), kScaleLogMin);
-          lv[n][1] = fmaxf(lg2_approx(v2.y), kScaleLogMin);
-        }
-        uint32_t w[4];
+        uint32_t w[GROUPS][4];
         // A masked tile has a body of its own: selections would lengthen the
         // other's.
         auto weigh = [&](auto hidden) {
           uint32_t unseen = 0u;  // bit 4 n + 2 h + e
           if constexpr (hidden.value) {
 #pragma unroll
-            for (int n = 0; n < 2; ++n)
+            for (int n = 0; n < kN; ++n)
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
                 const int key = key0 + n * 8 + 2 * t + e;
@@ -486,19 +480,22 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS>::kThreads, TreeTile<D, WARP
                     unseen |= 1u << (4 * n + 2 * h + e);
               }
           }
-          float y[2][4];
           float most[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
+          for (int n = 0; n < kN; ++n) {
+            const float2 ks = *reinterpret_cast<const float2*>(scales + key0 + 8 * n + 2 * t);
+            const float2 vs = *reinterpret_cast<const float2*>(scales + S::kKeys + key0 + 8 * n + 2 * t);
+            const float lv[2] = {fmaxf(lg2_approx(vs.x), kScaleLogMin), fmaxf(lg2_approx(vs.y), kScaleLogMin)};
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-              y[n][x] = (s[0][n][x] + s[1][n][x]) * ks[n][x & 1];
+              y[n][x] *= (x & 1) ? ks.y : ks.x;
               // A key that a row does not see may hold anything.
               if (hidden.value && ((unseen >> (4 * n + x)) & 1u)) y[n][x] = -INFINITY;
-              float z = fmaf(y[n][x], factor[x / 2], lv[n][x & 1]);
+              float z = fmaf(y[n][x], factor[x / 2], lv[x & 1]);
               if (hidden.value && ((unseen >> (4 * n + x)) & 1u)) z = -INFINITY;
               most[x / 2] = fmaxf(most[x / 2], z);
             }
+          }
           if (__any_sync(0xffffffffu, most[0] - unit[0] > kSlack || most[1] - unit[1] > kSlack)) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
@@ -517,7 +514,8 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS>::kThreads, TreeTile<D, WARP
             }
           }
 #pragma unroll
-          for (int n = 0; n < 2; ++n)
+          for (int n = 0; n < kN; ++n) {
+            const float2 vs = *reinterpret_cast<const float2*>(scales + S::kKeys + key0 + 8 * n + 2 * t);
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               float p[2];
@@ -525,11 +523,12 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS>::kThreads, TreeTile<D, WARP
               for (int e = 0; e < 2; ++e) {
                 p[e] = ex2_approx(fmaf(y[n][2 * h + e], factor[h], -unit[h]));
                 l[h] += p[e];
-                p[e] *= vs[n][e];
+                p[e] *= e ? vs.y : vs.x;
                 if (hidden.value && ((unseen >> (4 * n + 2 * h + e)) & 1u)) p[e] = 0.0f;
               }
-              w[2 * n + h] = pack2(p[0], p[1], __half());
+              w[n / 2][2 * (n & 1) + h] = pack2(p[0], p[1], __half());
             }
+          }
         };
         if (masked)
           weigh(std::true_type());
@@ -538,14 +537,17 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS>::kThreads, TreeTile<D, WARP
         // ---- numerators: even, then odd head dimensions of each chunk
 #pragma unroll
         for (int c = 0; c < kChunks; c += 2) {
-          uint32_t v[4];
-          ldmatrix4_trans(tile_chunk<D>(base + S::kCodes, key0 + (lane & 15), c + (lane >> 4)), v);
 #pragma unroll
-          for (int x = 0; x < 4; ++x) v[x] ^= 0x80808080u;
+          for (int i = 0; i < GROUPS; ++i) {
+            uint32_t v[4];
+            ldmatrix4_trans(tile_chunk<D>(base + S::kCodes, key0 + 16 * i + (lane & 15), c + (lane >> 4)), v);
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            mma16816(o[2 * (c + x)], w, codes_f16<0x4240>(v[2 * x]), codes_f16<0x4240>(v[2 * x + 1]));
-            mma16816(o[2 * (c + x) + 1], w, codes_f16<0x4341>(v[2 * x]), codes_f16<0x4341>(v[2 * x + 1]));
+            for (int x = 0; x < 4; ++x) v[x] ^= 0x80808080u;
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              mma16816(o[2 * (c + x)], w[i], codes_f16<0x4240>(v[2 * x]), codes_f16<0x4240>(v[2 * x + 1]));
+              mma16816(o[2 * (c + x) + 1], w[i], codes_f16<0x4341>(v[2 * x]), codes_f16<0x4341>(v[2 * x + 1]));
+            }
           }
         }
       }
