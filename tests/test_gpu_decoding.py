@@ -500,3 +500,27 @@ def test_attention_over_a_written_prompt_is_close_to_unquantised_attention() -> 
     off = float(query.double().abs().sum(-1).max() * most_k) / 254 * d**-0.5
     allowed = float(value.double().abs().max()) * (1 / 254 + 2 * off) + 2.0**-8 * float(expected.abs().max())
     assert float((out - expected).abs().max()) <= allowed
+
+
+def test_the_example_keeps_every_layer_consistent_with_its_tokens() -> None:
+    # After the last step the caches hold the rows of the prompt and of every
+    # token but the last: the first layer's rows depend on the token alone, so
+    # they are the quantised projections of the embeddings.
+    from piper_kernels.decoding import example
+
+    dev = require_b200()
+    model = example.ToyModel()
+    prompt = torch.randint(0, model.vocab, (3, 21), generator=torch.Generator().manual_seed(13)).to(dev)
+    with torch.no_grad():
+        generated, caches, table, lengths = example.generate(model, prompt, 5)
+        for b, tokens in enumerate(generated):
+            assert 6 <= len(tokens) <= 1 + 5 * 3 and all(0 <= t < model.vocab for t in tokens)
+            assert int(lengths[b]) == prompt.shape[1] + len(tokens) - 1
+            sequence = torch.cat([prompt[b], torch.tensor(tokens[:-1], device=dev)])[None]
+            h = torch.nn.functional.normalize(model.embedding[sequence].float(), dim=-1).to(torch.bfloat16) * 8
+            # (The projection of one row and of a batch of rows may round differently: one bf16 step and one code.)
+            k, v = pk.read_kv_cache(caches[0], table[b : b + 1], torch.zeros_like(lengths[:1]), sequence.shape[1])
+            for got, weight in ((k, model.key[0]), (v, model.value[0])):
+                expected = model.heads_of(h, weight).float()
+                step = expected.abs().amax(-1, keepdim=True) / 127
+                assert bool(((got.float() - expected).abs() <= 1.6 * step + 2.0**-6 * expected.abs()).all())
