@@ -16,11 +16,11 @@
 // 128-255 of the row tile over the same keys (more than 128 rows).  Otherwise
 // they are alternate key tiles of the same 128 rows, joined at the end.
 //
-// A softmax warp reads its 16 rows' scores twice, 32 columns at a time, first
-// for the maxima, then for the weights.  A row has one reference, the unit of
-// its numerators and of its total: 2^unit follows the largest weight times its
-// value scale, trails by a factor of at most 2^14, and moves only when a tile
-// could outgrow it.
+// A softmax warp takes its 16 rows' scores 32 columns at a time.  A row has one
+// reference, the unit of its numerators and of its total: 2^unit follows the
+// largest weight times its value scale, trails by a factor of at most 2^14, and
+// moves only when 32 columns could outgrow it; then what is there already, the
+// tile's first weights among it, is scaled down.
 //
 // Warps: 0-7 and 8-15 softmax of streams 0 and 1 (two for each 32 TMEM lanes),
 // 16-17 conversion of K, 18-19 of V, 20 fetches, 21 issues MMAs, 22 owns
@@ -167,6 +167,79 @@ __device__ __forceinline__ float2 f2_of(uint32_t x, uint32_t y) {
   return make_float2(__uint_as_float(x), __uint_as_float(y));
 }
 
+// New references of a lane's two rows, and by how much they moved.
+struct WideMove {
+  float2 unit, shrink;
+};
+
+// Moves the references to the largest logarithm of a weight times its value
+// scale in chunk c of a tile (bit 8 n + e of seen0 and seen1: column 8 n + e
+// after the lane's first is seen), and scales down the tile's weights so far
+// and `numerators` columns at tm_o.  Not inlined: it is rare, and its registers
+// would be the common path's spills.
+template <typename S>
+__device__ __noinline__ WideMove wide_move(uint32_t tm_s, uint32_t tm_o, uint32_t scales, int c, float2 factor,
+                                           float2 unit, uint32_t seen0, uint32_t seen1, int numerators) {
+  const int t = threadIdx.x % 4;
+  float most[2] = {-INFINITY, -INFINITY};
+  const float factors[2] = {factor.x, factor.y};
+  float units[2] = {unit.x, unit.y}, shrink[2] = {1.0f, 1.0f};
+  const uint32_t seen[2] = {seen0, seen1};
+  uint32_t v[16];
+  tmem_ld_16x256b_x4(tm_s + 32 * c, v);
+  tmem_ld_wait();
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    const float2 ks = lds64(scales + 128 * c + 32 * n + 8 * t);
+    const float2 vs = lds64(scales + S::kKeys * 4 + 128 * c + 32 * n + 8 * t);
+    const float lx = fmaxf(lg2_approx(vs.x), kScaleLogMin), ly = fmaxf(lg2_approx(vs.y), kScaleLogMin);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float zx = fmaf(__uint_as_float(v[4 * n + 2 * h]) * ks.x, factors[h], lx);
+      const float zy = fmaf(__uint_as_float(v[4 * n + 2 * h + 1]) * ks.y, factors[h], ly);
+      if ((seen[h] >> (8 * n)) & 1u) most[h] = fmaxf(most[h], zx);
+      if ((seen[h] >> (8 * n + 1)) & 1u) most[h] = fmaxf(most[h], zy);
+    }
+  }
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 1));
+    most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 2));
+    if (most[h] > units[h]) {
+      // By whole powers of two: the weights that are in TMEM already stay exact.
+      const float up = units[h] == kNoReference ? most[h] : units[h] + ceilf(most[h] - units[h]);
+      shrink[h] = ex2_approx(units[h] - up);
+      units[h] = up;
+    }
+  }
+  tmem_st_wait();
+#pragma unroll 1
+  for (int d = 0; d < c; ++d) {
+    uint32_t u[8];
+    tmem_ld_16x128b_x4(tm_s + 16 * d, u);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const __half2 z = __hmul2(*reinterpret_cast<const __half2*>(&u[i]), __float2half2_rn(shrink[i & 1]));
+      u[i] = *reinterpret_cast<const uint32_t*>(&z);
+    }
+    tmem_st_16x128b_x4(tm_s + 16 * d, u);
+  }
+  // (The stream's last numerator MMAs are complete: the scores of this tile
+  // were committed after them.)
+#pragma unroll 1
+  for (int d = 0; d < numerators; d += 16) {
+    uint32_t u[8];
+    tmem_ld_16x256b_x2(tm_o + d, u);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) u[i] = __float_as_uint(__uint_as_float(u[i]) * shrink[(i / 2) & 1]);
+    tmem_st_16x256b_x2(tm_o + d, u);
+  }
+  tmem_st_wait();
+  return WideMove{make_float2(units[0], units[1]), make_float2(shrink[0], shrink[1])};
+}
+
 template <typename T, int D, bool kShared>
 __global__ void __launch_bounds__(kWideThreads, 1)
     tree_wide_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map,
@@ -246,7 +319,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
       if (w.count == 0) continue;
       const int kv = w.hr / a.row_tiles;
       const int row0 = (w.hr % a.row_tiles) * S::kRows + (kShared ? x * 128 : 0);
-      const int64_t length = max(0, __ldg(a.c.lengths + w.b));
+      const int full_tiles = max(0, __ldg(a.c.lengths + w.b)) / S::kKeys;  // without drafted keys
       if (kShared || x == 0) {
         if (half == 0) {
           const int row = row0 + lane0 + lane;
@@ -291,151 +364,85 @@ __global__ void __launch_bounds__(kWideThreads, 1)
         tc_fence_after();
         if (!idle) {
           const uint32_t scales = sbase + S::kOffScales + entry * S::kEntry;
-          const int64_t first = static_cast<int64_t>(w.tile + j) * S::kKeys;
           const uint32_t goods = valid[entry];
-          const bool masked = first + S::kKeys > length || goods != (1u << boxes) - 1u;
-          const int open = static_cast<int>(max(min(length - first, int64_t(256)), int64_t(-256)));
+          const bool masked = w.tile + j >= full_tiles || goods != (1u << boxes) - 1u;
           // Bit 8 n + e: column 32 c + 8 n + 2 t + e of row h is seen.
           auto seen_of = [&](int c, int h) {
-            return wide_seen(goods, box_shift, open, words[own + r16 + 8 * h], c) >> (2 * t);
+            const int64_t open = max(0, __ldg(a.c.lengths + w.b)) - static_cast<int64_t>(w.tile + j) * S::kKeys;
+            return wide_seen(goods, box_shift, static_cast<int>(max(min(open, int64_t(256)), int64_t(-256))),
+                             words[own + r16 + 8 * h], c) >> (2 * t);
           };
-          // ---- first reading: the largest scores and value scale
-          float top[2] = {-INFINITY, -INFINITY};
+          // The largest value scale of the tile, as a logarithm.  (NaN: 0; floats
+          // that are not negative order as their bits.)
           const float4 four = lds128(scales + S::kKeys * 4 + 16 * lane);
-          float reach = fmaxf(fmaxf(fmaxf(four.x, four.y), fmaxf(four.z, four.w)), 0.0f);  // (NaN: 0)
-          // (A masked tile has a body of its own: branches inside would cut
-          // the other's instructions into short chains.)
-          auto largest = [&](auto hidden) {
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              uint32_t v[16];
-              tmem_ld_16x256b_x4(tm_s + 32 * c, v);
-              float2 ks[4];
-#pragma unroll
-              for (int n = 0; n < 4; ++n) ks[n] = lds64(scales + 128 * c + 32 * n + 8 * t);
-              tmem_ld_wait();
-#pragma unroll
-              for (int k = 0; k < 1; ++k) {
-                uint32_t seen[2];
-                if constexpr (hidden.value) {
-                  seen[0] = seen_of(c + k, 0);
-                  seen[1] = seen_of(c + k, 1);
-                }
-#pragma unroll
-                for (int n = 0; n < 4; ++n)
-#pragma unroll
-                  for (int h = 0; h < 2; ++h) {
-                    float2 y = mul2(f2_of(v[16 * k + 4 * n + 2 * h], v[16 * k + 4 * n + 2 * h + 1]), ks[4 * k + n]);
-                    if constexpr (hidden.value) hide(y, seen[h] >> (8 * n));
-                    top[h] = fmax3(top[h], y.x, y.y);
-                  }
-              }
-            }
-          };
-          if (masked)
-            largest(std::true_type());
-          else
-            largest(std::false_type());
-          // (Floats that are not negative order as their bits.)
+          float reach = fmaxf(fmaxf(fmaxf(four.x, four.y), fmaxf(four.z, four.w)), 0.0f);
           reach = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(reach)));
           const float reach_log = fmaxf(lg2_approx(reach), kScaleLogMin);
-          // A weight times its value scale is at most 2^(top + reach_log - unit).
-          bool renew = false;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) renew |= fmaf(top[h], factor[h], reach_log - unit[h]) > kSlack;
-          if (__any_sync(0xffffffffu, renew)) {
-            // The largest logarithm of a weight times its value scale.
-            float most[2] = {-INFINITY, -INFINITY};
-            uint32_t v[16];
-#pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              tmem_ld_16x256b_x4(tm_s + 32 * c, v);
-              tmem_ld_wait();
-#pragma unroll
-              for (int h = 0; h < 2; ++h) {
-                const uint32_t seen = masked ? seen_of(c, h) : ~0u;
-#pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                  const float2 ks = lds64(scales + 128 * c + 32 * n + 8 * t);
-                  const float2 vs = lds64(scales + S::kKeys * 4 + 128 * c + 32 * n + 8 * t);
-                  const float zx = fmaf(__uint_as_float(v[4 * n + 2 * h]) * ks.x, factor[h],
-                                        fmaxf(lg2_approx(vs.x), kScaleLogMin));
-                  const float zy = fmaf(__uint_as_float(v[4 * n + 2 * h + 1]) * ks.y, factor[h],
-                                        fmaxf(lg2_approx(vs.y), kScaleLogMin));
-                  if ((seen >> (8 * n)) & 1u) most[h] = fmaxf(most[h], zx);
-                  if ((seen >> (8 * n + 1)) & 1u) most[h] = fmaxf(most[h], zy);
-                }
-              }
-            }
-            float shrink[2];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 1));
-              most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 2));
-              shrink[h] = 1.0f;
-              if (most[h] > unit[h]) {
-                shrink[h] = ex2_approx(unit[h] - most[h]);
-                unit[h] = most[h];
-                l[h] *= shrink[h];
-              }
-            }
-            // The stream's last numerator MMAs are complete: the scores of
-            // this tile were committed after them.
-            if (!first_job) {
-#pragma unroll 1
-              for (int d = 0; d < D; d += 32) {
-                tmem_ld_16x256b_x4(tm_o + d, v);
-                tmem_ld_wait();
-#pragma unroll
-                for (int n = 0; n < 4; ++n)
-#pragma unroll
-                  for (int e = 0; e < 4; ++e)
-                    v[4 * n + e] = __float_as_uint(__uint_as_float(v[4 * n + e]) * shrink[e / 2]);
-                tmem_st_16x256b_x4(tm_o + d, v);
-              }
-            }
-          }
-          // ---- second reading: the weights, over the spent scores (column
-          // c / 2: what it covers has been read)
           float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+          // (A masked tile has a body of its own: branches inside would cut
+          // the other's instructions into short chains.)
           auto weigh = [&](auto hidden) {
+            bool moved = false;  // the references have, for this chunk
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
-              {
-                uint32_t v[16];
-                tmem_ld_16x256b_x4(tm_s + 32 * c, v);
-                float2 ks[4], vs[4];
+            for (int c = 0; c < 4;) {
+              uint32_t v[16];
+              tmem_ld_16x256b_x4(tm_s + 32 * c, v);
+              float2 ks[4], vs[4];
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                  ks[n] = lds64(scales + 128 * c + 32 * n + 8 * t);
-                  vs[n] = lds64(scales + S::kKeys * 4 + 128 * c + 32 * n + 8 * t);
-                }
-                tmem_ld_wait();
-                uint32_t seen[2];
-                if constexpr (hidden.value) {
-                  seen[0] = seen_of(c, 0);
-                  seen[1] = seen_of(c, 1);
-                }
-                uint32_t p16[8];
-#pragma unroll
-                for (int n = 0; n < 4; ++n)
-#pragma unroll
-                  for (int h = 0; h < 2; ++h) {
-                    float2 p = __ffma2_rn(mul2(f2_of(v[4 * n + 2 * h], v[4 * n + 2 * h + 1]), ks[n]),
-                                          make_float2(factor[h], factor[h]), make_float2(-unit[h], -unit[h]));
-                    if constexpr (hidden.value) hide(p, seen[h] >> (8 * n));
-                    p.x = ex2_approx(p.x);
-                    p.y = ex2_approx(p.y);
-                    sum[h] = __fadd2_rn(sum[h], p);
-                    p = mul2(p, vs[n]);
-                    uint32_t x16 = pack2(p.x, p.y, __half());
-                    if constexpr (hidden.value)  // an unseen key's value scale may be anything
-                      x16 &= ((seen[h] >> (8 * n)) & 1u ? 0xffffu : 0u) |
-                             ((seen[h] >> (8 * n + 1)) & 1u ? 0xffff0000u : 0u);
-                    p16[2 * n + h] = x16;
-                  }
-                tmem_st_16x128b_x4(tm_s + 16 * c, p16);
+              for (int n = 0; n < 4; ++n) {
+                ks[n] = lds64(scales + 128 * c + 32 * n + 8 * t);
+                vs[n] = lds64(scales + S::kKeys * 4 + 128 * c + 32 * n + 8 * t);
               }
+              tmem_ld_wait();
+              uint32_t seen[2] = {~0u, ~0u};
+              if constexpr (hidden.value) {
+                seen[0] = seen_of(c, 0);
+                seen[1] = seen_of(c, 1);
+              }
+              float2 y[4][2];
+              float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+              for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  y[n][h] = mul2(f2_of(v[4 * n + 2 * h], v[4 * n + 2 * h + 1]), ks[n]);
+                  if constexpr (hidden.value) hide(y[n][h], seen[h] >> (8 * n));
+                  top[h] = fmax3(top[h], y[n][h].x, y[n][h].y);
+                }
+              // A weight times its value scale is at most 2^(top + reach_log - unit).
+              if (!moved && __any_sync(0xffffffffu, fmaf(top[0], factor[0], reach_log - unit[0]) > kSlack ||
+                                                        fmaf(top[1], factor[1], reach_log - unit[1]) > kSlack)) {
+                const WideMove m = wide_move<S>(tm_s, tm_o, scales, c, make_float2(factor[0], factor[1]),
+                                                make_float2(unit[0], unit[1]), seen[0], seen[1], first_job ? 0 : D);
+                unit[0] = m.unit.x;
+                unit[1] = m.unit.y;
+                l[0] *= m.shrink.x;
+                l[1] *= m.shrink.y;
+                sum[0] = mul2(sum[0], make_float2(m.shrink.x, m.shrink.x));
+                sum[1] = mul2(sum[1], make_float2(m.shrink.y, m.shrink.y));
+                moved = true;  // and take the chunk again
+                continue;
+              }
+              uint32_t p16[8];
+#pragma unroll
+              for (int n = 0; n < 4; ++n)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  float2 p = __ffma2_rn(y[n][h], make_float2(factor[h], factor[h]), make_float2(-unit[h], -unit[h]));
+                  p.x = ex2_approx(p.x);
+                  p.y = ex2_approx(p.y);
+                  sum[h] = __fadd2_rn(sum[h], p);
+                  p = mul2(p, vs[n]);
+                  uint32_t x16 = pack2(p.x, p.y, __half());
+                  if constexpr (hidden.value)  // an unseen key's value scale may be anything
+                    x16 &= ((seen[h] >> (8 * n)) & 1u ? 0xffffu : 0u) |
+                           ((seen[h] >> (8 * n + 1)) & 1u ? 0xffff0000u : 0u);
+                  p16[2 * n + h] = x16;
+                }
+              // Over spent scores: columns 16 c .. of chunk c / 2.
+              tmem_st_16x128b_x4(tm_s + 16 * c, p16);
+              moved = false;
+              ++c;
             }
           };
           if (masked)
