@@ -504,18 +504,14 @@ __global__ void __launch_bounds__(kWideThreads, 1)
           to[S::kRows * D + 2 * lr + 1] = whole_l;
         }
 #pragma unroll 1
-        for (int d = share * kShare; d < (share + 1) * kShare; d += 16) {
-          uint32_t u0[16], u1[16];
+        for (int d = share * kShare; d < (share + 1) * kShare; d += 8) {
+          uint32_t u0[8], u1[8];
           tmem_ld8(from + d, u0);
-          tmem_ld8(from + d + 8, u0 + 8);
-          if (two) {
-            tmem_ld8(from + 128 + d, u1);
-            tmem_ld8(from + 128 + d + 8, u1 + 8);
-          }
+          if (two) tmem_ld8(from + 128 + d, u1);
           tmem_ld_wait();
-          float z[16];
+          float z[8];
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
+          for (int i = 0; i < 8; ++i) {
             z[i] = __uint_as_float(u0[i]) * f0;
             if (two) z[i] += __uint_as_float(u1[i]) * f1;
           }
@@ -523,19 +519,15 @@ __global__ void __launch_bounds__(kWideThreads, 1)
           if (w.all) {
             T* out = static_cast<T*>(a.out) + ((static_cast<int64_t>(w.b) * a.heads + kv * a.group + row / a.nodes) *
                                                    a.nodes + row % a.nodes) * D + d;
-#pragma unroll
-            for (int i = 0; i < 16; i += 8) {
-              uint4 h;
-              h.x = pack2(z[i], z[i + 1], T());
-              h.y = pack2(z[i + 2], z[i + 3], T());
-              h.z = pack2(z[i + 4], z[i + 5], T());
-              h.w = pack2(z[i + 6], z[i + 7], T());
-              *reinterpret_cast<uint4*>(out + i) = h;
-            }
+            uint4 h;
+            h.x = pack2(z[0], z[1], T());
+            h.y = pack2(z[2], z[3], T());
+            h.z = pack2(z[4], z[5], T());
+            h.w = pack2(z[6], z[7], T());
+            *reinterpret_cast<uint4*>(out) = h;
           } else {
-#pragma unroll
-            for (int i = 0; i < 16; i += 4)
-              *reinterpret_cast<float4*>(to + lr * D + d + i) = make_float4(z[i], z[i + 1], z[i + 2], z[i + 3]);
+            *reinterpret_cast<float4*>(to + lr * D + d) = make_float4(z[0], z[1], z[2], z[3]);
+            *reinterpret_cast<float4*>(to + lr * D + d + 4) = make_float4(z[4], z[5], z[6], z[7]);
           }
         }
         tc_fence_before();
