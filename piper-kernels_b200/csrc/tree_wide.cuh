@@ -7,9 +7,8 @@
 //   S = Q K^T   Q (fp16, scaled by row) and K from shared memory
 //   O += W V    W (fp16 weights) from TMEM, over the spent scores; V from
 //               shared memory with the head dimension contiguous
-// kind::f16 needs 16-bit operands, so a warpgroup turns each tile's codes into
-// fp16 between the TMA ring and the MMAs: 128 rows then pay for one
-// conversion.
+// kind::f16 needs 16-bit operands, so warps turn each tile's codes into fp16
+// between the TMA ring and the MMAs: 128 rows or more pay for one conversion.
 //
 // Two streams of 128 TMEM lanes hide each other's latency: while one stream's
 // softmax runs, the other's MMAs do.  kShared: the streams are rows 0-127 and
@@ -25,12 +24,24 @@
 // Warps: 0-7 and 8-15 softmax of streams 0 and 1 (two for each 32 TMEM lanes),
 // 16-17 conversion of K, 18-19 of V, 20 fetches, 21 issues MMAs, 22 owns
 // TMEM.
+//
+// Measured: 16 nodes of 40 over 8 heads of 128 and 131072 tokens (80 rows) 126
+// us, 341 TFLOP/s; 16 requests of 4000 to 8191 tokens, 47 nodes, 32 over 8 heads
+// (188 rows) 185 us, 410 TFLOP/s.  The time hardly depends on the rows up to
+// 128 (17 rows 122 us, 128 rows 137 us): what bounds it is a stream's chain of
+// scores, weights and numerators, some 8000 cycles a tile with two tiles under
+// way, the tensor pipe being busy a quarter of the time.  Tried and slower: a
+// thread a row with all 128 scores in registers (204 us; one long unrolled
+// body), half tiles with both halves' scores in TMEM (191 us; twice the
+// hand-overs, and QK^T of 64 keys reads Q twice).
 #pragma once
 
 #include "tree_attention.cuh"
 
 namespace piper {
 
+// 23 warps at 80 registers: what a softmax warp needs without spilling in its
+// loop (more columns at a time, or a look ahead, spilled and measured slower).
 constexpr int kWideThreads = 736;
 
 template <int D, bool kShared>
@@ -192,7 +203,7 @@ __device__ __noinline__ WideMove wide_move(uint32_t tm_s, uint32_t tm_o, uint32_
   for (int n = 0; n < 4; ++n) {
     const float2 ks = lds64(scales + 128 * c + 32 * n + 8 * t);
     const float2 vs = lds64(scales + S::kKeys * 4 + 128 * c + 32 * n + 8 * t);
-    const float lx = fmaxf(lg2_approx(vs.x), kScaleLogMin), ly = fmaxf(lg2_approx(vs.y), kScaleLogMin);
+    const float lx = fmaxf(lg2_approx(fabsf(vs.x)), kScaleLogMin), ly = fmaxf(lg2_approx(fabsf(vs.y)), kScaleLogMin);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const float zx = fmaf(__uint_as_float(v[4 * n + 2 * h]) * ks.x, factors[h], lx);
@@ -375,7 +386,7 @@ __global__ void __launch_bounds__(kWideThreads, 1)
           // The largest value scale of the tile, as a logarithm.  (NaN: 0; floats
           // that are not negative order as their bits.)
           const float4 four = lds128(scales + S::kKeys * 4 + 16 * lane);
-          float reach = fmaxf(fmaxf(fmaxf(four.x, four.y), fmaxf(four.z, four.w)), 0.0f);
+          float reach = fmaxf(fmaxf(fmaxf(fabsf(four.x), fabsf(four.y)), fmaxf(fabsf(four.z), fabsf(four.w))), 0.0f);
           reach = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(reach)));
           const float reach_log = fmaxf(lg2_approx(reach), kScaleLogMin);
           float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};

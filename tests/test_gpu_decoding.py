@@ -524,3 +524,73 @@ def test_the_example_keeps_every_layer_consistent_with_its_tokens() -> None:
                 expected = model.heads_of(h, weight).float()
                 step = expected.abs().amax(-1, keepdim=True) / 127
                 assert bool(((got.float() - expected).abs() <= 1.6 * step + 2.0**-6 * expected.abs()).all())
+
+
+@pytest.mark.parametrize("nodes", [1, 11, 40])
+def test_attention_of_many_short_requests(nodes) -> None:
+    # More requests than a warp has lanes, segments of a few tiles: runs hold
+    # many of them whole and cut others.
+    dev = require_b200()
+    g = torch.Generator().manual_seed(nodes + 70)
+    lengths = [int(x) for x in torch.randint(0, 1500, (70,), generator=g)]
+    lengths[3], lengths[33], lengths[69] = 2600, 0, 2049
+    _attend(g, dev, d=64, page=128, kv_heads=2, group=2, nodes=nodes, lengths=lengths, dtype=torch.float16)
+
+
+@pytest.mark.parametrize("nodes", [1, 6, 50])
+def test_attention_with_scales_of_either_sign(nodes) -> None:
+    # The handle takes any scales; a negative one only turns its row around.
+    dev = require_b200()
+    g = torch.Generator().manual_seed(nodes + 80)
+    cache = _pool(g, 20, 1, 64, 128)
+    for name in ("key_scales", "value_scales"):
+        getattr(cache, name).mul_(torch.randint(0, 2, (20, 1, 64), generator=g) * 2 - 1)
+    table = torch.randperm(20, generator=g)[:18].view(1, 18).to(torch.int32)
+    lengths = torch.tensor([1100], dtype=torch.int32)
+    query = torch.randn((1, 4, nodes, 128), generator=g).bfloat16()
+    out = pk.tree_attention(query.to(dev), _on(cache, dev), table.to(dev), lengths.to(dev)).cpu().double()
+    expected, _ = oracle.attention(query, cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales,
+                                   table, lengths, None, 128**-0.5)
+    _, bound = oracle.attention(query, cache.key_codes, cache.key_scales, cache.value_codes,
+                                cache.value_scales.abs(), table, lengths, None, 128**-0.5)
+    assert bool(((out - expected).abs() <= 2.0**-8 * expected.abs() + 1.01 * bound).all())
+
+
+@pytest.mark.parametrize("nodes", [1, 20, 64])
+def test_attention_ends_before_what_follows_on_its_stream(nodes) -> None:
+    # The joining kernel may be placed early; the next kernel on the stream must
+    # still find attention done with the cache.
+    dev = require_b200()
+    g = torch.Generator().manual_seed(nodes + 90)
+    cache = _on(_pool(g, 300, 2, 64, 128), dev)
+    table = torch.randperm(300, generator=g)[:280].view(4, 70).to(torch.int32).to(dev)
+    lengths = torch.tensor([4000, 17, 3000, 900], dtype=torch.int32, device=dev)
+    query = torch.randn((4, 8, nodes, 128), generator=g).bfloat16().to(dev)
+    saved = cache.value_codes.clone()
+    expected = pk.tree_attention(query, cache, table, lengths).clone()
+    torch.cuda.synchronize()
+    for _ in range(20):
+        out = pk.tree_attention(query, cache, table, lengths)
+        cache.value_codes.zero_()
+        cache.value_codes.copy_(saved)
+        assert torch.equal(out, expected)
+
+
+def test_calls_on_two_streams_at_once_do_not_share_anything() -> None:
+    dev = require_b200()
+    g = torch.Generator().manual_seed(95)
+    cache = _on(_pool(g, 200, 2, 64, 128), dev)
+    table = torch.randperm(200, generator=g)[:192].view(4, 48).to(torch.int32).to(dev)
+    lengths = torch.tensor([3000, 2000, 1, 2900], dtype=torch.int32, device=dev)
+    queries = [torch.randn((4, 8, n, 128), generator=g).bfloat16().to(dev) for n in (1, 1, 24, 50)]
+    expected = [pk.tree_attention(q, cache, table, lengths) for q in queries]
+    streams = [torch.cuda.Stream() for _ in queries]
+    torch.cuda.synchronize()
+    outs = []
+    for _ in range(5):
+        for q, stream in zip(queries, streams):
+            with torch.cuda.stream(stream):
+                outs.append(pk.tree_attention(q, cache, table, lengths))
+    torch.cuda.synchronize()
+    for i, out in enumerate(outs):
+        assert torch.equal(out, expected[i % len(queries)])
