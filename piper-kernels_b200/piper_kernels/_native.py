@@ -9,11 +9,14 @@ fallback: if the shared library is missing, every entry point raises
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 import threading
 from pathlib import Path
 
 LIB_DIR = Path(__file__).resolve().parent / "_lib"
 LIB_PATH = LIB_DIR / "libpiper_b200.so"
+BINDING_PATH = LIB_DIR / "decoding_binding.so"
 
 OK = 0
 ERR_INVALID_ARGUMENT = 1
@@ -234,6 +237,32 @@ def library() -> ctypes.CDLL:
             _declare(lib)
             _lib = lib
     return _lib
+
+
+_binding = None
+
+
+def binding():
+    """Load (once) and return the extension module that calls the decoding entry points on torch tensors.
+
+    Its functions check their arguments natively and return the outputs, a
+    status for :func:`check`, or None for arguments that the operator does not
+    take (csrc/decoding_binding.cpp).
+    """
+    global _binding
+    if _binding is None:
+        library()
+        if not BINDING_PATH.exists():
+            raise NativeLibraryMissing(
+                f"{BINDING_PATH} is missing: build the sm_100a extension with "
+                "`python piper-kernels_b200/build.py` (or __graft_entry__.build())"
+            )
+        loader = importlib.machinery.ExtensionFileLoader("decoding_binding", str(BINDING_PATH))
+        spec = importlib.util.spec_from_loader("decoding_binding", loader)
+        module = importlib.util.module_from_spec(spec)
+        loader.exec_module(module)
+        _binding = module
+    return _binding
 
 
 def last_error() -> str:

@@ -2,8 +2,9 @@
 
 Everything here runs on the host before any device work.  These operators are
 called once per layer and token, often with a few microseconds of GPU work, so
-a call first asks :func:`fits` of each argument, one expression without
-messages; only a misfit goes to :func:`check_tensor`, which says what is wrong.
+an eager call goes to the native binding first (:func:`direct`), which checks
+its arguments without messages; only what it does not take comes to the checks
+here, which say what is wrong.
 """
 
 from __future__ import annotations
@@ -16,6 +17,26 @@ from .._targets import AcceleratorTarget
 DTYPE_CODES = {torch.float16: _native.FLOAT16, torch.bfloat16: _native.BFLOAT16}
 SUPPORTED_HEAD_DIMS = (64, 128)
 MAX_NODES = 64
+
+_binding = None
+
+
+def direct(name: str, what: str, *args):
+    """Outputs of the native binding's function, or None: the call goes on through the checks.
+
+    That is so under ``torch.compile``, and for arguments that the operator
+    does not take.
+    """
+    global _binding
+    if torch.compiler.is_compiling():
+        return None
+    if _binding is None:
+        _binding = _native.binding()
+    out = getattr(_binding, name)(*args)
+    if type(out) is int:
+        _native.check(out, what)
+    return out
+
 
 _sm100_devices: dict[int, bool] = {}
 

@@ -9,7 +9,7 @@ from functools import lru_cache
 import torch
 
 from .. import _native
-from ._common import DTYPE_CODES, MAX_NODES, check_half, check_tensor, fits, launch, refuse_grad, require_device
+from ._common import DTYPE_CODES, MAX_NODES, check_half, check_tensor, direct, fits, launch, refuse_grad, require_device
 from .cache import QuantizedKVCache, check_batch
 
 OPERATOR = "tree_attention"
@@ -43,6 +43,11 @@ def tree_attention(
     Returns a contiguous ``[batch, heads, nodes, head_dim]`` of ``query``'s
     type.  Inference only.
     """
+    out = direct(
+        "attend", "piper_b200_tree_attention", cache.buffers, query, block_table, lengths, tree_mask, scale
+    )
+    if out is not None:
+        return out
     if query.ndim != 4:
         raise ValueError(
             f"{OPERATOR} query must have shape [batch, heads, sequence, head_dim], got {tuple(query.shape)}"

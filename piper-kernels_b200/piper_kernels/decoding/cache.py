@@ -29,6 +29,7 @@ from ._common import (
     SUPPORTED_HEAD_DIMS,
     check_half,
     check_tensor,
+    direct,
     fits,
     launch,
     refuse_grad,
@@ -46,11 +47,12 @@ class QuantizedKVCache:
     kv_heads, page_size]``, all contiguous on one device.  ``key_mean`` is
     float32 ``[kv_heads, head_dim]`` or None; it belongs to the rows written
     with it.  ``page_size`` is 16, 32, 64, 128 or 256, ``head_dim`` 64 or 128.
-    The buffers are read-only attributes, like the sizes ``pages``,
-    ``kv_heads``, ``page_size`` and ``head_dim`` and the ``device``.
+    The buffers are read-only attributes (``buffers``: all five), like the
+    sizes ``pages``, ``kv_heads``, ``page_size`` and ``head_dim`` and the
+    ``device``.
     """
 
-    __slots__ = ("_buffers", "device", "pages", "kv_heads", "page_size", "head_dim")
+    __slots__ = ("buffers", "device", "pages", "kv_heads", "page_size", "head_dim")
 
     def __init__(
         self,
@@ -78,7 +80,7 @@ class QuantizedKVCache:
             and (key_mean is None or fits(key_mean, shape[1::2], torch.float32, device) and key_mean.is_contiguous())
         ):
             _refuse_buffers(key_codes, key_scales, value_codes, value_scales, key_mean)
-        self._buffers = (key_codes, key_scales, value_codes, value_scales, key_mean)
+        self.buffers = (key_codes, key_scales, value_codes, value_scales, key_mean)
         self.device = device
         self.pages, self.kv_heads, self.page_size, self.head_dim = shape
 
@@ -107,27 +109,27 @@ class QuantizedKVCache:
 
     @property
     def key_codes(self) -> torch.Tensor:
-        return self._buffers[0]
+        return self.buffers[0]
 
     @property
     def key_scales(self) -> torch.Tensor:
-        return self._buffers[1]
+        return self.buffers[1]
 
     @property
     def value_codes(self) -> torch.Tensor:
-        return self._buffers[2]
+        return self.buffers[2]
 
     @property
     def value_scales(self) -> torch.Tensor:
-        return self._buffers[3]
+        return self.buffers[3]
 
     @property
     def key_mean(self) -> torch.Tensor | None:
-        return self._buffers[4]
+        return self.buffers[4]
 
     def native(self, block_table: torch.Tensor, lengths: torch.Tensor) -> _native.KVCache:
         """The C ABI's description of this cache for one batch."""
-        key_codes, key_scales, value_codes, value_scales, key_mean = self._buffers
+        key_codes, key_scales, value_codes, value_scales, key_mean = self.buffers
         batch, width = block_table.shape
         return _native.KVCache(
             key_codes.data_ptr(), key_scales.data_ptr(), value_codes.data_ptr(), value_scales.data_ptr(),
@@ -205,6 +207,10 @@ def write_kv_cache(
     entry that is no page of the cache, such as -1) are not written.  Pages
     that are written must not be shared between requests.
     """
+    if direct(
+        "write", "piper_b200_kv_cache_write", cache.buffers, key, value, block_table, lengths, counts
+    ) is not None:
+        return
     operator = "write_kv_cache"
     if key.ndim != 4:
         raise ValueError(f"{operator} key must have shape [batch, heads, sequence, head_dim], got {tuple(key.shape)}")
@@ -255,6 +261,13 @@ def read_kv_cache(
     (``lengths`` of zeros reads from the start); tokens from ``counts[b]`` on
     (default: none), and positions without a page, read as zeros.
     """
+    if dtype in DTYPE_CODES:
+        out = direct(
+            "read", "piper_b200_kv_cache_read", cache.buffers, block_table, lengths, counts, tokens,
+            dtype is torch.float16,
+        )
+        if out is not None:
+            return out
     operator = "read_kv_cache"
     if dtype not in DTYPE_CODES:
         check_half(operator, "dtype", dtype)
@@ -302,6 +315,8 @@ def keep_draft_path(
     counts[b]``.  ``lengths`` is not changed; the committed length is then
     ``lengths + counts``.
     """
+    if direct("keep", "piper_b200_kv_cache_keep", cache.buffers, block_table, lengths, path, counts) is not None:
+        return
     operator = "keep_draft_path"
     if path.ndim != 2:
         raise ValueError(f"{operator} path must have shape [batch, nodes], got {tuple(path.shape)}")

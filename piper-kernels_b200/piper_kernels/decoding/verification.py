@@ -7,7 +7,7 @@ from typing import NamedTuple
 import torch
 
 from .. import _native
-from ._common import MAX_NODES, check_tensor, fits, launch, refuse_grad, require_device
+from ._common import MAX_NODES, check_tensor, direct, fits, launch, refuse_grad, require_device
 
 OPERATOR = "verify_draft_tree"
 
@@ -56,6 +56,11 @@ def verify_draft_tree(
     ``tokens`` int64, ``parents`` int32 and ``uniform`` float32 ``[batch,
     nodes]``, ``noise`` float32 ``[batch, vocab]`` (positive); 1 to 64 nodes.
     """
+    found = direct(
+        "verify", "piper_b200_verify_draft_tree", target_probs, draft_probs, tokens, parents, uniform, noise
+    )
+    if found is not None:
+        return DraftVerification(*found)
     if target_probs.ndim != 3:
         raise ValueError(
             f"{OPERATOR} target_probs must have shape [batch, nodes, vocab], got {tuple(target_probs.shape)}"

@@ -204,3 +204,27 @@ def test_oracle_verification_follows_the_target_distribution() -> None:
     for x in range(vocab):
         p = float(target[0, 0, x])
         assert abs(int((first == x).sum()) - tries * p) <= 5 * (tries * p * (1 - p)) ** 0.5 + 1
+
+
+def test_the_binding_passes_on_what_it_does_not_take() -> None:
+    # None: the checks that explain come next.  (On CPU tensors that is always so.)
+    binding = _native.binding()
+    table, lengths = _batch()
+    x = torch.zeros(2, 2, 3, 64).half()
+    buffers = _cache().buffers
+    assert binding.attend(buffers, x, table, lengths, None, None) is None
+    assert binding.attend(None, x, table, lengths, None, None) is None
+    assert binding.attend(buffers, "query", table, None, 3, 1) is None
+    assert binding.attend() is None
+    assert binding.write(buffers, x, None, table, lengths, None) is None
+    assert binding.read(buffers, table, lengths, None, 1 << 80, True) is None
+    assert binding.read((1, 2, 3, 4, 5), table, lengths, None, 1, True) is None
+    assert binding.keep(buffers, table, lengths, x, lengths) is None
+    assert binding.verify(x, x, x, x, x, x) is None
+
+
+def test_missing_binding_fails_loudly(monkeypatch: pytest.MonkeyPatch, tmp_path) -> None:
+    monkeypatch.setattr(_native, "_binding", None)
+    monkeypatch.setattr(_native, "BINDING_PATH", tmp_path / "absent.so")
+    with pytest.raises(_native.NativeLibraryMissing, match="build"):
+        _native.binding()
