@@ -1,6 +1,11 @@
 // The quantised paged KV cache: writing new rows, reading rows back, and
-// moving the accepted rows of a drafted tree together.  All three are bound
-// by memory.
+// moving the accepted rows of a drafted tree together.  All three would be
+// bound by memory; writing is by its arithmetic (19 instructions a value, the
+// near-tie test of the division-free rounding among them) and reading nearly.
+//
+// Measured (4 prompts of 5001 to 8192 tokens, 32 heads of 128, bf16): written and
+// read back in 345 us, 3.8 TB/s or 0.59 of the copy rate; IEEE division in place
+// of the division-free rounding, and eight values a lane, took 392 us.
 //
 // A row is one token of one KV head: D codes q[d] and a scale s, standing for
 // q[d] * s (plus the key mean for keys), with

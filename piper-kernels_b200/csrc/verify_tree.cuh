@@ -16,7 +16,11 @@
 // Bound: memory (12 bytes a word for the last pass), and with few requests the
 // latency of the passes that follow one another.  A cluster of CTAs shares a
 // request's vocabulary and joins its sums and maxima through distributed
-// shared memory, in rank order.
+// shared memory, in rank order (one CTA a request took four times as long).
+//
+// Measured: a chain of 8 over 32768 words 8.8 us; 16 trees of 16 over 50001 words
+// (rows that start at any element) 17 us; 64 trees of 32 over 131072 words 66 us,
+// where the mean request reads some 3.5 MB: half of the copy rate.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -29,6 +33,7 @@ namespace piper {
 
 constexpr int kVerifyThreads = 512;
 constexpr int kVerifyUnroll = 4;  // 16-byte loads in flight of each row
+constexpr int kVerifySingle = 8;   // 4-byte ones, where rows are not aligned
 
 struct VerifyArgs {
   const float* target;
@@ -97,10 +102,10 @@ __device__ __forceinline__ void verify_words(const VerifyArgs& a, const float* p
     }
     v = whole + threadIdx.x;
   }
-  for (; v < end; v += kVerifyThreads * kVerifyUnroll) {
-    float pw[kVerifyUnroll], qw[kVerifyUnroll], ew[kVerifyUnroll];
+  for (; v < end; v += kVerifyThreads * kVerifySingle) {
+    float pw[kVerifySingle], qw[kVerifySingle], ew[kVerifySingle];
 #pragma unroll
-    for (int k = 0; k < kVerifyUnroll; ++k) {
+    for (int k = 0; k < kVerifySingle; ++k) {
       const int w = v + k * kVerifyThreads;
       pw[k] = qw[k] = ew[k] = 0.0f;
       if (w < end) {
@@ -110,7 +115,7 @@ __device__ __forceinline__ void verify_words(const VerifyArgs& a, const float* p
       }
     }
 #pragma unroll
-    for (int k = 0; k < kVerifyUnroll; ++k)
+    for (int k = 0; k < kVerifySingle; ++k)
       if (v + k * kVerifyThreads < end) body(v + k * kVerifyThreads, pw[k], qw[k], ew[k]);
   }
 }
