@@ -6,21 +6,29 @@
 // the target's distribution and q the draft's,
 //   total = sum_v max(r[v] - q[v], 0),   r <- max(r - q, 0) / total
 // before a further sibling can be tested, and at the end for the next token,
-//   argmax_v r[v] / noise[v].
+//   argmax_v r[v] / noise[v],
+// which takes the last rejected draft out on the way: its total is not needed.
 // The rest after several rejections is computed again from the rows and the
-// over, so that nothing is written back.  All is fp32; a total divides as its
+// totals, so that nothing is written back.  All is fp32; a total divides as its
 // reciprocal multiplies (an IEEE division for each word and rejection made the
 // passes twice as long), the last division, by the noise, is IEEE: equal
 // quotients are equal, and go to the lowest index.
+//
+// A warp divides only near its best quotient (a division for every word: 51 us
+// instead of 45 in the largest case below).
 //
 // Bound: memory (12 bytes a word for the last pass), and with few requests the
 // latency of the passes that follow one another.  A cluster of CTAs shares a
 // request's vocabulary and joins its sums and maxima through distributed
 // shared memory, in rank order (one CTA a request took four times as long).
 //
-// Measured: a chain of 8 over 32768 words 8.8 us; 16 trees of 16 over 50001 words
-// (rows that start at any element) 17 us; 64 trees of 32 over 131072 words 66 us,
-// where the mean request reads some 3.5 MB: half of the copy rate.
+// Measured: a chain of 8 over 32768 words 7.1 us; 16 trees of 16 over 50001 words
+// (rows that start at any element) 11 us; 64 trees of 32 over 131072 words 45 us,
+// where the mean request reads 1.7 to 1.8 MB: 0.4 of the copy rate, as 512 CTAs run
+// in two turns and a request of four rejections takes four passes.  No faster: the
+// noise fetched into L2 in advance (52 before, 53), half the loads under way and three
+// CTAs on an SM (47), 1024 threads (64 against 52), one turn of 4 CTAs a request
+// (60 against 51), passes made for no earlier rejection (45, with spills).
 #pragma once
 
 #include <cooperative_groups.h>
@@ -33,7 +41,9 @@ namespace piper {
 
 constexpr int kVerifyThreads = 512;
 constexpr int kVerifyUnroll = 4;  // 16-byte loads in flight of each row
-constexpr int kVerifySingle = 8;   // 4-byte ones, where rows are not aligned
+constexpr int kVerifySingle = 8;  // 4-byte ones, where rows are not aligned
+constexpr float kVerifyLeast = 0x1p-126f;  // the least total whose reciprocal is finite
+constexpr float kVerifyTold = 0x1p-64f;    // a quotient far above what fp32 rounds to zero
 
 struct VerifyArgs {
   const float* target;
@@ -70,15 +80,16 @@ __device__ __forceinline__ VerifyBest verify_better(VerifyBest x, VerifyBest y) 
 
 // Calls body(v, p, q, e) for this thread's words of [begin, end): the target's,
 // the draft's and the noise's values (0 where a pass does not read them).
-// `begin` is a multiple of 4.
-template <bool kDraft, bool kNoise, typename Body>
+// `begin` is a multiple of 4.  After every few words a warp calls turn(), together.
+template <bool kDraft, bool kNoise, typename Body, typename Turn>
 __device__ __forceinline__ void verify_words(const VerifyArgs& a, const float* p, const float* q, const float* e,
-                                             int begin, int end, Body body) {
+                                             int begin, int end, Body body, Turn turn) {
+  const int lane = threadIdx.x % 32;
   int v = begin + threadIdx.x;
   if (a.vec) {
     const int whole = begin + (end - begin) / 4 * 4;
     constexpr int kStep = kVerifyThreads * 4;
-    for (int u = begin + threadIdx.x * 4; u < whole; u += kStep * kVerifyUnroll) {
+    for (int u = begin + threadIdx.x * 4; u - lane * 4 < whole; u += kStep * kVerifyUnroll) {
       float4 pw[kVerifyUnroll], qw[kVerifyUnroll], ew[kVerifyUnroll];
 #pragma unroll
       for (int k = 0; k < kVerifyUnroll; ++k) {
@@ -98,11 +109,12 @@ __device__ __forceinline__ void verify_words(const VerifyArgs& a, const float* p
           body(w + 2, pw[k].z, qw[k].z, ew[k].z);
           body(w + 3, pw[k].w, qw[k].w, ew[k].w);
         }
+        turn();
       }
     }
     v = whole + threadIdx.x;
   }
-  for (; v < end; v += kVerifyThreads * kVerifySingle) {
+  for (; v - lane < end; v += kVerifyThreads * kVerifySingle) {
     float pw[kVerifySingle], qw[kVerifySingle], ew[kVerifySingle];
 #pragma unroll
     for (int k = 0; k < kVerifySingle; ++k) {
@@ -115,8 +127,10 @@ __device__ __forceinline__ void verify_words(const VerifyArgs& a, const float* p
       }
     }
 #pragma unroll
-    for (int k = 0; k < kVerifySingle; ++k)
+    for (int k = 0; k < kVerifySingle; ++k) {
       if (v + k * kVerifyThreads < end) body(v + k * kVerifyThreads, pw[k], qw[k], ew[k]);
+      if (k % 4 == 3) turn();
+    }
   }
 }
 
@@ -138,84 +152,123 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(VerifyAr
   const int vocab = static_cast<int>(a.vocab);
   const int per = ((vocab + ranks - 1) / ranks + 3) / 4 * 4;
   const int begin = min(vocab, per * rank), end = min(vocab, begin + per);
-  if (tid < a.nodes) {
-    const int64_t x = tid == 0 ? -1 : __ldg(reinterpret_cast<const long long*>(a.tokens) + b * a.tokens_stride + tid);
-    const int parent = tid == 0 ? -1 : __ldg(a.parents + b * a.parents_stride + tid);
-    const bool there = x >= 0 && x < a.vocab && parent >= 0 && parent < tid;
-    node_parent[tid] = there ? parent : -1;
-    if (there) {
-      node_p[tid] = __ldg(a.target + b * a.ts[0] + parent * a.ts[1] + x);
-      node_q[tid] = __ldg(a.draft + b * a.ds[0] + parent * a.ds[1] + x);
-      node_u[tid] = __ldg(a.uniform + b * a.uniform_stride + tid);
+  if (tid < kMaxNodes) {
+    node_parent[tid] = -1;
+    if (tid > 0 && tid < a.nodes) {
+      const int64_t x = __ldg(reinterpret_cast<const long long*>(a.tokens) + b * a.tokens_stride + tid);
+      const int parent = __ldg(a.parents + b * a.parents_stride + tid);
+      if (x >= 0 && x < a.vocab && parent >= 0 && parent < tid) {
+        node_parent[tid] = parent;
+        node_p[tid] = __ldg(a.target + b * a.ts[0] + parent * a.ts[1] + x);
+        node_q[tid] = __ldg(a.draft + b * a.ds[0] + parent * a.ds[1] + x);
+        node_u[tid] = __ldg(a.uniform + b * a.uniform_stride + tid);
+      }
     }
   }
   __syncthreads();
-  // Every thread of the cluster takes the same walk.
+  // Every thread of the cluster takes the same walk.  A node's children, as
+  // bits (they all come after it):
+  auto children_of = [&](int node) {
+    const uint64_t low = __ballot_sync(0xffffffffu, node_parent[lane] == node);
+    const uint64_t high = __ballot_sync(0xffffffffu, node_parent[lane + 32] == node);
+    return low | (high << 32);
+  };
   int current = 0, rejected = 0, count = 1, turn = 0;
   int32_t* path = a.path + b * a.nodes;
   if (rank == 0 && tid == 0) path[0] = 0;
-  for (int i = 1; i < a.nodes; ++i) {
-    if (node_parent[i] != current) continue;
-    const float p = node_p[i], q = node_q[i];
-    if (node_u[i] * q < rest_of(p, q, over, rejected)) {
-      if (rank == 0 && tid == 0) path[count] = i;
-      ++count;
-      current = i;
-      rejected = 0;
-      continue;
+  uint64_t children = children_of(0);
+  // Nothing is tested against the rest of the last rejection, and the next
+  // token does not depend on its total: the last pass takes that draft out
+  // without it, unless its scores come out too small to be told from nothing.
+  bool open_end = false, may_end = true;
+  VerifyBest best;
+  const float* er = a.noise + b * a.noise_stride;
+  for (;;) {  // twice at most
+    while (children != 0) {
+      const int i = __ffsll(static_cast<long long>(children)) - 1;
+      const float p = node_p[i], q = node_q[i];
+      if (node_u[i] * q < rest_of(p, q, over, rejected)) {
+        if (rank == 0 && tid == 0) path[count] = i;
+        ++count;
+        current = i;
+        rejected = 0;
+        children = children_of(i);
+        continue;
+      }
+      if (may_end && (children & (children - 1)) == 0) {
+        open_end = true;
+        break;
+      }
+      children &= children - 1;
+      const float* pr = a.target + b * a.ts[0] + current * a.ts[1];
+      const float* qr = a.draft + b * a.ds[0] + current * a.ds[1];
+      float sum = 0.0f;
+      verify_words<true, false>(
+          a, pr, qr, nullptr, begin, end,
+          [&](int, float x, float y, float) { sum += fmaxf(rest_of(x, y, over, rejected) - y, 0.0f); }, [] {});
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      if (lane == 0) warp_sum[warp] = sum;
+      __syncthreads();
+      if (tid == 0) {
+        float mine = 0.0f;
+        for (int w = 0; w < kWarps; ++w) mine += warp_sum[w];
+        joined_sum[turn] = mine;
+      }
+      cluster.sync();
+      float total = 0.0f;
+      for (int r = 0; r < ranks; ++r) total += *cluster.map_shared_rank(&joined_sum[turn], r);
+      // The other turn's sums are written only after every rank has read these:
+      // each passes the next cluster.sync after its reading.
+      turn ^= 1;
+      if (total >= kVerifyLeast) {  // else nothing would be left: rest stays as it was
+        if (tid == 0) over[rejected] = 1.0f / total;
+        ++rejected;
+      }
+      __syncthreads();
     }
     const float* pr = a.target + b * a.ts[0] + current * a.ts[1];
     const float* qr = a.draft + b * a.ds[0] + current * a.ds[1];
-    float sum = 0.0f;
-    verify_words<true, false>(a, pr, qr, nullptr, begin, end, [&](int, float x, float y, float) {
-      sum += fmaxf(rest_of(x, y, over, rejected) - y, 0.0f);
-    });
+    best = VerifyBest{-1.0f, 0};
+    // Only a word near the warp's best is divided: r < score * e, by more than
+    // the product's rounding, cannot win (nor does it tie).
+    float bound = 0.0f;
+    auto race = [&](int v, float r, float e) {
+      if (!(r < bound * e)) {
+        const float s = __fdiv_rn(r, e);
+        if (s > best.score) best = VerifyBest{s, v};  // (a thread's words ascend)
+        bound = fmaxf(bound, fminf(s, 0x1p127f) * 0x1.fffffp-1f);
+      }
+    };
+    auto share = [&] { bound = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(bound))); };
+    if (rejected == 0 && !open_end)
+      verify_words<false, true>(a, pr, qr, er, begin, end, [&](int v, float x, float, float e) { race(v, x, e); }, share);
+    else
+      verify_words<true, true>(
+          a, pr, qr, er, begin, end,
+          [&](int v, float x, float y, float e) {
+            const float r = rest_of(x, y, over, rejected);
+            race(v, open_end ? fmaxf(r - y, 0.0f) : r, e);
+          },
+          share);
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) warp_sum[warp] = sum;
+    for (int o = 16; o > 0; o >>= 1)
+      best = verify_better(best, VerifyBest{__shfl_xor_sync(0xffffffffu, best.score, o),
+                                            __shfl_xor_sync(0xffffffffu, best.at, o)});
+    if (lane == 0) warp_best[warp] = best;
     __syncthreads();
     if (tid == 0) {
-      float mine = 0.0f;
-      for (int w = 0; w < kWarps; ++w) mine += warp_sum[w];
-      joined_sum[turn] = mine;
+      for (int w = 1; w < kWarps; ++w) best = verify_better(best, warp_best[w]);
+      joined_best = best;
     }
     cluster.sync();
-    float total = 0.0f;
-    for (int r = 0; r < ranks; ++r) total += *cluster.map_shared_rank(&joined_sum[turn], r);
-    // The other turn's sums are written only after every rank has read these:
-    // each passes the next cluster.sync after its reading.
-    turn ^= 1;
-    if (total > 0.0f) {  // else nothing would be left: rest stays as it was
-      if (tid == 0) over[rejected] = 1.0f / total;
-      ++rejected;
-    }
-    __syncthreads();
+    if (!open_end) break;
+    bool told = false;
+    for (int r = 0; r < ranks; ++r) told |= cluster.map_shared_rank(&joined_best, r)->score > kVerifyTold;
+    if (told) break;
+    open_end = may_end = false;
+    cluster.sync();  // every rank has read the scores that are written again
   }
-  const float* pr = a.target + b * a.ts[0] + current * a.ts[1];
-  const float* qr = a.draft + b * a.ds[0] + current * a.ds[1];
-  const float* er = a.noise + b * a.noise_stride;
-  VerifyBest best{-1.0f, 0};
-  auto race = [&](int v, float r, float e) {
-    const float s = __fdiv_rn(r, e);
-    if (s > best.score) best = VerifyBest{s, v};  // (a thread's words ascend)
-  };
-  if (rejected == 0)
-    verify_words<false, true>(a, pr, qr, er, begin, end, [&](int v, float x, float, float e) { race(v, x, e); });
-  else
-    verify_words<true, true>(a, pr, qr, er, begin, end, [&](int v, float x, float y, float e) {
-      race(v, rest_of(x, y, over, rejected), e);
-    });
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    best = verify_better(best, VerifyBest{__shfl_xor_sync(0xffffffffu, best.score, o),
-                                          __shfl_xor_sync(0xffffffffu, best.at, o)});
-  if (lane == 0) warp_best[warp] = best;
-  __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < kWarps; ++w) best = verify_better(best, warp_best[w]);
-    joined_best = best;
-  }
-  cluster.sync();
   if (rank == 0) {
     if (tid == 0) {
       for (int r = 1; r < ranks; ++r) best = verify_better(best, *cluster.map_shared_rank(&joined_best, r));

@@ -409,6 +409,33 @@ def test_verification_when_nothing_is_left() -> None:
         assert torch.equal(x.cpu(), y)
 
 
+@pytest.mark.parametrize("left,scale", [(1e-30, 1e20), (1e-20, 1.0), (0.25, 1e38), (1e-37, 1e9)])
+@pytest.mark.parametrize("children", [1, 2])
+def test_verification_of_a_rest_that_is_nearly_nothing(left, scale, children) -> None:
+    # One word is all that is left (everywhere else the target is at most the
+    # draft, in the same bits), so the next token is that word whatever the
+    # noise, even where left / noise is below the least fp32 number.
+    dev = require_b200()
+    g = torch.Generator().manual_seed(21)
+    batch, vocab, word = 3, 5003, 4444
+    nodes = 1 + children
+    draft = torch.softmax(torch.randn((batch, 1, vocab), generator=g), -1).repeat(1, nodes, 1)
+    draft[:, :, word] = 0.0
+    target = draft.clone()
+    tokens = torch.arange(nodes).repeat(batch, 1) + 10
+    target[:, :, 11 : 11 + children] = 0.0
+    target[:, :, word] = left
+    parents = torch.zeros((batch, nodes), dtype=torch.int32)
+    parents[:, 0] = -1
+    uniform = torch.full((batch, nodes), 0.5)
+    noise = torch.empty((batch, vocab)).exponential_(generator=g).clamp(0.1, 3.0) * scale
+    args = (target, draft, tokens, parents, uniform, noise)
+    got = pk.verify_draft_tree(*(x.to(dev) for x in args))
+    assert got[2].tolist() == [word] * batch
+    for x, y in zip(got, oracle.verify(*args)):
+        assert torch.equal(x.cpu(), y)
+
+
 def test_verification_follows_the_target_distribution() -> None:
     # Binomial counts within five standard deviations (plus one).
     dev = require_b200()
