@@ -14,26 +14,15 @@ have.
 
 from .attention.piper_attention import piper_attention
 from .attention.sage_attention_2pp import sage_attention_2pp
-from .decoding import (
-    DraftVerification,
-    QuantizedKVCache,
-    keep_draft_path,
-    read_kv_cache,
-    tree_attention,
-    tree_mask_from_parents,
-    verify_draft_tree,
-    write_kv_cache,
-)
+from .decoding import DraftVerification as DraftVerification
+from .decoding import QuantizedKVCache as QuantizedKVCache
+from .decoding import keep_draft_path as keep_draft_path
+from .decoding import read_kv_cache as read_kv_cache
+from .decoding import tree_attention as tree_attention
+from .decoding import tree_mask_from_parents as tree_mask_from_parents
+from .decoding import verify_draft_tree as verify_draft_tree
+from .decoding import write_kv_cache as write_kv_cache
 
-__all__ = [
-    "DraftVerification",
-    "QuantizedKVCache",
-    "keep_draft_path",
-    "piper_attention",
-    "read_kv_cache",
-    "sage_attention_2pp",
-    "tree_attention",
-    "tree_mask_from_parents",
-    "verify_draft_tree",
-    "write_kv_cache",
-]
+# A star import gives the reference package's names and no others; the decoding
+# operators are attributes of the package, and decoding.__all__ lists them.
+__all__ = ["piper_attention", "sage_attention_2pp"]
