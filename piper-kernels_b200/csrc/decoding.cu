@@ -126,21 +126,23 @@ TreePlan tree_plan(int64_t batch, int64_t kv_heads, int64_t rows, int64_t positi
   return p;
 }
 
-// The kernel for a number of query rows of a KV head: up to 16 one m16 tile
-// on four warps, up to 128 a tcgen05 tile whose streams take alternate keys,
+// The kernel for a number of query rows of a KV head: up to 8 and up to 16 one
+// mma tile on four warps, whose n or m they are, up to 128 a tcgen05 tile whose streams take alternate keys,
 // more a pair of them over the same keys.
-enum class TreeKind { kFew, kAlternate, kPair };
+enum class TreeKind { kEight, kSixteen, kAlternate, kPair };
 TreeKind tree_kind(int64_t rows) {
-  return rows <= 16 ? TreeKind::kFew : rows <= 128 ? TreeKind::kAlternate : TreeKind::kPair;
+  if (rows <= 16) return rows <= 8 ? TreeKind::kEight : TreeKind::kSixteen;
+  return rows <= 128 ? TreeKind::kAlternate : TreeKind::kPair;
 }
 constexpr int kFewGroups = 2;
-template <int D>
-using FewRows = piper::TreeTile<D, 4, kFewGroups>;
+template <int D, int ROWS>
+using FewRows = piper::TreeTile<D, 4, kFewGroups, ROWS>;
 
 template <int D>
 TreePlan tree_plan(int64_t batch, int64_t kv_heads, int64_t rows, int64_t positions, int sms) {
   switch (tree_kind(rows)) {
-    case TreeKind::kFew: return tree_plan<FewRows<D>>(batch, kv_heads, rows, positions, sms);
+    case TreeKind::kEight: return tree_plan<FewRows<D, 8>>(batch, kv_heads, rows, positions, sms);
+    case TreeKind::kSixteen: return tree_plan<FewRows<D, 16>>(batch, kv_heads, rows, positions, sms);
     case TreeKind::kAlternate: return tree_plan<piper::WideTile<D, false>>(batch, kv_heads, rows, positions, sms);
     default: return tree_plan<piper::WideTile<D, true>>(batch, kv_heads, rows, positions, sms);
   }
@@ -151,6 +153,12 @@ int allow_smem(const void* kernel, int bytes) {
   return PIPER_B200_OK;
 }
 
+template <typename T, int D, int ROWS>
+int set_up_few() {
+  const void* kernel = reinterpret_cast<const void*>(piper::tree_attention_kernel<T, D, 4, kFewGroups, ROWS>);
+  return allow_smem(kernel, FewRows<D, ROWS>::kAlloc);
+}
+
 template <typename T, int D, bool kShared>
 int set_up_wide() {
   const void* kernel = reinterpret_cast<const void*>(piper::tree_wide_kernel<T, D, kShared>);
@@ -159,8 +167,9 @@ int set_up_wide() {
 
 template <typename T, int D>
 int set_up_instances() {
-  int rc = allow_smem(reinterpret_cast<const void*>(piper::tree_attention_kernel<T, D, 4, kFewGroups>), FewRows<D>::kAlloc);
+  int rc = set_up_few<T, D, 8>();
   if (rc != PIPER_B200_OK) return rc;
+  if ((rc = set_up_few<T, D, 16>()) != PIPER_B200_OK) return rc;
   if ((rc = set_up_wide<T, D, false>()) != PIPER_B200_OK) return rc;
   return set_up_wide<T, D, true>();
 }
@@ -214,9 +223,12 @@ int launch_tree(piper::TreeArgs a, Kernel kernel, int threads, int sms, size_t w
 template <typename T, int D>
 int launch_tree_rows(const piper::TreeArgs& a, int sms, size_t workspace_bytes, cudaStream_t stream) {
   switch (tree_kind(a.rows)) {
-    case TreeKind::kFew:
-      return launch_tree<T, D, FewRows<D>>(a, piper::tree_attention_kernel<T, D, 4, kFewGroups>, FewRows<D>::kThreads, sms,
-                                           workspace_bytes, stream);
+    case TreeKind::kEight:
+      return launch_tree<T, D, FewRows<D, 8>>(a, piper::tree_attention_kernel<T, D, 4, kFewGroups, 8>,
+                                              FewRows<D, 8>::kThreads, sms, workspace_bytes, stream);
+    case TreeKind::kSixteen:
+      return launch_tree<T, D, FewRows<D, 16>>(a, piper::tree_attention_kernel<T, D, 4, kFewGroups, 16>,
+                                               FewRows<D, 16>::kThreads, sms, workspace_bytes, stream);
     case TreeKind::kAlternate:
       return launch_tree<T, D, piper::WideTile<D, false>>(a, piper::tree_wide_kernel<T, D, false>,
                                                           piper::kWideThreads, sms, workspace_bytes, stream);

@@ -7,6 +7,12 @@
 // over the keys j that the row sees.  Reading the cache once (2 D + 8 bytes a
 // key) bounds it while the rows are few: 16 rows need 64 products a byte.
 //
+// Up to 8 rows are the n of the products' m16n8k16: keys are the m of
+// S^T = K Q^T and head dimensions that of O^T = V^T P^T, and the weights are
+// transposed in registers between the two.  9 to 16 rows are the m, S = Q K^T
+// and O = P V: for 8 rows that was half empty (110 against 94 us in the first
+// case measured below).
+//
 // Products: fp16 tensor-core MMAs (m16n8k16, fp32 accumulators).  Codes are
 // exact in fp16.  fp16 queries are used as they are; a bf16 row is scaled by
 // a power of two to [1, 2) at its largest element, which loses only what lies
@@ -21,7 +27,8 @@
 // elements, ldmatrix gives lane (g, t) the bytes 4t .. 4t+3 of key g: the
 // fragment's two pairs, if query elements are permuted alike.  ldmatrix.trans
 // gives keys 2t, 2t+1 of bytes 2g, 2g+1: fragments of the even and of the odd
-// head dimensions.  A byte becomes fp16 by a byte permute under 0x64 (1024 +
+// head dimensions.  These are the b of 16 rows' products, and pairs of them the
+// a of 8 rows'.  A byte becomes fp16 by a byte permute under 0x64 (1024 +
 // code + 128) and one subtraction.
 //
 // Work: a segment is one (request, KV head, row tile); it has S::kLead units
@@ -34,9 +41,11 @@
 // tree_merge_kernel joins the parts.
 //
 // Measured (32 query over 8 KV heads of 128, pages of 64, one token each): 64
-// requests of 1 to 8192 tokens 110 us, 5.0 TB/s or 0.78 of the copy rate; one
-// request of 131072 tokens 61 us.  Instructions bound it, 320 of some 660 for
-// 32 keys a warp turning codes into fp16: 16 keys a warp took 131 us.
+// requests of 1 to 8192 tokens 94 us, 5.9 TB/s or 0.92 of the copy rate; one
+// request of 256 tokens 7.6 us.  24 heads of 64, 5 nodes, 32 requests of 333 to
+// 4097 tokens in pages of 16: 65 us, 0.55 of the copy rate.  With 16 rows
+// instructions bound it, 320 of some 660 for 32 keys a warp turning codes into
+// fp16: 16 keys a warp took 131 us for 110.
 #pragma once
 
 #include <math.h>
@@ -68,23 +77,26 @@ struct TreeArgs {
   float scale_log2e;
 };
 
-// Tile of up to 16 rows: a warp takes 16 * GROUPS keys of it.
-template <int D, int WARPS, int GROUPS>
+// Tile of up to ROWS (8 or 16) rows: a warp takes 16 * GROUPS keys of it.
+template <int D, int WARPS, int GROUPS, int ROWS>
 struct TreeTile {
-  static constexpr int kRows = 16;
+  static constexpr int kRows = ROWS;
   static constexpr int kKeys = 16 * GROUPS * WARPS;
   static constexpr int kThreads = 32 * (WARPS + 1);  // and one warp that fetches
   static constexpr int kCodes = kKeys * D;
   static constexpr int kScales = kKeys * 4;
   static constexpr int kStage = 2 * kCodes + 2 * kScales;
   static constexpr int kStageAlloc = (kStage + 1023) / 1024 * 1024;
-  static constexpr int kJoinStride = 48;  // floats, 32 of them used; 16 banks between rows
-  static constexpr int kJoin = WARPS * 16 * kJoinStride * 4;
+  static constexpr int kJoinColumns = 512 / ROWS;
+  static constexpr int kJoinStride = kJoinColumns + 16;  // floats; 16 banks between rows
+  static constexpr int kJoin = WARPS * ROWS * kJoinStride * 4;
   static constexpr int kState = 2 * WARPS * kRows * 4;
-  static constexpr int kQuery = (D / 16) * 32 * 16;  // fragments
+  static constexpr int kQuery = ROWS == 16 ? (D / 16) * 32 * 16 : 0;  // fragments
   static constexpr int kFixed = kJoin + kState + kQuery + kRows * 8 + 512;
-  static constexpr int kCtas = D == 64 ? 3 : 2;  // per SM, what registers and stages allow
-  static constexpr int kLead = 4;  // a segment's start and end, in key tiles
+  // Per SM, what registers and stages allow (8 rows: of 128, three spilled
+  // and took 115 us instead of 94; of 64, three took 73 us instead of 68, five 82).
+  static constexpr int kCtas = D == 64 ? (ROWS == 8 ? 4 : 3) : 2;
+  static constexpr int kLead = ROWS == 8 ? 3 : 4;  // a segment's start and end, in key tiles
   static constexpr int kFit = (227 * 1024 / kCtas - 1024 * 2 - kFixed) / kStageAlloc;
   static constexpr int kStages = kFit > 8 ? 8 : kFit;
   static constexpr int kAlloc = kStages * kStageAlloc + kFixed + 1024;
@@ -225,6 +237,13 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// An 8 x 8 matrix of 16-bit elements, a row's pair to each lane, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
 // Two of the four codes in x (each plus 128), chosen by `select`, as fp16.
 template <uint32_t select>
 __device__ __forceinline__ uint32_t codes_f16(uint32_t x) {
@@ -265,15 +284,15 @@ __device__ __forceinline__ void query4(const T* p, bool vec, float (&x)[4]) {
   for (int i = 0; i < 4; ++i) x[i] = to_f32<T>(reinterpret_cast<const T*>(e)[i]);
 }
 
-// The fragments of query rows r0 + lane / 4 and that plus 8 (zeros past the
-// last row), scaled to fp16, and what undoes the scaling times the softmax
+// The fragments of query rows r0 + lane / 4 and, of two halves, that plus 8
+// (zeros past the last row), scaled to fp16, and what undoes the scaling times the softmax
 // scale.
-template <typename T, int D>
-__device__ __forceinline__ void query_fragments(const TreeArgs& a, int b, int kv, int r0, uint32_t (&q)[D / 16][4],
-                                                float (&factor)[2]) {
+template <typename T, int D, int HALVES = 2>
+__device__ __forceinline__ void query_fragments(const TreeArgs& a, int b, int kv, int r0, uint32_t (&q)[D / 16][2 * HALVES],
+                                                float (&factor)[HALVES]) {
   const int lane = threadIdx.x % 32;
 #pragma unroll
-  for (int half = 0; half < 2; ++half) {
+  for (int half = 0; half < HALVES; ++half) {
     const int row = r0 + lane / 4 + 8 * half;
     float x[D / 16][4] = {};
     if (row < a.rows) {
@@ -300,17 +319,18 @@ __device__ __forceinline__ void query_fragments(const TreeArgs& a, int b, int kv
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) {
       q[c][half] = pack2(x[c][0] * up, x[c][1] * up, __half());
-      q[c][half + 2] = pack2(x[c][2] * up, x[c][3] * up, __half());
+      q[c][half + HALVES] = pack2(x[c][2] * up, x[c][3] * up, __half());
     }
   }
 }
 
-template <typename T, int D, int WARPS, int GROUPS>
-__global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS>::kThreads, TreeTile<D, WARPS, GROUPS>::kCtas)
+template <typename T, int D, int WARPS, int GROUPS, int ROWS>
+__global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS, ROWS>::kThreads, TreeTile<D, WARPS, GROUPS, ROWS>::kCtas)
     tree_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map,
                           TreeArgs a) {
-  using S = TreeTile<D, WARPS, GROUPS>;
-  constexpr int kN = 2 * GROUPS;  // groups of eight keys of a warp
+  using S = TreeTile<D, WARPS, GROUPS, ROWS>;
+  constexpr bool kEight = ROWS == 8;
+  constexpr int kN = kEight ? GROUPS : 2 * GROUPS;  // score fragments of a warp
   constexpr int kStages = S::kStages;
   constexpr int kChunks = D / 16;
   extern __shared__ uint8_t smem_raw[];
@@ -399,6 +419,18 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS>::kThreads, TreeTile
 
   // ---- computing warps: some keys of each tile, all rows.
   const int g = lane / 4, t = lane % 4;
+  // Element x of score fragment n is row row_at(h), h = row_half(x), and key
+  // key_at(n, e), e = key_half(x), of the warp's.
+  auto row_half = [](int x) { return kEight ? (x & 1) : x / 2; };
+  auto key_half = [](int x) { return kEight ? x / 2 : (x & 1); };
+  auto row_at = [&](int h) { return kEight ? 2 * t + h : g + 8 * h; };
+  auto key_at = [&](int n, int e) { return kEight ? 16 * n + g + 8 * e : 8 * n + 2 * t + e; };
+  // Over the lanes that hold the same rows.
+  auto of_row = [&](float x, auto join2) {
+#pragma unroll
+    for (int o = kEight ? 4 : 1; o < (kEight ? 32 : 4); o <<= 1) x = join2(x, __shfl_xor_sync(0xffffffffu, x, o));
+    return x;
+  };
   int stage = 0;
   uint32_t phase = 0;
   bool ok = true;
@@ -409,10 +441,16 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS>::kThreads, TreeTile
     const int row0 = (run.hr % a.row_tiles) * S::kRows;
     const bool all = run.all;
     const int64_t length = max(0, __ldg(a.c.lengths + b));
-    // Every warp has the rows' factors; warp 0's fragments serve all (holding
-    // them cost each thread 32 registers, and the SM a CTA).
     float factor[2];
-    {
+    uint32_t held[kEight ? kChunks : 1][2];
+    if constexpr (kEight) {
+      float mine[1];
+      query_fragments<T, D, 1>(a, b, kv, row0, held, mine);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) factor[h] = __shfl_sync(0xffffffffu, mine[0], 4 * row_at(h));
+    } else {
+      // Every warp has the rows' factors; warp 0's fragments serve all (holding
+      // them cost each thread 32 registers, and the SM a CTA).
       uint32_t q[kChunks][4];
       query_fragments<T, D>(a, b, kv, row0, q, factor);
       if (warp == 0) {
@@ -433,7 +471,7 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS>::kThreads, TreeTile
       words[tid] = word;
     }
     bar_sync(1, WARPS * 32);
-    float o[2 * kChunks][4] = {};
+    float o[kEight ? kChunks : 2 * kChunks][4] = {};
     float unit[2] = {kNoReference, kNoReference}, l[2] = {0.0f, 0.0f};
     for (int tile = run.tile; tile < run.tile + run.count; ++tile) {
       if (ok) ok = mbar_wait_block_warp(smem_u32(&full_bar[stage]), phase, a.wait_budget_ns, a.status, kStatusTimeoutFull,
@@ -451,7 +489,8 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS>::kThreads, TreeTile
         for (int c = 0; c < kChunks; c += 2) {
           uint4 f[2];
 #pragma unroll
-          for (int x = 0; x < 2; ++x) f[x] = query[(c + x) * 32 + lane];
+          for (int x = 0; x < 2; ++x)
+            if constexpr (!kEight) f[x] = query[(c + x) * 32 + lane];
 #pragma unroll
           for (int i = 0; i < GROUPS; ++i) {
             uint32_t k[4];
@@ -460,79 +499,92 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS>::kThreads, TreeTile
             for (int x = 0; x < 4; ++x) k[x] ^= 0x80808080u;
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              const uint32_t q[4] = {f[x].x, f[x].y, f[x].z, f[x].w};
+              if constexpr (kEight) {
+                const uint32_t keys[4] = {codes_f16<0x4140>(k[2 * x]), codes_f16<0x4140>(k[2 * x + 1]),
+                                          codes_f16<0x4342>(k[2 * x]), codes_f16<0x4342>(k[2 * x + 1])};
+                mma16816(y[i], keys, held[c + x][0], held[c + x][1]);
+              } else {
+                const uint32_t q[4] = {f[x].x, f[x].y, f[x].z, f[x].w};
 #pragma unroll
-              for (int n = 0; n < 2; ++n)
-                mma16816(y[2 * i + n], q, codes_f16<0x4140>(k[2 * x + n]), codes_f16<0x4342>(k[2 * x + n]));
+                for (int n = 0; n < 2; ++n)
+                  mma16816(y[2 * i + n], q, codes_f16<0x4140>(k[2 * x + n]), codes_f16<0x4342>(k[2 * x + n]));
+              }
             }
           }
         }
-        uint32_t w[GROUPS][4];
+        uint32_t w[GROUPS][kEight ? 2 : 4];
+        auto two = [&](const float* p, int n) {
+          if constexpr (kEight) return make_float2(p[key_at(n, 0)], p[key_at(n, 1)]);
+          return *reinterpret_cast<const float2*>(p + key_at(n, 0));
+        };
         // A masked tile has a body of its own: selections would lengthen the
         // other's.
         auto weigh = [&](auto hidden) {
-          uint32_t unseen = 0u;  // bit 4 n + 2 h + e
+          uint32_t unseen = 0u;  // bit 4 n + x
           if constexpr (hidden.value) {
 #pragma unroll
             for (int n = 0; n < kN; ++n)
 #pragma unroll
               for (int e = 0; e < 2; ++e) {
-                const int key = key0 + n * 8 + 2 * t + e;
+                const int key = key0 + key_at(n, e);
                 const int64_t j = first + key - length;
                 const bool there = (goods >> (key >> box_shift)) & 1u;
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
-                  if (!(there && (j < 0 || (j < a.nodes && ((words[g + 8 * h] >> (j & 63)) & 1u)))))
-                    unseen |= 1u << (4 * n + 2 * h + e);
+                  if (!(there && (j < 0 || (j < a.nodes && ((words[row_at(h)] >> (j & 63)) & 1u)))))
+                    unseen |= 1u << (4 * n + (kEight ? 2 * e + h : 2 * h + e));
               }
           }
           float most[2] = {-INFINITY, -INFINITY};
 #pragma unroll
           for (int n = 0; n < kN; ++n) {
-            const float2 ks = *reinterpret_cast<const float2*>(scales + key0 + 8 * n + 2 * t);
-            const float2 vs = *reinterpret_cast<const float2*>(scales + S::kKeys + key0 + 8 * n + 2 * t);
+            const float2 ks = two(scales + key0, n);
+            const float2 vs = two(scales + S::kKeys + key0, n);
             const float lv[2] = {fmaxf(lg2_approx(fabsf(vs.x)), kScaleLogMin), fmaxf(lg2_approx(fabsf(vs.y)), kScaleLogMin)};
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-              y[n][x] *= (x & 1) ? ks.y : ks.x;
+              y[n][x] *= key_half(x) ? ks.y : ks.x;
               // A key that a row does not see may hold anything.
               if (hidden.value && ((unseen >> (4 * n + x)) & 1u)) y[n][x] = -INFINITY;
-              float z = fmaf(y[n][x], factor[x / 2], lv[x & 1]);
+              float z = fmaf(y[n][x], factor[row_half(x)], lv[key_half(x)]);
               if (hidden.value && ((unseen >> (4 * n + x)) & 1u)) z = -INFINITY;
-              most[x / 2] = fmaxf(most[x / 2], z);
+              most[row_half(x)] = fmaxf(most[row_half(x)], z);
             }
           }
           if (__any_sync(0xffffffffu, most[0] - unit[0] > kSlack || most[1] - unit[1] > kSlack)) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 1));
-              most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 2));
-              if (most[h] > unit[h]) {
-                const float shrink = ex2_approx(unit[h] - most[h]);
-                unit[h] = most[h];
-                l[h] *= shrink;
+              most[h] = of_row(most[h], [](float u, float v) { return fmaxf(u, v); });
+              // (The numerators' columns are rows as the scores' are.)
+              const float shrink = most[h] > unit[h] ? ex2_approx(unit[h] - most[h]) : 1.0f;
+              unit[h] = fmaxf(unit[h], most[h]);
+              l[h] *= shrink;
 #pragma unroll
-                for (int c = 0; c < 2 * kChunks; ++c) {
-                  o[c][2 * h] *= shrink;
-                  o[c][2 * h + 1] *= shrink;
-                }
-              }
+              for (auto& c : o)
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                  if (row_half(x) == h) c[x] *= shrink;
             }
           }
 #pragma unroll
           for (int n = 0; n < kN; ++n) {
-            const float2 vs = *reinterpret_cast<const float2*>(scales + S::kKeys + key0 + 8 * n + 2 * t);
+            const float2 vs = two(scales + S::kKeys + key0, n);
+            float p[4];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float p[2];
+            for (int x = 0; x < 4; ++x) {
+              const int h = row_half(x);
+              p[x] = ex2_approx(fmaf(y[n][x], factor[h], -unit[h]));
+              l[h] += p[x];
+              p[x] *= key_half(x) ? vs.y : vs.x;
+              if (hidden.value && ((unseen >> (4 * n + x)) & 1u)) p[x] = 0.0f;
+            }
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                p[e] = ex2_approx(fmaf(y[n][2 * h + e], factor[h], -unit[h]));
-                l[h] += p[e];
-                p[e] *= e ? vs.y : vs.x;
-                if (hidden.value && ((unseen >> (4 * n + 2 * h + e)) & 1u)) p[e] = 0.0f;
-              }
-              w[n / 2][2 * (n & 1) + h] = pack2(p[0], p[1], __half());
+            for (int z = 0; z < 2; ++z) {
+              const uint32_t pair = pack2(p[2 * z], p[2 * z + 1], __half());
+              if constexpr (kEight)
+                w[n][z] = transpose8(pair);
+              else
+                w[n / 2][2 * (n & 1) + z] = pair;
             }
           }
         };
@@ -551,8 +603,14 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS>::kThreads, TreeTile
             for (int x = 0; x < 4; ++x) v[x] ^= 0x80808080u;
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              mma16816(o[2 * (c + x)], w[i], codes_f16<0x4240>(v[2 * x]), codes_f16<0x4240>(v[2 * x + 1]));
-              mma16816(o[2 * (c + x) + 1], w[i], codes_f16<0x4341>(v[2 * x]), codes_f16<0x4341>(v[2 * x + 1]));
+              if constexpr (kEight) {
+                const uint32_t values[4] = {codes_f16<0x4240>(v[2 * x]), codes_f16<0x4341>(v[2 * x]),
+                                            codes_f16<0x4240>(v[2 * x + 1]), codes_f16<0x4341>(v[2 * x + 1])};
+                mma16816(o[c + x], values, w[i][0], w[i][1]);
+              } else {
+                mma16816(o[2 * (c + x)], w[i], codes_f16<0x4240>(v[2 * x]), codes_f16<0x4240>(v[2 * x + 1]));
+                mma16816(o[2 * (c + x) + 1], w[i], codes_f16<0x4341>(v[2 * x]), codes_f16<0x4341>(v[2 * x + 1]));
+              }
             }
           }
         }
@@ -565,15 +623,14 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS>::kThreads, TreeTile
       }
     }
     // ---- join the warps' parts: each row's reference and total, then the
-    // numerators, 32 head dimensions at a time.
+    // numerators, kJoinColumns head dimensions at a time.
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+      l[h] = of_row(l[h], [](float u, float v) { return u + v; });
       if (unit[h] == kNoReference) unit[h] = -INFINITY;
-      if (t == 0) {
-        state[warp * 16 + g + 8 * h] = unit[h];
-        state[(WARPS + warp) * 16 + g + 8 * h] = l[h];
+      if ((kEight ? g : t) == 0) {
+        state[warp * ROWS + row_at(h)] = unit[h];
+        state[(WARPS + warp) * ROWS + row_at(h)] = l[h];
       }
     }
     bar_sync(1, WARPS * 32);
@@ -581,11 +638,11 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS>::kThreads, TreeTile
     auto joined = [&](int r, float* total) {
       float top = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) top = fmaxf(top, state[w * 16 + r]);
+      for (int w = 0; w < WARPS; ++w) top = fmaxf(top, state[w * ROWS + r]);
       const float ref = top == -INFINITY ? 0.0f : top;
       *total = 0.0f;
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) *total += state[(WARPS + w) * 16 + r] * ex2_approx(state[w * 16 + r] - ref);
+      for (int w = 0; w < WARPS; ++w) *total += state[(WARPS + w) * ROWS + r] * ex2_approx(state[w * ROWS + r] - ref);
       return top;
     };
     float share[2];
@@ -593,34 +650,41 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS>::kThreads, TreeTile
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float total;
-      const float top = joined(g + 8 * h, &total);
+      const float top = joined(row_at(h), &total);
       share[h] = ex2_approx(unit[h] - (top == -INFINITY ? 0.0f : top));
-      if (!all && warp == 0 && t == 0) {
-        to[16 * D + 2 * (g + 8 * h)] = top;
-        to[16 * D + 2 * (g + 8 * h) + 1] = total;
+      if (!all && warp == 0 && (kEight ? g : t) == 0) {
+        to[ROWS * D + 2 * row_at(h)] = top;
+        to[ROWS * D + 2 * row_at(h) + 1] = total;
       }
     }
 #pragma unroll
-    for (int d0 = 0; d0 < D; d0 += 32) {
-      float* mine = join + warp * 16 * S::kJoinStride;
+    for (int d0 = 0; d0 < D; d0 += S::kJoinColumns) {
+      float* mine = join + warp * ROWS * S::kJoinStride;
 #pragma unroll
-      for (int c = 0; c < 2; ++c)
+      for (int c = 0; c < S::kJoinColumns / 16; ++c)
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float(&even)[4] = o[2 * (d0 / 16 + c)];
-          const float(&odd)[4] = o[2 * (d0 / 16 + c) + 1];
           const float f = share[h];
-          *reinterpret_cast<float4*>(mine + (g + 8 * h) * S::kJoinStride + c * 16 + 4 * t) =
-              make_float4(even[2 * h] * f, odd[2 * h] * f, even[2 * h + 1] * f, odd[2 * h + 1] * f);
+          float* row = mine + row_at(h) * S::kJoinStride + c * 16;
+          if constexpr (kEight) {
+            const float(&both)[4] = o[d0 / 16 + c];
+            *reinterpret_cast<float2*>(row + 2 * g) = make_float2(both[h] * f, both[2 + h] * f);
+          } else {
+            const float(&even)[4] = o[2 * (d0 / 16 + c)];
+            const float(&odd)[4] = o[2 * (d0 / 16 + c) + 1];
+            *reinterpret_cast<float4*>(row + 4 * t) =
+                make_float4(even[2 * h] * f, odd[2 * h] * f, even[2 * h + 1] * f, odd[2 * h + 1] * f);
+          }
         }
       bar_sync(1, WARPS * 32);
-      // 16 rows x 32 columns, four columns a thread.
+      // Four columns a thread.
       for (int x = tid; x < 128; x += WARPS * 32) {
-        const int r = x / 8, d = (x % 8) * 4;
+        constexpr int kFours = S::kJoinColumns / 4;
+        const int r = x / kFours, d = (x % kFours) * 4;
         float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
-          const float4 y = *reinterpret_cast<const float4*>(join + (w * 16 + r) * S::kJoinStride + d);
+          const float4 y = *reinterpret_cast<const float4*>(join + (w * ROWS + r) * S::kJoinStride + d);
           sum.x += y.x;
           sum.y += y.y;
           sum.z += y.z;
