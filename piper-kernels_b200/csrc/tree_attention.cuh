@@ -43,7 +43,7 @@
 // Measured (32 query over 8 KV heads of 128, pages of 64, one token each): 64
 // requests of 1 to 8192 tokens 94 us, 5.9 TB/s or 0.92 of the copy rate; one
 // request of 256 tokens 7.6 us.  24 heads of 64, 5 nodes, 32 requests of 333 to
-// 4097 tokens in pages of 16: 65 us, 0.55 of the copy rate.  With 16 rows
+// 4097 tokens in pages of 16: 58 us, 0.63 of the copy rate.  With 16 rows
 // instructions bound it, 320 of some 660 for 32 keys a warp turning codes into
 // fp16: 16 keys a warp took 131 us for 110.
 #pragma once
@@ -237,6 +237,14 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ void cp_async16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+// This thread's arrival, once its earlier cp_async16 have landed.
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+
 // An 8 x 8 matrix of 16-bit elements, a row's pair to each lane, transposed.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
@@ -346,7 +354,7 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS, ROWS>::kThreads, Tr
   const uint32_t abort_flag = smem_u32(&abort_word);
   if (tid == 0) {
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(smem_u32(&full_bar[s]), 1);
+      mbar_init(smem_u32(&full_bar[s]), 1 + 32);  // the codes' bytes, and each lane's scales
       mbar_init(smem_u32(&empty_bar[s]), WARPS);
     }
     abort_word = 0u;
@@ -361,7 +369,10 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS, ROWS>::kThreads, Tr
   const int boxes = S::kKeys >> box_shift;
 
   if (warp == WARPS) {
-    // ---- fetching warp: lane i brings box i of each tile.
+    // ---- fetching warp: lane i brings box i of each tile's codes and four rows'
+    // scales (a copy of a box's scales each, with pages of 16, made the copies so
+    // many that they bound it: 65 us instead of 58).
+    static_assert(S::kKeys == 32 * 4, "a lane brings four rows' scales");
     int stage = 0, issued = 0;
     uint32_t phase = 1;  // a fresh barrier's previous phase counts as done
     bool ok = true;
@@ -388,19 +399,24 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS, ROWS>::kThreads, Tr
         const uint32_t bar = smem_u32(&full_bar[stage]);
         if (lane == 0) {
           valid[stage] = goods;
-          mbar_arrive_expect_tx(bar, __popc(goods) * box * (2 * D + 8));
+          mbar_arrive_expect_tx(bar, __popc(goods) * box * 2 * D);
         }
         __syncwarp();
+        const uint32_t base = smem_u32(smem + stage * S::kStageAlloc);
+        const int z = page * a.c.kv_heads + head;
+        const int y = static_cast<int>(position & (a.c.page_size - 1));
         if (good) {
-          const int z = page * a.c.kv_heads + head;
-          const int y = static_cast<int>(position & (a.c.page_size - 1));
-          const uint32_t base = smem_u32(smem + stage * S::kStageAlloc);
-          const int64_t at = (static_cast<int64_t>(z) << a.page_shift) + y;
           tma_load_3d(base + lane * box * D, &key_map, bar, 0, y, z);
-          bulk_load(base + 2 * S::kCodes + lane * box * 4, a.c.key_scales + at, box * 4, bar);
           tma_load_3d(base + S::kCodes + lane * box * D, &value_map, bar, 0, y, z);
-          bulk_load(base + 2 * S::kCodes + S::kScales + lane * box * 4, a.c.value_scales + at, box * 4, bar);
         }
+        const int from = (4 * lane) >> box_shift;  // the box of this lane's four rows
+        const int64_t at = (static_cast<int64_t>(__shfl_sync(0xffffffffu, z, from)) << a.page_shift) +
+                           __shfl_sync(0xffffffffu, y, from) + (4 * lane & (box - 1));
+        if ((goods >> from) & 1u) {
+          cp_async16(base + 2 * S::kCodes + lane * 16, a.c.key_scales + at);
+          cp_async16(base + 2 * S::kCodes + S::kScales + lane * 16, a.c.value_scales + at);
+        }
+        cp_async_arrive(bar);
         ++issued;
         if (++stage == kStages) {
           stage = 0;
