@@ -126,12 +126,18 @@ TreePlan tree_plan(int64_t batch, int64_t kv_heads, int64_t rows, int64_t positi
   return p;
 }
 
-// The kernel for a number of query rows of a KV head: up to 8 and up to 16 one
-// mma tile on four warps, whose n or m they are, up to 128 a tcgen05 tile whose streams take alternate keys,
-// more a pair of them over the same keys.
-enum class TreeKind { kEight, kSixteen, kAlternate, kPair };
+// The kernel for a number of query rows of a KV head: up to kMoreRows an mma
+// tile of 8, 16 or that many rows on four warps, up to 128 a tcgen05 tile whose
+// streams take alternate keys, more a pair of them over the same keys.  Both
+// sides of the limits, 32 requests of 1000 to 8191 tokens, 8 KV heads of 128 (of
+// 64): 8 and 16 rows 58 and 69 us (39 and 47); 24 rows on the mma tile 108, on the
+// tcgen05 tile 160 (32 rows 93 and 143), which is as long for 32 rows (64: 174).
+enum class TreeKind { kEight, kSixteen, kMore, kAlternate, kPair };
+template <int D>
+constexpr int kMoreRows = D == 64 ? 32 : 24;
+template <int D>
 TreeKind tree_kind(int64_t rows) {
-  if (rows <= 16) return rows <= 8 ? TreeKind::kEight : TreeKind::kSixteen;
+  if (rows <= kMoreRows<D>) return rows <= 8 ? TreeKind::kEight : rows <= 16 ? TreeKind::kSixteen : TreeKind::kMore;
   return rows <= 128 ? TreeKind::kAlternate : TreeKind::kPair;
 }
 constexpr int kFewGroups = 2;
@@ -140,9 +146,10 @@ using FewRows = piper::TreeTile<D, 4, kFewGroups, ROWS>;
 
 template <int D>
 TreePlan tree_plan(int64_t batch, int64_t kv_heads, int64_t rows, int64_t positions, int sms) {
-  switch (tree_kind(rows)) {
+  switch (tree_kind<D>(rows)) {
     case TreeKind::kEight: return tree_plan<FewRows<D, 8>>(batch, kv_heads, rows, positions, sms);
     case TreeKind::kSixteen: return tree_plan<FewRows<D, 16>>(batch, kv_heads, rows, positions, sms);
+    case TreeKind::kMore: return tree_plan<FewRows<D, kMoreRows<D>>>(batch, kv_heads, rows, positions, sms);
     case TreeKind::kAlternate: return tree_plan<piper::WideTile<D, false>>(batch, kv_heads, rows, positions, sms);
     default: return tree_plan<piper::WideTile<D, true>>(batch, kv_heads, rows, positions, sms);
   }
@@ -170,6 +177,7 @@ int set_up_instances() {
   int rc = set_up_few<T, D, 8>();
   if (rc != PIPER_B200_OK) return rc;
   if ((rc = set_up_few<T, D, 16>()) != PIPER_B200_OK) return rc;
+  if ((rc = set_up_few<T, D, kMoreRows<D>>()) != PIPER_B200_OK) return rc;
   if ((rc = set_up_wide<T, D, false>()) != PIPER_B200_OK) return rc;
   return set_up_wide<T, D, true>();
 }
@@ -222,13 +230,16 @@ int launch_tree(piper::TreeArgs a, Kernel kernel, int threads, int sms, size_t w
 
 template <typename T, int D>
 int launch_tree_rows(const piper::TreeArgs& a, int sms, size_t workspace_bytes, cudaStream_t stream) {
-  switch (tree_kind(a.rows)) {
+  switch (tree_kind<D>(a.rows)) {
     case TreeKind::kEight:
       return launch_tree<T, D, FewRows<D, 8>>(a, piper::tree_attention_kernel<T, D, 4, kFewGroups, 8>,
                                               FewRows<D, 8>::kThreads, sms, workspace_bytes, stream);
     case TreeKind::kSixteen:
       return launch_tree<T, D, FewRows<D, 16>>(a, piper::tree_attention_kernel<T, D, 4, kFewGroups, 16>,
                                                FewRows<D, 16>::kThreads, sms, workspace_bytes, stream);
+    case TreeKind::kMore:
+      return launch_tree<T, D, FewRows<D, kMoreRows<D>>>(a, piper::tree_attention_kernel<T, D, 4, kFewGroups, kMoreRows<D>>,
+                                               FewRows<D, kMoreRows<D>>::kThreads, sms, workspace_bytes, stream);
     case TreeKind::kAlternate:
       return launch_tree<T, D, piper::WideTile<D, false>>(a, piper::tree_wide_kernel<T, D, false>,
                                                           piper::kWideThreads, sms, workspace_bytes, stream);

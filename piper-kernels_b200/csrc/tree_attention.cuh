@@ -11,7 +11,9 @@
 // S^T = K Q^T and head dimensions that of O^T = V^T P^T, and the weights are
 // transposed in registers between the two.  9 to 16 rows are the m, S = Q K^T
 // and O = P V: for 8 rows that was half empty (110 against 94 us in the first
-// case measured below).
+// case measured below).  Up to 24 (heads of 64: 32) rows are several blocks of
+// 8 that share each converted fragment, as many as the numerators fit in
+// registers.
 //
 // Products: fp16 tensor-core MMAs (m16n8k16, fp32 accumulators).  Codes are
 // exact in fp16.  fp16 queries are used as they are; a bf16 row is scaled by
@@ -45,7 +47,9 @@
 // request of 256 tokens 7.6 us.  24 heads of 64, 5 nodes, 32 requests of 333 to
 // 4097 tokens in pages of 16: 58 us, 0.63 of the copy rate.  With 16 rows
 // instructions bound it, 320 of some 660 for 32 keys a warp turning codes into
-// fp16: 16 keys a warp took 131 us for 110.
+// fp16: 16 keys a warp took 131 us for 110.  32 requests of 1000 to 8191 tokens,
+// 8 KV heads of 128: 8 rows 58 us, 16 rows 69, 24 rows 108; of 64: 39, 47, 32 rows
+// 93.
 #pragma once
 
 #include <math.h>
@@ -77,7 +81,7 @@ struct TreeArgs {
   float scale_log2e;
 };
 
-// Tile of up to ROWS (8 or 16) rows: a warp takes 16 * GROUPS keys of it.
+// Tile of up to ROWS rows (16, or blocks of 8 that are the products' n): a warp takes 16 * GROUPS keys of it.
 template <int D, int WARPS, int GROUPS, int ROWS>
 struct TreeTile {
   static constexpr int kRows = ROWS;
@@ -87,15 +91,19 @@ struct TreeTile {
   static constexpr int kScales = kKeys * 4;
   static constexpr int kStage = 2 * kCodes + 2 * kScales;
   static constexpr int kStageAlloc = (kStage + 1023) / 1024 * 1024;
-  static constexpr int kJoinColumns = 512 / ROWS;
-  static constexpr int kJoinStride = kJoinColumns + 16;  // floats; 16 banks between rows
+  static constexpr bool kThin = ROWS != 16;
+  static constexpr int kBlocks = kThin ? ROWS / 8 : 1;
+  static constexpr int kJoinColumns = ROWS <= 16 ? 512 / ROWS : 16;
+  static constexpr int kJoinStride = kJoinColumns + (ROWS <= 16 ? 16 : 4);  // floats; spreads rows over banks
   static constexpr int kJoin = WARPS * ROWS * kJoinStride * 4;
   static constexpr int kState = 2 * WARPS * kRows * 4;
-  static constexpr int kQuery = ROWS == 16 ? (D / 16) * 32 * 16 : 0;  // fragments
+  static constexpr bool kHeld = ROWS == 8;  // query fragments in registers
+  static constexpr int kQuery = kHeld ? 0 : (D / 16) * 32 * ROWS;
   static constexpr int kFixed = kJoin + kState + kQuery + kRows * 8 + 512;
   // Per SM, what registers and stages allow (8 rows: of 128, three spilled
-  // and took 115 us instead of 94; of 64, three took 73 us instead of 68, five 82).
-  static constexpr int kCtas = D == 64 ? (ROWS == 8 ? 4 : 3) : 2;
+  // and took 115 us instead of 94; of 64, three took 73 us instead of 68, five
+  // 82; 16 rows of 64: four 81 us instead of 69).
+  static constexpr int kCtas = D == 64 ? (ROWS == 8 ? 4 : ROWS == 16 ? 3 : 2) : 2;
   static constexpr int kLead = ROWS == 8 ? 3 : 4;  // a segment's start and end, in key tiles
   static constexpr int kFit = (227 * 1024 / kCtas - 1024 * 2 - kFixed) / kStageAlloc;
   static constexpr int kStages = kFit > 8 ? 8 : kFit;
@@ -337,8 +345,10 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS, ROWS>::kThreads, Tr
     tree_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map,
                           TreeArgs a) {
   using S = TreeTile<D, WARPS, GROUPS, ROWS>;
-  constexpr bool kEight = ROWS == 8;
-  constexpr int kN = kEight ? GROUPS : 2 * GROUPS;  // score fragments of a warp
+  constexpr bool kThin = S::kThin, kHeld = S::kHeld;
+  constexpr int kBlocks = S::kBlocks;
+  constexpr int kSlots = 2 * kBlocks;  // rows of a thread
+  constexpr int kN = kThin ? GROUPS * kBlocks : 2 * GROUPS;  // score fragments of a warp
   constexpr int kStages = S::kStages;
   constexpr int kChunks = D / 16;
   extern __shared__ uint8_t smem_raw[];
@@ -372,7 +382,7 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS, ROWS>::kThreads, Tr
     // ---- fetching warp: lane i brings box i of each tile's codes and four rows'
     // scales (a copy of a box's scales each, with pages of 16, made the copies so
     // many that they bound it: 65 us instead of 58).
-    static_assert(S::kKeys == 32 * 4, "a lane brings four rows' scales");
+    static_assert(S::kKeys == 32 * 4 && S::kBlocks <= WARPS, "a lane brings four rows' scales");
     int stage = 0, issued = 0;
     uint32_t phase = 1;  // a fresh barrier's previous phase counts as done
     bool ok = true;
@@ -435,16 +445,16 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS, ROWS>::kThreads, Tr
 
   // ---- computing warps: some keys of each tile, all rows.
   const int g = lane / 4, t = lane % 4;
-  // Element x of score fragment n is row row_at(h), h = row_half(x), and key
+  // Element x of score fragment n is row row_at(h), h = row_slot(n, x), and key
   // key_at(n, e), e = key_half(x), of the warp's.
-  auto row_half = [](int x) { return kEight ? (x & 1) : x / 2; };
-  auto key_half = [](int x) { return kEight ? x / 2 : (x & 1); };
-  auto row_at = [&](int h) { return kEight ? 2 * t + h : g + 8 * h; };
-  auto key_at = [&](int n, int e) { return kEight ? 16 * n + g + 8 * e : 8 * n + 2 * t + e; };
+  auto row_slot = [](int n, int x) { return kThin ? 2 * (n % kBlocks) + (x & 1) : x / 2; };
+  auto key_half = [](int x) { return kThin ? x / 2 : (x & 1); };
+  auto row_at = [&](int h) { return kThin ? 8 * (h / 2) + 2 * t + (h & 1) : g + 8 * h; };
+  auto key_at = [&](int n, int e) { return kThin ? 16 * (n / kBlocks) + g + 8 * e : 8 * n + 2 * t + e; };
   // Over the lanes that hold the same rows.
   auto of_row = [&](float x, auto join2) {
 #pragma unroll
-    for (int o = kEight ? 4 : 1; o < (kEight ? 32 : 4); o <<= 1) x = join2(x, __shfl_xor_sync(0xffffffffu, x, o));
+    for (int o = kThin ? 4 : 1; o < (kThin ? 32 : 4); o <<= 1) x = join2(x, __shfl_xor_sync(0xffffffffu, x, o));
     return x;
   };
   int stage = 0;
@@ -457,13 +467,25 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS, ROWS>::kThreads, Tr
     const int row0 = (run.hr % a.row_tiles) * S::kRows;
     const bool all = run.all;
     const int64_t length = max(0, __ldg(a.c.lengths + b));
-    float factor[2];
-    uint32_t held[kEight ? kChunks : 1][2];
-    if constexpr (kEight) {
-      float mine[1];
-      query_fragments<T, D, 1>(a, b, kv, row0, held, mine);
+    float factor[kSlots];
+    uint32_t held[kHeld ? kChunks : 1][2];
+    uint2* query_pairs = reinterpret_cast<uint2*>(query);
+    if constexpr (kThin) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) factor[h] = __shfl_sync(0xffffffffu, mine[0], 4 * row_at(h));
+      for (int k = 0; k < kBlocks; ++k) {
+        uint32_t q[kChunks][2];
+        float mine[1];
+        query_fragments<T, D, 1>(a, b, kv, row0 + 8 * k, q, mine);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) factor[2 * k + h] = __shfl_sync(0xffffffffu, mine[0], 4 * row_at(h));
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+          if constexpr (kHeld)
+            held[c][0] = q[c][0], held[c][1] = q[c][1];
+          else if (warp == k)
+            query_pairs[(c * kBlocks + k) * 32 + lane] = make_uint2(q[c][0], q[c][1]);
+        }
+      }
     } else {
       // Every warp has the rows' factors; warp 0's fragments serve all (holding
       // them cost each thread 32 registers, and the SM a CTA).
@@ -487,8 +509,10 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS, ROWS>::kThreads, Tr
       words[tid] = word;
     }
     bar_sync(1, WARPS * 32);
-    float o[kEight ? kChunks : 2 * kChunks][4] = {};
-    float unit[2] = {kNoReference, kNoReference}, l[2] = {0.0f, 0.0f};
+    float o[kThin ? kChunks * kBlocks : 2 * kChunks][4] = {};
+    float unit[kSlots], l[kSlots];
+#pragma unroll
+    for (int h = 0; h < kSlots; ++h) unit[h] = kNoReference, l[h] = 0.0f;
     for (int tile = run.tile; tile < run.tile + run.count; ++tile) {
       if (ok) ok = mbar_wait_block_warp(smem_u32(&full_bar[stage]), phase, a.wait_budget_ns, a.status, kStatusTimeoutFull,
                                   abort_flag);
@@ -506,7 +530,7 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS, ROWS>::kThreads, Tr
           uint4 f[2];
 #pragma unroll
           for (int x = 0; x < 2; ++x)
-            if constexpr (!kEight) f[x] = query[(c + x) * 32 + lane];
+            if constexpr (!kThin) f[x] = query[(c + x) * 32 + lane];
 #pragma unroll
           for (int i = 0; i < GROUPS; ++i) {
             uint32_t k[4];
@@ -515,10 +539,18 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS, ROWS>::kThreads, Tr
             for (int x = 0; x < 4; ++x) k[x] ^= 0x80808080u;
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              if constexpr (kEight) {
+              if constexpr (kThin) {
                 const uint32_t keys[4] = {codes_f16<0x4140>(k[2 * x]), codes_f16<0x4140>(k[2 * x + 1]),
                                           codes_f16<0x4342>(k[2 * x]), codes_f16<0x4342>(k[2 * x + 1])};
-                mma16816(y[i], keys, held[c + x][0], held[c + x][1]);
+#pragma unroll
+                for (int n = 0; n < kBlocks; ++n) {
+                  uint2 q;
+                  if constexpr (kHeld)
+                    q = make_uint2(held[c + x][0], held[c + x][1]);
+                  else
+                    q = query_pairs[((c + x) * kBlocks + n) * 32 + lane];
+                  mma16816(y[i * kBlocks + n], keys, q.x, q.y);
+                }
               } else {
                 const uint32_t q[4] = {f[x].x, f[x].y, f[x].z, f[x].w};
 #pragma unroll
@@ -528,9 +560,9 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS, ROWS>::kThreads, Tr
             }
           }
         }
-        uint32_t w[GROUPS][kEight ? 2 : 4];
+        uint32_t w[GROUPS][kThin ? kSlots : 4];
         auto two = [&](const float* p, int n) {
-          if constexpr (kEight) return make_float2(p[key_at(n, 0)], p[key_at(n, 1)]);
+          if constexpr (kThin) return make_float2(p[key_at(n, 0)], p[key_at(n, 1)]);
           return *reinterpret_cast<const float2*>(p + key_at(n, 0));
         };
         // A masked tile has a body of its own: selections would lengthen the
@@ -546,12 +578,15 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS, ROWS>::kThreads, Tr
                 const int64_t j = first + key - length;
                 const bool there = (goods >> (key >> box_shift)) & 1u;
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-                  if (!(there && (j < 0 || (j < a.nodes && ((words[row_at(h)] >> (j & 63)) & 1u)))))
-                    unseen |= 1u << (4 * n + (kEight ? 2 * e + h : 2 * h + e));
+                for (int x = 0; x < 4; ++x)
+                  if (key_half(x) == e &&
+                      !(there && (j < 0 || (j < a.nodes && ((words[row_at(row_slot(n, x))] >> (j & 63)) & 1u)))))
+                    unseen |= 1u << (4 * n + x);
               }
           }
-          float most[2] = {-INFINITY, -INFINITY};
+          float most[kSlots];
+#pragma unroll
+          for (int h = 0; h < kSlots; ++h) most[h] = -INFINITY;
 #pragma unroll
           for (int n = 0; n < kN; ++n) {
             const float2 ks = two(scales + key0, n);
@@ -562,24 +597,27 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS, ROWS>::kThreads, Tr
               y[n][x] *= key_half(x) ? ks.y : ks.x;
               // A key that a row does not see may hold anything.
               if (hidden.value && ((unseen >> (4 * n + x)) & 1u)) y[n][x] = -INFINITY;
-              float z = fmaf(y[n][x], factor[row_half(x)], lv[key_half(x)]);
+              float z = fmaf(y[n][x], factor[row_slot(n, x)], lv[key_half(x)]);
               if (hidden.value && ((unseen >> (4 * n + x)) & 1u)) z = -INFINITY;
-              most[row_half(x)] = fmaxf(most[row_half(x)], z);
+              most[row_slot(n, x)] = fmaxf(most[row_slot(n, x)], z);
             }
           }
-          if (__any_sync(0xffffffffu, most[0] - unit[0] > kSlack || most[1] - unit[1] > kSlack)) {
+          bool above = false;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
+          for (int h = 0; h < kSlots; ++h) above |= most[h] - unit[h] > kSlack;
+          if (__any_sync(0xffffffffu, above)) {
+#pragma unroll
+            for (int h = 0; h < kSlots; ++h) {
               most[h] = of_row(most[h], [](float u, float v) { return fmaxf(u, v); });
               // (The numerators' columns are rows as the scores' are.)
               const float shrink = most[h] > unit[h] ? ex2_approx(unit[h] - most[h]) : 1.0f;
               unit[h] = fmaxf(unit[h], most[h]);
               l[h] *= shrink;
 #pragma unroll
-              for (auto& c : o)
+              for (int c = 0; c < static_cast<int>(sizeof(o) / sizeof(o[0])); ++c)
 #pragma unroll
                 for (int x = 0; x < 4; ++x)
-                  if (row_half(x) == h) c[x] *= shrink;
+                  if (row_slot(c, x) == h) o[c][x] *= shrink;
             }
           }
 #pragma unroll
@@ -588,7 +626,7 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS, ROWS>::kThreads, Tr
             float p[4];
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-              const int h = row_half(x);
+              const int h = row_slot(n, x);
               p[x] = ex2_approx(fmaf(y[n][x], factor[h], -unit[h]));
               l[h] += p[x];
               p[x] *= key_half(x) ? vs.y : vs.x;
@@ -597,8 +635,8 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS, ROWS>::kThreads, Tr
 #pragma unroll
             for (int z = 0; z < 2; ++z) {
               const uint32_t pair = pack2(p[2 * z], p[2 * z + 1], __half());
-              if constexpr (kEight)
-                w[n][z] = transpose8(pair);
+              if constexpr (kThin)
+                w[n / kBlocks][2 * (n % kBlocks) + z] = transpose8(pair);
               else
                 w[n / 2][2 * (n & 1) + z] = pair;
             }
@@ -619,10 +657,12 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS, ROWS>::kThreads, Tr
             for (int x = 0; x < 4; ++x) v[x] ^= 0x80808080u;
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              if constexpr (kEight) {
+              if constexpr (kThin) {
                 const uint32_t values[4] = {codes_f16<0x4240>(v[2 * x]), codes_f16<0x4341>(v[2 * x]),
                                             codes_f16<0x4240>(v[2 * x + 1]), codes_f16<0x4341>(v[2 * x + 1])};
-                mma16816(o[c + x], values, w[i][0], w[i][1]);
+#pragma unroll
+                for (int n = 0; n < kBlocks; ++n)
+                  mma16816(o[(c + x) * kBlocks + n], values, w[i][2 * n], w[i][2 * n + 1]);
               } else {
                 mma16816(o[2 * (c + x)], w[i], codes_f16<0x4240>(v[2 * x]), codes_f16<0x4240>(v[2 * x + 1]));
                 mma16816(o[2 * (c + x) + 1], w[i], codes_f16<0x4341>(v[2 * x]), codes_f16<0x4341>(v[2 * x + 1]));
@@ -641,10 +681,10 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS, ROWS>::kThreads, Tr
     // ---- join the warps' parts: each row's reference and total, then the
     // numerators, kJoinColumns head dimensions at a time.
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < kSlots; ++h) {
       l[h] = of_row(l[h], [](float u, float v) { return u + v; });
       if (unit[h] == kNoReference) unit[h] = -INFINITY;
-      if ((kEight ? g : t) == 0) {
+      if ((kThin ? g : t) == 0) {
         state[warp * ROWS + row_at(h)] = unit[h];
         state[(WARPS + warp) * ROWS + row_at(h)] = l[h];
       }
@@ -661,14 +701,14 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS, ROWS>::kThreads, Tr
       for (int w = 0; w < WARPS; ++w) *total += state[(WARPS + w) * ROWS + r] * ex2_approx(state[w * ROWS + r] - ref);
       return top;
     };
-    float share[2];
+    float share[kSlots];
     float* to = a.parts + (static_cast<int64_t>(blockIdx.x) * 2 + part) * S::kPart;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+    for (int h = 0; h < kSlots; ++h) {
       float total;
       const float top = joined(row_at(h), &total);
       share[h] = ex2_approx(unit[h] - (top == -INFINITY ? 0.0f : top));
-      if (!all && warp == 0 && (kEight ? g : t) == 0) {
+      if (!all && warp == 0 && (kThin ? g : t) == 0) {
         to[ROWS * D + 2 * row_at(h)] = top;
         to[ROWS * D + 2 * row_at(h) + 1] = total;
       }
@@ -679,12 +719,12 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS, ROWS>::kThreads, Tr
 #pragma unroll
       for (int c = 0; c < S::kJoinColumns / 16; ++c)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < kSlots; ++h) {
           const float f = share[h];
           float* row = mine + row_at(h) * S::kJoinStride + c * 16;
-          if constexpr (kEight) {
-            const float(&both)[4] = o[d0 / 16 + c];
-            *reinterpret_cast<float2*>(row + 2 * g) = make_float2(both[h] * f, both[2 + h] * f);
+          if constexpr (kThin) {
+            const float(&both)[4] = o[(d0 / 16 + c) * kBlocks + h / 2];
+            *reinterpret_cast<float2*>(row + 2 * g) = make_float2(both[h & 1] * f, both[2 + (h & 1)] * f);
           } else {
             const float(&even)[4] = o[2 * (d0 / 16 + c)];
             const float(&odd)[4] = o[2 * (d0 / 16 + c) + 1];
@@ -694,7 +734,7 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS, ROWS>::kThreads, Tr
         }
       bar_sync(1, WARPS * 32);
       // Four columns a thread.
-      for (int x = tid; x < 128; x += WARPS * 32) {
+      for (int x = tid; x < ROWS * S::kJoinColumns / 4; x += WARPS * 32) {
         constexpr int kFours = S::kJoinColumns / 4;
         const int r = x / kFours, d = (x % kFours) * 4;
         float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);

@@ -246,6 +246,28 @@ def test_attention_over_a_long_ragged_batch(nodes) -> None:
             dtype=torch.bfloat16)
 
 
+@pytest.mark.parametrize(("group", "nodes"), [
+    (8, 1), (3, 3), (4, 4), (1, 17), (8, 3), (5, 5), (4, 8), (11, 3), (1, 31),
+])
+@pytest.mark.parametrize(("d", "page", "lengths", "mask"), [
+    (64, 16, [2900, 0, 1, 70, 1500], "random"), (128, 32, [2900, 0, 1, 70, 1500], "tree"),
+    (64, 64, [5, 200], None), (128, 64, [0, 333], "random"),
+])
+def test_attention_of_few_rows_on_both_sides_of_each_tile(group, nodes, d, page, lengths, mask) -> None:
+    dev = require_b200()
+    g = torch.Generator().manual_seed(group * 100 + nodes + d)
+    _attend(g, dev, d=d, page=page, kv_heads=2, group=group, nodes=nodes, lengths=lengths, dtype=torch.bfloat16,
+            mask=mask)
+
+
+def test_attention_of_24_rows_with_sharp_scores() -> None:
+    dev = require_b200()
+    g = torch.Generator().manual_seed(4)
+    for d in (64, 128):
+        _attend(g, dev, d=d, page=64, kv_heads=1, group=6, nodes=4, lengths=[900, 3], dtype=torch.float16, scale=0.9,
+                gain=4.0)
+
+
 def test_attention_of_sharp_scores_and_explicit_scale() -> None:
     dev = require_b200()
     g = torch.Generator().manual_seed(3)
