@@ -7,14 +7,16 @@
 // calls the C ABI on the current stream.  It returns
 //   the outputs   when the call was made,
 //   a status      (int) when the C ABI refused or failed, and
-//   None          when an argument is not what the operator takes: the Python
-//                 layer then says what is wrong.
+//   None          when an argument is not what the operator takes, or the call
+//                 is being traced: the Python layer then says what is wrong, or
+//                 calls the registered operator.
 // Nothing else is decided here, so that the Python path stays the whole
 // contract.
 #include <ATen/core/TensorBody.h>
 #include <ATen/core/grad_mode.h>
 #include <ATen/ops/empty.h>
 #include <Python.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -28,10 +30,31 @@ namespace {
 
 using at::Tensor;
 
-// Argument i as a tensor; nullptr when it is none.
-const Tensor* tensor_at(PyObject* const* args, Py_ssize_t i) {
-  return THPVariable_Check(args[i]) ? &THPVariable_Unpack(args[i]) : nullptr;
+// What stands between a call and its kernels: modes and transforms that record
+// or replace operators, and tensors whose memory is not their value.  Such calls
+// belong to torch's dispatcher, which knows the operators by their registered names.
+constexpr c10::DispatchKeySet kIntercepts({
+    c10::DispatchKey::Python, c10::DispatchKey::PythonTLSSnapshot, c10::DispatchKey::PythonDispatcher,
+    c10::DispatchKey::PreDispatch, c10::DispatchKey::Fake, c10::DispatchKey::Functionalize,
+    c10::DispatchKey::FuncTorchDynamicLayerFrontMode, c10::DispatchKey::FuncTorchDynamicLayerBackMode,
+    c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchVmapMode, c10::DispatchKey::Batched,
+    c10::DispatchKey::VmapMode, c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Tracer,
+    c10::DispatchKey::DeferredInit, c10::DispatchKey::Conjugate, c10::DispatchKey::Negative,
+    c10::DispatchKey::ZeroTensor,
+});
+
+bool intercepted() {
+  const c10::impl::LocalDispatchKeySet keys = c10::impl::tls_local_dispatch_key_set();
+  return (keys.included_ - keys.excluded_).has_any(kIntercepts);
 }
+
+// A tensor that is nothing but one; nullptr for anything else, subclasses among it.
+const Tensor* tensor_of(PyObject* x) {
+  if (!THPVariable_CheckExact(x)) return nullptr;
+  const Tensor& t = THPVariable_Unpack(x);
+  return t.key_set().has_any(kIntercepts) ? nullptr : &t;
+}
+const Tensor* tensor_at(PyObject* const* args, Py_ssize_t i) { return tensor_of(args[i]); }
 
 bool fits(const Tensor* t, std::initializer_list<int64_t> sizes, at::ScalarType type, c10::Device device) {
   if (t == nullptr || t->layout() != at::kStrided || t->dim() != static_cast<int64_t>(sizes.size()) ||
@@ -60,8 +83,7 @@ struct Cache {
     for (int i = 0; i < 5; ++i) {
       PyObject* item = PyTuple_GET_ITEM(buffers, i);
       if (i == 4 && item == Py_None) break;
-      if (!THPVariable_Check(item)) return false;
-      t[i] = &THPVariable_Unpack(item);
+      if ((t[i] = tensor_of(item)) == nullptr) return false;
     }
     device = t[0]->device();
     if (!device.is_cuda() || t[0]->dim() != 4 || batch <= 0 || table == nullptr || table->dim() != 2 ||
@@ -91,10 +113,9 @@ struct Cache {
 bool take_counts(PyObject* arg, int64_t batch, c10::Device device, const int32_t** out) {
   *out = nullptr;
   if (arg == Py_None) return true;
-  if (!THPVariable_Check(arg)) return false;
-  const Tensor& t = THPVariable_Unpack(arg);
-  if (!fits(&t, {batch}, at::kInt, device)) return false;
-  *out = static_cast<const int32_t*>(t.data_ptr());
+  const Tensor* t = tensor_of(arg);
+  if (!fits(t, {batch}, at::kInt, device)) return false;
+  *out = static_cast<const int32_t*>(t->data_ptr());
   return true;
 }
 
@@ -114,7 +135,7 @@ PyObject* guarded(Body body) {
 // attend(buffers, query, table, lengths, mask or None, scale or None)
 PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    if (n != 6) return none();
+    if (n != 6 || intercepted()) return none();
     const Tensor* q = tensor_at(args, 1);
     if (q == nullptr || q->dim() != 4 || !half_type(q->scalar_type()) || wants_grad(*q)) return none();
     const int64_t batch = q->size(0), heads = q->size(1), nodes = q->size(2);
@@ -163,7 +184,7 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
 // write(buffers, key, value, table, lengths, counts or None): True
 PyObject* write(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    if (n != 6) return none();
+    if (n != 6 || intercepted()) return none();
     const Tensor *k = tensor_at(args, 1), *v = tensor_at(args, 2);
     if (k == nullptr || v == nullptr || k->dim() != 4 || !half_type(k->scalar_type()) || wants_grad(*k) ||
         wants_grad(*v))
@@ -189,7 +210,7 @@ PyObject* write(PyObject*, PyObject* const* args, Py_ssize_t n) {
 // read(buffers, table, lengths, counts or None, tokens, half precision?): (key, value)
 PyObject* read(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    if (n != 6 || !PyLong_Check(args[4])) return none();
+    if (n != 6 || intercepted() || !PyLong_Check(args[4])) return none();
     const Tensor* lengths = tensor_at(args, 2);
     const int64_t tokens = PyLong_AsLongLong(args[4]);
     if (PyErr_Occurred()) {
@@ -222,7 +243,7 @@ PyObject* read(PyObject*, PyObject* const* args, Py_ssize_t n) {
 // keep(buffers, table, lengths, path, counts): True
 PyObject* keep(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    if (n != 5) return none();
+    if (n != 5 || intercepted()) return none();
     const Tensor* path = tensor_at(args, 3);
     if (path == nullptr || path->dim() != 2 || args[4] == Py_None) return none();
     const int64_t batch = path->size(0), nodes = path->size(1);
@@ -242,7 +263,7 @@ PyObject* keep(PyObject*, PyObject* const* args, Py_ssize_t n) {
 // verify(target, draft, tokens, parents, uniform, noise): (path, count, next)
 PyObject* verify(PyObject*, PyObject* const* args, Py_ssize_t n) {
   return guarded([&]() -> PyObject* {
-    if (n != 6) return none();
+    if (n != 6 || intercepted()) return none();
     const Tensor* t[6];
     for (int i = 0; i < 6; ++i)
       if ((t[i] = tensor_at(args, i)) == nullptr) return none();

@@ -246,8 +246,8 @@ def binding():
     """Load (once) and return the extension module that calls the decoding entry points on torch tensors.
 
     Its functions check their arguments natively and return the outputs, a
-    status for :func:`check`, or None for arguments that the operator does not
-    take (csrc/decoding_binding.cpp).
+    status for :func:`check`, or None for calls that are traced and arguments
+    that the operator does not take (csrc/decoding_binding.cpp).
     """
     global _binding
     if _binding is None:

@@ -24,8 +24,9 @@ _binding = None
 def direct(name: str, what: str, *args):
     """Outputs of the native binding's function, or None: the call goes on through the checks.
 
-    That is so under ``torch.compile``, and for arguments that the operator
-    does not take.
+    That is so under ``torch.compile`` and other modes that trace or transform
+    operators, for tensor subclasses (both then reach the registered operator),
+    and for arguments that the operator does not take.
     """
     global _binding
     if torch.compiler.is_compiling():

@@ -73,12 +73,10 @@ def tree_attention(
     if not math.isfinite(effective) or effective <= 0:
         raise ValueError(f"{OPERATOR} scale must be finite and positive, got {scale}")
     require_device(OPERATOR, device)
-    if torch.compiler.is_compiling():
-        return torch.ops.piper_kernels.tree_attention(
-            query, cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales, block_table, lengths,
-            tree_mask, effective,
-        )
-    return _run(query, cache, block_table, lengths, tree_mask, effective)
+    return torch.ops.piper_kernels.tree_attention(
+        query, cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales, block_table, lengths,
+        tree_mask, effective,
+    )
 
 
 def workspace_bytes(batch: int, heads: int, kv_heads: int, nodes: int, head_dim: int, positions: int) -> int:

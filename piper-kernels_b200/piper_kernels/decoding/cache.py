@@ -229,13 +229,10 @@ def write_kv_cache(
     if (key.requires_grad or value.requires_grad) and torch.is_grad_enabled():
         refuse_grad(operator)
     require_device(operator, cache.device)
-    if torch.compiler.is_compiling():
-        torch.ops.piper_kernels.write_kv_cache(
-            cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales, cache.key_mean, key, value,
-            block_table, lengths, counts,
-        )
-    else:
-        _write(cache, key, value, block_table, lengths, counts)
+    torch.ops.piper_kernels.write_kv_cache(
+        cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales, cache.key_mean, key, value,
+        block_table, lengths, counts,
+    )
 
 
 def _write(cache, key, value, block_table, lengths, counts) -> None:
@@ -280,12 +277,10 @@ def read_kv_cache(
     if counts is not None and not fits(counts, (lengths.shape[0],), torch.int32, cache.device):
         check_tensor(operator, "counts", counts, (lengths.shape[0],), torch.int32, cache.device)
     require_device(operator, cache.device)
-    if torch.compiler.is_compiling():
-        return torch.ops.piper_kernels.read_kv_cache(
-            cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales, cache.key_mean, block_table,
-            lengths, counts, tokens, dtype,
-        )
-    return _read(cache, block_table, lengths, counts, tokens, dtype)
+    return torch.ops.piper_kernels.read_kv_cache(
+        cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales, cache.key_mean, block_table,
+        lengths, counts, tokens, dtype,
+    )
 
 
 def _read(cache, block_table, lengths, counts, tokens, dtype) -> tuple[torch.Tensor, torch.Tensor]:
@@ -329,13 +324,9 @@ def keep_draft_path(
         check_tensor(operator, "path", path, (batch, nodes), torch.int32, device)
         check_tensor(operator, "counts", counts, (batch,), torch.int32, device)
     require_device(operator, cache.device)
-    if torch.compiler.is_compiling():
-        torch.ops.piper_kernels.keep_draft_path(
-            cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales, block_table, lengths, path,
-            counts,
-        )
-    else:
-        _keep(cache, block_table, lengths, path, counts)
+    torch.ops.piper_kernels.keep_draft_path(
+        cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales, block_table, lengths, path, counts
+    )
 
 
 def _keep(cache, block_table, lengths, path, counts) -> None:

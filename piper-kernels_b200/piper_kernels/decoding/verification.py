@@ -89,11 +89,9 @@ def verify_draft_tree(
     if (target_probs.requires_grad or draft_probs.requires_grad) and torch.is_grad_enabled():
         refuse_grad(OPERATOR)
     require_device(OPERATOR, device)
-    if torch.compiler.is_compiling():
-        return DraftVerification(
-            *torch.ops.piper_kernels.verify_draft_tree(target_probs, draft_probs, tokens, parents, uniform, noise)
-        )
-    return DraftVerification(*_run(target_probs, draft_probs, tokens, parents, uniform, noise))
+    return DraftVerification(
+        *torch.ops.piper_kernels.verify_draft_tree(target_probs, draft_probs, tokens, parents, uniform, noise)
+    )
 
 
 def _run(target, draft, tokens, parents, uniform, noise) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:

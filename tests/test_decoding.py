@@ -228,3 +228,38 @@ def test_missing_binding_fails_loudly(monkeypatch: pytest.MonkeyPatch, tmp_path)
     monkeypatch.setattr(_native, "BINDING_PATH", tmp_path / "absent.so")
     with pytest.raises(_native.NativeLibraryMissing, match="build"):
         _native.binding()
+
+
+def _operators_of(graph_module) -> list[str]:
+    return [str(n.target) for n in graph_module.graph.nodes if str(n.target).startswith("piper_kernels.")]
+
+
+def test_traced_calls_record_the_registered_operators(monkeypatch: pytest.MonkeyPatch) -> None:
+    # (Fake tensors need no GPU; only the device's check would ask for one.)
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    from piper_kernels.decoding import attention, cache, verification
+
+    for module in (attention, cache, verification):
+        monkeypatch.setattr(module, "require_device", lambda *_: None)
+
+    def step(c, x, table, lengths, probs, tokens, parents, path, uniform, noise):
+        pk.write_kv_cache(c, x, x, table, lengths)
+        out = pk.tree_attention(x, c, table, lengths) + 1
+        found = pk.verify_draft_tree(probs, probs, tokens, parents, uniform, noise)
+        pk.keep_draft_path(c, table, lengths, path, lengths)
+        return out, *found, *pk.read_kv_cache(c, table, lengths, 2)
+
+    with FakeTensorMode():
+        kw = dict(device="cuda")
+        handle = pk.QuantizedKVCache.allocate(3, 2, 16, 64, device="cuda")
+        ints = torch.zeros((2, 3), dtype=torch.int32, **kw)
+        args = (torch.zeros((2, 2, 3, 64), dtype=torch.float16, **kw), ints, ints[:, 0].contiguous(),
+                torch.zeros((2, 3, 5), **kw), torch.zeros((2, 3), dtype=torch.int64, **kw), ints, ints,
+                torch.zeros((2, 3), **kw), torch.zeros((2, 5), **kw))
+        shapes = [tuple(x.shape) for x in step(handle, *args)]
+        traced = make_fx(lambda *a: step(handle, *a))(*args)
+    assert shapes == [(2, 2, 3, 64), (2, 3), (2,), (2,), (2, 2, 2, 64), (2, 2, 2, 64)]
+    assert [name.split(".")[1] for name in _operators_of(traced)] == [
+        "write_kv_cache", "tree_attention", "verify_draft_tree", "keep_draft_path", "read_kv_cache"]

@@ -643,3 +643,25 @@ def test_calls_on_two_streams_at_once_do_not_share_anything() -> None:
     torch.cuda.synchronize()
     for i, out in enumerate(outs):
         assert torch.equal(out, expected[i % len(queries)])
+
+
+def test_a_step_traced_from_real_tensors_computes_what_it_records() -> None:
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    dev = require_b200()
+    step = _step(dev, torch.Generator().manual_seed(96))
+    expected = [x.clone() for x in step()]
+    traced = make_fx(lambda: step())()
+    for out in (traced(), traced()):
+        assert all(torch.equal(a, b) for a, b in zip(expected, out))
+
+
+def test_attention_of_a_tensor_whose_memory_is_not_its_value() -> None:
+    # A lazily negated view: the fast path may not read its memory.
+    dev = require_b200()
+    g = torch.Generator().manual_seed(97)
+    cache = _on(_pool(g, 2, 2, 16, 64), dev)
+    table, lengths = torch.tensor([[1, 0]], dtype=torch.int32, device=dev), torch.tensor([20], dtype=torch.int32, device=dev)
+    query = torch.randn((1, 4, 3, 64), generator=g).half().to(dev)
+    assert torch.equal(pk.tree_attention(torch._neg_view(query), cache, table, lengths),
+                       pk.tree_attention(-query, cache, table, lengths))
