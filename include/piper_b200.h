@@ -353,7 +353,8 @@ int piper_b200_kv_cache_keep(const piper_b200_kv_cache_t* cache, const int32_t* 
 
 /* Workspace bytes of piper_b200_tree_attention on the current device for a
  * block table with room for `positions` tokens a request (table_width *
- * page_size); 0 when it needs none. */
+ * page_size); 0 when it needs none.  The sizes are those that the call takes:
+ * heads a multiple of kv_heads, 1 to 64 nodes. */
 int piper_b200_tree_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads,
                                               int64_t nodes, int64_t head_dim, int64_t positions,
                                               size_t* bytes);

@@ -48,6 +48,14 @@ int check_cache(const piper_b200_kv_cache_t* c) {
   return PIPER_B200_OK;
 }
 
+// The sizes of an attention call that do not come from the cache.
+int check_rows(int64_t heads, int64_t kv_heads, int64_t nodes) {
+  if (nodes <= 0 || nodes > piper::kMaxNodes) return invalid("nodes must be in [1, 64], got " + std::to_string(nodes));
+  if (heads <= 0 || heads > 65535 || heads % kv_heads != 0)
+    return invalid("heads must be a multiple of kv_heads, at most 65535");
+  return PIPER_B200_OK;
+}
+
 int check_dtype(int dtype) {
   if (dtype != PIPER_B200_FLOAT16 && dtype != PIPER_B200_BFLOAT16)
     return invalid("dtype must be PIPER_B200_FLOAT16 or PIPER_B200_BFLOAT16");
@@ -341,8 +349,11 @@ extern "C" int piper_b200_kv_cache_keep(const piper_b200_kv_cache_t* cache, cons
 extern "C" int piper_b200_tree_attention_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t nodes,
                                                          int64_t head_dim, int64_t positions, size_t* bytes) {
   if (bytes == nullptr) return invalid("bytes is NULL");
-  if (batch <= 0 || heads <= 0 || kv_heads <= 0 || nodes <= 0 || positions <= 0)
-    return invalid("sizes must be positive");
+  if (batch <= 0 || kv_heads <= 0 || positions <= 0) return invalid("sizes must be positive");
+  if (kv_heads > 65535 || batch > 65535) return invalid("kv_heads and batch must be at most 65535");
+  if (positions > (int64_t(1) << 39)) return invalid("positions must be at most 2^39");  // the widest table, pages of 256
+  const int rc = check_rows(heads, kv_heads, nodes);
+  if (rc != PIPER_B200_OK) return rc;
   if (head_dim != 64 && head_dim != 128)
     return invalid("head_dim must be 64 or 128, got " + std::to_string(head_dim));
   int device = 0, sms = 148;
@@ -365,9 +376,7 @@ extern "C" int piper_b200_tree_attention(const piper_b200_kv_cache_t* cache, con
   if (rc != PIPER_B200_OK) return rc;
   if ((rc = check_dtype(dtype)) != PIPER_B200_OK) return rc;
   if (!query || !query_strides || !out) return invalid("NULL pointer argument");
-  if (nodes <= 0 || nodes > piper::kMaxNodes) return invalid("nodes must be in [1, 64], got " + std::to_string(nodes));
-  if (heads <= 0 || heads > 65535 || heads % cache->kv_heads != 0)
-    return invalid("heads must be a multiple of kv_heads, at most 65535");
+  if ((rc = check_rows(heads, cache->kv_heads, nodes)) != PIPER_B200_OK) return rc;
   if (!(std::isfinite(scale) && scale > 0.0)) return invalid("scale must be finite and positive");
   if (reinterpret_cast<uintptr_t>(out) % 16 != 0) return invalid("output must be 16-byte aligned");
   if (reinterpret_cast<uintptr_t>(cache->key_scales) % 16 != 0 ||

@@ -263,3 +263,31 @@ def test_traced_calls_record_the_registered_operators(monkeypatch: pytest.Monkey
     assert shapes == [(2, 2, 3, 64), (2, 3), (2,), (2,), (2, 2, 2, 64), (2, 2, 2, 64)]
     assert [name.split(".")[1] for name in _operators_of(traced)] == [
         "write_kv_cache", "tree_attention", "verify_draft_tree", "keep_draft_path", "read_kv_cache"]
+
+
+def test_the_workspace_function_refuses_what_the_call_refuses() -> None:
+    # In a process of its own: an integer division by zero would end it.
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    code = """
+import sys
+sys.path.insert(0, sys.argv[1])
+from piper_kernels.decoding.attention import workspace_bytes
+good = dict(batch=1, heads=4, kv_heads=4, nodes=1, head_dim=64, positions=4096)
+assert workspace_bytes(**good) > 0 and workspace_bytes(**(good | dict(positions=64))) == 0
+for match, change in [("multiple", dict(heads=2)), ("multiple", dict(heads=6)), ("multiple", dict(heads=0)),
+                      ("nodes", dict(nodes=65)), ("nodes", dict(nodes=0)), ("positive", dict(kv_heads=0)),
+                      ("positive", dict(positions=-1)), ("65535", dict(batch=1 << 40)), ("2^39", dict(positions=1 << 62)),
+                      ("head_dim", dict(head_dim=96))]:
+    try:
+        workspace_bytes(**(good | change))
+    except ValueError as refused:
+        assert match in str(refused), (change, refused)
+    else:
+        raise AssertionError(change)
+"""
+    package = Path(pk.__file__).resolve().parents[1]
+    done = subprocess.run([sys.executable, "-c", code, str(package)], capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, (done.returncode, done.stderr)
