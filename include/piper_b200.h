@@ -366,7 +366,8 @@ int piper_b200_tree_attention_workspace_bytes(int64_t batch, int64_t heads, int6
  * heads, nodes, head_dim] with element strides (B, H, N), heads a multiple of
  * kv_heads (query head h reads KV head h / (heads / kv_heads)); out is
  * contiguous and of the same type.  tree_mask is int64 [batch, nodes], rows
- * mask_stride elements apart (0: one tree for all). */
+ * mask_stride elements apart (0: one tree for all).  scale is from 2^-126 to
+ * 2^127. */
 int piper_b200_tree_attention(const piper_b200_kv_cache_t* cache, const void* query,
                               const int64_t query_strides[3], void* out, int dtype, int64_t heads,
                               int64_t nodes, const int64_t* tree_mask, int64_t mask_stride,

@@ -6,7 +6,6 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <cmath>
 #include <mutex>
 #include <string>
 
@@ -377,7 +376,8 @@ extern "C" int piper_b200_tree_attention(const piper_b200_kv_cache_t* cache, con
   if ((rc = check_dtype(dtype)) != PIPER_B200_OK) return rc;
   if (!query || !query_strides || !out) return invalid("NULL pointer argument");
   if ((rc = check_rows(heads, cache->kv_heads, nodes)) != PIPER_B200_OK) return rc;
-  if (!(std::isfinite(scale) && scale > 0.0)) return invalid("scale must be finite and positive");
+  // (fp32 holds its product with log2(e) as a normal number.)
+  if (!(scale >= 0x1p-126 && scale <= 0x1p127)) return invalid("scale must be from 2^-126 to 2^127");
   if (reinterpret_cast<uintptr_t>(out) % 16 != 0) return invalid("output must be 16-byte aligned");
   if (reinterpret_cast<uintptr_t>(cache->key_scales) % 16 != 0 ||
       reinterpret_cast<uintptr_t>(cache->value_scales) % 16 != 0)

@@ -162,7 +162,7 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
     } else {
       if (!PyFloat_Check(args[5])) return none();
       scale = PyFloat_AS_DOUBLE(args[5]);
-      if (!(scale > 0.0 && scale <= 1.7976931348623157e308)) return none();
+      if (!(scale >= 0x1p-126 && scale <= 0x1p127)) return none();
     }
     const c10::cuda::OptionalCUDAGuard guard(cache.device);
     size_t bytes = 0;

@@ -627,10 +627,14 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS, ROWS>::kThreads, Tr
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
               const int h = row_slot(n, x);
+              // (An unseen key's value scale may be anything, and -infinity times a
+              // factor that underflowed is no number.)
+              const bool out = hidden.value && ((unseen >> (4 * n + x)) & 1u);
               p[x] = ex2_approx(fmaf(y[n][x], factor[h], -unit[h]));
+              if (out) p[x] = 0.0f;
               l[h] += p[x];
               p[x] *= key_half(x) ? vs.y : vs.x;
-              if (hidden.value && ((unseen >> (4 * n + x)) & 1u)) p[x] = 0.0f;
+              if (out) p[x] = 0.0f;
             }
 #pragma unroll
             for (int z = 0; z < 2; ++z) {

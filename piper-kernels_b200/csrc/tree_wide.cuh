@@ -442,6 +442,10 @@ __global__ void __launch_bounds__(kWideThreads, 1)
                   float2 p = __ffma2_rn(y[n][h], make_float2(factor[h], factor[h]), make_float2(-unit[h], -unit[h]));
                   p.x = ex2_approx(p.x);
                   p.y = ex2_approx(p.y);
+                  if constexpr (hidden.value) {  // (-infinity times a factor that underflowed is no number)
+                    if (!((seen[h] >> (8 * n)) & 1u)) p.x = 0.0f;
+                    if (!((seen[h] >> (8 * n + 1)) & 1u)) p.y = 0.0f;
+                  }
                   sum[h] = __fadd2_rn(sum[h], p);
                   p = mul2(p, vs[n]);
                   uint32_t x16 = pack2(p.x, p.y, __half());

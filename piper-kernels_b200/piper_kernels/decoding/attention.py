@@ -38,7 +38,8 @@ def tree_attention(
     nodes]``, or ``[nodes]`` for one tree for all;
     :func:`~piper_kernels.tree_mask_from_parents`); by default node ``t`` sees
     nodes 0 to ``t``, which for one node is plain decoding.  A node that sees
-    nothing gets zeros.  ``scale`` defaults to ``head_dim ** -0.5``.
+    nothing gets zeros.  ``scale`` defaults to ``head_dim ** -0.5`` (from 2**-126
+    to 2**127).
 
     Returns a contiguous ``[batch, heads, nodes, head_dim]`` of ``query``'s
     type.  Inference only.
@@ -72,6 +73,8 @@ def tree_attention(
     effective = head_dim**-0.5 if scale is None else float(scale)
     if not math.isfinite(effective) or effective <= 0:
         raise ValueError(f"{OPERATOR} scale must be finite and positive, got {scale}")
+    if not 2.0**-126 <= effective <= 2.0**127:
+        raise ValueError(f"{OPERATOR} scale must be from 2**-126 to 2**127, got {scale}")
     require_device(OPERATOR, device)
     return torch.ops.piper_kernels.tree_attention(
         query, cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales, block_table, lengths,

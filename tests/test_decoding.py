@@ -291,3 +291,17 @@ for match, change in [("multiple", dict(heads=2)), ("multiple", dict(heads=6)), 
     package = Path(pk.__file__).resolve().parents[1]
     done = subprocess.run([sys.executable, "-c", code, str(package)], capture_output=True, text=True, timeout=300)
     assert done.returncode == 0, (done.returncode, done.stderr)
+
+
+@pytest.mark.parametrize("scale", [1e-46, 1e-39, 2.4e38, 1e39, 5e-324])
+def test_scales_that_fp32_does_not_hold_are_refused(scale) -> None:
+    table, lengths = _batch()
+    with pytest.raises(ValueError, match="scale"):
+        pk.tree_attention(torch.zeros(2, 4, 3, 64).half(), _cache(), table, lengths, scale=scale)
+    lib = _native.library()
+    cache = _native.KVCache(key_codes=256, key_scales=256, value_codes=256, value_scales=256, key_mean=None,
+                            block_table=256, lengths=256, pages=2, table_stride=1, kv_heads=1, page_size=16,
+                            head_dim=64, batch=1, table_width=1)
+    assert lib.piper_b200_tree_attention(ctypes.byref(cache), 256, _native._STRIDES(1, 1, 1), 256, 0, 1, 1, None, 0,
+                                         scale, None, 0, None) == _native.ERR_INVALID_ARGUMENT
+    assert "scale" in _native.last_error()

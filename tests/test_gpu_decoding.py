@@ -665,3 +665,30 @@ def test_attention_of_a_tensor_whose_memory_is_not_its_value() -> None:
     query = torch.randn((1, 4, 3, 64), generator=g).half().to(dev)
     assert torch.equal(pk.tree_attention(torch._neg_view(query), cache, table, lengths),
                        pk.tree_attention(-query, cache, table, lengths))
+
+
+# Query rows of a KV head (heads, nodes) that take each of the five tiles.
+EACH_TILE = [(4, 1), (4, 4), (6, 4), (8, 5), (4, 47)]
+
+
+@pytest.mark.parametrize(("group", "nodes"), EACH_TILE)
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_of_factors_that_underflow_skips_unseen_keys(group, nodes, d) -> None:
+    # A bf16 row of zeros counts every key it sees alike, whatever the scale; so
+    # does any row at the least scale (its scores are below 2^-90).  The bound is
+    # the oracle's; half of the keys of the last tile are unseen.
+    dev = require_b200()
+    g = torch.Generator().manual_seed(group + nodes + d)
+    cache = _pool(g, 12, 1, 32, d)
+    table = torch.randperm(12, generator=g).view(2, 6).to(torch.int32)
+    lengths = torch.tensor([70, 3], dtype=torch.int32)
+    words = torch.randint(0, 2**62, (2, nodes), generator=g)
+    for dtype, gain, scale in ((torch.bfloat16, 0.0, 1e-9), (torch.bfloat16, 0.0, 2.0**-126),
+                               (torch.float16, 1.0, 2.0**-126), (torch.bfloat16, 2.0**-60, 1e-20)):
+        query = (gain * torch.randn((2, group, nodes, d), generator=g)).to(dtype)
+        out = pk.tree_attention(query.to(dev), _on(cache, dev), table.to(dev), lengths.to(dev),
+                                tree_mask=words.to(dev), scale=scale).cpu().double()
+        expected, bound = oracle.attention(query, cache.key_codes, cache.key_scales, cache.value_codes,
+                                           cache.value_scales, table, lengths, words, scale)
+        allowed = UNIT[dtype] * expected.abs() + (1 + UNIT[dtype]) * bound + TINY[dtype]
+        assert bool(((out - expected).abs() <= allowed).all())
