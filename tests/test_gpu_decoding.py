@@ -692,3 +692,77 @@ def test_attention_of_factors_that_underflow_skips_unseen_keys(group, nodes, d) 
                                            cache.value_scales, table, lengths, words, scale)
         allowed = UNIT[dtype] * expected.abs() + (1 + UNIT[dtype]) * bound + TINY[dtype]
         assert bool(((out - expected).abs() <= allowed).all())
+
+
+def _check_rows(dev, cache, table, lengths, words, query, scale):
+    """Attention against the oracle, within its bound; the output."""
+    dtype = query.dtype
+    out = pk.tree_attention(query.to(dev), _on(cache, dev), table.to(dev), lengths.to(dev),
+                            tree_mask=None if words is None else words.to(dev), scale=scale).cpu()
+    expected, bound = oracle.attention(query, cache.key_codes, cache.key_scales, cache.value_codes,
+                                       cache.value_scales, table, lengths, words, scale)
+    allowed = UNIT[dtype] * expected.abs() + (1 + UNIT[dtype]) * bound + TINY[dtype]
+    off = (out.double() - expected).abs()
+    assert bool((off <= allowed).all()), float((off / allowed).max())
+    return out
+
+
+@pytest.mark.parametrize(("group", "nodes"), EACH_TILE)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("pages", [8, 40])  # one CTA a segment, and runs that are joined
+def test_attention_of_scores_that_rise_along_the_keys(group, nodes, d, pages) -> None:
+    # Scores rise by about a factor of 2 every 5 keys: a row's reference moves
+    # several times within a tile and again in each later one, over weights and
+    # numerators that are not zero.  Rows rise, fall and stay, by their first element.
+    dev = require_b200()
+    g = torch.Generator().manual_seed(1000 * group + nodes + d + pages)
+    cache = _pool(g, 2 * pages, 1, 32, d)
+    table = torch.randperm(2 * pages, generator=g).view(2, pages).to(torch.int32)
+    most = 32 * pages - nodes
+    lengths = torch.tensor([most, most // 2 + 3], dtype=torch.int32)
+    cache.key_codes[..., 0] = 127
+    cache.key_codes[..., 1:] = torch.randint(-3, 4, cache.key_codes[..., 1:].shape, generator=g, dtype=torch.int8)
+    for b in range(2):
+        for column in range(pages):
+            rise = torch.arange(32) + 32 * column
+            # A step down now and then: a tile's largest score is not always its last.
+            cache.key_scales[table[b, column], 0] = (rise - 40 * (rise % 100 > 90)).clamp(min=0) / 127
+    query = torch.randn((2, group, nodes, d), generator=g)
+    query[..., 0] = torch.tensor([1.0, 0.6, -1.0, 0.0, 0.25])[torch.arange(group * nodes).view(group, nodes) % 5]
+    _check_rows(dev, cache, table, lengths, None, query.to(torch.float16), 0.14)
+    _check_rows(dev, cache, table, lengths, None, query.to(torch.bfloat16), 0.14)
+
+
+@pytest.mark.parametrize(("group", "nodes"), EACH_TILE)
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_with_value_scales_of_any_size_on_each_tile(group, nodes, d) -> None:
+    dev = require_b200()
+    g = torch.Generator().manual_seed(2000 * group + nodes + d)
+    cache = _pool(g, 60, 1, 32, d)
+    cache.value_scales.copy_(torch.exp2(torch.randint(-60, 40, cache.value_scales.shape, generator=g).float()))
+    table = torch.randperm(60, generator=g)[:56].view(2, 28).to(torch.int32)
+    lengths = torch.tensor([800, 37], dtype=torch.int32)
+    query = (4 * torch.randn((2, group, nodes, d), generator=g)).to(torch.bfloat16)
+    _check_rows(dev, cache, table, lengths, None, query, 0.3)
+
+
+@pytest.mark.parametrize(("group", "nodes"), EACH_TILE)
+@pytest.mark.parametrize("what", ["key", "value"])
+def test_attention_propagates_non_finite_rows_on_each_tile(group, nodes, what) -> None:
+    # The last node's row is not finite: the rows that see it are not, all others are as without it.
+    dev = require_b200()
+    g = torch.Generator().manual_seed(3000 * group + nodes)
+    cache = _pool(g, 40, 1, 32, 64)
+    table = torch.randperm(40, generator=g)[:38].view(1, 38).to(torch.int32)
+    lengths = torch.tensor([1100], dtype=torch.int32)
+    query = torch.randn((1, group, nodes, 64), generator=g).half()
+    words = torch.randint(0, 2**62, (1, nodes), generator=g) & ~(1 << (nodes - 1))
+    there = _on(cache, dev)
+    page, offset = oracle.find_row(table, 40, 32, 0, 1100 + nodes - 1)
+    getattr(there, what + "_scales")[page, 0, offset] = torch.nan
+    bad = words.clone()
+    bad[:, :: 2] |= 1 << (nodes - 1)
+    args = (query.to(dev), there, table.to(dev), lengths.to(dev))
+    out = pk.tree_attention(*args, tree_mask=bad.to(dev)).cpu()
+    clean = _check_rows(dev, cache, table, lengths, words, query, 0.125)
+    assert not torch.isfinite(out[:, :, ::2]).any() and torch.equal(out[:, :, 1::2], clean[:, :, 1::2])
