@@ -22,8 +22,11 @@
 // follows its largest p_j b_j: the total sums p_j / 2^unit, and the weights
 // w_j = p_j b_j / 2^unit are rounded to fp16 (11 bits, against 8 or 11 of the
 // output).  The reference moves, and the numerators with it, only when a
-// weight would exceed 2^14, so that w neither overflows nor goes subnormal
-// where it counts.  Scores, weights, totals and numerators are fp32.
+// weight would exceed 2^15.9, and then to 2^-10 of the largest: fp16 rounds
+// weights below 2^-14 to steps of 2^-24, which is 2^-34 of the row's largest, so
+// that the many small weights of a long context count beside a large one (a
+// reference at the largest itself lost weights of 2^-25; the room costs nothing
+// here).  Scores, weights, totals and numerators are fp32.
 //
 // Layout: a code of a page is the byte that a lane's fragment wants.  As 16-bit
 // elements, ldmatrix gives lane (g, t) the bytes 4t .. 4t+3 of key g: the
@@ -61,7 +64,8 @@
 
 namespace piper {
 
-constexpr float kSlack = 14.0f;         // log2 by which a weight may exceed 1: fp16 holds 2^15
+constexpr float kSlack = 15.9f;         // log2 of the largest weight: fp16 holds less than 2^16
+constexpr float kRoom = 10.0f;          // and of a row's largest one when its reference has just moved
 constexpr float kScaleLogMin = -90.0f;  // smaller value scales count as 2^-90 in the references
 constexpr float kNoReference = -1e30f;
 
@@ -609,9 +613,10 @@ __global__ void __launch_bounds__(TreeTile<D, WARPS, GROUPS, ROWS>::kThreads, Tr
 #pragma unroll
             for (int h = 0; h < kSlots; ++h) {
               most[h] = of_row(most[h], [](float u, float v) { return fmaxf(u, v); });
+              const float to = most[h] - kRoom;
               // (The numerators' columns are rows as the scores' are.)
-              const float shrink = most[h] > unit[h] ? ex2_approx(unit[h] - most[h]) : 1.0f;
-              unit[h] = fmaxf(unit[h], most[h]);
+              const float shrink = to > unit[h] ? ex2_approx(unit[h] - to) : 1.0f;
+              unit[h] = fmaxf(unit[h], to);
               l[h] *= shrink;
 #pragma unroll
               for (int c = 0; c < static_cast<int>(sizeof(o) / sizeof(o[0])); ++c)

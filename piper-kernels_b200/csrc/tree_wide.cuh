@@ -16,10 +16,11 @@
 // they are alternate key tiles of the same 128 rows, joined at the end.
 //
 // A softmax warp takes its 16 rows' scores 32 columns at a time.  A row has one
-// reference, the unit of its numerators and of its total: 2^unit follows the
-// largest weight times its value scale, trails by a factor of at most 2^14, and
-// moves only when 32 columns could outgrow it; then what is there already, the
-// tile's first weights among it, is scaled down.
+// reference, the unit of its numerators and of its total: 2^unit is 2^6 to 2^15.9
+// times smaller than the row's largest weight times its value scale, so that small
+// weights have room in fp16 (kWideRoom), and moves only when 32 columns could
+// outgrow that; then what is there already, the tile's first weights among it, is
+// scaled down.
 //
 // Warps: 0-7 and 8-15 softmax of streams 0 and 1 (two for each 32 TMEM lanes),
 // 16-17 conversion of K, 18-19 of V, 20 fetches, 21 issues MMAs, 22 owns
@@ -43,6 +44,11 @@ namespace piper {
 // 23 warps at 80 registers: what a softmax warp needs without spilling in its
 // loop (more columns at a time, or a look ahead, spilled and measured slower).
 constexpr int kWideThreads = 736;
+// log2 of a row's largest weight when its reference has just moved (less up to 1).
+// The smallest step of fp16 is then 2^-30 of it or less.  A move holds its stream
+// up, and the less the weights may grow the more there are: 131 us at 6 and below,
+// 133 at 7, 135 at 8, 140 at 10 for the first case measured above.
+constexpr float kWideRoom = 7.0f;
 
 template <int D, bool kShared>
 struct WideTile {
@@ -183,8 +189,8 @@ struct WideMove {
   float2 unit, shrink;
 };
 
-// Moves the references to the largest logarithm of a weight times its value
-// scale in chunk c of a tile (bit 8 n + e of seen0 and seen1: column 8 n + e
+// Moves the references to kWideRoom below the largest logarithm of a weight times
+// its value scale in chunk c of a tile (bit 8 n + e of seen0 and seen1: column 8 n + e
 // after the lane's first is seen), and scales down the tile's weights so far
 // and `numerators` columns at tm_o.  Not inlined: it is rare, and its registers
 // would be the common path's spills.
@@ -216,9 +222,10 @@ __device__ __noinline__ WideMove wide_move(uint32_t tm_s, uint32_t tm_o, uint32_
   for (int h = 0; h < 2; ++h) {
     most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 1));
     most[h] = fmaxf(most[h], __shfl_xor_sync(0xffffffffu, most[h], 2));
-    if (most[h] > units[h]) {
+    const float to = most[h] - kWideRoom;
+    if (to > units[h]) {
       // By whole powers of two: the weights that are in TMEM already stay exact.
-      const float up = units[h] == kNoReference ? most[h] : units[h] + ceilf(most[h] - units[h]);
+      const float up = units[h] == kNoReference ? to : units[h] + ceilf(to - units[h]);
       shrink[h] = ex2_approx(units[h] - up);
       units[h] = up;
     }
@@ -231,7 +238,7 @@ __device__ __noinline__ WideMove wide_move(uint32_t tm_s, uint32_t tm_o, uint32_
     tmem_ld_wait();
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      // In fp32: fp16 has no factor below 2^-24, which a weight of 2^14 outlives.
+      // In fp32: fp16 has no factor below 2^-24, which a weight of 2^15 outlives.
       const float2 z = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
       u[i] = pack2(z.x * shrink[i & 1], z.y * shrink[i & 1], __half());
     }

@@ -7,6 +7,8 @@ beside the rounding of the output.
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 from conftest import require_b200
@@ -766,3 +768,51 @@ def test_attention_propagates_non_finite_rows_on_each_tile(group, nodes, what) -
     out = pk.tree_attention(*args, tree_mask=bad.to(dev)).cpu()
     clean = _check_rows(dev, cache, table, lengths, words, query, 0.125)
     assert not torch.isfinite(out[:, :, ::2]).any() and torch.equal(out[:, :, 1::2], clean[:, :, 1::2])
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize(("group", "nodes"), EACH_TILE)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize(("kv_heads", "length", "bits"), [
+    (300, 8200, 26),  # runs of about a request's keys, so that one reference serves nearly all of them
+    (40, 900, 22),    # one CTA a segment
+])
+def test_attention_keeps_the_tail_of_a_peaked_softmax(kv_heads, length, bits, d, group, nodes, dtype) -> None:
+    # One key has 2^bits times the weight of each other, and zeros for values in
+    # the even channels: these come from the others alone.  A weight may be off
+    # by 2^-11 of itself or, where fp16 holds it as a subnormal, by 2^-25, the
+    # largest one standing at 2^10 (more than 24 or 32 rows: 2^6) or more: 2^-35
+    # of it, all alike at worst, or 2^-31 of it at random (the others' value scales
+    # are), which over N keys is 5 sqrt(N / 3) times that: both are below N 2^-33
+    # here.  A value is below 127.  fp32 sums and exponentials add 2^-16, the scores
+    # (bits * ln 2, in fp32) 2^-17 of a weight.
+    dev = require_b200()
+    g = torch.Generator(device=dev).manual_seed(group + nodes + d)
+    page = 64
+    pages = -(-(length + nodes) // page)
+    shape = (pages, kv_heads, page, d)
+    codes = torch.zeros(shape, dtype=torch.int8, device=dev)
+    values = torch.randint(40, 128, shape, generator=g, dtype=torch.int8, device=dev)
+    value_scales = torch.rand(shape[:3], generator=g, device=dev) * 0.5 + 0.5
+    table = torch.randperm(pages, generator=g, device=dev).view(1, pages).to(torch.int32)
+    at, offset = int(table[0, 70 // page]), 70 % page
+    codes[at, :, offset, 0] = 127
+    values[at, :, offset, ::2] = 0
+    cache = pk.QuantizedKVCache(codes, torch.ones(shape[:3], device=dev), values, value_scales)
+    query = torch.zeros((1, kv_heads * group, nodes, d), dtype=dtype, device=dev)
+    query[..., 0] = 1.0
+    out = pk.tree_attention(query, cache, table, torch.tensor([length], dtype=torch.int32, device=dev),
+                            tree_mask=torch.zeros(nodes, dtype=torch.int64, device=dev),
+                            scale=bits * math.log(2) / 127).double()
+    order = table[0].long()
+    total, sums = 0.0, 0.0
+    for i in range(0, pages, 16):  # (a part at a time: the values in fp64 are large)
+        position = torch.arange(i * page, min(pages, i + 16) * page, device=dev)
+        p = torch.where(position == 70, 1.0, 2.0**-bits) * (position < length).double()
+        v = (values[order[i : i + 16]].double() * value_scales[order[i : i + 16]].double()[..., None])
+        v = v.transpose(0, 1).reshape(kv_heads, -1, d)
+        total, sums = total + p.sum(), sums + torch.einsum("n,hnd->hd", p, v)
+    expected = (sums / total).repeat_interleave(group, 0)[None, :, None]
+    bound = (2.0**-11 + 2.0**-15) * expected.abs() + length * 2.0**-33 * 127
+    assert bool(((out - expected).abs() <= (UNIT[dtype] + bound / expected.abs().clamp(min=1e-30)) * expected.abs()
+                 + TINY[dtype]).all()), float(((out - expected).abs() / expected).max())
