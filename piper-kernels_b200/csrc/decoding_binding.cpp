@@ -72,7 +72,8 @@ int dtype_code(at::ScalarType type) { return type == at::kHalf ? PIPER_B200_FLOA
 bool wants_grad(const Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
 
 // The buffers of a handle (a tuple of four tensors and the key mean or None)
-// with a batch's table and lengths.  The handle checked its own buffers.
+// with a batch's table and lengths.  Buffers can be resized or replaced in place
+// after the handle was made, so that each call looks at all of them.
 struct Cache {
   piper_b200_kv_cache_t c{};
   c10::Device device{c10::kCPU};
@@ -89,6 +90,15 @@ struct Cache {
     if (!device.is_cuda() || t[0]->dim() != 4 || batch <= 0 || table == nullptr || table->dim() != 2 ||
         table->size(1) <= 0 || table->size(1) > INT32_MAX || batch > INT32_MAX)
       return false;
+    const int64_t pages = t[0]->size(0), heads = t[0]->size(1), page = t[0]->size(2), d = t[0]->size(3);
+    if (pages <= 0 || heads <= 0 || heads > INT32_MAX || page <= 0 || page > INT32_MAX || (d != 64 && d != 128))
+      return false;
+    for (int i = 0; i < 4; ++i)
+      if (!(i % 2 == 0 ? fits(t[i], {pages, heads, page, d}, at::kChar, device)
+                       : fits(t[i], {pages, heads, page}, at::kFloat, device)) ||
+          !t[i]->is_contiguous())
+        return false;
+    if (t[4] != nullptr && !(fits(t[4], {heads, d}, at::kFloat, device) && t[4]->is_contiguous())) return false;
     if (!fits(table, {batch, table->size(1)}, at::kInt, device) || !fits(lengths, {batch}, at::kInt, device))
       return false;
     c.key_codes = t[0]->data_ptr();
@@ -98,10 +108,10 @@ struct Cache {
     c.key_mean = t[4] ? static_cast<const float*>(t[4]->data_ptr()) : nullptr;
     c.block_table = static_cast<const int32_t*>(table->data_ptr());
     c.lengths = static_cast<const int32_t*>(lengths->data_ptr());
-    c.pages = t[0]->size(0);
-    c.kv_heads = static_cast<int32_t>(t[0]->size(1));
-    c.page_size = static_cast<int32_t>(t[0]->size(2));
-    c.head_dim = static_cast<int32_t>(t[0]->size(3));
+    c.pages = pages;
+    c.kv_heads = static_cast<int32_t>(heads);
+    c.page_size = static_cast<int32_t>(page);
+    c.head_dim = static_cast<int32_t>(d);
     c.batch = static_cast<int32_t>(batch);
     c.table_width = static_cast<int32_t>(table->size(1));
     c.table_stride = table->stride(0);

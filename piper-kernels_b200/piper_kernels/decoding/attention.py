@@ -49,6 +49,7 @@ def tree_attention(
     )
     if out is not None:
         return out
+    cache.check()
     if query.ndim != 4:
         raise ValueError(
             f"{OPERATOR} query must have shape [batch, heads, sequence, head_dim], got {tuple(query.shape)}"

@@ -49,10 +49,10 @@ class QuantizedKVCache:
     with it.  ``page_size`` is 16, 32, 64, 128 or 256, ``head_dim`` 64 or 128.
     The buffers are read-only attributes (``buffers``: all five), like the
     sizes ``pages``, ``kv_heads``, ``page_size`` and ``head_dim`` and the
-    ``device``.
+    ``device``; every call checks that they still belong together.
     """
 
-    __slots__ = ("buffers", "device", "pages", "kv_heads", "page_size", "head_dim")
+    __slots__ = ("_buffers",)
 
     def __init__(
         self,
@@ -62,6 +62,12 @@ class QuantizedKVCache:
         value_scales: torch.Tensor,
         key_mean: torch.Tensor | None = None,
     ) -> None:
+        self._buffers = (key_codes, key_scales, value_codes, value_scales, key_mean)
+        self.check()
+
+    def check(self) -> None:
+        """Raise ``ValueError`` unless the buffers are what the class says."""
+        key_codes, key_scales, value_codes, value_scales, key_mean = self._buffers
         shape, device = key_codes.shape, key_codes.device
         if not (
             len(shape) == 4
@@ -80,9 +86,6 @@ class QuantizedKVCache:
             and (key_mean is None or fits(key_mean, shape[1::2], torch.float32, device) and key_mean.is_contiguous())
         ):
             _refuse_buffers(key_codes, key_scales, value_codes, value_scales, key_mean)
-        self.buffers = (key_codes, key_scales, value_codes, value_scales, key_mean)
-        self.device = device
-        self.pages, self.kv_heads, self.page_size, self.head_dim = shape
 
     @classmethod
     def allocate(
@@ -108,24 +111,48 @@ class QuantizedKVCache:
         )
 
     @property
+    def buffers(self) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor | None]:
+        return self._buffers
+
+    @property
     def key_codes(self) -> torch.Tensor:
-        return self.buffers[0]
+        return self._buffers[0]
 
     @property
     def key_scales(self) -> torch.Tensor:
-        return self.buffers[1]
+        return self._buffers[1]
 
     @property
     def value_codes(self) -> torch.Tensor:
-        return self.buffers[2]
+        return self._buffers[2]
 
     @property
     def value_scales(self) -> torch.Tensor:
-        return self.buffers[3]
+        return self._buffers[3]
 
     @property
     def key_mean(self) -> torch.Tensor | None:
-        return self.buffers[4]
+        return self._buffers[4]
+
+    @property
+    def device(self) -> torch.device:
+        return self._buffers[0].device
+
+    @property
+    def pages(self) -> int:
+        return self._buffers[0].shape[0]
+
+    @property
+    def kv_heads(self) -> int:
+        return self._buffers[0].shape[1]
+
+    @property
+    def page_size(self) -> int:
+        return self._buffers[0].shape[2]
+
+    @property
+    def head_dim(self) -> int:
+        return self._buffers[0].shape[3]
 
     def native(self, block_table: torch.Tensor, lengths: torch.Tensor) -> _native.KVCache:
         """The C ABI's description of this cache for one batch."""
@@ -212,6 +239,7 @@ def write_kv_cache(
     ) is not None:
         return
     operator = "write_kv_cache"
+    cache.check()
     if key.ndim != 4:
         raise ValueError(f"{operator} key must have shape [batch, heads, sequence, head_dim], got {tuple(key.shape)}")
     batch, _, tokens, _ = key.shape
@@ -266,6 +294,7 @@ def read_kv_cache(
         if out is not None:
             return out
     operator = "read_kv_cache"
+    cache.check()
     if dtype not in DTYPE_CODES:
         check_half(operator, "dtype", dtype)
     tokens = int(tokens)
@@ -313,6 +342,7 @@ def keep_draft_path(
     if direct("keep", "piper_b200_kv_cache_keep", cache.buffers, block_table, lengths, path, counts) is not None:
         return
     operator = "keep_draft_path"
+    cache.check()
     if path.ndim != 2:
         raise ValueError(f"{operator} path must have shape [batch, nodes], got {tuple(path.shape)}")
     batch, nodes = path.shape

@@ -305,3 +305,23 @@ def test_scales_that_fp32_does_not_hold_are_refused(scale) -> None:
     assert lib.piper_b200_tree_attention(ctypes.byref(cache), 256, _native._STRIDES(1, 1, 1), 256, 0, 1, 1, None, 0,
                                          scale, None, 0, None) == _native.ERR_INVALID_ARGUMENT
     assert "scale" in _native.last_error()
+
+
+def test_a_handle_cannot_be_changed_and_notices_changed_buffers() -> None:
+    c = _cache(pages=4)
+    for name, value in (("buffers", c.buffers[:4] + (None,)), ("page_size", 32), ("pages", 9), ("kv_heads", 1),
+                        ("head_dim", 128), ("device", torch.device("cuda"))):
+        with pytest.raises(AttributeError):
+            setattr(c, name, value)
+    table, lengths = _batch()
+    x, ints = torch.zeros(2, 2, 3, 64).half(), torch.zeros((2, 3), dtype=torch.int32)
+    calls = (lambda c: pk.write_kv_cache(c, x, x, table, lengths), lambda c: pk.read_kv_cache(c, table, lengths, 2),
+             lambda c: pk.keep_draft_path(c, table, lengths, ints, lengths),
+             lambda c: pk.tree_attention(x, c, table, lengths))
+    for name, shape in (("value_codes", (2, 2, 16, 64)), ("key_scales", (4, 2, 8)), ("value_scales", (1,)),
+                        ("key_codes", (8, 2, 16, 64))):
+        for call in calls:
+            c = _cache(pages=4)
+            getattr(c, name).resize_(shape)
+            with pytest.raises(ValueError, match="QuantizedKVCache"):
+                call(c)

@@ -816,3 +816,20 @@ def test_attention_keeps_the_tail_of_a_peaked_softmax(kv_heads, length, bits, d,
     bound = (2.0**-11 + 2.0**-15) * expected.abs() + length * 2.0**-33 * 127
     assert bool(((out - expected).abs() <= (UNIT[dtype] + bound / expected.abs().clamp(min=1e-30)) * expected.abs()
                  + TINY[dtype]).all()), float(((out - expected).abs() / expected).max())
+
+
+def test_a_cache_whose_buffers_were_resized_is_refused() -> None:
+    # (Checked on the host, before anything is launched.)
+    dev = require_b200()
+    table = torch.zeros((2, 2), dtype=torch.int32, device=dev)
+    lengths, ints = torch.zeros(2, dtype=torch.int32, device=dev), torch.zeros((2, 3), dtype=torch.int32, device=dev)
+    x = torch.zeros((2, 2, 3, 64), dtype=torch.float16, device=dev)
+    for name, shape in (("value_codes", (2, 2, 16, 64)), ("key_scales", (4, 2, 8)), ("key_mean", (2, 32))):
+        for call in (lambda c: pk.write_kv_cache(c, x, x, table, lengths),
+                     lambda c: pk.read_kv_cache(c, table, lengths, 2),
+                     lambda c: pk.keep_draft_path(c, table, lengths, ints, lengths),
+                     lambda c: pk.tree_attention(x, c, table, lengths)):
+            cache = pk.QuantizedKVCache.allocate(4, 2, 16, 64, device=dev, key_mean=torch.zeros((2, 64), device=dev))
+            getattr(cache, name).resize_(shape)
+            with pytest.raises(ValueError, match="QuantizedKVCache"):
+                call(cache)
