@@ -42,7 +42,8 @@ namespace piper {
 constexpr int kVerifyThreads = 512;
 constexpr int kVerifyUnroll = 4;  // 16-byte loads in flight of each row
 constexpr int kVerifySingle = 8;  // 4-byte ones, where rows are not aligned
-constexpr float kVerifyLeast = 0x1p-126f;  // the least total whose reciprocal is finite
+constexpr float kVerifyLeast = 0x1p-126f;  // the least total whose reciprocal is surely finite
+constexpr float kVerifyUp = 0x1p64f;       // what a smaller one is scaled by
 constexpr float kVerifyTold = 0x1p-64f;    // a quotient far above what fp32 rounds to zero
 
 struct VerifyArgs {
@@ -63,10 +64,12 @@ struct VerifyArgs {
 };
 
 // What is left of probability p after taking out the draft's q n times:
-// max(r - q, 0) over each total, given as reciprocals.
-__device__ __forceinline__ float rest_of(float p, float q, const float* over, int n) {
+// max(r - q, 0) over each total, given as (up, 1 / (total * up)): up is 1, or
+// kVerifyUp where the total is subnormal.  (The second product costs 2 % of the
+// largest case; bodies of their own for such totals cost as much or more.)
+__device__ __forceinline__ float rest_of(float p, float q, const float2* over, int n) {
   float r = p;
-  for (int k = 0; k < n; ++k) r = fmaxf(r - q, 0.0f) * over[k];
+  for (int k = 0; k < n; ++k) r = fmaxf(r - q, 0.0f) * over[k].x * over[k].y;
   return r;
 }
 
@@ -141,7 +144,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(VerifyAr
   constexpr int kWarps = kVerifyThreads / 32;
   __shared__ float node_p[kMaxNodes], node_q[kMaxNodes], node_u[kMaxNodes];
   __shared__ int node_parent[kMaxNodes];  // -1: absent
-  __shared__ float over[kMaxNodes];
+  __shared__ float2 over[kMaxNodes];
   __shared__ float warp_sum[kWarps], joined_sum[2];  // by turn
   __shared__ VerifyBest warp_best[kWarps], joined_best;
   const int64_t b = blockIdx.y;
@@ -221,8 +224,9 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(VerifyAr
       // The other turn's sums are written only after every rank has read these:
       // each passes the next cluster.sync after its reading.
       turn ^= 1;
-      if (total >= kVerifyLeast) {  // else nothing would be left: rest stays as it was
-        if (tid == 0) over[rejected] = 1.0f / total;
+      if (total > 0.0f) {  // else nothing would be left: rest stays as it was
+        const float up = total < kVerifyLeast ? kVerifyUp : 1.0f;
+        if (tid == 0) over[rejected] = make_float2(up, 1.0f / (total * up));
         ++rejected;
       }
       __syncthreads();

@@ -833,3 +833,30 @@ def test_a_cache_whose_buffers_were_resized_is_refused() -> None:
             getattr(cache, name).resize_(shape)
             with pytest.raises(ValueError, match="QuantizedKVCache"):
                 call(cache)
+
+
+@pytest.mark.parametrize("left", [1e-39, 1e-42, 1e-44])
+@pytest.mark.parametrize("children", [1, 2, 3])
+def test_verification_of_a_rest_whose_total_is_subnormal(left, children) -> None:
+    # Two words are all that is left, the sum of both below the least normal fp32
+    # number; the rest is normalised all the same, and the next token is one of them.
+    dev = require_b200()
+    g = torch.Generator().manual_seed(22)
+    batch, vocab, words = 4, 5003, [1234, 4444]
+    nodes = 1 + children
+    draft = torch.softmax(torch.randn((batch, 1, vocab), generator=g), -1).repeat(1, nodes, 1)
+    draft[:, :, words] = 0.0
+    target = draft.clone()
+    tokens = torch.arange(nodes).repeat(batch, 1) + 10
+    target[:, :, 11 : 11 + children] = 0.0
+    target[:, :, words] = torch.tensor([left, 2 * left])
+    parents = torch.zeros((batch, nodes), dtype=torch.int32)
+    parents[:, 0] = -1
+    noise = torch.empty((batch, vocab)).exponential_(generator=g)
+    noise[:, words[0]] = torch.tensor([1.0, 1.0, 0.01, 1.0])
+    noise[:, words[1]] = torch.tensor([1.0, 3.0, 1.0, 1e-20])
+    args = (target, draft, tokens, parents, torch.full((batch, nodes), 0.5), noise)
+    got = pk.verify_draft_tree(*(x.to(dev) for x in args))
+    assert got.next_token.tolist() == [words[1], words[0], words[0], words[1]]
+    for x, y in zip(got, oracle.verify(*args)):
+        assert torch.equal(x.cpu(), y)
