@@ -84,7 +84,7 @@ def tree_attention(
 
 
 def workspace_bytes(batch: int, heads: int, kv_heads: int, nodes: int, head_dim: int, positions: int) -> int:
-    """Workspace of one call whose block table has room for ``positions`` tokens (0: it needs none)."""
+    """Workspace of one call on the current device, whose block table has room for ``positions`` tokens (0: none)."""
     size = ctypes.c_size_t(0)
     _native.check(
         _native.library().piper_b200_tree_attention_workspace_bytes(
@@ -95,7 +95,10 @@ def workspace_bytes(batch: int, heads: int, kv_heads: int, nodes: int, head_dim:
     return int(size.value)
 
 
-_workspace_bytes = lru_cache(maxsize=4096)(workspace_bytes)  # the same few shapes come back every step
+@lru_cache(maxsize=4096)  # the same few shapes come back every step
+def _workspace_bytes(device: int, *sizes: int) -> int:
+    with torch.cuda.device(device):  # (the plan goes by its SMs)
+        return workspace_bytes(*sizes)
 
 
 def _run(query, cache, block_table, lengths, tree_mask, scale) -> torch.Tensor:
@@ -103,7 +106,7 @@ def _run(query, cache, block_table, lengths, tree_mask, scale) -> torch.Tensor:
     device = query.device
     out = torch.empty_like(query, memory_format=torch.contiguous_format)
     nbytes = _workspace_bytes(
-        batch, heads, cache.kv_heads, nodes, head_dim, block_table.shape[1] * cache.page_size
+        device.index, batch, heads, cache.kv_heads, nodes, head_dim, block_table.shape[1] * cache.page_size
     )
     workspace = out.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     mask_ptr, mask_stride = None, 0

@@ -325,3 +325,27 @@ def test_a_handle_cannot_be_changed_and_notices_changed_buffers() -> None:
             getattr(c, name).resize_(shape)
             with pytest.raises(ValueError, match="QuantizedKVCache"):
                 call(c)
+
+
+def test_workspace_sizes_belong_to_a_device(monkeypatch: pytest.MonkeyPatch) -> None:
+    # Two fake devices whose plans differ, as GPUs with other SM counts' do.
+    from piper_kernels.decoding import attention
+
+    class Fake:
+        current = 0
+
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, Fake.current = Fake.current, self.index
+
+        def __exit__(self, *_):
+            Fake.current = self.before
+
+    monkeypatch.setattr(torch.cuda, "device", Fake)
+    monkeypatch.setattr(attention, "workspace_bytes", lambda *sizes: 1000 * Fake.current + len(sizes))
+    attention._workspace_bytes.cache_clear()
+    for _ in range(2):
+        assert [attention._workspace_bytes(i, 1, 2, 1, 1, 64, 4096) for i in (0, 1)] == [6, 1006]
+    attention._workspace_bytes.cache_clear()
