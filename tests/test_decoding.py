@@ -349,3 +349,47 @@ def test_workspace_sizes_belong_to_a_device(monkeypatch: pytest.MonkeyPatch) -> 
     for _ in range(2):
         assert [attention._workspace_bytes(i, 1, 2, 1, 1, 64, 4096) for i in (0, 1)] == [6, 1006]
     attention._workspace_bytes.cache_clear()
+
+
+def test_the_library_is_built_without_torch_and_the_binding_again_with_another(
+    monkeypatch: pytest.MonkeyPatch, tmp_path
+) -> None:
+    # Fake compilers that write their output, and a fake torch.
+    import importlib.util
+    import subprocess
+    from pathlib import Path
+
+    path = Path(pk.__file__).resolve().parents[1] / "build.py"
+    spec = importlib.util.spec_from_file_location("piper_build", path)
+    build = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(build)
+    for name in ("OUTPUT", "BINDING", "BINDING_TORCH"):
+        monkeypatch.setattr(build, name, tmp_path / getattr(build, name).name)
+    made = []
+
+    class Compiler:
+        def __init__(self, args, check=False):
+            self.args, self.returncode = args, 0
+            made.append(Path(args[args.index("-o") + 1]).name)
+            Path(args[args.index("-o") + 1]).write_text("")
+
+        def wait(self):
+            return 0
+
+    monkeypatch.setattr(subprocess, "Popen", Compiler)
+    monkeypatch.setattr(subprocess, "run", Compiler)
+
+    def outputs(**kw):
+        made.clear()
+        build.build(**kw)
+        return {name for name in made if not name.endswith(".o")}
+
+    version = [None]
+    monkeypatch.setattr(build, "torch_version", lambda: version[0])
+    assert outputs() == {"libpiper_b200.so"} and outputs() == set()
+    version[0] = "2.0 True"
+    assert outputs(library_only=True) == set()
+    assert outputs() == {"decoding_binding.so"} and outputs() == set()
+    version[0] = "2.1 True"
+    assert outputs() == {"decoding_binding.so"} and outputs() == set()
+    assert outputs(force=True) == {"libpiper_b200.so", "decoding_binding.so"}
