@@ -78,7 +78,8 @@ struct Cache {
   piper_b200_kv_cache_t c{};
   c10::Device device{c10::kCPU};
 
-  bool take(PyObject* buffers, const Tensor* table, const Tensor* lengths, int64_t batch) {
+  // `mean`: the call's result depends on the key mean.
+  bool take(PyObject* buffers, const Tensor* table, const Tensor* lengths, int64_t batch, bool mean) {
     if (!PyTuple_Check(buffers) || PyTuple_GET_SIZE(buffers) != 5) return false;
     const Tensor* t[5] = {};
     for (int i = 0; i < 5; ++i) {
@@ -99,6 +100,7 @@ struct Cache {
           !t[i]->is_contiguous())
         return false;
     if (t[4] != nullptr && !(fits(t[4], {heads, d}, at::kFloat, device) && t[4]->is_contiguous())) return false;
+    if (wants_grad(*t[1]) || wants_grad(*t[3]) || (mean && t[4] != nullptr && wants_grad(*t[4]))) return false;
     if (!fits(table, {batch, table->size(1)}, at::kInt, device) || !fits(lengths, {batch}, at::kInt, device))
       return false;
     c.key_codes = t[0]->data_ptr();
@@ -151,7 +153,7 @@ PyObject* attend(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int64_t batch = q->size(0), heads = q->size(1), nodes = q->size(2);
     const Tensor *table = tensor_at(args, 2), *lengths = tensor_at(args, 3);
     Cache cache;
-    if (!cache.take(args[0], table, lengths, batch)) return none();
+    if (!cache.take(args[0], table, lengths, batch, false)) return none();
     const int64_t d = cache.c.head_dim;
     if (!fits(q, {batch, heads, nodes, d}, q->scalar_type(), cache.device) || nodes < 1 || nodes > 64 || heads < 1 ||
         heads % cache.c.kv_heads != 0)
@@ -201,7 +203,7 @@ PyObject* write(PyObject*, PyObject* const* args, Py_ssize_t n) {
       return none();
     const int64_t batch = k->size(0), tokens = k->size(2);
     Cache cache;
-    if (!cache.take(args[0], tensor_at(args, 3), tensor_at(args, 4), batch) || tokens < 1) return none();
+    if (!cache.take(args[0], tensor_at(args, 3), tensor_at(args, 4), batch, true) || tokens < 1) return none();
     const std::initializer_list<int64_t> sizes = {batch, cache.c.kv_heads, tokens, cache.c.head_dim};
     const int32_t* counts = nullptr;
     if (!fits(k, sizes, k->scalar_type(), cache.device) || !fits(v, sizes, k->scalar_type(), cache.device) ||
@@ -231,7 +233,7 @@ PyObject* read(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int64_t batch = lengths->size(0);
     Cache cache;
     const int32_t* counts = nullptr;
-    if (!cache.take(args[0], tensor_at(args, 1), lengths, batch) ||
+    if (!cache.take(args[0], tensor_at(args, 1), lengths, batch, true) ||
         !take_counts(args[3], batch, cache.device, &counts))
       return none();
     const at::ScalarType type = args[5] == Py_True ? at::kHalf : at::kBFloat16;
@@ -259,7 +261,7 @@ PyObject* keep(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int64_t batch = path->size(0), nodes = path->size(1);
     Cache cache;
     const int32_t* counts = nullptr;
-    if (nodes < 1 || nodes > 64 || !cache.take(args[0], tensor_at(args, 1), tensor_at(args, 2), batch) ||
+    if (nodes < 1 || nodes > 64 || !cache.take(args[0], tensor_at(args, 1), tensor_at(args, 2), batch, false) ||
         !fits(path, {batch, nodes}, at::kInt, cache.device) || !take_counts(args[4], batch, cache.device, &counts))
       return none();
     const c10::cuda::OptionalCUDAGuard guard(cache.device);

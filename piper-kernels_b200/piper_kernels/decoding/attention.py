@@ -10,7 +10,7 @@ import torch
 
 from .. import _native
 from ._common import DTYPE_CODES, MAX_NODES, check_half, check_tensor, direct, fits, launch, refuse_grad, require_device
-from .cache import QuantizedKVCache, check_batch
+from .cache import QuantizedKVCache, check_batch, check_cache_grad
 
 OPERATOR = "tree_attention"
 
@@ -71,6 +71,7 @@ def tree_attention(
             check_tensor(OPERATOR, "tree_mask", tree_mask, shape, torch.int64, device)
     if query.requires_grad and torch.is_grad_enabled():
         refuse_grad(OPERATOR)
+    check_cache_grad(OPERATOR, cache, mean=False)
     effective = head_dim**-0.5 if scale is None else float(scale)
     if not math.isfinite(effective) or effective <= 0:
         raise ValueError(f"{OPERATOR} scale must be finite and positive, got {scale}")

@@ -214,6 +214,13 @@ def check_batch(
         raise ValueError(f"{operator} block_table must have at least one column")
 
 
+def check_cache_grad(operator: str, cache: QuantizedKVCache, *, mean: bool) -> None:
+    """Refuse a cache whose scales (or key mean, if the call's result depends on it) want a gradient."""
+    tensors = (cache.key_scales, cache.value_scales, cache.key_mean if mean else None)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        refuse_grad(operator)
+
+
 def write_kv_cache(
     cache: QuantizedKVCache,
     key: torch.Tensor,
@@ -256,6 +263,7 @@ def write_kv_cache(
         check_tensor(operator, "counts", counts, (batch,), torch.int32, device)
     if (key.requires_grad or value.requires_grad) and torch.is_grad_enabled():
         refuse_grad(operator)
+    check_cache_grad(operator, cache, mean=True)
     require_device(operator, cache.device)
     torch.ops.piper_kernels.write_kv_cache(
         cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales, cache.key_mean, key, value,
@@ -305,6 +313,7 @@ def read_kv_cache(
     check_batch(operator, cache, lengths.shape[0], block_table, lengths)
     if counts is not None and not fits(counts, (lengths.shape[0],), torch.int32, cache.device):
         check_tensor(operator, "counts", counts, (lengths.shape[0],), torch.int32, cache.device)
+    check_cache_grad(operator, cache, mean=True)
     require_device(operator, cache.device)
     return torch.ops.piper_kernels.read_kv_cache(
         cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales, cache.key_mean, block_table,
@@ -353,6 +362,7 @@ def keep_draft_path(
     if not (fits(path, (batch, nodes), torch.int32, device) and fits(counts, (batch,), torch.int32, device)):
         check_tensor(operator, "path", path, (batch, nodes), torch.int32, device)
         check_tensor(operator, "counts", counts, (batch,), torch.int32, device)
+    check_cache_grad(operator, cache, mean=False)
     require_device(operator, cache.device)
     torch.ops.piper_kernels.keep_draft_path(
         cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales, block_table, lengths, path, counts

@@ -393,3 +393,26 @@ def test_the_library_is_built_without_torch_and_the_binding_again_with_another(
     version[0] = "2.1 True"
     assert outputs() == {"decoding_binding.so"} and outputs() == set()
     assert outputs(force=True) == {"libpiper_b200.so", "decoding_binding.so"}
+
+
+def test_a_cache_that_wants_a_gradient_is_refused_where_it_would_lose_one() -> None:
+    table, lengths = _batch()
+    x, ints = torch.zeros(2, 2, 3, 64).half(), torch.zeros((2, 3), dtype=torch.int32)
+    calls = {
+        "write": lambda c: pk.write_kv_cache(c, x, x, table, lengths),
+        "read": lambda c: pk.read_kv_cache(c, table, lengths, 2),
+        "keep": lambda c: pk.keep_draft_path(c, table, lengths, ints, lengths),
+        "attend": lambda c: pk.tree_attention(x, c, table, lengths),
+    }
+    learned = _cache(key_mean=torch.zeros(2, 64, requires_grad=True))
+    scaled = _cache()
+    scaled.value_scales.requires_grad_()
+    for name, call in calls.items():
+        with pytest.raises(RuntimeError, match="autograd"):
+            call(scaled)
+        # A softmax does not see the mean, and moved rows keep their codes.
+        with pytest.raises(RuntimeError, match="autograd" if name in ("write", "read") else "no CPU"):
+            call(learned)
+        for cache in (scaled, learned):
+            with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU"):
+                call(cache)

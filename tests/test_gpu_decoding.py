@@ -860,3 +860,17 @@ def test_verification_of_a_rest_whose_total_is_subnormal(left, children) -> None
     assert got.next_token.tolist() == [words[1], words[0], words[0], words[1]]
     for x, y in zip(got, oracle.verify(*args)):
         assert torch.equal(x.cpu(), y)
+
+
+def test_a_learned_key_mean_serves_without_gradients_only() -> None:
+    dev = require_b200()
+    mean = torch.zeros((2, 64), device=dev, requires_grad=True)
+    cache = pk.QuantizedKVCache.allocate(2, 2, 16, 64, device=dev, key_mean=mean)
+    table, lengths = torch.tensor([[1]], dtype=torch.int32, device=dev), torch.zeros(1, dtype=torch.int32, device=dev)
+    x = torch.ones((1, 2, 3, 64), dtype=torch.float16, device=dev)
+    for call in (lambda: pk.write_kv_cache(cache, x, x, table, lengths), lambda: pk.read_kv_cache(cache, table, lengths, 2)):
+        with pytest.raises(RuntimeError, match="autograd"):
+            call()
+        with torch.no_grad():
+            call()
+    assert torch.equal(pk.tree_attention(x, cache, table, lengths), x)
