@@ -75,13 +75,13 @@ bool wants_grad(const Tensor& t) { return at::GradMode::is_enabled() && t.requir
 // with a batch's table and lengths.  Buffers can be resized or replaced in place
 // after the handle was made, so that each call looks at all of them.
 struct Cache {
+  const Tensor* t[5] = {};
   piper_b200_kv_cache_t c{};
   c10::Device device{c10::kCPU};
 
   // `mean`: the call's result depends on the key mean.
   bool take(PyObject* buffers, const Tensor* table, const Tensor* lengths, int64_t batch, bool mean) {
     if (!PyTuple_Check(buffers) || PyTuple_GET_SIZE(buffers) != 5) return false;
-    const Tensor* t[5] = {};
     for (int i = 0; i < 5; ++i) {
       PyObject* item = PyTuple_GET_ITEM(buffers, i);
       if (i == 4 && item == Py_None) break;
@@ -118,6 +118,12 @@ struct Cache {
     c.table_width = static_cast<int32_t>(table->size(1));
     c.table_stride = table->stride(0);
     return true;
+  }
+
+  // The rows have been written to: autograd, and whoever else saved a buffer, can tell.
+  void written() const {
+    for (int i = 0; i < 4; ++i)
+      if (!t[i]->is_inference()) t[i]->unsafeGetTensorImpl()->bump_version();
   }
 };
 
@@ -215,6 +221,7 @@ PyObject* write(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int rc = piper_b200_kv_cache_write(&cache.c, k->data_ptr(), ks, v->data_ptr(), vs,
                                              dtype_code(k->scalar_type()), tokens, counts, stream_of(cache.device));
     if (rc != PIPER_B200_OK) return status(rc);
+    cache.written();
     Py_RETURN_TRUE;
   });
 }
@@ -268,6 +275,7 @@ PyObject* keep(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int rc = piper_b200_kv_cache_keep(&cache.c, static_cast<const int32_t*>(path->data_ptr()), path->stride(0),
                                             nodes, counts, stream_of(cache.device));
     if (rc != PIPER_B200_OK) return status(rc);
+    cache.written();
     Py_RETURN_TRUE;
   });
 }

@@ -874,3 +874,32 @@ def test_a_learned_key_mean_serves_without_gradients_only() -> None:
         with torch.no_grad():
             call()
     assert torch.equal(pk.tree_attention(x, cache, table, lengths), x)
+
+
+def test_writes_raise_the_version_of_the_buffers() -> None:
+    dev = require_b200()
+    table, lengths = torch.tensor([[1]], dtype=torch.int32, device=dev), torch.zeros(1, dtype=torch.int32, device=dev)
+    path = torch.zeros((1, 3), dtype=torch.int32, device=dev)
+    x = torch.ones((1, 2, 3, 64), dtype=torch.float16, device=dev)
+    with torch.inference_mode():
+        inside = pk.QuantizedKVCache.allocate(2, 2, 16, 64, device=dev)
+        pk.write_kv_cache(inside, x, x, table, lengths)  # (tensors without versions)
+        pk.keep_draft_path(inside, table, lengths, path, lengths)
+    cache = pk.QuantizedKVCache.allocate(2, 2, 16, 64, device=dev)
+
+    def versions():
+        return [t._version for t in cache.buffers[:4]]
+
+    before = versions()
+    pk.read_kv_cache(cache, table, lengths, 3)
+    pk.tree_attention(x, cache, table, lengths)
+    assert versions() == before
+    pk.write_kv_cache(cache, x, x, table, lengths)
+    pk.keep_draft_path(cache, table, lengths, path, lengths)
+    assert all(now >= was + 2 for now, was in zip(versions(), before))
+    # What autograd saved of a buffer is no longer what it was.
+    weight = torch.ones((), device=dev, requires_grad=True)
+    product = (weight * cache.key_scales).sum()
+    pk.write_kv_cache(cache, 2 * x, x, table, lengths)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        product.backward()
