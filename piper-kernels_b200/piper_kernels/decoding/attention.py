@@ -49,6 +49,22 @@ def tree_attention(
     )
     if out is not None:
         return out
+    effective = _check(query, cache, block_table, lengths, tree_mask, scale)
+    return torch.ops.piper_kernels.tree_attention(
+        query, cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales, block_table, lengths,
+        tree_mask, effective,
+    )
+
+
+def _check(
+    query: torch.Tensor,
+    cache: QuantizedKVCache,
+    block_table: torch.Tensor,
+    lengths: torch.Tensor,
+    tree_mask: torch.Tensor | None,
+    scale: float | None,
+) -> float:
+    """Check a call's arguments; the scale that it uses."""
     cache.check()
     if query.ndim != 4:
         raise ValueError(
@@ -78,10 +94,7 @@ def tree_attention(
     if not 2.0**-126 <= effective <= 2.0**127:
         raise ValueError(f"{OPERATOR} scale must be from 2**-126 to 2**127, got {scale}")
     require_device(OPERATOR, device)
-    return torch.ops.piper_kernels.tree_attention(
-        query, cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales, block_table, lengths,
-        tree_mask, effective,
-    )
+    return effective
 
 
 def workspace_bytes(batch: int, heads: int, kv_heads: int, nodes: int, head_dim: int, positions: int) -> int:
@@ -161,6 +174,7 @@ def _tree_attention_op(
     scale: float,
 ) -> torch.Tensor:
     cache = QuantizedKVCache(key_codes, key_scales, value_codes, value_scales)
+    _check(query, cache, block_table, lengths, tree_mask, scale)
     return _run(query, cache, block_table, lengths, tree_mask, scale)
 
 

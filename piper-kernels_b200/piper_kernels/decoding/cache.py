@@ -245,6 +245,14 @@ def write_kv_cache(
         "write", "piper_b200_kv_cache_write", cache.buffers, key, value, block_table, lengths, counts
     ) is not None:
         return
+    _check_write(cache, key, value, block_table, lengths, counts)
+    torch.ops.piper_kernels.write_kv_cache(
+        cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales, cache.key_mean, key, value,
+        block_table, lengths, counts,
+    )
+
+
+def _check_write(cache, key, value, block_table, lengths, counts) -> None:
     operator = "write_kv_cache"
     cache.check()
     if key.ndim != 4:
@@ -265,10 +273,6 @@ def write_kv_cache(
         refuse_grad(operator)
     check_cache_grad(operator, cache, mean=True)
     require_device(operator, cache.device)
-    torch.ops.piper_kernels.write_kv_cache(
-        cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales, cache.key_mean, key, value,
-        block_table, lengths, counts,
-    )
 
 
 def _write(cache, key, value, block_table, lengths, counts) -> None:
@@ -301,11 +305,19 @@ def read_kv_cache(
         )
         if out is not None:
             return out
+    tokens = int(tokens)
+    _check_read(cache, block_table, lengths, counts, tokens, dtype)
+    return torch.ops.piper_kernels.read_kv_cache(
+        cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales, cache.key_mean, block_table,
+        lengths, counts, tokens, dtype,
+    )
+
+
+def _check_read(cache, block_table, lengths, counts, tokens, dtype) -> None:
     operator = "read_kv_cache"
     cache.check()
     if dtype not in DTYPE_CODES:
         check_half(operator, "dtype", dtype)
-    tokens = int(tokens)
     if tokens <= 0:
         raise ValueError(f"{operator} tokens must be positive, got {tokens}")
     if lengths.ndim != 1:
@@ -315,10 +327,6 @@ def read_kv_cache(
         check_tensor(operator, "counts", counts, (lengths.shape[0],), torch.int32, cache.device)
     check_cache_grad(operator, cache, mean=True)
     require_device(operator, cache.device)
-    return torch.ops.piper_kernels.read_kv_cache(
-        cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales, cache.key_mean, block_table,
-        lengths, counts, tokens, dtype,
-    )
 
 
 def _read(cache, block_table, lengths, counts, tokens, dtype) -> tuple[torch.Tensor, torch.Tensor]:
@@ -350,6 +358,13 @@ def keep_draft_path(
     """
     if direct("keep", "piper_b200_kv_cache_keep", cache.buffers, block_table, lengths, path, counts) is not None:
         return
+    _check_keep(cache, block_table, lengths, path, counts)
+    torch.ops.piper_kernels.keep_draft_path(
+        cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales, block_table, lengths, path, counts
+    )
+
+
+def _check_keep(cache, block_table, lengths, path, counts) -> None:
     operator = "keep_draft_path"
     cache.check()
     if path.ndim != 2:
@@ -364,9 +379,6 @@ def keep_draft_path(
         check_tensor(operator, "counts", counts, (batch,), torch.int32, device)
     check_cache_grad(operator, cache, mean=False)
     require_device(operator, cache.device)
-    torch.ops.piper_kernels.keep_draft_path(
-        cache.key_codes, cache.key_scales, cache.value_codes, cache.value_scales, block_table, lengths, path, counts
-    )
 
 
 def _keep(cache, block_table, lengths, path, counts) -> None:
@@ -394,6 +406,7 @@ def _write_op(
     counts: torch.Tensor | None,
 ) -> None:
     cache = QuantizedKVCache(key_codes, key_scales, value_codes, value_scales, key_mean)
+    _check_write(cache, key, value, block_table, lengths, counts)
     _write(cache, key, value, block_table, lengths, counts)
 
 
@@ -416,6 +429,7 @@ def _read_op(
     dtype: torch.dtype,
 ) -> tuple[torch.Tensor, torch.Tensor]:
     cache = QuantizedKVCache(key_codes, key_scales, value_codes, value_scales, key_mean)
+    _check_read(cache, block_table, lengths, counts, tokens, dtype)
     return _read(cache, block_table, lengths, counts, tokens, dtype)
 
 
@@ -438,7 +452,9 @@ def _keep_op(
     path: torch.Tensor,
     counts: torch.Tensor,
 ) -> None:
-    _keep(QuantizedKVCache(key_codes, key_scales, value_codes, value_scales), block_table, lengths, path, counts)
+    cache = QuantizedKVCache(key_codes, key_scales, value_codes, value_scales)
+    _check_keep(cache, block_table, lengths, path, counts)
+    _keep(cache, block_table, lengths, path, counts)
 
 
 @_keep_op.register_fake

@@ -61,6 +61,13 @@ def verify_draft_tree(
     )
     if found is not None:
         return DraftVerification(*found)
+    _check(target_probs, draft_probs, tokens, parents, uniform, noise)
+    return DraftVerification(
+        *torch.ops.piper_kernels.verify_draft_tree(target_probs, draft_probs, tokens, parents, uniform, noise)
+    )
+
+
+def _check(target_probs, draft_probs, tokens, parents, uniform, noise) -> None:
     if target_probs.ndim != 3:
         raise ValueError(
             f"{OPERATOR} target_probs must have shape [batch, nodes, vocab], got {tuple(target_probs.shape)}"
@@ -89,9 +96,6 @@ def verify_draft_tree(
     if (target_probs.requires_grad or draft_probs.requires_grad) and torch.is_grad_enabled():
         refuse_grad(OPERATOR)
     require_device(OPERATOR, device)
-    return DraftVerification(
-        *torch.ops.piper_kernels.verify_draft_tree(target_probs, draft_probs, tokens, parents, uniform, noise)
-    )
 
 
 def _run(target, draft, tokens, parents, uniform, noise) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
@@ -119,6 +123,7 @@ def _verify_op(
     uniform: torch.Tensor,
     noise: torch.Tensor,
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    _check(target_probs, draft_probs, tokens, parents, uniform, noise)
     return _run(target_probs, draft_probs, tokens, parents, uniform, noise)
 
 

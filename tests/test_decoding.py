@@ -416,3 +416,39 @@ def test_a_cache_that_wants_a_gradient_is_refused_where_it_would_lose_one() -> N
         for cache in (scaled, learned):
             with torch.no_grad(), pytest.raises(RuntimeError, match="no CPU"):
                 call(cache)
+
+
+def test_registered_operators_check_their_arguments() -> None:
+    # (On the CPU: the last check, after all others, is the device's.)
+    ops = torch.ops.piper_kernels
+    buffers, (table, lengths) = _cache().buffers, _batch()
+    x, ints = torch.zeros(2, 2, 3, 64).half(), torch.zeros((2, 3), dtype=torch.int32)
+    wide = table.long()
+
+    def write(b=buffers, k=x, v=x, t=table, n=lengths):
+        return ops.write_kv_cache(*b, k, v, t, n, None)
+
+    def read(t=table, n=lengths, tokens=2, dtype=torch.float16):
+        return ops.read_kv_cache(*buffers, t, n, None, tokens, dtype)
+
+    def keep(t=table, n=lengths, path=ints, counts=lengths):
+        return ops.keep_draft_path(*buffers[:4], t, n, path, counts)
+
+    def attend(q=x, t=table, n=lengths, mask=None, scale=0.1):
+        return ops.tree_attention(q, *buffers[:4], t, n, mask, scale)
+
+    def verify(target=torch.zeros(2, 3, 5), draft=torch.zeros(2, 3, 5), noise=torch.zeros(2, 5)):
+        return ops.verify_draft_tree(target, draft, ints.long(), ints, torch.zeros(2, 3), noise)
+
+    for call, changes in (
+        (write, [dict(t=wide), dict(n=lengths[:1]), dict(k=x[:, :1]), dict(v=x.float()), dict(b=_cache(d=128).buffers)]),
+        (read, [dict(t=wide), dict(t=table[:1]), dict(tokens=0), dict(dtype=torch.float32)]),
+        (keep, [dict(t=wide), dict(path=ints.long()), dict(counts=lengths[:1]), dict(n=lengths.long())]),
+        (attend, [dict(t=wide), dict(n=lengths[:1]), dict(q=x[..., :32]), dict(mask=ints.long()[:, :2]), dict(scale=0.0)]),
+        (verify, [dict(draft=torch.zeros(2, 3, 4)), dict(noise=torch.zeros(2, 4)), dict(target=torch.zeros(2, 3, 5).half())]),
+    ):
+        with pytest.raises(RuntimeError, match="no CPU or generic-GPU fallback"):
+            call()
+        for change in changes:
+            with pytest.raises(ValueError):
+                call(**change)
