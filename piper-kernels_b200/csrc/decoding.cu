@@ -72,7 +72,7 @@ bool rows_aligned16(const void* p, const int64_t s[3]) {
 
 // CTAs for `rows` rows of D/16 lanes each.
 int row_blocks(int64_t rows, int d, unsigned* blocks) {
-  const int64_t per = piper::kCacheThreads / (d / 16) * piper::kCachePasses;
+  const int64_t per = piper::kCacheThreads / (d / 16);
   const int64_t n = (rows + per - 1) / per;
   if (n > 0x7fffffff) return invalid("too many rows for one call");
   *blocks = static_cast<unsigned>(n);

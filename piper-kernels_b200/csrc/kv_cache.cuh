@@ -96,9 +96,9 @@ __device__ __forceinline__ void codes_f32(uint32_t w, float (&x)[8], int at) {
     x[at + i] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7540u + i)) - 8388736.0f;
 }
 
-// (token, head) of the rows that a thread takes: `row0` and every `step`-th
-// after it.  `inner` varies fastest.  Divisions are of 32 bits where the rows'
-// numbers are, and none for rows that stay near the first.
+// (token, head) of the rows that a CTA takes, from row0 on.  `inner` varies
+// fastest.  Divisions are of 32 bits where the rows' numbers are, and none for
+// rows that stay near the first.
 struct CacheRowWalk {
   int64_t outer0;
   unsigned inner0, inner;
@@ -114,75 +114,64 @@ struct CacheRowWalk {
   }
 };
 
-// D/16 consecutive lanes hold a row, sixteen values each: K and V of one
-// (token, head) per lane group, kCachePasses rows a thread with all their
-// loads in flight.  grid (ceil(rows / rows per CTA), batch).  Rows go by blocks
-// of up to 8 tokens, then heads, then tokens: a projection leaves the heads of
+// D/16 consecutive lanes hold K and V of one row (a token of a head), sixteen
+// values of each a lane (four rows' loads in flight a thread took 457 us for the
+// prompts above).  grid (ceil(rows / rows per CTA), batch).  Rows go by
+// blocks of up to 8 tokens, then heads, then tokens: a projection leaves the heads of
 // a token side by side, the cache has the tokens of a head side by side, and
 // such a block is a kilobyte in both.
-constexpr int kCachePasses = 1;
-
 template <typename T, int D, bool kVec16>
 __global__ void __launch_bounds__(kCacheThreads) cache_write_kernel(CacheRowsArgs a) {
   constexpr int kLanes = D / 16;
-  constexpr int kRows = kCacheThreads / kLanes;  // a pass
+  constexpr int kRows = kCacheThreads / kLanes;
   const int b = blockIdx.y;
   const int lane = threadIdx.x % kLanes;
-  const CacheRowWalk walk(static_cast<int64_t>(blockIdx.x) * (kRows * kCachePasses),
+  const CacheRowWalk walk(static_cast<int64_t>(blockIdx.x) * kRows,
                           static_cast<int64_t>(a.c.kv_heads) << a.block_shift);
   int64_t n = a.tokens;
   if (a.counts != nullptr) n = min(n, static_cast<int64_t>(__ldg(a.counts + b)));
   const int64_t length = __ldg(a.c.lengths + b);
-  uint4 raw[kCachePasses][2][2];
-  int64_t token[kCachePasses];
-  unsigned head[kCachePasses];
+  int64_t token;
+  unsigned head;
+  walk.at(threadIdx.x / kLanes, &token, &head);
+  token = (token << a.block_shift) + (head & ((1u << a.block_shift) - 1u));
+  head >>= a.block_shift;
+  uint4 raw[2][2];
 #pragma unroll
-  for (int p = 0; p < kCachePasses; ++p) {
-    walk.at(threadIdx.x / kLanes + p * kRows, &token[p], &head[p]);
-    token[p] = (token[p] << a.block_shift) + (head[p] & ((1u << a.block_shift) - 1u));
-    head[p] >>= a.block_shift;
-#pragma unroll
-    for (int side = 0; side < 2; ++side) {
-      raw[p][side][0] = raw[p][side][1] = make_uint4(0u, 0u, 0u, 0u);
-      if (token[p] < n) {
-        const T* from = static_cast<const T*>(a.in[side]) + b * a.stride[side][0] + head[p] * a.stride[side][1] +
-                        token[p] * a.stride[side][2] + lane * 16;
-        raw[p][side][0] = load_raw8<T, kVec16>(from);
-        raw[p][side][1] = load_raw8<T, kVec16>(from + 8);
-      }
+  for (int side = 0; side < 2; ++side) {
+    raw[side][0] = raw[side][1] = make_uint4(0u, 0u, 0u, 0u);
+    if (token < n) {
+      const T* from = static_cast<const T*>(a.in[side]) + b * a.stride[side][0] + head * a.stride[side][1] +
+                      token * a.stride[side][2] + lane * 16;
+      raw[side][0] = load_raw8<T, kVec16>(from);
+      raw[side][1] = load_raw8<T, kVec16>(from + 8);
     }
   }
-  int64_t at[kCachePasses];
+  const int64_t at = token < n ? cache_row(a.c, a.page_shift, b, head, length + token) : -1;
 #pragma unroll
-  for (int p = 0; p < kCachePasses; ++p)
-    at[p] = token[p] < n ? cache_row(a.c, a.page_shift, b, head[p], length + token[p]) : -1;
+  for (int side = 0; side < 2; ++side) {
+    float x[2][8];
+    float amax = 0.0f;
 #pragma unroll
-  for (int p = 0; p < kCachePasses; ++p) {
+    for (int k = 0; k < 2; ++k) {
+      unpack8<T>(raw[side][k], x[k]);
+      if (side == 0 && a.c.key_mean != nullptr && at >= 0) {
+        float m[8];
+        mean8(a.c.key_mean + head * D + lane * 16 + k * 8, m);
 #pragma unroll
-    for (int side = 0; side < 2; ++side) {
-      float x[2][8];
-      float amax = 0.0f;
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        unpack8<T>(raw[p][side][k], x[k]);
-        if (side == 0 && a.c.key_mean != nullptr && at[p] >= 0) {
-          float m[8];
-          mean8(a.c.key_mean + head[p] * D + lane * 16 + k * 8, m);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[k][i] = __fsub_rn(x[k][i], m[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) amax = amax3(amax, x[k][i], x[k][i + 1]);
+        for (int i = 0; i < 8; ++i) x[k][i] = __fsub_rn(x[k][i], m[i]);
       }
 #pragma unroll
-      for (int o = kLanes / 2; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-      if (at[p] < 0) continue;
-      const float scale = amax == 0.0f ? 1.0f : __fmul_rn(amax, 1.0f / 127.0f);
-      int8_t* codes = static_cast<int8_t*>(side == 0 ? a.c.key_codes : a.c.value_codes);
-      const uint2 lo = row_codes(x[0], scale), hi = row_codes(x[1], scale);
-      *reinterpret_cast<uint4*>(codes + at[p] * D + lane * 16) = make_uint4(lo.x, lo.y, hi.x, hi.y);
-      if (lane == 0) (side == 0 ? a.c.key_scales : a.c.value_scales)[at[p]] = scale;
+      for (int i = 0; i < 8; i += 2) amax = amax3(amax, x[k][i], x[k][i + 1]);
     }
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    if (at < 0) continue;
+    const float scale = amax == 0.0f ? 1.0f : __fmul_rn(amax, 1.0f / 127.0f);
+    int8_t* codes = static_cast<int8_t*>(side == 0 ? a.c.key_codes : a.c.value_codes);
+    const uint2 lo = row_codes(x[0], scale), hi = row_codes(x[1], scale);
+    *reinterpret_cast<uint4*>(codes + at * D + lane * 16) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+    if (lane == 0) (side == 0 ? a.c.key_scales : a.c.value_scales)[at] = scale;
   }
 }
 
@@ -203,65 +192,57 @@ __global__ void __launch_bounds__(kCacheThreads) cache_read_kernel(CacheRowsArgs
   constexpr int kRows = kCacheThreads / kLanes;
   const int b = blockIdx.y;
   const int lane = threadIdx.x % kLanes;
-  const CacheRowWalk walk(static_cast<int64_t>(blockIdx.x) * (kRows * kCachePasses), a.tokens);
+  const CacheRowWalk walk(static_cast<int64_t>(blockIdx.x) * kRows, a.tokens);
   int64_t n = a.tokens;
   if (a.counts != nullptr) n = min(n, static_cast<int64_t>(__ldg(a.counts + b)));
   const int64_t length = __ldg(a.c.lengths + b);
-  int64_t at[kCachePasses], head[kCachePasses];
-  unsigned token[kCachePasses];
+  int64_t head;
+  unsigned token;
+  walk.at(threadIdx.x / kLanes, &head, &token);
+  const int64_t at = head < a.c.kv_heads && token < n
+                         ? cache_row(a.c, a.page_shift, b, static_cast<int>(head), length + token)
+                         : -1;
+  uint4 w[2];
+  float scale[2];
 #pragma unroll
-  for (int p = 0; p < kCachePasses; ++p) {
-    walk.at(threadIdx.x / kLanes + p * kRows, &head[p], &token[p]);
-    at[p] = head[p] < a.c.kv_heads && token[p] < n
-                ? cache_row(a.c, a.page_shift, b, static_cast<int>(head[p]), length + token[p])
-                : -1;
+  for (int side = 0; side < 2; ++side) {
+    if (at < 0) continue;
+    const int8_t* codes = static_cast<const int8_t*>(side == 0 ? a.c.key_codes : a.c.value_codes);
+    w[side] = *reinterpret_cast<const uint4*>(codes + at * D + lane * 16);
+    scale[side] = (side == 0 ? a.c.key_scales : a.c.value_scales)[at];
   }
-  uint4 w[kCachePasses][2];
-  float scale[kCachePasses][2];
+  if (head >= a.c.kv_heads) return;
+  const int64_t o = ((static_cast<int64_t>(b) * a.c.kv_heads + head) * a.tokens + token) * D + lane * 16;
 #pragma unroll
-  for (int p = 0; p < kCachePasses; ++p)
+  for (int side = 0; side < 2; ++side) {
 #pragma unroll
-    for (int side = 0; side < 2; ++side) {
-      if (at[p] < 0) continue;
-      const int8_t* codes = static_cast<const int8_t*>(side == 0 ? a.c.key_codes : a.c.value_codes);
-      w[p][side] = *reinterpret_cast<const uint4*>(codes + at[p] * D + lane * 16);
-      scale[p][side] = (side == 0 ? a.c.key_scales : a.c.value_scales)[at[p]];
-    }
+    for (int k = 0; k < 2; ++k) {
+      uint4 y = make_uint4(0u, 0u, 0u, 0u);
+      if (at >= 0) {
+        float x[8];
+        codes_f32(k == 0 ? w[side].x : w[side].z, x, 0);
+        codes_f32(k == 0 ? w[side].y : w[side].w, x, 4);
 #pragma unroll
-  for (int p = 0; p < kCachePasses; ++p) {
-    if (head[p] >= a.c.kv_heads) continue;
-    const int64_t o = ((static_cast<int64_t>(b) * a.c.kv_heads + head[p]) * a.tokens + token[p]) * D + lane * 16;
+        for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(x[i], scale[side]);
+        if (side == 0 && a.c.key_mean != nullptr) {
+          float m[8];
+          mean8(a.c.key_mean + head * D + lane * 16 + k * 8, m);
 #pragma unroll
-    for (int side = 0; side < 2; ++side) {
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        uint4 y = make_uint4(0u, 0u, 0u, 0u);
-        if (at[p] >= 0) {
-          float x[8];
-          codes_f32(k == 0 ? w[p][side].x : w[p][side].z, x, 0);
-          codes_f32(k == 0 ? w[p][side].y : w[p][side].w, x, 4);
-#pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = __fmul_rn(x[i], scale[p][side]);
-          if (side == 0 && a.c.key_mean != nullptr) {
-            float m[8];
-            mean8(a.c.key_mean + head[p] * D + lane * 16 + k * 8, m);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = __fadd_rn(x[i], m[i]);
-          }
-          y.x = pack2(x[0], x[1], T());
-          y.y = pack2(x[2], x[3], T());
-          y.z = pack2(x[4], x[5], T());
-          y.w = pack2(x[6], x[7], T());
+          for (int i = 0; i < 8; ++i) x[i] = __fadd_rn(x[i], m[i]);
         }
-        *reinterpret_cast<uint4*>(static_cast<T*>(a.out[side]) + o + k * 8) = y;
+        y.x = pack2(x[0], x[1], T());
+        y.y = pack2(x[2], x[3], T());
+        y.z = pack2(x[4], x[5], T());
+        y.w = pack2(x[6], x[7], T());
       }
+      *reinterpret_cast<uint4*>(static_cast<T*>(a.out[side]) + o + k * 8) = y;
     }
   }
 }
 
-// One CTA moves the rows of one (request, KV head), K then V: every source
-// row is in registers before the barrier, every target row is written after
-// it, because a row may be both.
+// One CTA moves the key rows of one (request, KV head), another its value rows
+// (blockIdx.z): every source row is in registers before the barrier, every target
+// row is written after it, because a row may be both.
 template <int D>
 __global__ void __launch_bounds__(kCacheThreads) cache_keep_kernel(piper_b200_kv_cache_t c, const int32_t* path,
                                                                    int64_t path_stride, int nodes,
