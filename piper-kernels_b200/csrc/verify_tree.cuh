@@ -64,12 +64,15 @@ struct VerifyArgs {
 };
 
 // What is left of probability p after taking out the draft's q n times:
-// max(r - q, 0) over each total, given as (up, 1 / (total * up)): up is 1, or
-// kVerifyUp where the total is subnormal.  (The second product costs 2 % of the
-// largest case; bodies of their own for such totals cost as much or more.)
-__device__ __forceinline__ float rest_of(float p, float q, const float2* over, int n) {
+// max(r - q, 0) over each total, given as reciprocals.  kSmall: a negative one is
+// that of a subnormal total times kVerifyUp.
+template <bool kSmall = false>
+__device__ __forceinline__ float rest_of(float p, float q, const float* over, int n) {
   float r = p;
-  for (int k = 0; k < n; ++k) r = fmaxf(r - q, 0.0f) * over[k].x * over[k].y;
+  for (int k = 0; k < n; ++k) {
+    r = fmaxf(r - q, 0.0f);
+    r = kSmall && over[k] < 0.0f ? r * kVerifyUp * -over[k] : r * over[k];
+  }
   return r;
 }
 
@@ -137,6 +140,29 @@ __device__ __forceinline__ void verify_words(const VerifyArgs& a, const float* p
   }
 }
 
+// The passes over this thread's words of [begin, end) when a total was subnormal.
+// Not inlined: they are rare, and their registers would be the others'.
+__device__ __noinline__ float verify_small_sum(const float* p, const float* q, int begin, int end, const float* over,
+                                               int n) {
+  float sum = 0.0f;
+  for (int v = begin + threadIdx.x; v < end; v += kVerifyThreads) {
+    const float y = __ldg(q + v);
+    sum += fmaxf(rest_of<true>(__ldg(p + v), y, over, n) - y, 0.0f);
+  }
+  return sum;
+}
+__device__ __noinline__ VerifyBest verify_small_best(const float* p, const float* q, const float* e, int begin,
+                                                     int end, const float* over, int n, bool less) {
+  VerifyBest best{-1.0f, 0};
+  for (int v = begin + threadIdx.x; v < end; v += kVerifyThreads) {
+    const float y = __ldg(q + v);
+    const float r = rest_of<true>(__ldg(p + v), y, over, n);
+    const float s = __fdiv_rn(less ? fmaxf(r - y, 0.0f) : r, __ldg(e + v));
+    if (s > best.score) best = VerifyBest{s, v};
+  }
+  return best;
+}
+
 // grid (CTAs of a cluster, batch), a cluster to a request.
 __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(VerifyArgs a) {
   namespace cg = cooperative_groups;
@@ -144,7 +170,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(VerifyAr
   constexpr int kWarps = kVerifyThreads / 32;
   __shared__ float node_p[kMaxNodes], node_q[kMaxNodes], node_u[kMaxNodes];
   __shared__ int node_parent[kMaxNodes];  // -1: absent
-  __shared__ float2 over[kMaxNodes];
+  __shared__ float over[kMaxNodes];
   __shared__ float warp_sum[kWarps], joined_sum[2];  // by turn
   __shared__ VerifyBest warp_best[kWarps], joined_best;
   const int64_t b = blockIdx.y;
@@ -184,17 +210,22 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(VerifyAr
   // token does not depend on its total: the last pass takes that draft out
   // without it, unless its scores come out too small to be told from nothing.
   bool open_end = false, may_end = true;
+  // A total since the last accepted node was subnormal: such a walk takes the two
+  // functions above (a second product for every word cost 5 % of the largest case,
+  // loops in place 3 %, the branch 1.5 %).
+  bool small = false;
   VerifyBest best;
   const float* er = a.noise + b * a.noise_stride;
   for (;;) {  // twice at most
     while (children != 0) {
       const int i = __ffsll(static_cast<long long>(children)) - 1;
       const float p = node_p[i], q = node_q[i];
-      if (node_u[i] * q < rest_of(p, q, over, rejected)) {
+      if (node_u[i] * q < rest_of<true>(p, q, over, rejected)) {
         if (rank == 0 && tid == 0) path[count] = i;
         ++count;
         current = i;
         rejected = 0;
+        small = false;
         children = children_of(i);
         continue;
       }
@@ -206,9 +237,13 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(VerifyAr
       const float* pr = a.target + b * a.ts[0] + current * a.ts[1];
       const float* qr = a.draft + b * a.ds[0] + current * a.ds[1];
       float sum = 0.0f;
-      verify_words<true, false>(
-          a, pr, qr, nullptr, begin, end,
-          [&](int, float x, float y, float) { sum += fmaxf(rest_of(x, y, over, rejected) - y, 0.0f); }, [] {});
+      if (!small) {
+        verify_words<true, false>(
+            a, pr, qr, nullptr, begin, end,
+            [&](int, float x, float y, float) { sum += fmaxf(rest_of(x, y, over, rejected) - y, 0.0f); }, [] {});
+      } else {
+        sum = verify_small_sum(pr, qr, begin, end, over, rejected);
+      }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
       if (lane == 0) warp_sum[warp] = sum;
@@ -225,9 +260,10 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(VerifyAr
       // each passes the next cluster.sync after its reading.
       turn ^= 1;
       if (total > 0.0f) {  // else nothing would be left: rest stays as it was
-        const float up = total < kVerifyLeast ? kVerifyUp : 1.0f;
-        if (tid == 0) over[rejected] = make_float2(up, 1.0f / (total * up));
+        const bool subnormal = total < kVerifyLeast;
+        if (tid == 0) over[rejected] = subnormal ? -1.0f / (total * kVerifyUp) : 1.0f / total;
         ++rejected;
+        small |= subnormal;
       }
       __syncthreads();
     }
@@ -245,9 +281,11 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(VerifyAr
       }
     };
     auto share = [&] { bound = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(bound))); };
-    if (rejected == 0 && !open_end)
+    if (rejected == 0 && !open_end) {
       verify_words<false, true>(a, pr, qr, er, begin, end, [&](int v, float x, float, float e) { race(v, x, e); }, share);
-    else
+    } else if (small) {
+      best = verify_small_best(pr, qr, er, begin, end, over, rejected, open_end);
+    } else {
       verify_words<true, true>(
           a, pr, qr, er, begin, end,
           [&](int v, float x, float y, float e) {
@@ -255,6 +293,7 @@ __global__ void __launch_bounds__(kVerifyThreads, 2) verify_tree_kernel(VerifyAr
             race(v, open_end ? fmaxf(r - y, 0.0f) : r, e);
           },
           share);
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
       best = verify_better(best, VerifyBest{__shfl_xor_sync(0xffffffffu, best.score, o),
