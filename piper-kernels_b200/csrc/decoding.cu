@@ -120,14 +120,19 @@ TreePlan tree_plan(int64_t batch, int64_t kv_heads, int64_t rows, int64_t positi
   p.row_tiles = static_cast<int>((rows + S::kRows - 1) / S::kRows);
   const int64_t segments = batch * kv_heads * p.row_tiles;
   const int64_t most = (positions + S::kKeys - 1) / S::kKeys;
-  // Tables of a few tiles: a CTA for each (request, head, row tile), one
-  // launch and nothing to merge.
+  // Tables of a few tiles: a CTA for each (request, head, row tile), one launch and
+  // nothing to merge.  Whole against shared segments, 32 over 8 heads of 128: one
+  // request of 256 tokens 7.4 and 12.2 us, of 1000 11.5 and 12.8, of 2000 (16 tiles)
+  // 18.6 and 13.3; 64 requests of 100 to 1000 26.8 and 28.5, of 100 to 2000 39.5 and
+  // 37.5.
   p.whole = most <= 8 && segments < (int64_t(1) << 31);
   if (p.whole) {
     p.grid = segments;
     return p;
   }
   const int64_t slots = static_cast<int64_t>(sms) * S::kCtas;
+  // No more CTAs than the segments have pairs of tiles: it takes as long as a full
+  // grid, whose other CTAs find nothing to do, for less workspace.
   p.grid = most > 2 * slots / segments ? slots : std::max<int64_t>(1, segments * most / 2);
   p.bytes = static_cast<size_t>(p.grid) * 2 * S::kPart * 4;
   return p;
@@ -137,8 +142,9 @@ TreePlan tree_plan(int64_t batch, int64_t kv_heads, int64_t rows, int64_t positi
 // tile of 8, 16 or that many rows on four warps, up to 128 a tcgen05 tile whose
 // streams take alternate keys, more a pair of them over the same keys.  Both
 // sides of the limits, 32 requests of 1000 to 8191 tokens, 8 KV heads of 128 (of
-// 64): 8 and 16 rows 58 and 69 us (39 and 47); 24 rows on the mma tile 108, on the
-// tcgen05 tile 160 (32 rows 93 and 143), which is as long for 32 rows (64: 174).
+// 64): 8 and 16 rows 58 and 69 us (38 and 47); 24 rows on the mma tile 110, on the
+// tcgen05 tile 161 (32 rows 93 and 143), which is as long for 32 rows (162; 64:
+// 170).  One request of 131072 tokens: 128 rows 138 us, 132 on the pair 196.
 enum class TreeKind { kEight, kSixteen, kMore, kAlternate, kPair };
 template <int D>
 constexpr int kMoreRows = D == 64 ? 32 : 24;

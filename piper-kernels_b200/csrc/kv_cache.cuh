@@ -1,13 +1,16 @@
 // The quantised paged KV cache: writing new rows, reading rows back, and
 // moving the accepted rows of a drafted tree together.  All three would be
-// bound by memory; writing is by its arithmetic (19 instructions a value, the
-// near-tie test of the division-free rounding among them) and reading nearly.
+// bound by memory.
 //
-// Measured (4 prompts of 5001 to 8192 tokens, 32 heads of 128, bf16): written and
-// read back in 336 us, 3.9 TB/s or 0.60 of the copy rate (0.65 with the zeros that
-// fill the shorter prompts); without the near-tie test, which exact codes need, 304
-// us; IEEE division in place of the division-free rounding, and eight values a
-// lane, 392 us.
+// Measured (4 prompts of 5001 to 8192 tokens, 32 heads of 128, bf16): written in
+// 181 us, read back in 156, where the copy rate allows 101 and 118 (the zeros that
+// fill the shorter prompts included).  Writing takes 17 instructions a value, the
+// near-tie test of the division-free rounding among them (both without it, which
+// exact codes need, 304 us instead of 336; with IEEE division, and eight values a
+// lane, 392), with the ALU pipe busy half the time and 43 % of an SM's warps
+// resident.  Reading takes 10 with 87 % resident and the issue slots busy 42 % of the
+// time: latency, of the table, the row and the key mean, which both kernels load
+// again for every row.
 //
 // A row is one token of one KV head: D codes q[d] and a scale s, standing for
 // q[d] * s (plus the key mean for keys), with

@@ -48,10 +48,11 @@
 // Measured (32 query over 8 KV heads of 128, pages of 64, one token each): 64
 // requests of 1 to 8192 tokens 94 us, 5.9 TB/s or 0.92 of the copy rate; one
 // request of 256 tokens 7.6 us.  24 heads of 64, 5 nodes, 32 requests of 333 to
-// 4097 tokens in pages of 16: 58 us, 0.63 of the copy rate.  With 16 rows
+// 4097 tokens in pages of 16: 57 us, 0.63 of the copy rate (pages of 64: 51), the
+// ALU pipe busy 46 % and the issue slots 58 % of the time.  With 16 rows
 // instructions bound it, 320 of some 660 for 32 keys a warp turning codes into
 // fp16: 16 keys a warp took 131 us for 110.  32 requests of 1000 to 8191 tokens,
-// 8 KV heads of 128: 8 rows 58 us, 16 rows 69, 24 rows 108; of 64: 39, 47, 32 rows
+// 8 KV heads of 128: 8 rows 58 us, 16 rows 69, 24 rows 110; of 64: 38, 47, 32 rows
 // 93.
 #pragma once
 
@@ -104,9 +105,10 @@ struct TreeTile {
   static constexpr bool kHeld = ROWS == 8;  // query fragments in registers
   static constexpr int kQuery = kHeld ? 0 : (D / 16) * 32 * ROWS;
   static constexpr int kFixed = kJoin + kState + kQuery + kRows * 8 + 512;
-  // Per SM, what registers and stages allow (8 rows: of 128, three spilled
-  // and took 115 us instead of 94; of 64, three took 73 us instead of 68, five
-  // 82; 16 rows of 64: four 81 us instead of 69).
+  // Per SM, what registers and stages allow.  8 rows of 128, 64 ragged requests as
+  // above: two 94 us, three 110 (they spill).  8 rows of 64, 24 heads as above:
+  // three 61 us, four 57, five 73.  16 rows of 64, 32 requests: two 52 us, three 47,
+  // four 57.
   static constexpr int kCtas = D == 64 ? (ROWS == 8 ? 4 : ROWS == 16 ? 3 : 2) : 2;
   static constexpr int kLead = ROWS == 8 ? 3 : 4;  // a segment's start and end, in key tiles
   static constexpr int kFit = (227 * 1024 / kCtas - 1024 * 2 - kFixed) / kStageAlloc;
@@ -174,7 +176,9 @@ __device__ __forceinline__ void tree_find(const TreeArgs& a, int64_t u, int* req
   *first = base;
 }
 
-// CTAs that share the units: at least two key tiles' worth each.
+// CTAs that share the units: at least two key tiles' worth each (one request of
+// 2000 tokens, 8 KV heads of 128: 13.3 us; at least four 14.8; at least one 12.0,
+// and twice the workspace for tables of few tiles).
 template <typename S>
 __device__ __forceinline__ int64_t tree_ctas(int64_t units, int grid) {
   return max(static_cast<int64_t>(1), min(static_cast<int64_t>(grid), units / (S::kLead + 2)));

@@ -26,12 +26,16 @@
 // 16-17 conversion of K, 18-19 of V, 20 fetches, 21 issues MMAs, 22 owns
 // TMEM.
 //
-// Measured: 16 nodes of 40 over 8 heads of 128 and 131072 tokens (80 rows) 126
-// us, 341 TFLOP/s; 16 requests of 4000 to 8191 tokens, 47 nodes, 32 over 8 heads
-// (188 rows) 185 us, 410 TFLOP/s.  The time hardly depends on the rows up to
-// 128 (17 rows 122 us, 128 rows 137 us): what bounds it is a stream's chain of
-// scores, weights and numerators, some 8000 cycles a tile with two tiles under
-// way, the tensor pipe being busy a quarter of the time.  Tried and slower: a
+// Measured: 16 nodes of 40 over 8 heads of 128 and 131072 tokens (80 rows) 130
+// us, 330 TFLOP/s; 16 requests of 4000 to 8191 tokens, 47 nodes, 32 over 8 heads
+// (188 rows) 186 us, 408 TFLOP/s.  The time hardly depends on the rows up to 128
+// (131072 tokens: 25 rows 119 us, 40 rows 122, 128 rows 138; in pairs 132 rows 196,
+// 256 rows 216).  What bounds it is a stream's chain of scores, weights and
+// numerators, some 8500 cycles a tile with two tiles under way (tensor pipe busy 24
+// and 27 % of the time, issue slots 45 and 44), and in it the fullest of an SM's four
+// sub-partitions: rows fill TMEM lanes, and with them the warps of sub-partitions,
+// from 0 up, so that 80 rows give one 132000 instructions and another 44000 (188
+// rows: 178000 and 86000).  Tried and slower: a
 // thread a row with all 128 scores in registers (204 us; one long unrolled
 // body), half tiles with both halves' scores in TMEM (191 us; twice the
 // hand-overs, and QK^T of 64 keys reads Q twice).

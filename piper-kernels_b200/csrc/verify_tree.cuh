@@ -14,16 +14,16 @@
 // passes twice as long), the last division, by the noise, is IEEE: equal
 // quotients are equal, and go to the lowest index.
 //
-// A warp divides only near its best quotient (a division for every word: 51 us
-// instead of 45 in the largest case below).
+// A warp divides only near its best quotient (a division for every word: 6 us more
+// in the largest case below).
 //
 // Bound: memory (12 bytes a word for the last pass), and with few requests the
 // latency of the passes that follow one another.  A cluster of CTAs shares a
 // request's vocabulary and joins its sums and maxima through distributed
 // shared memory, in rank order (one CTA a request took four times as long).
 //
-// Measured: a chain of 8 over 32768 words 7.1 us; 16 trees of 16 over 50001 words
-// (rows that start at any element) 11 us; 64 trees of 32 over 131072 words 45 us,
+// Measured: a chain of 8 over 32768 words 7.0 us; 16 trees of 16 over 50001 words
+// (rows that start at any element) 12 us; 64 trees of 32 over 131072 words 43 us,
 // where the mean request reads 1.7 to 1.8 MB: 0.4 of the copy rate, as 512 CTAs run
 // in two turns and a request of four rejections takes four passes.  No faster: the
 // noise fetched into L2 in advance (52 before, 53), half the loads under way and three
